@@ -8,6 +8,7 @@
 // status and records a message for fmkv_last_error().
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -168,10 +169,16 @@ struct ExtWorkspace {
 struct Workspace {
   float* ptr = nullptr;
   size_t bytes = 0;
+  // a pool's: earlier, smaller buffers stay until the handle's end, since a
+  // captured graph may use them (each at least half as large again as the one
+  // before, so together they stay below twice the last)
+  bool keep = false;
+  std::vector<float*> kept;
   // zero: a new allocation starts zeroed (head-block staging, whose
   // unwritten slots are read, masked, as the cache's own are)
   int ensure(size_t need, bool zero = false) {
     if (need <= bytes) return FMKV_OK;
+    if (keep) return grow(need);
     if (ptr) (void)hipFree(ptr);
     ptr = nullptr;
     bytes = 0;
@@ -184,7 +191,26 @@ struct Workspace {
     bytes = need;
     return FMKV_OK;
   }
+  // (allocating does not end a capture in this thread's relaxed mode)
+  int grow(size_t need) {
+    const size_t want = std::max(need, bytes + bytes / 2);
+    float* p = nullptr;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    const hipError_t e = hipMalloc(&p, want);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return fail(FMKV_ERR_OOM, "workspace allocation failed");
+    }
+    if (ptr) kept.push_back(ptr);
+    ptr = p;
+    bytes = want;
+    return FMKV_OK;
+  }
   void release() {
+    for (float* p : kept) (void)hipFree(p);
+    kept.clear();
     if (ptr) (void)hipFree(ptr);
     ptr = nullptr;
     bytes = 0;
@@ -275,6 +301,7 @@ struct fmkv_pool {
   Workspace ws;
   PrefillScratch* split = nullptr;
   int cus;
+  int device;  // the GPU that holds the pool
 };
 
 namespace {
@@ -590,6 +617,29 @@ int prepare_attention(fmkv_cache* c, int64_t T, const void* q, int32_t n_q_heads
                                   out, out_dtype, wg_per_cu, 1, 1, new_col, a, ext);
 }
 
+// The most blocks that hold a window of `win` positions and `sinks` first ones.
+int64_t window_blocks(int64_t win, int64_t sinks) {
+  constexpr int64_t B = fmkv::kBlockTokens;
+  return (win + B - 2) / B + 1 + (sinks + B - 1) / B;
+}
+
+// A window's arguments; the GPU of a call.
+int check_window(int32_t window, int32_t sinks) {
+  if (window < 1 || window > (1 << 30))
+    return fail(FMKV_ERR_INVALID_ARG, "window must be in [1, 2^30]");
+  if (sinks < 0 || sinks > (1 << 30)) return fail(FMKV_ERR_INVALID_ARG, "sinks must be in [0, 2^30]");
+  return FMKV_OK;
+}
+int check_device(const fmkv_pool* p) {
+  int dev = -1;
+  const hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return hip_fail(e, "hipGetDevice");
+  if (dev != p->device)
+    return fail(FMKV_ERR_INVALID_ARG, "the pool is on GPU " + std::to_string(p->device) +
+                                          ", the current GPU is " + std::to_string(dev));
+  return FMKV_OK;
+}
+
 int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
                          const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
                          int32_t n_seqs, int32_t n_new, fmkv::AppendArgs* a, int* tasks) {
@@ -615,10 +665,12 @@ int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
   return FMKV_OK;
 }
 
+// win > 0: over the last `win` positions and the first `sinks` ones.
 int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
                             int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
                             int32_t max_seq_len, int32_t n_q_heads, float scale, float tau,
-                            void* out, int32_t out_dtype, int new_col, fmkv::AttnArgs* a) {
+                            void* out, int32_t out_dtype, int new_col, fmkv::AttnArgs* a,
+                            int32_t win = 0, int32_t sinks = 0) {
   if (n_seqs < 0 || max_seq_len < 0 || max_blocks < 1)
     return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / max_seq_len / max_blocks");
   if (n_seqs > 0 && (!block_tables || !seq_lens))
@@ -630,7 +682,14 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   a->seq_len = 0;
   a->window = 0;
   a->vis_begin = 0;
-  const int64_t nblk = (max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
+  if (win > 0) {
+    int rc = check_attn_args(p->desc, q, n_q_heads, tau, out, out_dtype);
+    if (rc || (rc = check_device(p))) return rc;
+  }
+  a->win = win;
+  a->sinks = sinks;
+  int64_t nblk = ((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
+  if (win > 0) nblk = std::min(nblk, window_blocks(win, sinks));
   // Ragged lengths: the bound counts every sequence at max_seq_len, so the
   // plan aims at several work-groups per CU (the dispatcher balances their
   // uneven sizes), but at least 64 blocks each (a work-group's prologue and
@@ -1113,6 +1172,9 @@ int fmkv_pool_create(const fmkv_cache_desc* desc, int64_t n_blocks, fmkv_pool** 
   sign_bits_of(*desc, p->sign_bits);
   p->cus = device_cus();
   p->split = prefill_scratch_join();
+  p->device = 0;
+  (void)hipGetDevice(&p->device);
+  p->ws.keep = true;
   *out = p;
   return FMKV_OK;
 }
@@ -1136,12 +1198,17 @@ int fmkv_paged_prefill_step(fmkv_pool* p, const void* k, const void* v,
                                          n_new, 0, q, n_q_heads, scale, out, out_dtype, stream);
 }
 
-int fmkv_paged_prefill_step_bounded(fmkv_pool* p, const void* k, const void* v,
-                                    const int32_t* block_tables, int32_t max_blocks,
-                                    const int32_t* start_pos, int32_t n_seqs, int32_t n_new,
-                                    int32_t max_seq_len, const void* q, int32_t n_q_heads,
-                                    float scale, void* out, int32_t out_dtype, void* stream) {
-  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+}  // extern "C"
+
+namespace {
+
+// Batched prefill: the append of k and v (both null with `stored`: the rows are
+// in the pool), then the attention, over a window with sinks where window > 0.
+int paged_prefill_impl(fmkv_pool* p, bool stored, const void* k, const void* v,
+                       const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
+                       int32_t n_seqs, int32_t n_new, int32_t max_seq_len, const void* q,
+                       int32_t n_q_heads, float scale, int32_t window, int32_t sinks, void* out,
+                       int32_t out_dtype, void* stream) {
   if (max_seq_len < 0) return fail(FMKV_ERR_INVALID_ARG, "max_seq_len must be >= 0 (0: unknown)");
   if (n_seqs < 1 || n_new < 1)
     return fail(FMKV_ERR_INVALID_ARG, "a prefill step needs n_seqs >= 1 and n_new >= 1");
@@ -1153,17 +1220,20 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* p, const void* k, const void* v,
     return fail(FMKV_ERR_INVALID_ARG, "n_new too large for one prefill step");
   fmkv::AppendArgs ap;
   int tasks = 0;
-  rc = prepare_paged_append(p, k, v, block_tables, max_blocks, start_pos, n_seqs, n_new, &ap,
-                            &tasks);
+  // (stored: q stands in for the rows, which are not read)
+  rc = prepare_paged_append(p, stored ? q : k, stored ? q : v, block_tables, max_blocks, start_pos,
+                            n_seqs, n_new, &ap, &tasks);
   if (rc) return rc;
+  if (window > 0 && (rc = check_device(p))) return rc;
   fmkv::PrefillArgs pa;
   pa.old_st = ap.st;
   pa.new_st = ap.st;
+  pa.sinks = sinks;
   pa.p0 = 0;
   pa.start_pos = start_pos;
   pa.n_seqs = n_seqs;
   pa.n_q = n_new;
-  pa.window = 0;
+  pa.window = window;
   pa.ring_slots = 0;
   pa.vis_begin = 0;
   pa.p_split = 0;
@@ -1177,13 +1247,79 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* p, const void* k, const void* v,
   pa.out = out;
   pa.out_f32 = out_dtype == FMKV_DTYPE_F32 ? 1 : 0;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipError_t e = fmkv::launch_append(ap, n_seqs, tasks, s);
-  if (e != hipSuccess) return hip_fail(e, "paged append launch");
+  hipError_t e = hipSuccess;
+  if (!stored) {
+    e = fmkv::launch_append(ap, n_seqs, tasks, s);
+    if (e != hipSuccess) return hip_fail(e, "paged append launch");
+  }
   // (starts are on the device: the caller or the table's width bounds the lengths)
   int64_t blocks = ((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
   if (blocks == 0 || blocks > max_blocks) blocks = max_blocks;
+  // (a tile of 64 rows sees a window, its own positions and the sinks)
+  if (window > 0) blocks = std::min(blocks, window_blocks((int64_t)window + 64, sinks));
   e = run_prefill(pa, p->split, p->cus, blocks / 2 + 2, s);
   if (e != hipSuccess) return hip_fail(e, "prefill attention launch");
+  return FMKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmkv_paged_prefill_step_bounded(fmkv_pool* p, const void* k, const void* v,
+                                    const int32_t* block_tables, int32_t max_blocks,
+                                    const int32_t* start_pos, int32_t n_seqs, int32_t n_new,
+                                    int32_t max_seq_len, const void* q, int32_t n_q_heads,
+                                    float scale, void* out, int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  return paged_prefill_impl(p, false, k, v, block_tables, max_blocks, start_pos, n_seqs, n_new,
+                            max_seq_len, q, n_q_heads, scale, 0, 0, out, out_dtype, stream);
+}
+
+int fmkv_paged_window_prefill_step(fmkv_pool* p, const void* k, const void* v,
+                                   const int32_t* block_tables, int32_t max_blocks,
+                                   const int32_t* start_pos, int32_t n_seqs, int32_t n_new,
+                                   int32_t max_seq_len, const void* q, int32_t n_q_heads,
+                                   float scale, int32_t window, int32_t sinks, void* out,
+                                   int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  const int rc = check_window(window, sinks);
+  if (rc) return rc;
+  return paged_prefill_impl(p, false, k, v, block_tables, max_blocks, start_pos, n_seqs, n_new,
+                            max_seq_len, q, n_q_heads, scale, window, sinks, out, out_dtype, stream);
+}
+
+int fmkv_paged_window_prefill_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
+                                        int32_t max_blocks, const int32_t* start_pos,
+                                        int32_t n_seqs, int32_t n_new, int32_t max_seq_len,
+                                        int32_t n_q_heads, float scale, int32_t window,
+                                        int32_t sinks, void* out, int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  const int rc = check_window(window, sinks);
+  if (rc) return rc;
+  return paged_prefill_impl(p, true, nullptr, nullptr, block_tables, max_blocks, start_pos, n_seqs,
+                            n_new, max_seq_len, q, n_q_heads, scale, window, sinks, out, out_dtype,
+                            stream);
+}
+
+int fmkv_paged_window_decode_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
+                                       int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
+                                       int32_t max_seq_len, int32_t n_q_heads, float scale,
+                                       int32_t window, int32_t sinks, void* out, int32_t out_dtype,
+                                       void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  int rc = check_window(window, sinks);
+  if (rc) return rc;
+  if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  fmkv::AttnArgs a;
+  rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
+                               n_q_heads, scale, 0.0f, out, out_dtype, 0, &a, window, sinks);
+  if (rc || n_seqs == 0) return rc;
+  hipEvent_t e0, e1;
+  next_events(&e0, &e1);
+  hipError_t e = launch_attention(a, n_seqs, p->desc.n_kv_heads, static_cast<hipStream_t>(stream),
+                                  e0, e1);
+  if (e != hipSuccess) return hip_fail(e, "paged window attention launch");
   return FMKV_OK;
 }
 
@@ -1244,7 +1380,7 @@ int paged_decode_step_impl(fmkv_pool* p, const void* k, const void* v,
                            const int32_t* start_pos, const int32_t* seq_lens, int32_t n_seqs,
                            int32_t n_new, int32_t max_seq_len, const void* q, int32_t n_q_heads,
                            float scale, float tau, void* out, int32_t out_dtype, void* stream,
-                           const fmkv_kv_prologue* pro) {
+                           const fmkv_kv_prologue* pro, int32_t win = 0, int32_t sinks = 0) {
   if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
   if (n_new < 1) return fail(FMKV_ERR_INVALID_ARG, "a decode step appends at least one token");
   int rc;
@@ -1260,7 +1396,7 @@ int paged_decode_step_impl(fmkv_pool* p, const void* k, const void* v,
   const int fused = n_new == 1 ? 1 : 0;
   fmkv::AttnArgs at;
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
-                               n_q_heads, scale, tau, out, out_dtype, fused, &at);
+                               n_q_heads, scale, tau, out, out_dtype, fused, &at, win, sinks);
   if (rc || n_seqs == 0) return rc;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e;
@@ -1293,6 +1429,21 @@ int fmkv_paged_decode_step(fmkv_pool* p, const void* k, const void* v,
                                 stream, nullptr);
 }
 
+int fmkv_paged_window_decode_step(fmkv_pool* p, const void* k, const void* v,
+                                  const int32_t* block_tables, int32_t max_blocks,
+                                  const int32_t* start_pos, const int32_t* seq_lens,
+                                  int32_t n_seqs, int32_t max_seq_len, const void* q,
+                                  int32_t n_q_heads, float scale, int32_t window, int32_t sinks,
+                                  void* out, int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  int rc = check_window(window, sinks);
+  if (rc) return rc;
+  if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  return paged_decode_step_impl(p, k, v, block_tables, max_blocks, start_pos, seq_lens, n_seqs, 1,
+                                max_seq_len, q, n_q_heads, scale, 0.0f, out, out_dtype, stream,
+                                nullptr, window, sinks);
+}
+
 int fmkv_paged_decode_step_projected(fmkv_pool* p, const void* k_proj, const void* v_proj,
                                      const int32_t* block_tables, int32_t max_blocks,
                                      const int32_t* start_pos, const int32_t* seq_lens,
@@ -1304,6 +1455,13 @@ int fmkv_paged_decode_step_projected(fmkv_pool* p, const void* k_proj, const voi
   return paged_decode_step_impl(p, k_proj, v_proj, block_tables, max_blocks, start_pos, seq_lens,
                                 n_seqs, n_new, max_seq_len, q, n_q_heads, scale, tau, out,
                                 out_dtype, stream, pro);
+}
+
+int fmkv_pool_storage(const fmkv_pool* p, void** base, int64_t* block_bytes) {
+  if (!p || !base || !block_bytes) return fail(FMKV_ERR_INVALID_ARG, "null argument");
+  *base = p->arena;
+  *block_bytes = p->layout.block_bytes * p->desc.n_kv_heads;
+  return FMKV_OK;
 }
 
 int fmkv_pool_read_codes(const fmkv_pool* p, void* codes, void* meta, void* stream) {

@@ -473,8 +473,9 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // per KV head -- the 16 matrix-core columns carry (group, head, high /
   // residual) instead of (head, high / residual), so each lane forms the
   // scores and P' of one group only (build_q_table)
-  static_assert(!PACK || (MODE == kDense && P::kSolo && D == 256 && BITS == 4),
+  static_assert(!PACK || ((MODE == kDense || MODE == kWindow) && P::kSolo && D == 256 && BITS == 4),
                 "packed columns: dense solo streams, head_dim 256, 4 bits");
+  static_assert(MODE != kWindow || PAGED, "a window with sinks is a paged pool's");
   constexpr int E = D / 64;
   constexpr int QS = P::kQS;
   // copy instructions per wave per block (the stats pass copies no V codes)
@@ -519,6 +520,14 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
     if (geo.blk_hi > a.st.table_stride) geo.blk_hi = a.st.table_stride;
     if (geo.blk_hi < geo.blk_lo) geo.blk_hi = geo.blk_lo;
   }
+  // kWindow: blocks below are numbered over the visible ones, wg.block(v) is
+  // the sequence's own number
+  WinGeom wg{};
+  if constexpr (MODE == kWindow) {
+    wg = win_geometry(Tg, a.win, a.sinks, a.st.table_stride);
+    geo = wg.geo;
+  }
+  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
   // one sequence: the host planned max_splits for exactly this block range
   // (no division before the first copies); paged: per sequence
   const int n_splits = PAGED ? n_splits_for(geo, bps0, bps, max_splits, skew_p) : max_splits;
@@ -562,18 +571,25 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // with LDS reads, so no later LDS access could go ahead of it either).
   // (the copy starts at the 16-byte boundary at or below the range's first
   // entry, tsh entries before it, in the same page)
-  int64_t n_tbl = 0;
+  // (kWindow: the part of the range past the sinks' blocks, the few of which
+  // are read from the table itself)
+  int64_t n_tbl = 0, tbl0 = b_begin;  // entries copied, the first one's block
   int tsh = 0;
   if constexpr (PAGED) {
-    tsh = (int)(((uintptr_t)(a.st.block_table + (int64_t)seq * a.st.table_stride + b_begin) & 15) >> 2);
     n_tbl = b_end - b_begin;
+    if constexpr (MODE == kWindow) {
+      const int64_t v0 = b_begin < wg.sink_blks ? wg.sink_blks : b_begin;
+      tbl0 = v0 + wg.skip;
+      n_tbl = b_end - v0;
+    }
+    tsh = (int)(((uintptr_t)(a.st.block_table + (int64_t)seq * a.st.table_stride + tbl0) & 15) >> 2);
     n_tbl = n_tbl < 0 ? 0 : (n_tbl > kTblCap - tsh ? kTblCap - tsh : n_tbl);
   }
   auto blk_ptr_loop = [&](int64_t lb) -> const uint8_t* {
     if constexpr (!PAGED) {
       return blk_ptr(lb);
     } else {
-      const int64_t r = lb - b_begin;
+      const int64_t r = lb - tbl0;
       int64_t phys = (r >= 0 && r < n_tbl) ? (int64_t)__builtin_amdgcn_readfirstlane(tbl_s[tsh + r])
                                            : (int64_t)table[lb];
       phys = phys < 0 ? 0 : (phys >= a.st.n_blocks ? a.st.n_blocks - 1 : phys);
@@ -618,6 +634,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // (a stage's first fill follows no reads of it: no wait, so that the
   // first copies do not wait for the argument struct's scalar loads)
   auto copy_block = [&](int st, int64_t lb, bool refill) {
+    lb = block_of(lb);
     const u32x4 rs = buffer_rsrc(refill ? blk_ptr_loop(lb) : blk_ptr(lb), (uint32_t)L.block_bytes);
     const uint32_t sl = pstage_lds + st * SB;
     if (refill) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // reads of this stage are done
@@ -644,7 +661,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // table's barrier publishes it to the other waves before any refill
   if constexpr (PAGED) {
     if (wave == 0 && n_tbl > 0) {
-      const u32x4 trs = buffer_rsrc(a.st.block_table + (int64_t)seq * a.st.table_stride + b_begin - tsh,
+      const u32x4 trs = buffer_rsrc(a.st.block_table + (int64_t)seq * a.st.table_stride + tbl0 - tsh,
                                     (uint32_t)((n_tbl + tsh) * 4));
       const int nk = (int)((n_tbl + tsh + 255) / 256);
       for (int k = 0; k < nk; k++) dma16(lds_addr(tbl_s) + k * kChunk, k * kChunk + lane * 16, trs);
@@ -845,15 +862,35 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
     // visibility: whole block in the common case (uniform test), per token
     // only at the edges of the visible range
     const int64_t t0 = b * kBlockTokens;
-    const bool full = t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim &&
-                      (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
+    const bool full =
+        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+                         : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
+        (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
+      // kWindow: a hidden token's weight is 0, but 0 * inf is NaN, and its V
+      // scale and bias may be anything (a page's earlier owner's, the slot that
+      // the new-token column writes meanwhile). They become 0 in the stage,
+      // lane (j, c < GH) clearing group c's of tokens 4j .. 4j + 3.
+      uint8_t* const vmeta_c =
+          const_cast<uint8_t*>(sp) + P::kMetaOff + half * 2 * MH + MH + c * 64 + j * 16;
+      u32x4 m = (u32x4){0, 0, 0, 0};
+      if (MODE == kWindow && c < GH) m = lds16(vmeta_c);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int64_t slot = t0 + 4 * j + i;
-        bool vis = slot >= vis_lo && slot < vis_hi && slot != ex_slot;
-        if (ring_trim) vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
-        if (!vis) s[i] = -INFINITY;
+        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+                                    : slot >= vis_lo && slot < vis_hi) &&
+                   slot != ex_slot;
+        if (MODE != kWindow && ring_trim)
+          vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
+        if (!vis) {
+          s[i] = -INFINITY;
+          m[i] = 0;
+        }
+      }
+      if constexpr (MODE == kWindow) {
+        if (c < GH) *reinterpret_cast<u32x4*>(vmeta_c) = m;
+        vm = lds16(sp + P::kMetaOff + half * 2 * MH + MH + (PACK ? grp * 64 : 0) + j * 16);
       }
     }
     if constexpr (MODE == kGated) {
@@ -975,7 +1012,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   for (int i = 0; i < nbx; i++) {
     const int rest = nbx - 1 - i;
     wait_copies<CP, NST - 1>(rest < NST - 1 ? rest : NST - 1);
-    process(pstage + st * SB, pb0 + (int64_t)NS * (MODE == kGated ? blist.pop() : i), i);
+    process(pstage + st * SB, block_of(pb0 + (int64_t)NS * (MODE == kGated ? blist.pop() : i)), i);
     if (i + NST < nbx)
       copy_block(st, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : i + NST), true);
     st = st + 1 == NST ? 0 : st + 1;
@@ -1155,7 +1192,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part_o, const
   if (n_cols < 0) {
     const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
     const SeqGeom geo =
-        seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
+        a.win > 0 ? win_geometry(T, a.win, a.sinks, a.st.table_stride).geo
+                  : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
     n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p) + a.new_col;
   }
   const int64_t stride = (int64_t)nqh;
@@ -1242,10 +1280,17 @@ template <int D, int BITS, int MODE>
 hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t ev0, hipEvent_t ev1) {
   // a paged pool has per-sequence lengths; a cache has neither
   if ((a.st.block_table != nullptr) != (a.seq_lens != nullptr)) return hipErrorInvalidValue;
+  if (MODE == kWindow && !a.st.block_table) return hipErrorInvalidValue;
   if constexpr (kSoloCapable<D, BITS>) {
     if (a.bps >= kSoloMinBlocks) {
       // head_dim 256 at 4 bits with at most 2 q heads per KV head (Gemma-4's
       // sliding layers): the packed-column form of the solo streams
+      if constexpr (MODE == kWindow) {
+        if constexpr (D == 256 && BITS == 4)
+          if (a.group <= 2)
+            return launch_kind<D, BITS, MODE, kPagedSoloWaves, true, true>(a, grid, s, ev0, ev1);
+        return launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1);
+      } else {
       if constexpr (MODE == kDense && D == 256 && BITS == 4) {
         if (a.group <= 2)
           return a.st.block_table
@@ -1254,10 +1299,15 @@ hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t 
       }
       return a.st.block_table ? launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1)
                               : launch_kind<D, BITS, MODE, 12, false>(a, grid, s, ev0, ev1);
+      }
     }
   }
+  if constexpr (MODE == kWindow) {
+    return launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1);
+  } else {
   return a.st.block_table ? launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1)
                           : launch_kind<D, BITS, MODE, 0, false>(a, grid, s, ev0, ev1);
+  }
 }
 
 template <int D, int BITS>
@@ -1292,7 +1342,8 @@ hipError_t launch_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_t s
       return e;
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
-  e = launch_split<D, BITS, kDense>(a, grid, s, ev0, ev1);
+  e = a.win > 0 ? launch_split<D, BITS, kWindow>(a, grid, s, ev0, ev1)
+                : launch_split<D, BITS, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);
 }

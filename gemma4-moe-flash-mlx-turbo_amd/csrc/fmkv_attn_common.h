@@ -27,7 +27,9 @@ constexpr float kRescaleSlack = 8.0f;
 // from those, visits only the blocks that hold a score at or above it and
 // is the dense pass with every score below theta dropped; the combine
 // divides by the full L of the stats pass.
-constexpr int kDense = 0, kStats = 1, kGated = 2;
+// kWindow: softmax attention of a paged sequence over its last a.win positions
+// and its first a.sinks ones (WinGeom), tau 0.
+constexpr int kDense = 0, kStats = 1, kGated = 2, kWindow = 3;
 
 // A stream's visiting order in the gated pass: the set bits of `mask` in
 // increasing order, then next, next + 1, ... below n (scalar values).

@@ -294,7 +294,7 @@ __device__ void cb_new_token_column(const AttnArgs& a, uint8_t* tab, float2* rop
   }
 }
 
-// MODE: kDense, or the statistics (kStats: keys only, split (m, l) and block
+// MODE: kDense, kWindow (dense over a paged window with sinks), or the statistics (kStats: keys only, split (m, l) and block
 // maxima) and gated (kGated) passes of sparse-V, as the affine kernel runs
 // them.
 template <int D, int BITS, int MODE>
@@ -333,8 +333,15 @@ void cb_decode_kernel(AttnArgs a) {
   const int kvh = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
 
   const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
+  // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
+  // is the sequence's own number
+  WinGeom wg{};
+  if constexpr (MODE == kWindow) wg = win_geometry(T, a.win, a.sinks, a.st.table_stride);
+  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
   const SeqGeom geo =
-      seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
+      MODE == kWindow
+          ? wg.geo
+          : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
   const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
   if constexpr (MODE != kGated) {
     if (a.new_col && split == (int)gridDim.z - 1) {
@@ -368,7 +375,7 @@ void cb_decode_kernel(AttnArgs a) {
   // sparse-V: this (sequence, KV head)'s row of block maxima; the gated pass
   // visits only the blocks holding a score at or above a head's threshold
   const int64_t blk_row =
-      MODE == kDense ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
+      MODE == kDense || MODE == kWindow ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
   BlockList blist{0ull, 0, nb};
   int nbx = nb;  // blocks visited
   if constexpr (MODE == kGated) {
@@ -385,7 +392,7 @@ void cb_decode_kernel(AttnArgs a) {
   // This wave's half of block lb into stage st: its K half, its V half, and
   // with one partial instruction (lanes 0..3) the block's K and V norms.
   auto copy_block = [&](int st, int64_t lb) {
-    const u32x4 rs = buffer_rsrc(blk_ptr(lb), (uint32_t)L.block_bytes);
+    const u32x4 rs = buffer_rsrc(blk_ptr(block_of(lb)), (uint32_t)L.block_bytes);
     const uint32_t sl = pstage_lds + st * SB;
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // reads of this stage are done
 #pragma unroll
@@ -498,8 +505,8 @@ void cb_decode_kernel(AttnArgs a) {
     const float4_t s1 = half == 0 ? other : acc;
     const float kscale[4] = {lo16(kn.x) * inv_sd, hi16(kn.x) * inv_sd, lo16(kn.y) * inv_sd,
                              hi16(kn.y) * inv_sd};
-    const float vscale[4] = {lo16(vn.x) * inv_sd, hi16(vn.x) * inv_sd, lo16(vn.y) * inv_sd,
-                             hi16(vn.y) * inv_sd};
+    float vscale[4] = {lo16(vn.x) * inv_sd, hi16(vn.x) * inv_sd, lo16(vn.y) * inv_sd,
+                       hi16(vn.y) * inv_sd};
     float sc[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -508,15 +515,24 @@ void cb_decode_kernel(AttnArgs a) {
     }
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
-    const bool full = t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim &&
-                      (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
+    const bool full =
+        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+                         : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
+        (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int64_t slot = t0 + 4 * j + i;
-        bool vis = slot >= vis_lo && slot < vis_hi && slot != ex_slot;
-        if (ring_trim) vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
-        if (!vis) sc[i] = -INFINITY;
+        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+                                    : slot >= vis_lo && slot < vis_hi) &&
+                   slot != ex_slot;
+        if (MODE != kWindow && ring_trim)
+          vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
+        if (!vis) {
+          sc[i] = -INFINITY;
+          // (a hidden token's norm may be anything, and 0 * inf is NaN)
+          if constexpr (MODE == kWindow) vscale[i] = 0.0f;
+        }
       }
     }
     if constexpr (MODE == kGated) {
@@ -595,7 +611,7 @@ void cb_decode_kernel(AttnArgs a) {
   for (int i = 0; i < nbx; i++) {
     const int rest = nbx - 1 - i;
     wait_copies<CP, NST - 1>(rest < NST - 1 ? rest : NST - 1);
-    process(pstage + st * SB, pb0 + (int64_t)NS * (MODE == kGated ? blist.pop() : i), i);
+    process(pstage + st * SB, block_of(pb0 + (int64_t)NS * (MODE == kGated ? blist.pop() : i)), i);
     if (i + NST < nbx)
       copy_block(st, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : i + NST));
     st = st + 1 == NST ? 0 : st + 1;
@@ -738,7 +754,9 @@ hipError_t launch_cb_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_
       return e;
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
-  e = launch_cb_mode<D, BITS, kDense>(a, grid, s, ev0, ev1);
+  if (a.win > 0 && !a.st.block_table) return hipErrorInvalidValue;
+  e = a.win > 0 ? launch_cb_mode<D, BITS, kWindow>(a, grid, s, ev0, ev1)
+                : launch_cb_mode<D, BITS, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);
 }

@@ -338,6 +338,36 @@ __host__ __device__ inline SeqGeom seq_geometry(int64_t T, int64_t window, int64
   return g;
 }
 
+// A paged sequence whose query at position T - 1 sees the last `win` positions
+// and the first `sinks` ones: the blocks that hold them, numbered on from 0.
+// Block v of that numbering is block v of the sequence below sink_blks (the
+// sinks' blocks) and block v + skip from there on, so the kernels' splits and
+// streams run over the visible blocks alone and the pages between, which a
+// server may have given back, are never looked up.
+struct WinGeom {
+  SeqGeom geo;        // visible blocks [0, blk_hi)
+  int64_t lo;         // first position of the window
+  int64_t sink_blks;  // blocks below it keep their number
+  int64_t skip;
+  __host__ __device__ int64_t block(int64_t v) const { return v < sink_blks ? v : v + skip; }
+};
+__host__ __device__ inline WinGeom win_geometry(int64_t T, int64_t win, int64_t sinks,
+                                                int64_t table_stride) {
+  WinGeom w;
+  int64_t nb = T > 0 ? (T + kBlockTokens - 1) / kBlockTokens : 0;
+  if (nb > table_stride) nb = table_stride;
+  w.lo = T > win ? T - win : 0;
+  const int64_t sb = (sinks + kBlockTokens - 1) / kBlockTokens;
+  w.sink_blks = sb < nb ? sb : nb;
+  int64_t first = w.lo / kBlockTokens;  // the window's first block, where the sinks do not hold it
+  if (first < w.sink_blks) first = w.sink_blks;
+  if (first > nb) first = nb;
+  w.skip = first - w.sink_blks;
+  w.geo.blk_lo = 0;
+  w.geo.blk_hi = nb - w.skip;
+  return w;
+}
+
 // Split count of a sequence (>= 1, so split 0 always writes a result),
 // never more than the grid provides.
 // Split 0 covers bps0 blocks, every later split bps (bps0 >= bps): a

@@ -124,6 +124,10 @@ struct AttnArgs {
   int32_t* sv_count = nullptr;
   int32_t gather_parts = 0;  // work-groups per (sequence, q head) of the gather
   int32_t gather_rows = 0;   // the most visible head-blocks of a sequence (<= kGatherMaxRows)
+  // A paged window (> 0): a query sees the last `win` positions and the first
+  // `sinks` ones (WinGeom, fmkv_device.h).
+  int64_t win = 0;
+  int64_t sinks = 0;
 };
 
 // Prefill (chunked) attention: n_q queries at positions p0 .. p0 + n_q - 1,
@@ -162,6 +166,9 @@ struct PrefillArgs {
   float* part_ml = nullptr;
   // eight waves a work-group at head_dim 128 and 256 too, sharing its rows
   bool share_rows = false;
+  // A paged pool's window (`window` > 0, ring_slots 0) and the positions at a
+  // sequence's start that every query sees besides.
+  int32_t sinks = 0;
 };
 
 struct ReadArgs {

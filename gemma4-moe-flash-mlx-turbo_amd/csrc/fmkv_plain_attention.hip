@@ -158,7 +158,7 @@ __device__ void plain_new_token_column(const AttnArgs& a, float2* rope, int64_t 
   }
 }
 
-// MODE: kDense, or the statistics (kStats: keys only, split (m, l) and block
+// MODE: kDense, kWindow (dense over a paged window with sinks), or the statistics (kStats: keys only, split (m, l) and block
 // maxima) and gated (kGated) passes of sparse-V, as the affine kernel runs
 // them.
 template <int D, int MODE>
@@ -180,8 +180,15 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   const int kvh = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
 
   const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
+  // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
+  // is the sequence's own number
+  WinGeom wg{};
+  if constexpr (MODE == kWindow) wg = win_geometry(T, a.win, a.sinks, a.st.table_stride);
+  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
   const SeqGeom geo =
-      seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
+      MODE == kWindow
+          ? wg.geo
+          : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
   const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
   if constexpr (MODE != kGated) {
     if (a.new_col && split == (int)gridDim.z - 1) {
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   // sparse-V: this (sequence, KV head)'s row of block maxima; the gated pass
   // visits only the blocks holding a score at or above a head's threshold
   const int64_t blk_row =
-      MODE == kDense ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
+      MODE == kDense || MODE == kWindow ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
   BlockList blist{0ull, 0, nb};
   int nbx = nb;  // blocks visited
   if constexpr (MODE == kGated) {
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   const int k_off = (int)L.k_codes + (c * D + wave * SW * 32 + 8 * j) * 2;         // t = c, jj = j
   const int v_off = (int)L.v_codes + ((wave * TW * 16 + c) * kBlockTokens + 4 * j) * 2;  // n = c, q = j
   auto load_ops = [&](int64_t lb, PlainOps<D>& o) {
-    const uint8_t* p = blk_ptr(lb);
+    const uint8_t* p = blk_ptr(block_of(lb));
 #pragma unroll
     for (int s = 0; s < SW; s++) o.k[s] = *reinterpret_cast<const u32x4*>(p + k_off + s * 64);
     if constexpr (MODE != kStats) {
@@ -265,8 +272,8 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   float m_run = -1e30f, l_run = 0.0f;
 
   for (int i = 0; i < nbx; i++) {
-    const int64_t b = b_begin + (MODE == kGated ? blist.pop() : i);
-    const PlainOps<D> cur = nxt;
+    const int64_t b = block_of(b_begin + (MODE == kGated ? blist.pop() : i));
+    PlainOps<D> cur = nxt;
     if (i + 1 < nbx) load_ops(b_begin + (MODE == kGated ? bcopy.pop() : i + 1), nxt);
 
     // -- this wave's quarter of S^T, summed over the waves in wave order --
@@ -287,15 +294,27 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
     for (int r = 0; r < 4; r++) s4[r] = head < G ? st[r] * a.qscale : -INFINITY;
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
-    const bool full = t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim &&
-                      (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
+    const bool full =
+        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+                         : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
+        (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
+      uint32_t seen[2] = {0u, 0u};  // kWindow: the lane's visible tokens as masks of bf16 pairs
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int64_t slot = t0 + 4 * j + r;
-        bool vis = slot >= vis_lo && slot < vis_hi && slot != ex_slot;
-        if (ring_trim) vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
+        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+                                    : slot >= vis_lo && slot < vis_hi) &&
+                   slot != ex_slot;
+        if (MODE != kWindow && ring_trim)
+          vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if (!vis) s4[r] = -INFINITY;
+        seen[r >> 1] |= vis ? 0xffffu << 16 * (r & 1) : 0u;
+      }
+      // a hidden token's weight is 0, but its V row may be anything, and 0 * inf is NaN
+      if constexpr (MODE == kWindow) {
+#pragma unroll
+        for (int t = 0; t < TW; t++) cur.v[t].x &= seen[0], cur.v[t].y &= seen[1];
       }
     }
     if constexpr (MODE == kGated) {
@@ -446,7 +465,9 @@ hipError_t launch_plain_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStre
       return e;
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
-  e = launch_plain_mode<D, kDense>(a, grid, s, ev0, ev1);
+  if (a.win > 0 && !a.st.block_table) return hipErrorInvalidValue;
+  e = a.win > 0 ? launch_plain_mode<D, kWindow>(a, grid, s, ev0, ev1)
+                : launch_plain_mode<D, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);
 }

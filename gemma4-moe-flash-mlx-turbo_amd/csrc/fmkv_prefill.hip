@@ -239,7 +239,7 @@ __device__ inline void lds_barrier() {
 __device__ inline int prefill_steps(const PrefillArgs& a, int64_t p0) {
   const int64_t lo = a.vis_begin > 0 ? a.vis_begin : 0;
   int64_t keys = p0 + a.n_q - lo;
-  if (a.window > 0 && keys > a.window + kPfRows) keys = a.window + kPfRows;
+  if (a.window > 0 && keys > a.window + kPfRows + a.sinks) keys = a.window + kPfRows + a.sinks;
   if (keys > ((int64_t)1 << 25)) keys = (int64_t)1 << 25;  // (64 sequences' steps add up in 32 bits)
   return (int)((keys > 0 ? keys : 0) / kPfKeys) + 2;
 }
@@ -305,7 +305,11 @@ __device__ inline PrefillUnit prefill_unit(const PrefillArgs& a, int u, int seq,
   return r;
 }
 
-template <int D, int BITS, int MODE, int RW>
+// WIN: a paged pool's window with sinks (a.window, a.sinks): position p sees j
+// <= p with j > p - window or j < sinks. The sinks' blocks take the place of
+// the old store's, in the pool itself, and the blocks between them and the
+// window, whose pages a server may have given back, are never looked up.
+template <int D, int BITS, int MODE, int RW, bool WIN>
 __global__ __launch_bounds__(D * RW)  // RW waves per 64 dims
 __attribute__((amdgpu_waves_per_eu(RW == 4 ? 4 : 2, RW == 4 ? 4 : 2)))
 void prefill_attn_kernel(PrefillArgs a) {
@@ -358,10 +362,11 @@ void prefill_attn_kernel(PrefillArgs a) {
   const int64_t wg_lo = lo_of(pA), wg_hi = pB;
   const int64_t b_lo = wg_lo / kBlockTokens, b_hi = wg_hi / kBlockTokens;
   const int64_t ps = a.p_split;
-  int64_t old_last = (ps + kBlockTokens - 1) / kBlockTokens - 1;  // last block with keys < ps
+  // (WIN: last block with keys < sinks; virtual block i < n_old is block i)
+  int64_t old_last = ((WIN ? a.sinks : ps) + kBlockTokens - 1) / kBlockTokens - 1;  // last block with keys < ps
   if (old_last > b_hi) old_last = b_hi;
-  const int64_t n_old = old_last >= b_lo ? old_last - b_lo + 1 : 0;
-  int64_t new_first = ps / kBlockTokens;
+  const int64_t n_old = WIN ? old_last + 1 : old_last >= b_lo ? old_last - b_lo + 1 : 0;
+  int64_t new_first = WIN ? n_old : ps / kBlockTokens;
   if (new_first < b_lo) new_first = b_lo;
   const int64_t n_new = b_hi >= new_first ? b_hi - new_first + 1 : 0;
   const int nvb = (int)(n_old + n_new);
@@ -401,7 +406,14 @@ void prefill_attn_kernel(PrefillArgs a) {
       (cint_ptr)(uintptr_t)(a.new_st.block_table + (int64_t)seq * a.new_st.table_stride);
   auto blk_ptr = [&](int i) __attribute__((always_inline)) -> gptr_t {
     i = i < nvb ? i : nvb > 0 ? nvb - 1 : 0;
-    if (i < n_old_i) {
+    if (WIN && i < n_old_i) {
+      // (a lookup and an address of its own: one for both sides, of a selected
+      // block, made the whole loop spill 85 registers)
+      const int32_t e = (uint32_t)i < t_width ? table[i] : 0;
+      const uint32_t phys = (uint32_t)(e < 0 ? 0 : (e >= n_pool ? n_pool - 1 : e));
+      return (gptr_t)(base_old + (uint64_t)phys * (uint64_t)a.old_st.block_stride);
+    }
+    if (!WIN && i < n_old_i) {
       uint32_t phys = (uint32_t)(b_lo_i + i);
       if (nrb > 0) {
         int r = ring0 + i;
@@ -424,7 +436,17 @@ void prefill_attn_kernel(PrefillArgs a) {
   // every key of virtual block i is visible to every row: at or past the
   // largest lower bound, at or before the first position, not cut by p_split
   const int lo_max = lo_rel(pA_r + nq - 1);
+  // WIN: virtual block i's first key, and the end of the sinks, relative too
+  // (past the last virtual block: keys past every row's position)
+  const int sink_r = (int)(a.sinks - bl16);
+  auto first_key = [&](int i) __attribute__((always_inline)) -> int {
+    return (i < n_old_i ? i - b_lo_i : i + vb_shift) * kBlockTokens;
+  };
   auto blk_full = [&](int i) __attribute__((always_inline)) -> bool {
+    if constexpr (WIN) {
+      const int k0 = first_key(i);
+      return (k0 >= lo_max || k0 + kBlockTokens <= sink_r) && k0 + kBlockTokens - 1 <= pA_r;
+    }
     int vlo, vhi;
     vb_range(i, vlo, vhi);
     return vhi - vlo == kBlockTokens && vlo >= lo_max && vhi - 1 <= pA_r;
@@ -820,7 +842,19 @@ void prefill_attn_kernel(PrefillArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; i++) s[t][i] = s[t][i] * a.qscale;
       }
-      if (!full) {
+      if (WIN && !full) {
+        const int p = p_row[u], lo = p - win + 1;
+#pragma unroll
+        for (int t = 0; t < NQ; t++) {
+          const int kp = first_key(2 * step + (kOwn ? t : quad0 >> 2)) + 4 * (quad0 & 3);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (kp + i > p || (kp + i < lo && kp + i >= sink_r)) {
+              s[t][i] = -INFINITY;
+              if constexpr (MODE == kCodebook) vscale[t][i] = 0.0f;
+            }
+        }
+      } else if (!full) {
         const int p = p_row[u], lo = lo_rel(p);
 #pragma unroll
         for (int t = 0; t < NQ; t++) {
@@ -1022,6 +1056,10 @@ void prefill_attn_kernel(PrefillArgs a) {
     // 1 for the keys 4 j + i of block kt that row 16 (rt0 + rt) + c sees, else 0
     auto seen_of = [&](int rt, int kt, int i) __attribute__((always_inline)) -> uint32_t {
       const int p = pos_at((rt0 + rt) * 16 + c), lo = lo_rel(p), vi = 2 * step + kt;
+      if constexpr (WIN) {
+        const int k = first_key(vi) + 4 * j + i;
+        return k > p || (k < p - win + 1 && k >= sink_r) ? 0u : 1u;
+      }
       int vlo, vhi;
       vb_range(vi, vlo, vhi);
       vlo = vlo > lo ? vlo : lo;
@@ -1286,12 +1324,12 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int t
   }
 }
 
-template <int D, int BITS, int MODE, int RW>
+template <int D, int BITS, int MODE, int RW, bool WIN>
 hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   const int qp = kPfRows / a.group;
   const int tiles = (a.n_q + qp - 1) / qp, H = a.new_st.n_kv_heads;
   dim3 grid(tiles, H, a.units > 0 ? a.units : a.n_seqs);
-  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW>), grid, dim3(D * RW), 0, s, a);
+  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, WIN>), grid, dim3(D * RW), 0, s, a);
   if (a.units > 0) {
     dim3 mgrid(tiles * (kPfRows / kPfMergeRows), H, a.n_seqs);
     hipLaunchKernelGGL((prefill_merge_kernel<D, MODE != kPlain>), mgrid, dim3(256), 0, s, a, tiles);
@@ -1300,9 +1338,13 @@ hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
 }
 template <int D, int BITS, int MODE>
 hipError_t launch_t(const PrefillArgs& a, hipStream_t s) {
+  // (a window without a ring is a paged pool's)
+  const bool win = a.window > 0 && a.ring_slots == 0;
+  if (win && !a.new_st.block_table) return hipErrorInvalidValue;
   if constexpr (D < 512)
-    if (a.share_rows) return launch_rw<D, BITS, MODE, 512 / D>(a, s);
-  return launch_rw<D, BITS, MODE, 1>(a, s);
+    if (a.share_rows)
+      return win ? launch_rw<D, BITS, MODE, 512 / D, true>(a, s) : launch_rw<D, BITS, MODE, 512 / D, false>(a, s);
+  return win ? launch_rw<D, BITS, MODE, 1, true>(a, s) : launch_rw<D, BITS, MODE, 1, false>(a, s);
 }
 
 }  // namespace

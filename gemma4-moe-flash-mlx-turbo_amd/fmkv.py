@@ -53,6 +53,8 @@ EXPORTED = (
     "fmkv_prefill_step", "fmkv_paged_prefill_step", "fmkv_paged_prefill_step_bounded",
     "fmkv_decode_step_noalloc",
     "fmkv_decode_step_projected", "fmkv_paged_decode_step_projected",
+    "fmkv_paged_window_decode_attention", "fmkv_paged_window_decode_step",
+    "fmkv_paged_window_prefill_attention", "fmkv_paged_window_prefill_step", "fmkv_pool_storage",
 )
 
 
@@ -168,6 +170,16 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         "fmkv_paged_decode_step_projected": ([vp, vp, vp, vp, i32, vp, vp, i32, i32, i32,
                                               P(KvPrologue), vp, i32, ctypes.c_float,
                                               ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_window_decode_attention": ([vp, vp, vp, i32, vp, i32, i32, i32, ctypes.c_float,
+                                                i32, i32, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_window_decode_step": ([vp, vp, vp, vp, i32, vp, vp, i32, i32, vp, i32,
+                                           ctypes.c_float, i32, i32, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_window_prefill_attention": ([vp, vp, vp, i32, vp, i32, i32, i32, i32,
+                                                 ctypes.c_float, i32, i32, vp, i32, vp],
+                                                ctypes.c_int),
+        "fmkv_paged_window_prefill_step": ([vp, vp, vp, vp, i32, vp, i32, i32, i32, vp, i32,
+                                            ctypes.c_float, i32, i32, vp, i32, vp], ctypes.c_int),
+        "fmkv_pool_storage": ([vp, P(vp), P(i64)], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -606,9 +618,121 @@ class PagedPool:
             _dtype_code(out.dtype), _stream(stream)))
         return out
 
+    def window_attention(self, q, block_tables, seq_lens, max_seq_len: int, window: int,
+                         sinks: int = 0, scale: float = 1.0, out=None, dtype=torch.bfloat16,
+                         stream=None):
+        """attention() of each sequence's newest token over its last `window`
+        positions and its first `sinks` ones. q bf16 [n_seqs, n_q_heads, D];
+        seq_lens int32 [n_seqs]. Pages that hold neither are not looked up."""
+        d = self.desc
+        n = q.shape[0]
+        _check_tensor("q", q, torch.bfloat16, (n, None, d.head_dim))
+        self._check_tables(block_tables, n, seq_lens=seq_lens)
+        out = _out(out, q, dtype)
+        _check(self._lib.fmkv_paged_window_decode_attention(
+            self._h, _ptr(q), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), n,
+            max_seq_len, q.shape[1], scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
+            _stream(stream)))
+        return out
+
+    def window_decode_step(self, keys, values, block_tables, start_pos, seq_lens, max_seq_len: int,
+                           q, window: int, sinks: int = 0, scale: float = 1.0, out=None,
+                           dtype=torch.bfloat16, stream=None):
+        """append(keys, values, ...) of one token per sequence at start_pos
+        (= seq_lens - 1), then window_attention, in one call. keys/values bf16
+        [n_seqs, 1, n_kv_heads, D]."""
+        d = self.desc
+        n = q.shape[0]
+        _check_tensor("q", q, torch.bfloat16, (n, None, d.head_dim))
+        for name, t in (("keys", keys), ("values", values)):
+            _check_tensor(name, t, torch.bfloat16, (n, 1, d.n_kv_heads, d.head_dim))
+        self._check_tables(block_tables, n, seq_lens=seq_lens, start_pos=start_pos)
+        out = _out(out, q, dtype)
+        _check(self._lib.fmkv_paged_window_decode_step(
+            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), block_tables.shape[1],
+            _ptr(start_pos), _ptr(seq_lens), n, max_seq_len, _ptr(q), q.shape[1], scale, window,
+            sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+        return out
+
+    def window_prefill(self, q, block_tables, start_pos, window: int, sinks: int = 0,
+                       scale: float = 1.0, max_seq_len: int = 0, out=None, dtype=torch.bfloat16,
+                       stream=None):
+        """Attention of q bf16 [n_seqs, n_new, n_q_heads, D] at positions
+        start_pos .. start_pos + n_new - 1, whose keys and values were appended
+        before, over the window and the sinks of each. max_seq_len: see
+        prefill_step."""
+        d = self.desc
+        n, n_new = q.shape[:2]
+        _check_tensor("q", q, torch.bfloat16, (n, n_new, None, d.head_dim))
+        self._check_tables(block_tables, n, start_pos=start_pos)
+        out = _out(out, q, dtype)
+        _check(self._lib.fmkv_paged_window_prefill_attention(
+            self._h, _ptr(q), _ptr(block_tables), block_tables.shape[1], _ptr(start_pos), n, n_new,
+            max_seq_len, q.shape[2], scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
+            _stream(stream)))
+        return out
+
+    def window_prefill_step(self, keys, values, block_tables, start_pos, q, window: int,
+                            sinks: int = 0, scale: float = 1.0, max_seq_len: int = 0, out=None,
+                            dtype=torch.bfloat16, stream=None):
+        """append(keys, values, ...) at start_pos, then window_prefill(q, ...).
+        keys/values bf16 [n_seqs, n_new, n_kv_heads, D]."""
+        d = self.desc
+        n, n_new = q.shape[:2]
+        _check_tensor("q", q, torch.bfloat16, (n, n_new, None, d.head_dim))
+        for name, t in (("keys", keys), ("values", values)):
+            _check_tensor(name, t, torch.bfloat16, (n, n_new, d.n_kv_heads, d.head_dim))
+        self._check_tables(block_tables, n, start_pos=start_pos)
+        out = _out(out, q, dtype)
+        _check(self._lib.fmkv_paged_window_prefill_step(
+            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), block_tables.shape[1],
+            _ptr(start_pos), n, n_new, max_seq_len, _ptr(q), q.shape[2], scale, window, sinks,
+            _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+        return out
+
+    def storage(self) -> torch.Tensor:
+        """The pool's blocks as a uint8 tensor [n_blocks, n_kv_heads, bytes of a
+        head-block] over the pool's own memory (which it keeps alive): to move
+        blocks to other pools of the same description or to the host and back."""
+        base, size = ctypes.c_void_p(), ctypes.c_int64()
+        _check(self._lib.fmkv_pool_storage(self._h, ctypes.byref(base), ctypes.byref(size)))
+        return torch.as_tensor(_Storage(self, base.value, (
+            self.n_blocks, self.desc.n_kv_heads, size.value // self.desc.n_kv_heads)), device="cuda")
+
+    def _check_tables(self, block_tables, n_seqs: int, **per_seq) -> None:
+        _check_tensor("block_tables", block_tables, torch.int32, (n_seqs, None))
+        for name, t in per_seq.items():
+            _check_tensor(name, t, torch.int32, (n_seqs,))
+
     def read_codes(self, stream=None):
         return _read_codes(self._lib.fmkv_pool_read_codes, self._h, self.desc,
                            self.n_blocks * BLOCK_TOKENS, stream)
+
+
+class _Storage:
+    """A pool's memory for torch (the tensor holds this object, and it the pool)."""
+
+    def __init__(self, owner, ptr: int, shape):
+        self.owner = owner
+        self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape),
+                                         "typestr": "|u1", "strides": None, "version": 2}
+
+
+def _check_tensor(name: str, t: torch.Tensor, dtype, shape) -> None:
+    """Type, shape (None: any extent) of an argument that the library takes as
+    a bare pointer."""
+    if t.dtype != dtype or t.dim() != len(shape) or any(
+            want is not None and have != want for have, want in zip(t.shape, shape)):
+        want = ", ".join("*" if x is None else str(x) for x in shape)
+        raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {tuple(t.shape)}")
+
+
+def _out(out, like: torch.Tensor, dtype) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=dtype, device=like.device)
+    if out.shape != like.shape:
+        raise ValueError(f"out must have the shape {tuple(like.shape)}, got {tuple(out.shape)}")
+    return out
 
 
 def _dtype_code(dtype) -> int:

@@ -335,6 +335,66 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
                                     int32_t max_seq_len, const void* q_bf16, int32_t n_q_heads,
                                     float scale, void* out, int32_t out_dtype, void* stream);
 
+/* Attention over a window with sinks: position p sees the positions j <= p
+ * with j > p - window (the sliding layers' band, create_sliding_mask,
+ * src/model/mod.rs:707-753) or j < sinks (the first positions of a sequence,
+ * which a model that was trained without a window leans on). 1 <= window <=
+ * 2^30, 0 <= sinks <= 2^30. Every cache mode and head layout of the calls
+ * above, whose other arguments, plans and errors these share. A position that
+ * no query of a call sees is never read, nor its block's table entry: the
+ * pages between the sinks and the window of the earliest query can be given
+ * to other sequences (entries -1, say). What hidden slots of a block hold,
+ * infinities and NaN included, does not reach an output. A sequence of length
+ * 0 gets zeros. The current GPU has to be the pool's. Calls on one pool share
+ * its workspace, so calls on several streams, and replays of graphs that
+ * captured them, have to be ordered by the caller; a workspace that a later,
+ * larger call outgrows stays until the pool is destroyed, so captured calls
+ * stay valid. */
+
+/* One token per sequence: fmkv_paged_decode_attention over a window. */
+int fmkv_paged_window_decode_attention(fmkv_pool* pool, const void* q_bf16,
+                                       const int32_t* block_tables, int32_t max_blocks,
+                                       const int32_t* seq_lens, int32_t n_seqs,
+                                       int32_t max_seq_len, int32_t n_q_heads, float scale,
+                                       int32_t window, int32_t sinks, void* out,
+                                       int32_t out_dtype, void* stream);
+
+/* fmkv_paged_decode_step of one new token per sequence (at seq_lens - 1 =
+ * start_pos) over a window; the attention launch appends the tokens. */
+int fmkv_paged_window_decode_step(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
+                                  const int32_t* block_tables, int32_t max_blocks,
+                                  const int32_t* start_pos, const int32_t* seq_lens,
+                                  int32_t n_seqs, int32_t max_seq_len, const void* q_bf16,
+                                  int32_t n_q_heads, float scale, int32_t window, int32_t sinks,
+                                  void* out, int32_t out_dtype, void* stream);
+
+/* n_new consecutive queries per sequence at start_pos .. start_pos + n_new - 1,
+ * whose keys and values are in the pool already (fmkv_paged_append or
+ * fmkv_paged_append_projected came first). max_seq_len: as
+ * fmkv_paged_prefill_step_bounded takes it. */
+int fmkv_paged_window_prefill_attention(fmkv_pool* pool, const void* q_bf16,
+                                        const int32_t* block_tables, int32_t max_blocks,
+                                        const int32_t* start_pos, int32_t n_seqs, int32_t n_new,
+                                        int32_t max_seq_len, int32_t n_q_heads, float scale,
+                                        int32_t window, int32_t sinks, void* out,
+                                        int32_t out_dtype, void* stream);
+
+/* fmkv_paged_append of n_new tokens per sequence, then their
+ * fmkv_paged_window_prefill_attention. */
+int fmkv_paged_window_prefill_step(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
+                                   const int32_t* block_tables, int32_t max_blocks,
+                                   const int32_t* start_pos, int32_t n_seqs, int32_t n_new,
+                                   int32_t max_seq_len, const void* q_bf16, int32_t n_q_heads,
+                                   float scale, int32_t window, int32_t sinks, void* out,
+                                   int32_t out_dtype, void* stream);
+
+/* The pool's storage: n_blocks blocks of *block_bytes (all KV heads), on the
+ * pool's GPU, as fmkv_pool_create laid it out (zeros, until tokens are
+ * appended). A block is moved by copying its bytes, to the same place of
+ * another pool of the same description or to host memory and back; nothing else
+ * about them is promised. */
+int fmkv_pool_storage(const fmkv_pool* pool, void** base, int64_t* block_bytes);
+
 /* Canonical codes of every pool block, indexed by (physical block * 16 + t). */
 int fmkv_pool_read_codes(const fmkv_pool* pool, void* codes, void* meta, void* stream);
 

@@ -1,0 +1,72 @@
+"""Refusals of the windowed calls, before any HIP call (no GPU needed)."""
+import ctypes
+
+import pytest
+
+import fmkv
+
+
+def test_null_pool_is_refused():
+    lib = fmkv.load_library()
+    calls = [
+        lib.fmkv_paged_window_decode_attention(None, 1, 1, 4, 1, 1, 64, 8, 1.0, 16, 0, 1, 0, None),
+        lib.fmkv_paged_window_decode_step(None, 1, 1, 1, 4, 1, 1, 1, 64, 1, 8, 1.0, 16, 0, 1, 0, None),
+        lib.fmkv_paged_window_prefill_attention(None, 1, 1, 4, 1, 1, 4, 0, 8, 1.0, 16, 0, 1, 0, None),
+        lib.fmkv_paged_window_prefill_step(None, 1, 1, 1, 4, 1, 1, 4, 0, 1, 8, 1.0, 16, 0, 1, 0, None),
+        lib.fmkv_pool_storage(None, ctypes.byref(ctypes.c_void_p()), ctypes.byref(ctypes.c_int64())),
+    ]
+    assert calls == [fmkv.FMKV_ERR_INVALID_ARG] * len(calls)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change,code", [
+    (dict(window=0), fmkv.FMKV_ERR_INVALID_ARG), (dict(window=-1), fmkv.FMKV_ERR_INVALID_ARG),
+    (dict(window=(1 << 30) + 1), fmkv.FMKV_ERR_INVALID_ARG), (dict(sinks=-1), fmkv.FMKV_ERR_INVALID_ARG),
+    (dict(sinks=(1 << 30) + 1), fmkv.FMKV_ERR_INVALID_ARG), (dict(scale=float("inf")), fmkv.FMKV_ERR_INVALID_ARG),
+    (dict(scale=float("nan")), fmkv.FMKV_ERR_INVALID_ARG), (dict(Hq=18), fmkv.FMKV_ERR_UNSUPPORTED),
+    (dict(Hq=3), fmkv.FMKV_ERR_INVALID_ARG), (dict(max_seq_len=65), fmkv.FMKV_ERR_INVALID_ARG),
+])
+def test_bad_arguments_are_refused(gpu, change, code):
+    import torch
+
+    a = dict(window=16, sinks=4, scale=1.0, Hq=4, max_seq_len=64, **{})
+    a.update(change)
+    pool = gpu.PagedPool(gpu.make_desc(2, 128, 4), 4)
+    q = torch.zeros((1, a["Hq"], 128), dtype=torch.bfloat16, device="cuda")
+    kv = torch.zeros((1, 1, 2, 128), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((1, 4), dtype=torch.int32, device="cuda")
+    n = torch.ones(1, dtype=torch.int32, device="cuda")
+    before = pool.storage().clone()
+    out = torch.full_like(q, 7.0)
+    kw = dict(window=a["window"], sinks=a["sinks"], scale=a["scale"], out=out)
+    with pytest.raises(fmkv.Exception_) as e:
+        pool.window_attention(q, table, n, a["max_seq_len"], **kw)
+    assert e.value.code == code
+    with pytest.raises(fmkv.Exception_) as e:
+        pool.window_decode_step(kv, kv, table, n - 1, n, a["max_seq_len"], q, **kw)
+    assert e.value.code == code
+    if "max_seq_len" not in change:
+        kw["out"] = out[:, None]
+        for call in (lambda: pool.window_prefill(q[:, None], table, n - 1, **kw),
+                     lambda: pool.window_prefill_step(kv, kv, table, n - 1, q[:, None], **kw)):
+            with pytest.raises(fmkv.Exception_) as e:
+                call()
+            assert e.value.code == code
+    torch.cuda.synchronize()
+    assert torch.equal(pool.storage(), before) and bool((out == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_wrong_tensors_are_refused(gpu):
+    import torch
+
+    pool = gpu.PagedPool(gpu.make_desc(2, 128, 4), 4)
+    q = torch.zeros((1, 4, 128), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((1, 4), dtype=torch.int32, device="cuda")
+    n = torch.ones(1, dtype=torch.int32, device="cuda")
+    for bad in ((q.float(), table, n), (q[..., :64].contiguous(), table, n), (q, table.long(), n),
+                (q, table.repeat(2, 1), n), (q, table, n.repeat(2)), (q, table, n.long()), (q.cpu(), table, n)):
+        with pytest.raises(ValueError):
+            pool.window_attention(*bad, 64, 16)
+    with pytest.raises(ValueError):
+        pool.window_attention(q, table, n, 64, 16, out=torch.zeros((1, 4, 64), device="cuda"))
