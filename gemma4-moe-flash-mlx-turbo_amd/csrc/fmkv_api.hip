@@ -12,8 +12,10 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/fmkv.h"
@@ -1457,6 +1459,172 @@ int fmkv_paged_decode_step_projected(fmkv_pool* p, const void* k_proj, const voi
                                 out_dtype, stream, pro);
 }
 
+int fmkv_pools_copy_blocks(fmkv_pool* const* pools, int32_t n_pools, const int32_t* src,
+                           const int32_t* dst, int64_t n_pairs, void* stream) {
+  if (n_pools < 0 || n_pairs < 0) return fail(FMKV_ERR_INVALID_ARG, "n_pools and n_pairs must be >= 0");
+  if (n_pools == 0 || n_pairs == 0) return FMKV_OK;
+  if (!pools || !src || !dst) return fail(FMKV_ERR_INVALID_ARG, "pools/src/dst are null");
+  for (int32_t i = 0; i < n_pools; i++)
+    if (!pools[i]) return fail(FMKV_ERR_INVALID_ARG, "pool " + std::to_string(i) + " is null");
+  for (int32_t i = 0; i < n_pools; i++) {
+    const int rc = check_device(pools[i]);
+    if (rc) return rc;
+  }
+  for (int32_t i0 = 0; i0 < n_pools; i0 += fmkv::kCopyPools) {
+    fmkv::CopyArgs a;
+    const int n = std::min<int32_t>(n_pools - i0, fmkv::kCopyPools);
+    for (int i = 0; i < n; i++) {
+      const fmkv_pool* p = pools[i0 + i];
+      a.base[i] = p->arena;
+      a.block_bytes[i] = p->layout.block_bytes * p->desc.n_kv_heads;
+      a.n_blocks[i] = (int32_t)p->n_blocks;
+    }
+    a.src = src;
+    a.dst = dst;
+    const hipError_t e = fmkv::launch_copy_blocks(a, n, n_pairs, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "block copy launch");
+  }
+  return FMKV_OK;
+}
+
+int fmkv_paged_compact(fmkv_pool* p, const int32_t* block_tables, int32_t max_blocks,
+                       const int32_t* keep, int32_t max_keep, const int32_t* n_keep,
+                       const int32_t* dst_tables, int32_t dst_max_blocks, int32_t n_seqs,
+                       void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  if (n_seqs < 0 || max_keep < 0 || max_blocks < 1 || dst_max_blocks < 1)
+    return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / max_keep / max_blocks / dst_max_blocks");
+  if (n_seqs > 65535) return fail(FMKV_ERR_INVALID_ARG, "at most 65535 sequences per call");
+  if (n_seqs == 0 || max_keep == 0) return FMKV_OK;
+  if (!block_tables || !keep || !n_keep || !dst_tables)
+    return fail(FMKV_ERR_INVALID_ARG, "block_tables/keep/n_keep/dst_tables are null");
+  if (max_keep > (int64_t)dst_max_blocks * fmkv::kBlockTokens)
+    return fail(FMKV_ERR_INVALID_ARG, "max_keep exceeds dst_max_blocks * 16");
+  const int rc = check_device(p);
+  if (rc) return rc;
+  fmkv::CompactArgs a;
+  a.st = pool_store(p, block_tables, max_blocks);
+  a.dst_table = dst_tables;
+  a.dst_stride = dst_max_blocks;
+  a.keep = keep;
+  a.max_keep = max_keep;
+  a.n_keep = n_keep;
+  const hipError_t e = fmkv::launch_compact(a, n_seqs, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "compact launch");
+  return FMKV_OK;
+}
+
+int fmkv_qkv_norm_rope(const fmkv_qkv_prologue* pro, int32_t head_dim, int32_t n_q_heads,
+                       int32_t n_kv_heads, int64_t n_tokens, const void* q, int64_t q_stride,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       const int32_t* positions, void* q_out, void* k_out, void* v_out,
+                       void* stream) {
+  if (!pro) return fail(FMKV_ERR_INVALID_ARG, "prologue is null");
+  if (head_dim != 128 && head_dim != 256 && head_dim != 512)
+    return fail(FMKV_ERR_UNSUPPORTED, "head_dim must be 128, 256 or 512");
+  if (n_q_heads < 0 || n_kv_heads < 0 || n_q_heads > 65535 || n_kv_heads > 65535 ||
+      n_q_heads + n_kv_heads == 0)
+    return fail(FMKV_ERR_INVALID_ARG, "n_q_heads and n_kv_heads must be in [0, 65535], one of them > 0");
+  if (n_tokens < 0 || n_tokens > INT32_MAX) return fail(FMKV_ERR_INVALID_ARG, "n_tokens must be in [0, 2^31)");
+  if (!(pro->eps > 0.0f) || !std::isfinite(pro->eps))
+    return fail(FMKV_ERR_INVALID_ARG, "eps must be finite and > 0");
+  if (!(pro->rope_theta >= 1.0f) || !std::isfinite(pro->rope_theta))
+    return fail(FMKV_ERR_INVALID_ARG, "rope_theta must be finite and >= 1");
+  if (pro->rope_dims < 0 || pro->rope_dims > head_dim || pro->rope_dims % 8 != 0)
+    return fail(FMKV_ERR_UNSUPPORTED, "rope_dims must be a multiple of 8 in [0, head_dim]");
+  if (pro->n_axes < 1 || pro->n_axes > 4) return fail(FMKV_ERR_INVALID_ARG, "n_axes must be 1 to 4");
+  if ((pro->v_norm != 0 && pro->v_norm != 1) || (pro->v_from_k != 0 && pro->v_from_k != 1))
+    return fail(FMKV_ERR_INVALID_ARG, "v_norm and v_from_k must be 0 or 1");
+  fmkv::NormRopeArgs a;
+  int64_t pairs = 0;
+  for (int i = 0; i < 4; i++) {
+    if (i < pro->n_axes && pro->n_axes > 1) {
+      if (pro->sections[i] < 0) return fail(FMKV_ERR_INVALID_ARG, "sections must be >= 0");
+      pairs += pro->sections[i];
+    }
+    // (pairs from the last axis's end on do not exist)
+    a.axis_end[i] = i < pro->n_axes - 1 ? (int32_t)std::min<int64_t>(pairs, INT32_MAX) : INT32_MAX;
+  }
+  if (pro->n_axes > 1 && 2 * pairs != pro->rope_dims)
+    return fail(FMKV_ERR_INVALID_ARG, "sections must add up to rope_dims / 2");
+  const bool has_v = v != nullptr;
+  if (pro->v_from_k && (has_v || n_kv_heads == 0))
+    return fail(FMKV_ERR_INVALID_ARG, "v_from_k takes V from k: k rows and no v");
+  const bool out_v = has_v || pro->v_from_k;
+  // arguments of the rows that are there
+  struct Rows {
+    const char* name;
+    bool there;
+    const void* in;
+    void* out;
+    int64_t heads, stride;
+    bool reads;
+  } rows[3] = {{"q", n_q_heads > 0, q, q_out, n_q_heads, q_stride, true},
+               {"k", n_kv_heads > 0, k, k_out, n_kv_heads, k_stride, true},
+               {"v", n_kv_heads > 0 && out_v, v, v_out, n_kv_heads, v_stride, has_v}};
+  for (const Rows& r : rows) {
+    if (!r.there) {
+      if (r.in) return fail(FMKV_ERR_INVALID_ARG, std::string(r.name) + " without heads");
+      continue;
+    }
+    if ((r.reads && !r.in) || !r.out)
+      return fail(FMKV_ERR_INVALID_ARG, std::string(r.name) + " and its output must be device pointers");
+    if (r.reads && r.stride < r.heads * head_dim)
+      return fail(FMKV_ERR_INVALID_ARG, std::string(r.name) + "_stride must be >= heads * head_dim");
+    if (r.reads && r.stride > ((int64_t)1 << 31))
+      return fail(FMKV_ERR_INVALID_ARG, std::string(r.name) + "_stride must be <= 2^31");
+  }
+  if ((n_q_heads > 0 && !pro->q_norm_weight) || (n_kv_heads > 0 && !pro->k_norm_weight))
+    return fail(FMKV_ERR_INVALID_ARG, "norm weights must be device pointers");
+  if (pro->rope_dims > 0 && !positions) return fail(FMKV_ERR_INVALID_ARG, "positions is null");
+  if (n_tokens == 0) return FMKV_OK;
+  // an output over an input or another output: rows would be read after they
+  // were written (its own input, row for row, is read first)
+  auto span = [&](const void* p, int64_t bytes) {
+    return std::pair<uintptr_t, uintptr_t>((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
+  };
+  for (int i = 0; i < 3; i++) {
+    if (!rows[i].there) continue;
+    const auto o = span(rows[i].out, n_tokens * rows[i].heads * head_dim * 2);
+    for (int j = 0; j < 3; j++) {
+      if (!rows[j].there) continue;
+      const auto in = span(rows[j].in, ((n_tokens - 1) * rows[j].stride + rows[j].heads * head_dim) * 2);
+      const bool same = i == j && rows[i].in == rows[i].out && rows[i].stride == rows[i].heads * head_dim;
+      if (rows[j].reads && !same && o.first < in.second && in.first < o.second)
+        return fail(FMKV_ERR_INVALID_ARG, std::string(rows[i].name) + "'s output overlaps " + rows[j].name);
+      const auto p = span(rows[j].out, n_tokens * rows[j].heads * head_dim * 2);
+      if (j > i && o.first < p.second && p.first < o.second)
+        return fail(FMKV_ERR_INVALID_ARG, std::string("the outputs of ") + rows[i].name + " and " +
+                                              rows[j].name + " overlap");
+    }
+  }
+  a.q = static_cast<const uint16_t*>(q);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.k_out = static_cast<uint16_t*>(k_out);
+  a.v_out = static_cast<uint16_t*>(v_out);
+  a.q_w = static_cast<const uint16_t*>(pro->q_norm_weight);
+  a.k_w = static_cast<const uint16_t*>(pro->k_norm_weight);
+  a.pos = positions;
+  a.n_tokens = n_tokens;
+  a.n_q = n_q_heads;
+  a.n_k = n_kv_heads;
+  a.n_v = has_v ? n_kv_heads : 0;
+  a.v_norm = pro->v_norm;
+  a.v_from_k = pro->v_from_k;
+  a.eps = pro->eps;
+  a.rope_dims = pro->rope_dims;
+  a.log2_theta = std::log2((double)pro->rope_theta);
+  const hipError_t e =
+      fmkv::launch_norm_rope(a, head_dim, device_cus(), static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "norm and rotation launch");
+  return FMKV_OK;
+}
+
 int fmkv_pool_storage(const fmkv_pool* p, void** base, int64_t* block_bytes) {
   if (!p || !base || !block_bytes) return fail(FMKV_ERR_INVALID_ARG, "null argument");
   *base = p->arena;
@@ -1535,6 +1703,155 @@ int fmkv_profile_collect_each(float* ms_out, int32_t capacity, int32_t* n_record
   }
   *n_records = g_prof.used;
   g_prof.used = 0;
+  return FMKV_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The book of a pool's blocks (host only)
+// ---------------------------------------------------------------------------
+
+struct fmkv_pages {
+  std::vector<int32_t> users;  // of each block
+  std::vector<int32_t> free;   // blocks without users, the next one last
+};
+
+namespace {
+
+int check_block(const fmkv_pages* p, int32_t block) {
+  if (block < 0 || (size_t)block >= p->users.size())
+    return fail(FMKV_ERR_INVALID_ARG, "block " + std::to_string(block) + " is not one of " +
+                                          std::to_string(p->users.size()));
+  if (p->users[block] == 0)
+    return fail(FMKV_ERR_INVALID_ARG, "block " + std::to_string(block) + " is free");
+  return FMKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmkv_pages_create(int64_t n_blocks, fmkv_pages** out) {
+  if (!out) return fail(FMKV_ERR_INVALID_ARG, "out is null");
+  *out = nullptr;
+  if (n_blocks < 1 || n_blocks > ((int64_t)1 << 31) - 1)
+    return fail(FMKV_ERR_INVALID_ARG, "n_blocks must be in [1, 2^31)");
+  fmkv_pages* p = nullptr;
+  try {
+    p = new fmkv_pages();
+    p->users.assign((size_t)n_blocks, 0);
+    p->free.resize((size_t)n_blocks);
+  } catch (const std::exception&) {
+    delete p;
+    return fail(FMKV_ERR_OOM, "no memory for the book of blocks");
+  }
+  for (int64_t i = 0; i < n_blocks; i++) p->free[i] = (int32_t)(n_blocks - 1 - i);
+  *out = p;
+  return FMKV_OK;
+}
+
+int fmkv_pages_destroy(fmkv_pages* p) {
+  delete p;
+  return FMKV_OK;
+}
+
+int fmkv_pages_free_count(const fmkv_pages* p, int64_t* out) {
+  if (!p || !out) return fail(FMKV_ERR_INVALID_ARG, "null argument");
+  *out = (int64_t)p->free.size();
+  return FMKV_OK;
+}
+
+int fmkv_pages_users(const fmkv_pages* p, int32_t block, int32_t* out) {
+  if (!p || !out) return fail(FMKV_ERR_INVALID_ARG, "null argument");
+  if (block < 0 || (size_t)block >= p->users.size())
+    return fail(FMKV_ERR_INVALID_ARG, "unknown block");
+  *out = p->users[block];
+  return FMKV_OK;
+}
+
+int fmkv_pages_alloc(fmkv_pages* p, int64_t n, int32_t* blocks) {
+  if (!p || n < 0 || (n > 0 && !blocks)) return fail(FMKV_ERR_INVALID_ARG, "bad pages / n / blocks");
+  if (n > (int64_t)p->free.size())
+    return fail(FMKV_ERR_CAPACITY, std::to_string(n) + " blocks asked for, " +
+                                       std::to_string(p->free.size()) + " free");
+  for (int64_t i = 0; i < n; i++) {
+    blocks[i] = p->free.back();
+    p->free.pop_back();
+    p->users[blocks[i]] = 1;
+  }
+  return FMKV_OK;
+}
+
+int fmkv_pages_release(fmkv_pages* p, const int32_t* blocks, int64_t n) {
+  if (!p || n < 0 || (n > 0 && !blocks)) return fail(FMKV_ERR_INVALID_ARG, "bad pages / n / blocks");
+  // (the free list has room for every block from the start: nothing is allocated)
+  // The users first, so that a block listed more often than it is used is
+  // noticed (and everything put back); then the free list
+  for (int64_t i = 0; i < n; i++) {
+    if (blocks[i] == -1) continue;
+    const int rc = check_block(p, blocks[i]);
+    if (rc) {
+      while (i-- > 0)
+        if (blocks[i] != -1) p->users[blocks[i]]++;
+      return rc;
+    }
+    p->users[blocks[i]]--;
+  }
+  for (int64_t i = n; i-- > 0;) {  // (backwards: the first listed is the first taken again)
+    if (blocks[i] == -1 || p->users[blocks[i]] != 0) continue;
+    p->free.push_back(blocks[i]);
+    p->users[blocks[i]] = -1;  // listed once, whatever its users were
+  }
+  for (int64_t i = 0; i < n; i++)
+    if (blocks[i] != -1 && p->users[blocks[i]] == -1) p->users[blocks[i]] = 0;
+  return FMKV_OK;
+}
+
+int fmkv_pages_fork(fmkv_pages* p, const int32_t* blocks, int64_t n_tokens, int32_t* child,
+                    int32_t* copy_src, int32_t* copy_dst) {
+  if (!p || n_tokens < 0 || !copy_src || !copy_dst || (n_tokens > 0 && (!blocks || !child)))
+    return fail(FMKV_ERR_INVALID_ARG, "bad pages / blocks / n_tokens / child / copy_src / copy_dst");
+  const int64_t n = (n_tokens + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
+  const bool part = n_tokens % fmkv::kBlockTokens != 0 && blocks[n - 1] != -1;
+  for (int64_t i = 0; i < n; i++) {
+    if (blocks[i] == -1) continue;
+    const int rc = check_block(p, blocks[i]);
+    if (rc) return rc;
+    if (p->users[blocks[i]] == INT32_MAX) return fail(FMKV_ERR_CAPACITY, "a block has 2^31 - 1 users");
+  }
+  int32_t fresh = -1;
+  if (part) {
+    const int rc = fmkv_pages_alloc(p, 1, &fresh);
+    if (rc) return rc;
+  }
+  *copy_src = part ? blocks[n - 1] : -1;
+  *copy_dst = fresh;
+  for (int64_t i = 0; i < n; i++) {
+    const bool copied = part && i == n - 1;
+    if (blocks[i] != -1 && !copied) p->users[blocks[i]]++;
+    child[i] = copied ? fresh : blocks[i];
+  }
+  return FMKV_OK;
+}
+
+int fmkv_pages_slide(fmkv_pages* p, int32_t* blocks, int64_t n_tokens, int32_t window,
+                     int32_t sinks, int64_t* n_freed) {
+  if (!p || n_tokens < 0 || (n_tokens > 0 && !blocks) || !n_freed)
+    return fail(FMKV_ERR_INVALID_ARG, "bad pages / blocks / n_tokens / n_freed");
+  int rc = check_window(window, sinks);
+  if (rc) return rc;
+  constexpr int64_t B = fmkv::kBlockTokens;
+  // blocks [first, last) hold hidden positions alone: from the sinks' end to the
+  // window of the next query, at position n_tokens
+  const int64_t first = ((int64_t)sinks + B - 1) / B, last = std::max<int64_t>(n_tokens + 1 - window, 0) / B;
+  *n_freed = 0;
+  if (last <= first) return FMKV_OK;
+  if ((rc = fmkv_pages_release(p, blocks + first, last - first))) return rc;
+  for (int64_t i = first; i < last; i++) {
+    *n_freed += blocks[i] != -1;
+    blocks[i] = -1;
+  }
   return FMKV_OK;
 }
 

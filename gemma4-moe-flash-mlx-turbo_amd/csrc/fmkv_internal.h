@@ -229,6 +229,44 @@ inline bool split_pre(const AttnArgs& a, SplitPre* p) {
   return true;
 }
 
+// Blocks src[i] to dst[i] in each of the pools (at most kCopyPools a launch).
+constexpr int kCopyPools = 32;
+struct CopyArgs {
+  uint8_t* base[kCopyPools];
+  int64_t block_bytes[kCopyPools];  // of all KV heads
+  int32_t n_blocks[kCopyPools];
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t parts;  // work-groups per pair
+};
+
+// Token keep[s][i] of sequence s (st's block table) to position i of dst_table.
+struct CompactArgs {
+  Store st;
+  const int32_t* dst_table;  // [n_seqs][dst_stride]
+  int32_t dst_stride;
+  const int32_t* keep;  // [n_seqs][max_keep]
+  int32_t max_keep;
+  const int32_t* n_keep;  // [n_seqs]
+};
+
+// Norms and rotation of projected rows (fmkv_norm_rope.hip).
+struct NormRopeArgs {
+  const uint16_t *q, *k, *v;  // rows of a token: heads x D from its start
+  int64_t q_stride, k_stride, v_stride;  // elements from token to token
+  uint16_t *q_out, *k_out, *v_out;       // [n_tokens][heads][D]
+  const uint16_t *q_w, *k_w;             // bf16 [D]
+  const int32_t* pos;                    // [n_axes][n_tokens]
+  int64_t n_tokens;
+  int32_t n_q, n_k, n_v;  // rows of a token (n_v 0 with v_from_k: V comes with K's rows)
+  int32_t v_norm, v_from_k;
+  float eps;
+  int32_t rope_dims;
+  double log2_theta;
+  int32_t axis_end[4];  // pairs of the axes before and with this one
+  int32_t chunks;       // parts that a token's rows are split into
+};
+
 hipError_t launch_append(const AppendArgs& a, int n_seqs, int max_tasks, hipStream_t s);
 // ev_begin / ev_end (optional, both or neither) are recorded by the split-K
 // kernel's dispatch: the start and end of its execution.
@@ -260,5 +298,8 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split);
 size_t prefill_scratch_bytes(int cus);
 hipError_t launch_read_codes(const ReadArgs& a, hipStream_t s);
 hipError_t launch_fetch(const FetchArgs& a, hipStream_t s);
+hipError_t launch_copy_blocks(CopyArgs& a, int n_pools, int64_t n_pairs, hipStream_t s);
+hipError_t launch_compact(const CompactArgs& a, int n_seqs, hipStream_t s);
+hipError_t launch_norm_rope(NormRopeArgs& a, int head_dim, int cus, hipStream_t s);
 
 }  // namespace fmkv

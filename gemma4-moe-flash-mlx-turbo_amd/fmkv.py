@@ -55,6 +55,9 @@ EXPORTED = (
     "fmkv_decode_step_projected", "fmkv_paged_decode_step_projected",
     "fmkv_paged_window_decode_attention", "fmkv_paged_window_decode_step",
     "fmkv_paged_window_prefill_attention", "fmkv_paged_window_prefill_step", "fmkv_pool_storage",
+    "fmkv_pools_copy_blocks", "fmkv_paged_compact", "fmkv_qkv_norm_rope",
+    "fmkv_pages_create", "fmkv_pages_destroy", "fmkv_pages_free_count", "fmkv_pages_users",
+    "fmkv_pages_alloc", "fmkv_pages_release", "fmkv_pages_fork", "fmkv_pages_slide",
 )
 
 
@@ -109,6 +112,40 @@ def _check_prologue_weight(prologue: KvPrologue, head_dim: int) -> None:
     w = getattr(prologue, "weight", None)
     if w is not None and w.numel() != head_dim:
         raise ValueError(f"k_norm_weight has {w.numel()} elements; head_dim is {head_dim}")
+
+
+class QkvPrologue(ctypes.Structure):
+    """fmkv_qkv_prologue: the norms of q, k and v and the rotation of q and k
+    (src/model/gemma4_attention.rs:50-81), see qkv_norm_rope."""
+    _fields_ = [
+        ("q_norm_weight", ctypes.c_void_p),
+        ("k_norm_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("rope_dims", ctypes.c_int32),
+        ("rope_theta", ctypes.c_float),
+        ("n_axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("v_norm", ctypes.c_int32),
+        ("v_from_k", ctypes.c_int32),
+    ]
+
+
+def make_qkv_prologue(q_norm_weight, k_norm_weight, eps: float, rope_dims: int, rope_theta: float,
+                      sections=None, v_norm: bool = True, v_from_k: bool = False) -> QkvPrologue:
+    """Weights bf16 [head_dim] on the device (None for rows that are never
+    given); sections: pairs of each position axis (None: one axis). The struct
+    keeps the weights alive, as make_prologue's does."""
+    for w in (q_norm_weight, k_norm_weight):
+        if w is not None and (w.dtype != torch.bfloat16 or w.dim() != 1 or not w.is_contiguous()):
+            raise ValueError("norm weights must be contiguous bf16 [head_dim]")
+    cut = tuple(sections) if sections is not None else (rope_dims // 2,)
+    if not 1 <= len(cut) <= 4:
+        raise ValueError("sections must be one to four counts of pairs")
+    pro = QkvPrologue(None if q_norm_weight is None else q_norm_weight.data_ptr(),
+                      None if k_norm_weight is None else k_norm_weight.data_ptr(), eps, rope_dims,
+                      rope_theta, len(cut), (ctypes.c_int32 * 4)(*cut), int(v_norm), int(v_from_k))
+    pro.weights = (q_norm_weight, k_norm_weight)
+    return pro
 
 
 _lib = None
@@ -180,6 +217,18 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         "fmkv_paged_window_prefill_step": ([vp, vp, vp, vp, i32, vp, i32, i32, i32, vp, i32,
                                             ctypes.c_float, i32, i32, vp, i32, vp], ctypes.c_int),
         "fmkv_pool_storage": ([vp, P(vp), P(i64)], ctypes.c_int),
+        "fmkv_pools_copy_blocks": ([P(vp), i32, vp, vp, i64, vp], ctypes.c_int),
+        "fmkv_paged_compact": ([vp, vp, i32, vp, i32, vp, vp, i32, i32, vp], ctypes.c_int),
+        "fmkv_qkv_norm_rope": ([P(QkvPrologue), i32, i32, i32, i64, vp, i64, vp, i64, vp, i64, vp,
+                                vp, vp, vp, vp], ctypes.c_int),
+        "fmkv_pages_create": ([i64, P(vp)], ctypes.c_int),
+        "fmkv_pages_destroy": ([vp], ctypes.c_int),
+        "fmkv_pages_free_count": ([vp, P(i64)], ctypes.c_int),
+        "fmkv_pages_users": ([vp, i32, P(i32)], ctypes.c_int),
+        "fmkv_pages_alloc": ([vp, i64, P(i32)], ctypes.c_int),
+        "fmkv_pages_release": ([vp, P(i32), i64], ctypes.c_int),
+        "fmkv_pages_fork": ([vp, P(i32), i64, P(i32), P(i32), P(i32)], ctypes.c_int),
+        "fmkv_pages_slide": ([vp, P(i32), i64, i32, i32, P(i64)], ctypes.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
@@ -690,6 +739,20 @@ class PagedPool:
             _ptr(out), _dtype_code(out.dtype), _stream(stream)))
         return out
 
+    def compact(self, block_tables, keep, n_keep, dst_tables, stream=None) -> None:
+        """Moves the tokens that sequences keep to the front of other blocks:
+        position keep[s, i] becomes position i of dst_tables' row s, i <
+        n_keep[s]. int32: block_tables [n_seqs, max_blocks], keep [n_seqs,
+        max_keep], n_keep [n_seqs], dst_tables [n_seqs, dst_max_blocks]. No
+        block of dst_tables is one of a sequence's sources, or listed twice."""
+        n = keep.shape[0]
+        _check_tensor("keep", keep, torch.int32, (n, None))
+        _check_tensor("dst_tables", dst_tables, torch.int32, (n, None))
+        self._check_tables(block_tables, n, n_keep=n_keep)
+        _check(self._lib.fmkv_paged_compact(
+            self._h, _ptr(block_tables), block_tables.shape[1], _ptr(keep), keep.shape[1],
+            _ptr(n_keep), _ptr(dst_tables), dst_tables.shape[1], n, _stream(stream)))
+
     def storage(self) -> torch.Tensor:
         """The pool's blocks as a uint8 tensor [n_blocks, n_kv_heads, bytes of a
         head-block] over the pool's own memory (which it keeps alive): to move
@@ -707,6 +770,136 @@ class PagedPool:
     def read_codes(self, stream=None):
         return _read_codes(self._lib.fmkv_pool_read_codes, self._h, self.desc,
                            self.n_blocks * BLOCK_TOKENS, stream)
+
+
+def copy_blocks(pools, src, dst, stream=None) -> None:
+    """Blocks src[i] to dst[i] in every pool of `pools` (a model's layers), in
+    one launch. src, dst: int32 [n] on the device; the destinations are distinct
+    and no sources."""
+    pools = list(pools)
+    _check_tensor("src", src, torch.int32, (None,))
+    _check_tensor("dst", dst, torch.int32, (src.shape[0],))
+    handles = (ctypes.c_void_p * max(len(pools), 1))(*[p._h for p in pools])
+    _check(load_library().fmkv_pools_copy_blocks(handles, len(pools), _ptr(src), _ptr(dst),
+                                                 src.shape[0], _stream(stream)))
+
+
+def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=None):
+    """(q, k, v) of a layer from its projections in one pass: per-head norms of
+    all three, q and k rotated by their positions (src/model/gemma4_attention.rs
+    :50-81). q bf16 [n_tokens, n_q_heads, D], k and v [n_tokens, n_kv_heads, D],
+    each row of heads contiguous and tokens any stride apart (slices of a fused
+    projection); q, or k and v, may be None. positions int32 [n_axes, n_tokens]
+    ([n_tokens] with one axis). Returns contiguous rows for append, decode_step
+    and the prefill calls (None for what was not given; with v_from_k V comes
+    from k). out: the three outputs, which may be the inputs themselves."""
+    rows = [t for t in (q, k, v) if t is not None]
+    if not rows:
+        raise ValueError("q or k must be given")
+    n, _, D = rows[0].shape
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t is None:
+            continue
+        _check_tensor(name, t, torch.bfloat16, (n, None, D))
+        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or not t.is_cuda:
+            raise ValueError(f"{name} must be a device tensor with contiguous rows of heads")
+    if v is not None and (k is None or k.shape != v.shape):
+        raise ValueError("v needs a k of its shape")
+    for w in getattr(prologue, "weights", ()):
+        if w is not None and w.numel() != D:
+            raise ValueError(f"a norm weight has {w.numel()} elements; head_dim is {D}")
+    if positions is not None:
+        shape = (n,) if prologue.n_axes == 1 and positions.dim() == 1 else (prologue.n_axes, n)
+        _check_tensor("positions", positions, torch.int32, shape)
+    like = (q, k, k if prologue.v_from_k else v)
+    if out is None:
+        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in like]
+    for t, o in zip(like, out):
+        if (t is None) != (o is None):
+            raise ValueError("out must have a tensor for each output")
+        if t is not None:
+            _check_tensor("out", o, torch.bfloat16, tuple(t.shape))
+
+    def at(t):  # (a token's stride; one token: none)
+        return (None, 0) if t is None else (t.data_ptr(), t.stride(0) if n > 1 else t.shape[1] * D)
+
+    _check(load_library().fmkv_qkv_norm_rope(
+        ctypes.byref(prologue), D, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], n,
+        *at(q), *at(k), *at(v), _ptr(positions), *(_ptr(o) for o in out), _stream(stream)))
+    return tuple(out)
+
+
+class PageBook:
+    """The book of a pool's blocks (or of several pools that share their block
+    tables): which are free, how many sequences use each. Block lists are host
+    lists of ints (-1: given back)."""
+
+    def __init__(self, n_blocks: int):
+        self.n_blocks = n_blocks
+        self._lib = load_library()
+        h = ctypes.c_void_p()
+        _check(self._lib.fmkv_pages_create(n_blocks, ctypes.byref(h)))
+        self._h = h
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self._lib.fmkv_pages_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def free_count(self) -> int:
+        v = ctypes.c_int64()
+        _check(self._lib.fmkv_pages_free_count(self._h, ctypes.byref(v)))
+        return v.value
+
+    def users(self, block: int) -> int:
+        v = ctypes.c_int32()
+        _check(self._lib.fmkv_pages_users(self._h, block, ctypes.byref(v)))
+        return v.value
+
+    def alloc(self, n: int) -> list[int]:
+        """n free blocks (an error, and none taken, when fewer are free)."""
+        if n > self.n_blocks:
+            raise Exception_(FMKV_ERR_CAPACITY, f"{n} blocks asked for of {self.n_blocks}")
+        buf = (ctypes.c_int32 * max(n, 1))()
+        _check(self._lib.fmkv_pages_alloc(self._h, n, buf))
+        return list(buf[:max(n, 0)])
+
+    def release(self, blocks) -> None:
+        """One user less for each block."""
+        blocks = list(blocks)
+        _check(self._lib.fmkv_pages_release(self._h, _i32s(blocks), len(blocks)))
+
+    def fork(self, blocks, n_tokens: int):
+        """(blocks of a second sequence that goes on from n_tokens of a first,
+        the (src, dst) copy that copy_blocks has to make for it or None)."""
+        blocks = list(blocks)
+        n = (n_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS
+        if n > len(blocks):
+            raise ValueError(f"{n_tokens} tokens need {n} blocks, got {len(blocks)}")
+        child, src, dst = (ctypes.c_int32 * max(n, 1))(), ctypes.c_int32(), ctypes.c_int32()
+        _check(self._lib.fmkv_pages_fork(self._h, _i32s(blocks), n_tokens, child, ctypes.byref(src),
+                                         ctypes.byref(dst)))
+        return list(child[:max(n, 0)]), None if src.value < 0 else (src.value, dst.value)
+
+    def slide(self, blocks, n_tokens: int, window: int, sinks: int = 0) -> list[int]:
+        """The sequence's blocks after giving back those that no query at position
+        n_tokens or later sees through the window and the sinks (-1 there)."""
+        blocks = list(blocks)
+        if (n_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS > len(blocks):
+            raise ValueError(f"{n_tokens} tokens need more than {len(blocks)} blocks")
+        buf, n = _i32s(blocks), ctypes.c_int64()
+        _check(self._lib.fmkv_pages_slide(self._h, buf, n_tokens, window, sinks, ctypes.byref(n)))
+        return list(buf[:len(blocks)])
+
+
+def _i32s(values):
+    return (ctypes.c_int32 * max(len(values), 1))(*values)
 
 
 class _Storage:

@@ -388,6 +388,98 @@ int fmkv_paged_window_prefill_step(fmkv_pool* pool, const void* k_bf16, const vo
                                    float scale, int32_t window, int32_t sinks, void* out,
                                    int32_t out_dtype, void* stream);
 
+/* Blocks src[i] copied to dst[i], i < n_pairs, in every one of n_pools pools (the
+ * layers of a model that share their block tables), all KV heads: a forked
+ * sequence's partly filled last block, blocks moved together. src, dst: int32
+ * device [n_pairs]. A pair that names a block outside a pool is left out there.
+ * The destinations of a call are distinct, and no source of it is among them
+ * (the contents of a destination that breaks this are unspecified; a pair of
+ * one block and itself changes nothing). All pools on the current GPU. No
+ * counterpart in the reference, whose caches belong to one request each. */
+int fmkv_pools_copy_blocks(fmkv_pool* const* pools, int32_t n_pools, const int32_t* src,
+                           const int32_t* dst, int64_t n_pairs, void* stream);
+
+/* The tokens that each sequence keeps, moved to the front of other blocks:
+ * position keep[s][i] of sequence s (block_tables) becomes position i of its
+ * row of dst_tables, i < n_keep[s] (at most max_keep). Codes, scales and norms
+ * move as they are (a kept K keeps the rotation of the position it was computed
+ * at). keep: int32 device [n_seqs][max_keep], in any order; n_keep: int32 device
+ * [n_seqs]; dst_tables: int32 device [n_seqs][dst_max_blocks]. A token whose
+ * position or blocks lie outside the tables or the pool is left out, and its
+ * slot, like every slot behind the last kept token, stays as it was. The blocks
+ * written are distinct and no sequence's sources (else the contents of those
+ * blocks are unspecified). The pool is on the current GPU. */
+int fmkv_paged_compact(fmkv_pool* pool, const int32_t* block_tables, int32_t max_blocks,
+                       const int32_t* keep, int32_t max_keep, const int32_t* n_keep,
+                       const int32_t* dst_tables, int32_t dst_max_blocks, int32_t n_seqs,
+                       void* stream);
+
+/* The book of a pool's blocks (or of several pools that share block tables):
+ * which are free and how many sequences use each. Host memory only; block lists
+ * below are host arrays. A handle is used by one host thread at a time. */
+typedef struct fmkv_pages fmkv_pages;
+int fmkv_pages_create(int64_t n_blocks, fmkv_pages** out);
+int fmkv_pages_destroy(fmkv_pages* pages);
+int fmkv_pages_free_count(const fmkv_pages* pages, int64_t* out);
+/* Users of a block (0: free). */
+int fmkv_pages_users(const fmkv_pages* pages, int32_t block, int32_t* out);
+/* n free blocks, each with one user from now on (FMKV_ERR_CAPACITY and none
+ * taken when fewer are free). */
+int fmkv_pages_alloc(fmkv_pages* pages, int64_t n, int32_t* blocks);
+/* One user less for each of n blocks (entries of -1 are skipped); a block
+ * without users is free again. A free or unknown block in the list: nothing is
+ * changed. */
+int fmkv_pages_release(fmkv_pages* pages, const int32_t* blocks, int64_t n);
+/* A second sequence that goes on from n_tokens of a first: child gets its
+ * blocks (ceil(n_tokens / 16) of them), whole ones shared, a partly filled last
+ * one replaced by a free block. *copy_src and *copy_dst name the copy that
+ * fmkv_pools_copy_blocks then has to make (-1: none). Entries of -1 (blocks
+ * given back) stay -1. */
+int fmkv_pages_fork(fmkv_pages* pages, const int32_t* blocks, int64_t n_tokens, int32_t* child,
+                    int32_t* copy_src, int32_t* copy_dst);
+/* Gives back the blocks of a sequence of n_tokens that no later query sees
+ * through a window with sinks (a query at position p >= n_tokens sees j > p -
+ * window and j < sinks); their entries become -1. *n_freed: how many entries. */
+int fmkv_pages_slide(fmkv_pages* pages, int32_t* blocks, int64_t n_tokens, int32_t window,
+                     int32_t sinks, int64_t* n_freed);
+
+/* What an attention layer does to its projections before the cache and the
+ * attention (src/model/gemma4_attention.rs:50-81), for q, k and v in one pass:
+ *   q, k = rotate(x / sqrt(mean(x^2) + eps) * weight), per head (q_norm, k_norm)
+ *   v    = x / sqrt(mean(x^2) + eps) (v_norm 1) or x (v_norm 0)
+ * The first rope_dims dims of a head are rotated in pairs (i, i + rope_dims /
+ * 2) by the angle pos * rope_theta^(-2i / rope_dims); the rest are left as
+ * they are. With n_axes > 1 positions have several axes (time, height, width of
+ * pictures): the first sections[0] pairs turn with the first axis's position,
+ * the next sections[1] with the second's, and so on (the sections add up to
+ * rope_dims / 2). Everything in f32 with one rounding to bf16 at the end; angles
+ * keep 2^-24 of a turn at any position. (The projected appends repeat the
+ * reference's roundings instead, with f32 angles, for K and V alone.) */
+typedef struct fmkv_qkv_prologue {
+  const void* q_norm_weight; /* bf16 [head_dim], device (NULL without q) */
+  const void* k_norm_weight; /* bf16 [head_dim], device (NULL without k) */
+  float eps;
+  int32_t rope_dims;         /* a multiple of 8 in [0, head_dim]; 0: no rotation */
+  float rope_theta;          /* >= 1 */
+  int32_t n_axes;            /* 1 to 4 */
+  int32_t sections[4];       /* pairs of each axis (one axis: all, whatever is given) */
+  int32_t v_norm;
+  int32_t v_from_k;          /* 1: V rows are v_norm of the raw k rows (v NULL) */
+} fmkv_qkv_prologue;
+
+/* n_tokens rows of q [n_q_heads][head_dim], k and v [n_kv_heads][head_dim]
+ * (bf16), token t at ptr + t * stride elements, so that parts of one fused
+ * projection can be given; q, k or v may be absent (0 heads, NULL). head_dim
+ * 128, 256 or 512. positions: int32 device [n_axes][n_tokens] (NULL with
+ * rope_dims 0). Outputs are contiguous [n_tokens][heads][head_dim] bf16, the
+ * inputs of the append, decode step and prefill calls. An output may be its own
+ * input where that is contiguous; any other overlap is refused. */
+int fmkv_qkv_norm_rope(const fmkv_qkv_prologue* prologue, int32_t head_dim, int32_t n_q_heads,
+                       int32_t n_kv_heads, int64_t n_tokens, const void* q, int64_t q_stride,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       const int32_t* positions, void* q_out, void* k_out, void* v_out,
+                       void* stream);
+
 /* The pool's storage: n_blocks blocks of *block_bytes (all KV heads), on the
  * pool's GPU, as fmkv_pool_create laid it out (zeros, until tokens are
  * appended). A block is moved by copying its bytes, to the same place of
