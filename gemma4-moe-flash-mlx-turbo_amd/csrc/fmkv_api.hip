@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -115,10 +116,13 @@ int64_t n_slots_of(const fmkv_cache_desc& d) {
 }
 
 int device_cus() {
+  static std::atomic<int> known[64];  // by device: the query takes as long as a launch
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess) return 256;
+  if (dev >= 0 && dev < 64 && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
   if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     return 256;
+  if (dev >= 0 && dev < 64) known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
 
@@ -667,6 +671,45 @@ int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
   return FMKV_OK;
 }
 
+// Blocks per split of a window's call: nblk visible blocks at most for each of
+// `rows` (sequence, KV head) pairs. A split costs its blocks and a fixed part (q
+// table, merge of its streams: about 12 blocks' time, 3 of the plain kernel's),
+// each round of work-groups that the chip takes at once costs the longest split
+// in it, and every split a tenth of a block in the combine. So the splits of
+// each number of rounds are as many as fit it, or as the combine allows, and
+// equal; the cheapest wins. (us per call, by blocks per split: one sequence,
+// 66 blocks of 4 bits, 256 dims, 8 heads: 1: 20.1, 2: 15.4, 3: 10.9, 8: 11.0, 16:
+// 13.0; seven of 254 blocks, 8 bits, 512 dims, 2 heads: 14, which leaves 10
+// work-groups to a second round: 28.6, 16: 22.8, 32: 27.1; 32 ragged ones of up
+// to 258 blocks, 4 bits: 64 (4 splits and one of 2 blocks): 60.2, 86: 51.4, 129:
+// 53.9; the same all at 258: 66.5, 65.7, 63.9; one of 254 blocks, 2 heads of 512
+// dims: 2: 17.0, 4: 15.5, 8: 16.8, 16: 19.6.)
+int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows, int new_col) {
+  if (nblk < 1) return 1;
+  const bool plain = d.mode == FMKV_MODE_PLAIN;
+  const double fixed = plain ? 3.0 : 12.0;
+  const int64_t few = std::max<int64_t>((int64_t)std::sqrt(10.0 * (double)nblk), 1);
+  auto best = [&](int64_t per_cu, int64_t min_bps) {
+    int64_t slots = per_cu * cus;
+    if (new_col && rows <= slots / 2) slots -= rows;  // the new-token column's work-groups
+    int64_t bps = 0;
+    double cost = 0.0;
+    const int64_t r0 = (rows + slots - 1) / slots;
+    for (int64_t r = r0; r < r0 + 4; r++) {
+      const int64_t s = std::clamp<int64_t>(r * slots / rows, 1, std::min(few, nblk));
+      const int64_t b = std::max((nblk + s - 1) / s, min_bps), n = (nblk + b - 1) / b;
+      const double c = (double)((n * rows + slots - 1) / slots) * ((double)b + fixed) + 0.1 * (double)n;
+      if (bps == 0 || c < cost) bps = b, cost = c;
+    }
+    return bps;
+  };
+  if (paged_solo_slots(d) == 1) return best(plain ? 2 : 1, 1);
+  // wave pairs, one work-group per CU, while a round of them is enough; else
+  // single-wave streams, three per CU
+  const int64_t pairs = best(1, 1);
+  return pairs < 8 && (nblk + pairs - 1) / pairs * rows <= cus ? pairs : best(3, 8);
+}
+
 // win > 0: over the last `win` positions and the first `sinks` ones.
 int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
                             int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
@@ -719,6 +762,12 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   const int64_t share = (total + n_slots - 1) / n_slots;
   const int min_bps = (int)std::min<int64_t>(64, std::max<int64_t>(share, 1));
   const int wg_per_cu = 6 * slots * fmkv::kAttnWgPerCu;
+  if (win > 0) {
+    const int64_t b = window_bps(p->desc, p->cus, nblk, (int64_t)p->desc.n_kv_heads * n_s, new_col);
+    return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,
+                                    max_blocks, q, n_q_heads, scale, tau, out, out_dtype,
+                                    1 << 20 /* b is the blocks per split */, (int)b, 1, new_col, a);
+  }
   const int64_t bps = choose_bps(total, p->cus, wg_per_cu, 0, min_bps);
   const int first_mult = total >= 4 * n_slots * bps ? 4 : 1;
   return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,

@@ -46,10 +46,12 @@ __global__ __launch_bounds__(kNrThreads) void norm_rope_kernel(NormRopeArgs a) {
     double f = exp2(-(double)tid / half * a.log2_theta) * 0.15915494309189535;  // / 2 pi
     s_freq[tid] = (uint64_t)(f * 18446744073709551616.0);
   }
-  // the lane's dims da .. da + 3 and db .. db + 3: four pairs, or (past the
-  // rotated ones) eight dims in a row
+  // The lane's dims da .. da + 3 and db .. db + 3: four pairs, or (past the
+  // rotated ones) four of either half of the rest, so that a wave's loads and
+  // stores are whole lines. (Eight in a row: two accesses to every line.)
   const bool rot = l < half / 4;
-  const int da = rot ? 4 * l : 8 * l, db = rot ? da + half : da + 4;
+  const int da = rot ? 4 * l : a.rope_dims + 4 * (l - half / 4);
+  const int db = da + (rot ? half : D / 2 - half);
   float qw[8], kw[8];
   if (a.n_q) {
     widen(*reinterpret_cast<const u16x4_a2*>(a.q_w + da), qw);
@@ -154,7 +156,9 @@ hipError_t launch_norm_rope_t(NormRopeArgs& a, int cus, hipStream_t s) {
   int64_t chunks = (want + a.n_tokens - 1) / a.n_tokens;
   a.chunks = (int32_t)(chunks > groups ? groups : chunks);
   const int64_t wgs = (a.n_tokens * a.chunks + kWaves - 1) / kWaves;
-  const int64_t most = (int64_t)cus * 8;  // resident at once; they take the tasks in turn
+  // Work-groups that are resident at once (98 registers: five waves a SIMD);
+  // they take the tasks in turn, so that the frequencies are computed once each.
+  const int64_t most = (int64_t)cus * 5;
   hipLaunchKernelGGL((norm_rope_kernel<D>), dim3((unsigned)(wgs < most ? wgs : most)), dim3(kNrThreads), 0,
                      s, a);
   return hipGetLastError();

@@ -1276,8 +1276,11 @@ void prefill_attn_kernel(PrefillArgs a) {
 // Merges the key ranges of a split sequence's rows: a wave per row, lane l
 // holding dims E l .., out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k,
 // rotated back. Reads each partial once (bound by that: D * 4 bytes a row and
-// range). A work-group takes 16 rows of a tile.
-constexpr int kPfMergeRows = 16;
+// range). A work-group takes four rows of a tile, one a wave: the rows of few
+// queries then merge side by side (5 queries after 3000 positions, window 1024,
+// 8/4 heads of 128 dims, bf16: 20.1 us the call, 25.0 with 16 rows a work-group;
+// after 9000, window 4000, 8 bits, 16/2 heads of 512 dims: 39.6 and 58.7).
+constexpr int kPfMergeRows = 4;
 template <int D, bool ROT>
 __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int tiles) {
   constexpr int E = D / 64;
@@ -1291,37 +1294,36 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int t
   const int nq = a.n_q - tile * QP < QP ? a.n_q - tile * QP : QP;
   const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
   const float cs = ROT ? fwht_lane_sign(lane) * a.c : 1.0f;
-#pragma unroll 1
-  for (int r = r0 + wave; r < r0 + kPfMergeRows; r += 4) {
-    const int rq = r / G, rh = r - rq * G;
-    if (rq >= nq) break;
-    const int64_t step = (int64_t)gridDim.y * tiles * kPfRows;  // rows from range to range
-    const int64_t row = (((int64_t)un.first * gridDim.y + kvh) * tiles + tile) * kPfRows + r;
-    float M = -1e30f;
-    for (int k = lane; k < un.ranges; k += 64) M = fmaxf(M, a.part_ml[(row + k * step) * 2]);
-    M = group_max<64>(M, lane);
-    float x[E], l = 0.0f;
+  const int r = r0 + wave, rq = r / G, rh = r - rq * G;
+  if (rq >= nq) return;
+  const int64_t step = (int64_t)gridDim.y * tiles * kPfRows;  // rows from range to range
+  const int64_t row = (((int64_t)un.first * gridDim.y + kvh) * tiles + tile) * kPfRows + r;
+  float M = -1e30f;
+  for (int k = lane; k < un.ranges; k += 64) M = fmaxf(M, a.part_ml[(row + k * step) * 2]);
+  M = group_max<64>(M, lane);
+  float x[E], l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; i++) x[i] = 0.0f;
-#pragma unroll 2
-    for (int k = 0; k < un.ranges; k++) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (row + k * step) * 2);
-      const float w = __builtin_amdgcn_exp2f(ml.x - M);
-      const float* src = a.part_o + (row + k * step) * D + lane * E;
-      l = fmaf(w, ml.y, l);
+  for (int i = 0; i < E; i++) x[i] = 0.0f;
+  // (ranges whose loads are in flight together; 4 of 512 dims ran slower)
+  constexpr int kAhead = D == 512 ? 2 : 4;
+#pragma unroll kAhead
+  for (int k = 0; k < un.ranges; k++) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (row + k * step) * 2);
+    const float w = __builtin_amdgcn_exp2f(ml.x - M);
+    const float* src = a.part_o + (row + k * step) * D + lane * E;
+    l = fmaf(w, ml.y, l);
 #pragma unroll
-      for (int i = 0; i < E; i++) x[i] = fmaf(w, src[i], x[i]);
-    }
-    if constexpr (ROT) {
-#pragma unroll
-      for (int i = 0; i < E; i++) x[i] = apply_sign(x[i], sbits, i);
-      wave_fwht_signed<E>(x, lane);
-    }
-#pragma unroll
-    for (int i = 0; i < E; i++) x[i] = l > 0.0f ? (x[i] * cs) / l : 0.0f;
-    store_out<E>(a, (((int64_t)seq * a.n_q + tile * QP + rq) * a.n_q_heads + (int64_t)kvh * G + rh) * D +
-                        lane * E, x);
+    for (int i = 0; i < E; i++) x[i] = fmaf(w, src[i], x[i]);
   }
+  if constexpr (ROT) {
+#pragma unroll
+    for (int i = 0; i < E; i++) x[i] = apply_sign(x[i], sbits, i);
+    wave_fwht_signed<E>(x, lane);
+  }
+#pragma unroll
+  for (int i = 0; i < E; i++) x[i] = l > 0.0f ? (x[i] * cs) / l : 0.0f;
+  store_out<E>(a, (((int64_t)seq * a.n_q + tile * QP + rq) * a.n_q_heads + (int64_t)kvh * G + rh) * D +
+                      lane * E, x);
 }
 
 template <int D, int BITS, int MODE, int RW, bool WIN>

@@ -256,7 +256,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _stream(stream) -> int | None:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        # (the handle alone: making a torch.cuda.Stream takes longer than a launch)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -573,6 +574,7 @@ class PagedPool:
     def __init__(self, desc: CacheDesc, n_blocks: int):
         self.desc = desc
         self.n_blocks = n_blocks
+        self._D, self._H = desc.head_dim, desc.n_kv_heads  # (a struct's field takes longer to read)
         self._lib = load_library()
         h = ctypes.c_void_p()
         _check(self._lib.fmkv_pool_create(ctypes.byref(desc), n_blocks, ctypes.byref(h)))
@@ -673,15 +675,13 @@ class PagedPool:
         """attention() of each sequence's newest token over its last `window`
         positions and its first `sinks` ones. q bf16 [n_seqs, n_q_heads, D];
         seq_lens int32 [n_seqs]. Pages that hold neither are not looked up."""
-        d = self.desc
-        n = q.shape[0]
-        _check_tensor("q", q, torch.bfloat16, (n, None, d.head_dim))
-        self._check_tables(block_tables, n, seq_lens=seq_lens)
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
         out = _out(out, q, dtype)
         _check(self._lib.fmkv_paged_window_decode_attention(
-            self._h, _ptr(q), _ptr(block_tables), block_tables.shape[1], _ptr(seq_lens), n,
-            max_seq_len, q.shape[1], scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
-            _stream(stream)))
+            self._h, _ptr(q), _ptr(block_tables), width, _ptr(seq_lens), n, max_seq_len, heads, scale,
+            window, sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def window_decode_step(self, keys, values, block_tables, start_pos, seq_lens, max_seq_len: int,
@@ -690,17 +690,17 @@ class PagedPool:
         """append(keys, values, ...) of one token per sequence at start_pos
         (= seq_lens - 1), then window_attention, in one call. keys/values bf16
         [n_seqs, 1, n_kv_heads, D]."""
-        d = self.desc
-        n = q.shape[0]
-        _check_tensor("q", q, torch.bfloat16, (n, None, d.head_dim))
-        for name, t in (("keys", keys), ("values", values)):
-            _check_tensor(name, t, torch.bfloat16, (n, 1, d.n_kv_heads, d.head_dim))
-        self._check_tables(block_tables, n, seq_lens=seq_lens, start_pos=start_pos)
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        _check_tensor("keys", keys, torch.bfloat16, (n, 1, self._H, self._D))
+        _check_tensor("values", values, torch.bfloat16, (n, 1, self._H, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
         out = _out(out, q, dtype)
         _check(self._lib.fmkv_paged_window_decode_step(
-            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), block_tables.shape[1],
-            _ptr(start_pos), _ptr(seq_lens), n, max_seq_len, _ptr(q), q.shape[1], scale, window,
-            sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), width, _ptr(start_pos),
+            _ptr(seq_lens), n, max_seq_len, _ptr(q), heads, scale, window, sinks, _ptr(out),
+            _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def window_prefill(self, q, block_tables, start_pos, window: int, sinks: int = 0,
@@ -710,15 +710,13 @@ class PagedPool:
         start_pos .. start_pos + n_new - 1, whose keys and values were appended
         before, over the window and the sinks of each. max_seq_len: see
         prefill_step."""
-        d = self.desc
-        n, n_new = q.shape[:2]
-        _check_tensor("q", q, torch.bfloat16, (n, n_new, None, d.head_dim))
-        self._check_tables(block_tables, n, start_pos=start_pos)
+        n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
         out = _out(out, q, dtype)
         _check(self._lib.fmkv_paged_window_prefill_attention(
-            self._h, _ptr(q), _ptr(block_tables), block_tables.shape[1], _ptr(start_pos), n, n_new,
-            max_seq_len, q.shape[2], scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
-            _stream(stream)))
+            self._h, _ptr(q), _ptr(block_tables), width, _ptr(start_pos), n, n_new, max_seq_len, heads,
+            scale, window, sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def window_prefill_step(self, keys, values, block_tables, start_pos, q, window: int,
@@ -726,17 +724,16 @@ class PagedPool:
                             dtype=torch.bfloat16, stream=None):
         """append(keys, values, ...) at start_pos, then window_prefill(q, ...).
         keys/values bf16 [n_seqs, n_new, n_kv_heads, D]."""
-        d = self.desc
-        n, n_new = q.shape[:2]
-        _check_tensor("q", q, torch.bfloat16, (n, n_new, None, d.head_dim))
-        for name, t in (("keys", keys), ("values", values)):
-            _check_tensor(name, t, torch.bfloat16, (n, n_new, d.n_kv_heads, d.head_dim))
-        self._check_tables(block_tables, n, start_pos=start_pos)
+        n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
+        _check_tensor("keys", keys, torch.bfloat16, (n, n_new, self._H, self._D))
+        _check_tensor("values", values, torch.bfloat16, (n, n_new, self._H, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
         out = _out(out, q, dtype)
         _check(self._lib.fmkv_paged_window_prefill_step(
-            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), block_tables.shape[1],
-            _ptr(start_pos), n, n_new, max_seq_len, _ptr(q), q.shape[2], scale, window, sinks,
-            _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), width, _ptr(start_pos), n, n_new,
+            max_seq_len, _ptr(q), heads, scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
+            _stream(stream)))
         return out
 
     def compact(self, block_tables, keep, n_keep, dst_tables, stream=None) -> None:
@@ -745,13 +742,13 @@ class PagedPool:
         n_keep[s]. int32: block_tables [n_seqs, max_blocks], keep [n_seqs,
         max_keep], n_keep [n_seqs], dst_tables [n_seqs, dst_max_blocks]. No
         block of dst_tables is one of a sequence's sources, or listed twice."""
-        n = keep.shape[0]
-        _check_tensor("keep", keep, torch.int32, (n, None))
-        _check_tensor("dst_tables", dst_tables, torch.int32, (n, None))
-        self._check_tables(block_tables, n, n_keep=n_keep)
+        n, most = _check_tensor("keep", keep, torch.int32, (None, None))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        dst_width = _check_tensor("dst_tables", dst_tables, torch.int32, (n, None))[1]
+        _check_tensor("n_keep", n_keep, torch.int32, (n,))
         _check(self._lib.fmkv_paged_compact(
-            self._h, _ptr(block_tables), block_tables.shape[1], _ptr(keep), keep.shape[1],
-            _ptr(n_keep), _ptr(dst_tables), dst_tables.shape[1], n, _stream(stream)))
+            self._h, _ptr(block_tables), width, _ptr(keep), most, _ptr(n_keep), _ptr(dst_tables),
+            dst_width, n, _stream(stream)))
 
     def storage(self) -> torch.Tensor:
         """The pool's blocks as a uint8 tensor [n_blocks, n_kv_heads, bytes of a
@@ -761,11 +758,6 @@ class PagedPool:
         _check(self._lib.fmkv_pool_storage(self._h, ctypes.byref(base), ctypes.byref(size)))
         return torch.as_tensor(_Storage(self, base.value, (
             self.n_blocks, self.desc.n_kv_heads, size.value // self.desc.n_kv_heads)), device="cuda")
-
-    def _check_tables(self, block_tables, n_seqs: int, **per_seq) -> None:
-        _check_tensor("block_tables", block_tables, torch.int32, (n_seqs, None))
-        for name, t in per_seq.items():
-            _check_tensor(name, t, torch.int32, (n_seqs,))
 
     def read_codes(self, stream=None):
         return _read_codes(self._lib.fmkv_pool_read_codes, self._h, self.desc,
@@ -793,40 +785,46 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
     ([n_tokens] with one axis). Returns contiguous rows for append, decode_step
     and the prefill calls (None for what was not given; with v_from_k V comes
     from k). out: the three outputs, which may be the inputs themselves."""
-    rows = [t for t in (q, k, v) if t is not None]
-    if not rows:
+    if q is None and k is None:
         raise ValueError("q or k must be given")
-    n, _, D = rows[0].shape
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t is None:
-            continue
-        _check_tensor(name, t, torch.bfloat16, (n, None, D))
-        if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or not t.is_cuda:
-            raise ValueError(f"{name} must be a device tensor with contiguous rows of heads")
-    if v is not None and (k is None or k.shape != v.shape):
-        raise ValueError("v needs a k of its shape")
+    n, _, D = (k if q is None else q).shape
     for w in getattr(prologue, "weights", ()):
-        if w is not None and w.numel() != D:
-            raise ValueError(f"a norm weight has {w.numel()} elements; head_dim is {D}")
+        if w is not None and w.shape[0] != D:
+            raise ValueError(f"a norm weight has {w.shape[0]} elements; head_dim is {D}")
+    q_heads, q_ptr, q_stride = _head_rows("q", q, n, D)
+    k_heads, k_ptr, k_stride = _head_rows("k", k, n, D)
+    v_heads, v_ptr, v_stride = _head_rows("v", v, n, D)
+    if v is not None and v_heads != k_heads:
+        raise ValueError("v needs a k of its shape")
     if positions is not None:
-        shape = (n,) if prologue.n_axes == 1 and positions.dim() == 1 else (prologue.n_axes, n)
-        _check_tensor("positions", positions, torch.int32, shape)
+        axes = prologue.n_axes
+        _check_tensor("positions", positions, torch.int32,
+                      (n,) if axes == 1 and positions.dim() == 1 else (axes, n))
     like = (q, k, k if prologue.v_from_k else v)
     if out is None:
-        out = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in like]
-    for t, o in zip(like, out):
-        if (t is None) != (o is None):
-            raise ValueError("out must have a tensor for each output")
-        if t is not None:
-            _check_tensor("out", o, torch.bfloat16, tuple(t.shape))
-
-    def at(t):  # (a token's stride; one token: none)
-        return (None, 0) if t is None else (t.data_ptr(), t.stride(0) if n > 1 else t.shape[1] * D)
-
+        out = tuple(None if t is None else t.new_empty(t.shape) for t in like)
+    else:
+        for t, o in zip(like, out):
+            if (t is None) != (o is None):
+                raise ValueError("out must have a tensor for each output")
+            if t is not None:
+                _check_tensor("out", o, torch.bfloat16, tuple(t.shape))
+        out = tuple(out)
     _check(load_library().fmkv_qkv_norm_rope(
-        ctypes.byref(prologue), D, 0 if q is None else q.shape[1], 0 if k is None else k.shape[1], n,
-        *at(q), *at(k), *at(v), _ptr(positions), *(_ptr(o) for o in out), _stream(stream)))
-    return tuple(out)
+        ctypes.byref(prologue), D, q_heads, k_heads, n, q_ptr, q_stride, k_ptr, k_stride, v_ptr,
+        v_stride, _ptr(positions), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _stream(stream)))
+    return out
+
+
+def _head_rows(name: str, t, n: int, D: int):
+    """(heads, address, elements from token to token) of rows [n, heads, D]."""
+    if t is None:
+        return 0, None, 0
+    heads = _check_tensor(name, t, torch.bfloat16, (n, None, D))[1]
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s1 != D and heads > 1) or not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor with contiguous rows of heads")
+    return heads, t.data_ptr(), s0 if n > 1 else heads * D
 
 
 class PageBook:
@@ -911,18 +909,23 @@ class _Storage:
                                          "typestr": "|u1", "strides": None, "version": 2}
 
 
-def _check_tensor(name: str, t: torch.Tensor, dtype, shape) -> None:
-    """Type, shape (None: any extent) of an argument that the library takes as
-    a bare pointer."""
-    if t.dtype != dtype or t.dim() != len(shape) or any(
-            want is not None and have != want for have, want in zip(t.shape, shape)):
-        want = ", ".join("*" if x is None else str(x) for x in shape)
-        raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {tuple(t.shape)}")
+def _check_tensor(name: str, t: torch.Tensor, dtype, shape):
+    """Type and shape (None: any extent) of an argument that the library takes as
+    a bare pointer; its shape."""
+    have = t.shape
+    if t.dtype is dtype and len(have) == len(shape):
+        for n, want in zip(have, shape):
+            if n != want and want is not None:
+                break
+        else:
+            return have
+    want = ", ".join("*" if x is None else str(x) for x in shape)
+    raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {tuple(have)}")
 
 
 def _out(out, like: torch.Tensor, dtype) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=dtype, device=like.device)
+        return torch.empty_like(like) if dtype is like.dtype else torch.empty_like(like, dtype=dtype)
     if out.shape != like.shape:
         raise ValueError(f"out must have the shape {tuple(like.shape)}, got {tuple(out.shape)}")
     return out
