@@ -675,7 +675,8 @@ int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
 // `rows` (sequence, KV head) pairs. A split costs its blocks and a fixed part (q
 // table, merge of its streams: about 12 blocks' time, 3 of the plain kernel's),
 // each round of work-groups that the chip takes at once costs the longest split
-// in it, and every split a tenth of a block in the combine. So the splits of
+// in it, every split a tenth of a block in the combine, and the combine's launch
+// as much as the fixed part (one split a sequence has none). So the splits of
 // each number of rounds are as many as fit it, or as the combine allows, and
 // equal; the cheapest wins. (us per call, by blocks per split: one sequence,
 // 66 blocks of 4 bits, 256 dims, 8 heads: 1: 20.1, 2: 15.4, 3: 10.9, 8: 11.0, 16:
@@ -698,12 +699,18 @@ int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows
     for (int64_t r = r0; r < r0 + 4; r++) {
       const int64_t s = std::clamp<int64_t>(r * slots / rows, 1, std::min(few, nblk));
       const int64_t b = std::max((nblk + s - 1) / s, min_bps), n = (nblk + b - 1) / b;
-      const double c = (double)((n * rows + slots - 1) / slots) * ((double)b + fixed) + 0.1 * (double)n;
+      const double c = (double)((n * rows + slots - 1) / slots) * ((double)b + fixed) + 0.1 * (double)n +
+                       (n > 1 || new_col ? fixed : 0.0);
       if (bps == 0 || c < cost) bps = b, cost = c;
     }
     return bps;
   };
-  if (paged_solo_slots(d) == 1) return best(plain ? 2 : 1, 1);
+  // (the plain kernel's registers: five work-groups a CU, at 512 dims three, of
+  // which two are counted: 32 sequences of 66 blocks, 8 heads of 256 dims: five
+  // splits 57.2 us, two 64.8; 64 sequences, 2 heads of 512 dims: four splits 66.0,
+  // six 70.4)
+  if (plain) return best(d.head_dim == 512 ? 2 : 5, 1);
+  if (paged_solo_slots(d) == 1) return best(1, 1);
   // wave pairs, one work-group per CU, while a round of them is enough; else
   // single-wave streams, three per CU
   const int64_t pairs = best(1, 1);
