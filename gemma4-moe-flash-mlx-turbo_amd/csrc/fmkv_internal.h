@@ -169,6 +169,12 @@ struct PrefillArgs {
   // A paged pool's window (`window` > 0, ring_slots 0) and the positions at a
   // sequence's start that every query sees besides.
   int32_t sinks = 0;
+  // A window's call of more work-groups than run at once: those from tail_from on
+  // (counted tile by tile, KV head by KV head, sequence by sequence), which would
+  // leave most of the chip idle at the end, are split into tail_ranges ranges of
+  // keys each (0: none).
+  int32_t tail_ranges = 0;
+  uint32_t tail_from = 0;
 };
 
 struct ReadArgs {

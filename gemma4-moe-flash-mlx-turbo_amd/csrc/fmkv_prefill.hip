@@ -84,6 +84,7 @@
 // positions early queries still need), the rest from new_st (a staging
 // copy of the chunk, or the cache itself for linear caches). A block that
 // straddles p_split is visited once per store with the other part masked.
+#include <algorithm>
 #include <type_traits>
 
 #include "fmkv_device.h"
@@ -336,14 +337,26 @@ void prefill_attn_kernel(PrefillArgs a) {
   auto pos_of = [&](int r) __attribute__((always_inline)) {  // r / G for rows r < 64, G <= 64
     return (int)((uint32_t)r * g_inv >> 16);
   };
-  const int kvh = blockIdx.y;
+  int kvh = blockIdx.y, tile = blockIdx.x;
   int seq = blockIdx.z, range = 0, ranges = 1;
-  if (a.units > 0) {
+  if (WIN && a.tail_ranges > 0) {  // grid x counts work-groups
+    uint32_t w = blockIdx.x;
+    if (w >= a.tail_from) {
+      const uint32_t u = w - a.tail_from, t = u / (uint32_t)a.tail_ranges;
+      ranges = a.tail_ranges;
+      range = (int)(u - t * (uint32_t)a.tail_ranges);
+      w = a.tail_from + t;
+    }
+    const uint32_t tiles = (uint32_t)((a.n_q + QP - 1) / QP), th = w / tiles;
+    tile = (int)(w - th * tiles);
+    seq = (int)(th / (uint32_t)a.new_st.n_kv_heads);
+    kvh = (int)(th - (uint32_t)seq * (uint32_t)a.new_st.n_kv_heads);
+  } else if (a.units > 0) {
     const PrefillUnit un = prefill_unit(a, blockIdx.z, 0, lane);
     if (un.seq < 0) return;
     seq = un.seq, range = (int)blockIdx.z - un.first, ranges = un.ranges;
   }
-  const int qi0 = blockIdx.x * QP;
+  const int qi0 = tile * QP;
   // paged: the sequence's start, through a scalar load (everything derived
   // from it stays in scalar registers)
   const int64_t p0 = a.start_pos ? (int64_t)((cint_ptr)(uintptr_t)a.start_pos)[seq] : a.p0;
@@ -1232,7 +1245,9 @@ void prefill_attn_kernel(PrefillArgs a) {
   __syncthreads();
   if (ranges > 1) {  // partial rows, as accumulated, with their (m, l)
     const int64_t slot =
-        (((int64_t)blockIdx.z * gridDim.y + kvh) * gridDim.x + blockIdx.x) * kPfRows;
+        (WIN && a.tail_ranges > 0 ? (int64_t)(blockIdx.x - a.tail_from)
+                                  : ((int64_t)blockIdx.z * gridDim.y + kvh) * gridDim.x + blockIdx.x) *
+        kPfRows;
 #pragma unroll 2
     for (int k = 0; k < kPfRows / NW; k++) {
       const int r = wave + NW * k;
@@ -1285,21 +1300,36 @@ template <int D, bool ROT>
 __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int tiles) {
   constexpr int E = D / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int seq = blockIdx.z, kvh = blockIdx.y;
-  const int tile = blockIdx.x / (kPfRows / kPfMergeRows);
+  int seq = blockIdx.z, kvh = blockIdx.y;
+  int tile = blockIdx.x / (kPfRows / kPfMergeRows);
   const int r0 = (blockIdx.x % (kPfRows / kPfMergeRows)) * kPfMergeRows;
-  const PrefillUnit un = prefill_unit(a, -1, seq, lane);
-  if (un.ranges <= 1) return;
+  // the rows' first partial, from one range's to the next, ranges
+  int64_t row, step;
+  int ranges;
+  if (a.tail_ranges > 0) {  // grid x counts the work-groups that were split
+    ranges = a.tail_ranges;
+    row = (int64_t)tile * ranges * kPfRows;
+    step = kPfRows;
+    const uint32_t w = a.tail_from + (uint32_t)tile, th = w / (uint32_t)tiles;
+    tile = (int)(w - th * (uint32_t)tiles);
+    seq = (int)(th / (uint32_t)a.new_st.n_kv_heads);
+    kvh = (int)(th - (uint32_t)seq * (uint32_t)a.new_st.n_kv_heads);
+  } else {
+    const PrefillUnit un = prefill_unit(a, -1, seq, lane);
+    if (un.ranges <= 1) return;
+    ranges = un.ranges;
+    row = (((int64_t)un.first * gridDim.y + kvh) * tiles + tile) * kPfRows;
+    step = (int64_t)gridDim.y * tiles * kPfRows;
+  }
   const int G = a.group, QP = kPfRows / G;
   const int nq = a.n_q - tile * QP < QP ? a.n_q - tile * QP : QP;
   const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
   const float cs = ROT ? fwht_lane_sign(lane) * a.c : 1.0f;
   const int r = r0 + wave, rq = r / G, rh = r - rq * G;
   if (rq >= nq) return;
-  const int64_t step = (int64_t)gridDim.y * tiles * kPfRows;  // rows from range to range
-  const int64_t row = (((int64_t)un.first * gridDim.y + kvh) * tiles + tile) * kPfRows + r;
+  row += r;
   float M = -1e30f;
-  for (int k = lane; k < un.ranges; k += 64) M = fmaxf(M, a.part_ml[(row + k * step) * 2]);
+  for (int k = lane; k < ranges; k += 64) M = fmaxf(M, a.part_ml[(row + k * step) * 2]);
   M = group_max<64>(M, lane);
   float x[E], l = 0.0f;
 #pragma unroll
@@ -1307,7 +1337,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int t
   // (ranges whose loads are in flight together; 4 of 512 dims ran slower)
   constexpr int kAhead = D == 512 ? 2 : 4;
 #pragma unroll kAhead
-  for (int k = 0; k < un.ranges; k++) {
+  for (int k = 0; k < ranges; k++) {
     const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (row + k * step) * 2);
     const float w = __builtin_amdgcn_exp2f(ml.x - M);
     const float* src = a.part_o + (row + k * step) * D + lane * E;
@@ -1330,10 +1360,13 @@ template <int D, int BITS, int MODE, int RW, bool WIN>
 hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   const int qp = kPfRows / a.group;
   const int tiles = (a.n_q + qp - 1) / qp, H = a.new_st.n_kv_heads;
+  const unsigned split = a.tail_ranges > 0 ? (unsigned)tiles * H * a.n_seqs - a.tail_from : 0;
   dim3 grid(tiles, H, a.units > 0 ? a.units : a.n_seqs);
+  if (split) grid = dim3(a.tail_from + split * a.tail_ranges);
   hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, WIN>), grid, dim3(D * RW), 0, s, a);
-  if (a.units > 0) {
+  if (a.units > 0 || split) {
     dim3 mgrid(tiles * (kPfRows / kPfMergeRows), H, a.n_seqs);
+    if (split) mgrid = dim3(split * (kPfRows / kPfMergeRows));
     hipLaunchKernelGGL((prefill_merge_kernel<D, MODE != kPlain>), mgrid, dim3(256), 0, s, a, tiles);
   }
   return hipGetLastError();
@@ -1405,12 +1438,35 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
   may_split = may_split && a.n_seqs <= 64;
   const bool few = !may_split || max_steps < kPfFewSteps;
   a.units = 0;
+  a.tail_ranges = 0;
   a.share_rows = D < 512 && total <= (!few ? cus / 4 : D == 128 ? cus : cus / 2);
   const int64_t places = prefill_places(D, a.share_rows, cus);
   const int mean = a.n_q / (2 * kPfKeys);  // steps that a row has less than the last, on average
   a.min_split = D == 512 || (total <= cus && !(few && a.share_rows)) ? 8
                 : total <= cus / 4                                   ? 9 + mean
                                                                      : (int)(5 + 16 * total / cus) + mean;
+  // A window's call of more work-groups than run at once: the last round's are
+  // split over their keys where that fills the chip, and the round ends sooner by
+  // the steps saved (all tiles see about a window), less the rotations of the
+  // ranges' rows and the merge: 12 steps, 24 of 512 dims. Four 333-token chunks
+  // (336 work-groups), window 2000, 8 bits, 512 dims: 241 us, unsplit 271; a
+  // 2500-token chunk, window 1024, 4 bits, 256 dims (632): 169, unsplit 198. At
+  // head_dim 128 four work-groups a CU do run unless their LDS is the 3-bit
+  // codebook's (4 x 2048 tokens, 1024 work-groups, bf16: 135; counted as three a
+  // CU and split 168).
+  if (may_split && a.window > 0 && a.ring_slots == 0) {
+    const BlockLayout& L = a.new_st.layout;
+    const int64_t once =
+        D == 128 && !a.share_rows && !(L.mode == kCodebook && L.bits == 3) ? 4 * (int64_t)cus : places;
+    if (total > once && total <= (1 << 24)) {
+      const int64_t rem = total % once;
+      const int64_t ranges = rem > 0 ? std::min(places / rem, max_steps / (2 * kPfMinSteps)) : 0;
+      if (ranges < 2 || max_steps - max_steps / ranges < (D == 512 ? 24 : 12)) return 0;
+      a.tail_ranges = (int32_t)ranges;
+      a.tail_from = (uint32_t)(total - rem);
+      return prefill_part_bytes(rem * ranges, D);
+    }
+  }
   if (!may_split || max_steps < a.min_split) return 0;
   int64_t units = places / wgs;
   const int64_t most = a.n_seqs * ((max_steps + kPfMinSteps - 1) / kPfMinSteps);

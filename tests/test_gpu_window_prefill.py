@@ -105,3 +105,32 @@ def test_one_query_is_the_decode_call(gpu, ora):
                                     dtype=torch.float32)
         torch.cuda.synchronize()
         check_window(a[:, 0], b.double().cpu().numpy(), 12.0)
+
+
+@pytest.mark.parametrize("mode,D,bits,Hkv,Hq,n", [(AFFINE, 512, 8, 2, 16, 333), (PLAIN, 128, 16, 4, 32, 600),
+                                                  (CODEBOOK, 256, 3, 4, 32, 300), (AFFINE, 256, 4, 4, 32, 300)])
+def test_window_prefill_tail(gpu, ora, mode, D, bits, Hkv, Hq, n):
+    """More work-groups than run at once: the last ones' keys are split (eager
+    calls) or not (captured ones)."""
+    import torch
+
+    start, window, sinks = [900, 1000, 40, 700], 1000, 21
+    p = Paged(gpu, ora, mode, D, bits, Hkv, [x + n for x in start])
+    q = np.stack([queries(4 + s, n, Hq, Hkv, D) for s in range(len(start))])
+    qd, table, first = dev_bf16(q), p.table(), p.lens_dev(start)
+
+    def call(out):
+        return p.pool.window_prefill(qd, table, first, window, sinks, D ** -0.5, out=out)
+
+    eager = call(torch.empty(qd.shape, dtype=torch.float32, device="cuda"))
+    again = call(torch.empty(qd.shape, dtype=torch.float32, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(eager, again)
+    check(ora, p, eager, q, start, window, sinks, D ** -0.5, rows=(0, 1, n // 2, n - 9, n - 1))
+    held = torch.zeros_like(eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(held)
+    graph.replay()
+    torch.cuda.synchronize()
+    check_window(held, eager.double().cpu().numpy(), 12.0, "captured")
