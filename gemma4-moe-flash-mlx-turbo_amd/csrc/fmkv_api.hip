@@ -735,6 +735,7 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   a->window = 0;
   a->vis_begin = 0;
   if (win > 0) {
+    if (n_seqs == 0) return FMKV_OK;
     int rc = check_attn_args(p->desc, q, n_q_heads, tau, out, out_dtype);
     if (rc || (rc = check_device(p))) return rc;
   }

@@ -16,6 +16,7 @@ missing.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from dataclasses import dataclass
@@ -252,6 +253,28 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     if not t.is_contiguous():
         raise ValueError("fmkv needs contiguous tensors")
     return t.data_ptr()
+
+
+def _here(t: torch.Tensor | None, device: int) -> int | None:
+    """_ptr of a tensor that has to be on GPU `device`."""
+    if t is None:
+        return None
+    if t.get_device() != device:
+        raise ValueError(f"fmkv needs tensors on cuda:{device}, got one on {t.device}")
+    if not t.is_contiguous():
+        raise ValueError("fmkv needs contiguous tensors")
+    return t.data_ptr()
+
+
+def _on(stream):
+    """Where an output is allocated that a call on `stream` writes (None: the
+    current stream), so that torch does not reuse memory that another stream
+    still works on."""
+    if stream is None:
+        return contextlib.nullcontext()
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream))
+    return torch.cuda.stream(stream)
 
 
 def _stream(stream) -> int | None:
@@ -579,6 +602,7 @@ class PagedPool:
         h = ctypes.c_void_p()
         _check(self._lib.fmkv_pool_create(ctypes.byref(desc), n_blocks, ctypes.byref(h)))
         self._h = h
+        self._device = torch.cuda.current_device()
 
     def close(self) -> None:
         if getattr(self, "_h", None):
@@ -678,10 +702,12 @@ class PagedPool:
         n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
-        out = _out(out, q, dtype)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_attention(
-            self._h, _ptr(q), _ptr(block_tables), width, _ptr(seq_lens), n, max_seq_len, heads, scale,
-            window, sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+            self._h, _here(q, dev), _here(block_tables, dev), width, _here(seq_lens, dev), n,
+            max_seq_len, heads, scale, window, sinks, _here(out, dev), _dtype_code(out.dtype),
+            _stream(stream)))
         return out
 
     def window_decode_step(self, keys, values, block_tables, start_pos, seq_lens, max_seq_len: int,
@@ -696,11 +722,12 @@ class PagedPool:
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
-        out = _out(out, q, dtype)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_step(
-            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), width, _ptr(start_pos),
-            _ptr(seq_lens), n, max_seq_len, _ptr(q), heads, scale, window, sinks, _ptr(out),
-            _dtype_code(out.dtype), _stream(stream)))
+            self._h, _here(keys, dev), _here(values, dev), _here(block_tables, dev), width,
+            _here(start_pos, dev), _here(seq_lens, dev), n, max_seq_len, _here(q, dev), heads,
+            scale, window, sinks, _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def window_prefill(self, q, block_tables, start_pos, window: int, sinks: int = 0,
@@ -713,10 +740,12 @@ class PagedPool:
         n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
-        out = _out(out, q, dtype)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_attention(
-            self._h, _ptr(q), _ptr(block_tables), width, _ptr(start_pos), n, n_new, max_seq_len, heads,
-            scale, window, sinks, _ptr(out), _dtype_code(out.dtype), _stream(stream)))
+            self._h, _here(q, dev), _here(block_tables, dev), width, _here(start_pos, dev), n,
+            n_new, max_seq_len, heads, scale, window, sinks, _here(out, dev),
+            _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def window_prefill_step(self, keys, values, block_tables, start_pos, q, window: int,
@@ -729,11 +758,12 @@ class PagedPool:
         _check_tensor("values", values, torch.bfloat16, (n, n_new, self._H, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
-        out = _out(out, q, dtype)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_step(
-            self._h, _ptr(keys), _ptr(values), _ptr(block_tables), width, _ptr(start_pos), n, n_new,
-            max_seq_len, _ptr(q), heads, scale, window, sinks, _ptr(out), _dtype_code(out.dtype),
-            _stream(stream)))
+            self._h, _here(keys, dev), _here(values, dev), _here(block_tables, dev), width,
+            _here(start_pos, dev), n, n_new, max_seq_len, _here(q, dev), heads, scale, window, sinks,
+            _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
         return out
 
     def compact(self, block_tables, keep, n_keep, dst_tables, stream=None) -> None:
@@ -746,18 +776,21 @@ class PagedPool:
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         dst_width = _check_tensor("dst_tables", dst_tables, torch.int32, (n, None))[1]
         _check_tensor("n_keep", n_keep, torch.int32, (n,))
+        dev = self._device
         _check(self._lib.fmkv_paged_compact(
-            self._h, _ptr(block_tables), width, _ptr(keep), most, _ptr(n_keep), _ptr(dst_tables),
-            dst_width, n, _stream(stream)))
+            self._h, _here(block_tables, dev), width, _here(keep, dev), most, _here(n_keep, dev),
+            _here(dst_tables, dev), dst_width, n, _stream(stream)))
 
     def storage(self) -> torch.Tensor:
         """The pool's blocks as a uint8 tensor [n_blocks, n_kv_heads, bytes of a
-        head-block] over the pool's own memory (which it keeps alive): to move
-        blocks to other pools of the same description or to the host and back."""
+        head-block] over the pool's own memory (which it keeps alive, unless
+        close() ends it): to move blocks to other pools of the same description
+        or to the host and back."""
         base, size = ctypes.c_void_p(), ctypes.c_int64()
         _check(self._lib.fmkv_pool_storage(self._h, ctypes.byref(base), ctypes.byref(size)))
         return torch.as_tensor(_Storage(self, base.value, (
-            self.n_blocks, self.desc.n_kv_heads, size.value // self.desc.n_kv_heads)), device="cuda")
+            self.n_blocks, self.desc.n_kv_heads, size.value // self.desc.n_kv_heads)),
+            device=f"cuda:{self._device}")
 
     def read_codes(self, stream=None):
         return _read_codes(self._lib.fmkv_pool_read_codes, self._h, self.desc,
@@ -771,9 +804,10 @@ def copy_blocks(pools, src, dst, stream=None) -> None:
     pools = list(pools)
     _check_tensor("src", src, torch.int32, (None,))
     _check_tensor("dst", dst, torch.int32, (src.shape[0],))
+    dev = torch.cuda.current_device()
     handles = (ctypes.c_void_p * max(len(pools), 1))(*[p._h for p in pools])
-    _check(load_library().fmkv_pools_copy_blocks(handles, len(pools), _ptr(src), _ptr(dst),
-                                                 src.shape[0], _stream(stream)))
+    _check(load_library().fmkv_pools_copy_blocks(handles, len(pools), _here(src, dev),
+                                                 _here(dst, dev), src.shape[0], _stream(stream)))
 
 
 def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=None):
@@ -787,13 +821,14 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
     from k). out: the three outputs, which may be the inputs themselves."""
     if q is None and k is None:
         raise ValueError("q or k must be given")
+    dev = torch.cuda.current_device()
     n, _, D = (k if q is None else q).shape
     for w in getattr(prologue, "weights", ()):
         if w is not None and w.shape[0] != D:
             raise ValueError(f"a norm weight has {w.shape[0]} elements; head_dim is {D}")
-    q_heads, q_ptr, q_stride = _head_rows("q", q, n, D)
-    k_heads, k_ptr, k_stride = _head_rows("k", k, n, D)
-    v_heads, v_ptr, v_stride = _head_rows("v", v, n, D)
+    q_heads, q_ptr, q_stride = _head_rows("q", q, n, D, dev)
+    k_heads, k_ptr, k_stride = _head_rows("k", k, n, D, dev)
+    v_heads, v_ptr, v_stride = _head_rows("v", v, n, D, dev)
     if v is not None and v_heads != k_heads:
         raise ValueError("v needs a k of its shape")
     if positions is not None:
@@ -802,7 +837,8 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
                       (n,) if axes == 1 and positions.dim() == 1 else (axes, n))
     like = (q, k, k if prologue.v_from_k else v)
     if out is None:
-        out = tuple(None if t is None else t.new_empty(t.shape) for t in like)
+        with _on(stream):
+            out = tuple(None if t is None else t.new_empty(t.shape) for t in like)
     else:
         for t, o in zip(like, out):
             if (t is None) != (o is None):
@@ -810,20 +846,23 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
             if t is not None:
                 _check_tensor("out", o, torch.bfloat16, tuple(t.shape))
         out = tuple(out)
+    if n == 0:
+        return out
     _check(load_library().fmkv_qkv_norm_rope(
         ctypes.byref(prologue), D, q_heads, k_heads, n, q_ptr, q_stride, k_ptr, k_stride, v_ptr,
-        v_stride, _ptr(positions), _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _stream(stream)))
+        v_stride, _here(positions, dev), _here(out[0], dev), _here(out[1], dev), _here(out[2], dev),
+        _stream(stream)))
     return out
 
 
-def _head_rows(name: str, t, n: int, D: int):
+def _head_rows(name: str, t, n: int, D: int, dev: int):
     """(heads, address, elements from token to token) of rows [n, heads, D]."""
     if t is None:
         return 0, None, 0
     heads = _check_tensor(name, t, torch.bfloat16, (n, None, D))[1]
     s0, s1, s2 = t.stride()
-    if s2 != 1 or (s1 != D and heads > 1) or not t.is_cuda:
-        raise ValueError(f"{name} must be a device tensor with contiguous rows of heads")
+    if s2 != 1 or (s1 != D and heads > 1) or t.get_device() != dev:
+        raise ValueError(f"{name} must be on the current GPU, with contiguous rows of heads")
     return heads, t.data_ptr(), s0 if n > 1 else heads * D
 
 
@@ -923,9 +962,12 @@ def _check_tensor(name: str, t: torch.Tensor, dtype, shape):
     raise ValueError(f"{name} must be {dtype} [{want}], got {t.dtype} {tuple(have)}")
 
 
-def _out(out, like: torch.Tensor, dtype) -> torch.Tensor:
+def _out(out, like: torch.Tensor, dtype, stream) -> torch.Tensor:
     if out is None:
-        return torch.empty_like(like) if dtype is like.dtype else torch.empty_like(like, dtype=dtype)
+        if stream is None:
+            return torch.empty_like(like, dtype=dtype)
+        with _on(stream):
+            return torch.empty_like(like, dtype=dtype)
     if out.shape != like.shape:
         raise ValueError(f"out must have the shape {tuple(like.shape)}, got {tuple(out.shape)}")
     return out

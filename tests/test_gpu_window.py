@@ -134,6 +134,88 @@ def test_window_attention_bad_pages(gpu, ora):
     check_window(out[1], window_reference(ora, p.oracles[1], q[1], 199, window, sinks, 0.05), 6.0)
 
 
+def test_window_step_of_a_padded_batch(gpu, ora):
+    """Rows of length 0 (and below) write no slot and get zeros; an empty batch is
+    no call."""
+    import torch
+
+    mode, D, bits, Hkv, Hq = CONFIGS[0]
+    p = Paged(gpu, ora, mode, D, bits, Hkv, [50, 40, 30], room=2)
+    before = p.pool.storage().clone()
+    k, v = (dev_bf16(fast_kv(s, 3, Hkv, D, outliers=False))[:, None].contiguous() for s in (1, 2))
+    q = queries(3, 3, Hq, Hkv, D)
+    out = p.pool.window_decode_step(k, v, p.table(), p.lens_dev([50, -1, -6]), p.lens_dev([51, 0, -5]), 51,
+                                    dev_bf16(q), 20, 3, 0.06, dtype=torch.float32)
+    torch.cuda.synchronize()
+    p.oracles[0].append(fast_kv(1, 3, Hkv, D, outliers=False)[:1], fast_kv(2, 3, Hkv, D, outliers=False)[:1])
+    check_window(out[0], window_reference(ora, p.oracles[0], q[0], 50, 20, 3, 0.06), 6.0)
+    assert bool((out[1:] == 0).all())
+    blocks = torch.arange(p.n_blocks) != int(p.tables[0, 50 // 16])
+    assert torch.equal(p.pool.storage()[blocks], before[blocks])
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    empty = p.pool.window_attention(torch.zeros((0, Hq, D), dtype=torch.bfloat16, device="cuda"),
+                                    torch.zeros((0, 4), dtype=torch.int32, device="cuda"), none, 64, 20)
+    assert empty.shape == (0, Hq, D)
+
+
+def test_window_first_call_captured_and_other_stream(gpu, ora):
+    """A capture that is a pool's first call allocates its workspace; a stream
+    given to the call is the one it runs on."""
+    import torch
+
+    mode, D, bits, Hkv, Hq = CONFIGS[2]
+    lens = [900, 333]
+    p = Paged(gpu, ora, mode, D, bits, Hkv, lens)
+    q = dev_bf16(np.stack([queries(5 + s, 1, Hq, Hkv, D)[0] for s in range(2)]))
+    table, n = p.table(), p.lens_dev()
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.pool.window_attention(q, table, n, 900, 500, 4, 0.05, out=out)
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        want = p.pool.window_attention(q, table, n, 900, 500, 4, 0.05, stream=side)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("mode,D,bits,Hkv,Hq", [CONFIGS[2], CONFIGS[7], CONFIGS[11]])
+def test_pages_past_4_gib(gpu, ora, mode, D, bits, Hkv, Hq):
+    """A pool of more than 4 GiB whose last pages hold the sequence: attention, a
+    chunk, copied blocks and kept tokens as in a small pool."""
+    import torch
+
+    n, window, sinks = 150, 60, 5
+    small = Paged(gpu, ora, mode, D, bits, Hkv, [n], spare=40, dirty=False)
+    size = small.pool.storage()[0].numel()
+    big = gpu.PagedPool(gpu.make_desc(Hkv, D, bits, mode=mode), (9 << 29) // size + 64)
+    off = big.n_blocks - small.n_blocks
+    big.storage()[off:].copy_(small.pool.storage())
+    q = dev_bf16(queries(3, 4, Hq, Hkv, D))
+    keep = torch.arange(0, n, 3, dtype=torch.int32, device="cuda")[None]
+    count = torch.tensor([keep.shape[1]], dtype=torch.int32, device="cuda")
+    spare = torch.from_numpy(small.spare.astype(np.int32)).cuda()
+    outs = []
+    for pool, base in ((small.pool, 0), (big, off)):
+        table = small.table() + base
+        one = pool.window_attention(q[:1], table, small.lens_dev(), n, window, sinks, 0.05)
+        four = pool.window_prefill(q[None], table, small.lens_dev([n - 4]), window, sinks, 0.05)
+        gpu.copy_blocks([pool], table[0, :4].contiguous(), spare[:4] + base)
+        dst = (spare[8:8 + 4] + base)[None].contiguous()
+        pool.compact(table, keep, count, dst)
+        full = pool.window_attention(q[:1], dst, count, 64, 1000, 0, 0.05)
+        moved = pool.window_attention(q[:1], (spare[:4] + base)[None].contiguous(), small.lens_dev([64]), 64, 1000, 0,
+                                      0.05)
+        outs.append((one, four, full, moved))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert torch.equal(small.pool.storage(), big.storage()[off:])
+
+
 def test_window_step_graph(gpu, ora):
     """A captured step replayed as its inputs change, with eager calls between
     that need a larger workspace and with another stream: bit for bit the eager
