@@ -310,18 +310,7 @@ __device__ inline PrefillUnit prefill_unit(const PrefillArgs& a, int u, int seq,
 // <= p with j > p - window or j < sinks. The sinks' blocks take the place of
 // the old store's, in the pool itself, and the blocks between them and the
 // window, whose pages a server may have given back, are never looked up.
-// LEAN: a window's bf16 outputs weigh V with f16 weights alone (11 bits, the
-// product with V's scale rounded once more: 2^-10 of the weighted sum of |V| at
-// most; with errors of either sign, a sixteenth on top of the squared error of
-// the output's own rounding to 8 bits); the residuals are for f32 outputs. It saves a quarter
-// of the matrix instructions and half the weights' arithmetic: 2048 tokens, 4
-// bits, 256 dims, window 1024: 111 us, with residuals 123; four 333-token chunks,
-// 8 bits, 512 dims, window 2000: 217 and 241. Not where the high part is no f16
-// of the whole: plain caches (bf16, 8 bits) and the 4-bit codebook (norms
-// without a bound).
-template <int BITS, int MODE>
-constexpr bool kMayLean = MODE == kAffine || (MODE == kCodebook && kCbExact<BITS == 16 ? 2 : BITS>);
-template <int D, int BITS, int MODE, int RW, bool WIN, bool LEAN>
+template <int D, int BITS, int MODE, int RW, bool WIN>
 __global__ __launch_bounds__(D * RW)  // RW waves per 64 dims
 __attribute__((amdgpu_waves_per_eu(RW == 4 ? 4 : 2, RW == 4 ? 4 : 2)))
 void prefill_attn_kernel(PrefillArgs a) {
@@ -936,7 +925,7 @@ void prefill_attn_kernel(PrefillArgs a) {
               rest[i] = x - (float)h[i];
             } else {
               h[i] = (_Float16)x;
-              r[i] = LEAN ? (_Float16)0.0f : (_Float16)(x - (float)h[i]);
+              r[i] = (_Float16)(x - (float)h[i]);
             }
           }
           if constexpr (MODE == kCodebook && !kCbExact<CB>)
@@ -1026,9 +1015,8 @@ void prefill_attn_kernel(PrefillArgs a) {
           const half2_t ph = __builtin_bit_cast(half2_t, e < 2 ? w0[e] : w1[e - 2]);
           const half2_t pl = __builtin_bit_cast(half2_t, e < 2 ? w0[e + 2] : w1[e]);
           half2_t h = ph * vsc[e];
-          half2_t l = (half2_t){(_Float16)0.0f, (_Float16)0.0f};
-          if constexpr (!LEAN)
-            l = __builtin_elementwise_fma(pl, vsc[e], __builtin_elementwise_fma(ph, vsc[e], -h));
+          half2_t l = __builtin_elementwise_fma(
+              pl, vsc[e], __builtin_elementwise_fma(ph, vsc[e], -h));
           if constexpr (decltype(hide)::value) {
             const float x0 = ((float)ph[0] + (float)pl[0]) * (float)vsc[e][0];
             const float x1 = ((float)ph[1] + (float)pl[1]) * (float)vsc[e][1];
@@ -1039,7 +1027,7 @@ void prefill_attn_kernel(PrefillArgs a) {
           bh[2 * e + 1] = h[1];
           bl[2 * e] = l[0];
           bl[2 * e + 1] = l[1];
-          if constexpr (!LEAN) bacc[rt] = __builtin_amdgcn_fdot2(pl, vbi[e], bacc[rt], false);
+          bacc[rt] = __builtin_amdgcn_fdot2(pl, vbi[e], bacc[rt], false);
           bacc[rt] = __builtin_amdgcn_fdot2(ph, vbi[e], bacc[rt], false);
         }
         // (here, not sunk past the barrier with every weight and bias kept for it)
@@ -1060,8 +1048,7 @@ void prefill_attn_kernel(PrefillArgs a) {
           o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[ct], bh, o[rt][ct], 0, 0, 0);
           if constexpr (MODE == kCodebook && !kCbExact<CB>)
             o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[ct], bh, o[rt][ct], 0, 0, 0);
-          if constexpr (!LEAN || decltype(hide)::value)
-            o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[ct], bl, o[rt][ct], 0, 0, 0);
+          o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[ct], bl, o[rt][ct], 0, 0, 0);
         }
       }
     }
@@ -1376,10 +1363,7 @@ hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   const unsigned split = a.tail_ranges > 0 ? (unsigned)tiles * H * a.n_seqs - a.tail_from : 0;
   dim3 grid(tiles, H, a.units > 0 ? a.units : a.n_seqs);
   if (split) grid = dim3(a.tail_from + split * a.tail_ranges);
-  const auto kernel = WIN && kMayLean<BITS, MODE> && !a.out_f32
-                          ? prefill_attn_kernel<D, BITS, MODE, RW, WIN, WIN && kMayLean<BITS, MODE>>
-                          : prefill_attn_kernel<D, BITS, MODE, RW, WIN, false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(D * RW), 0, s, a);
+  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, WIN>), grid, dim3(D * RW), 0, s, a);
   if (a.units > 0 || split) {
     dim3 mgrid(tiles * (kPfRows / kPfMergeRows), H, a.n_seqs);
     if (split) mgrid = dim3(split * (kPfRows / kPfMergeRows));

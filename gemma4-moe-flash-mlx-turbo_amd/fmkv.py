@@ -838,7 +838,8 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
     like = (q, k, k if prologue.v_from_k else v)
     if out is None:
         with _on(stream):
-            out = tuple(None if t is None else t.new_empty(t.shape) for t in like)
+            out = tuple(None if t is None else
+                        torch.empty_like(t, memory_format=torch.contiguous_format) for t in like)
     else:
         for t, o in zip(like, out):
             if (t is None) != (o is None):

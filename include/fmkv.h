@@ -368,9 +368,6 @@ int fmkv_paged_window_decode_step(fmkv_pool* pool, const void* k_bf16, const voi
                                   int32_t n_q_heads, float scale, int32_t window, int32_t sinks,
                                   void* out, int32_t out_dtype, void* stream);
 
-/* (bf16 outputs of the two calls below weigh V with f16 weights, off by 2^-10 of
- * the weighted sum of |V| at most, where f32 outputs take about 22 bits.) */
-
 /* n_new consecutive queries per sequence at start_pos .. start_pos + n_new - 1,
  * whose keys and values are in the pool already (fmkv_paged_append or
  * fmkv_paged_append_projected came first). max_seq_len: as

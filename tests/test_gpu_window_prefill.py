@@ -19,8 +19,7 @@ def check(ora, p, out, q, start, window, sinks, scale, rows=None):
     for s, first in enumerate(start):
         for i in range(q.shape[1]) if rows is None else rows:
             ref = window_reference(ora, p.oracles[s], q[s, i], first + i, window, sinks, scale)
-            check_window(out[s, i], ref, 6.0, f"sequence {s} row {i} position {first + i}",
-                         lean="bfloat16" in str(out.dtype))
+            check_window(out[s, i], ref, 6.0, f"sequence {s} row {i} position {first + i}")
 
 
 @pytest.mark.parametrize("mode,D,bits,Hkv,Hq", CONFIGS)

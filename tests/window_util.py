@@ -116,20 +116,16 @@ def window_reference(ora, oc, q, pos, window, sinks, scale):
     return ora.attention_f64(ora.bf16_to_f32(q).astype(np.float64), k, v, None, scale)
 
 
-def check_window(out, ref, vmax, what="", lean=False):
+def check_window(out, ref, vmax, what=""):
     """f32 outputs: scores of soft scales stay below 64 in base 2 and come out of
     at most 32 roundings each, so they are off by 64 * 32 * 2^-24 = 2^-13 at most,
     weights and their sum by ln 2 times that each, and products with weights held
     as pairs of f16 (or bf16) by 2^-16: together below 2^-12 of the largest |V|.
-    bf16 outputs: half a step of their own besides. lean (several queries, bf16
-    outputs): weights rounded to f16, and their products with V's scale again, half
-    a step of 2^-11 each: 2^-10 of the weighted sum of |V|, at most the largest."""
+    bf16 outputs: half a step of their own besides."""
     import torch
 
     o = out.float().cpu().numpy().astype(np.float64)
     allow = 2.0 ** -12 * vmax + (2.0 ** -8 * np.abs(ref) if out.dtype == torch.bfloat16 else 0.0)
-    if lean:
-        allow = allow + 2.0 ** -10 * vmax
     err = np.abs(o - ref)
     bad = ~(err <= allow)  # (a NaN is bad too)
     assert not bad.any(), (f"{what}: {bad.sum()} of {bad.size} off, first at {np.argwhere(bad)[0]}, "
