@@ -5,7 +5,8 @@ pages without visible slots are given back (their table entries lead nowhere).""
 import numpy as np
 import pytest
 
-from gpu_util import check_codes, dev_bf16, fast_kv
+import synth
+from gpu_util import check_attention, check_codes, dev_bf16, fast_kv, kv_batch
 from window_util import AFFINE, CODEBOOK, PLAIN, Paged, check_window, queries, window_reference
 
 pytestmark = pytest.mark.gpu
@@ -255,3 +256,29 @@ def test_window_step_graph(gpu, ora):
         if i == 1:  # a batch that outgrows the workspace that the graph uses
             big = dev_bf16(queries(3, 24, Hq, Hkv, D))
             p.pool.window_attention(big, table[:1].repeat(24, 1), now[:1].repeat(24), 964, 900, 4, 0.06)
+
+
+@pytest.mark.parametrize("mode,D,bits,Hkv,Hq", CONFIGS)
+@pytest.mark.parametrize("scale", [1.0, 0.02])
+def test_window_of_outlier_channels(gpu, ora, mode, D, bits, Hkv, Hq, scale):
+    """K, V and q with channels 20 times the others, at the model's scale and a
+    soft one, both calls: within the 2e-2 that every attention of the library
+    holds (before a bf16 output's own rounding)."""
+    import torch
+
+    n, chunk, window, sinks = 230, 7, 70, 9
+    p = Paged(gpu, ora, mode, D, bits, Hkv, [0], room=n)
+    k, v = kv_batch(1, n, Hkv, D), kv_batch(2, n, Hkv, D)
+    p.oracles[0].append(k, v)
+    p.pool.append(dev_bf16(k[None]), dev_bf16(v[None]), p.table(), p.lens_dev([0]))
+    q = synth.q_rows(3, Hq, Hkv, D, synth.outlier_channels(1, Hkv, D), batch=chunk)
+    for dtype in (torch.float32, torch.bfloat16):
+        some = p.pool.window_prefill(dev_bf16(q[None]), p.table(), p.lens_dev([n - chunk]), window, sinks, scale,
+                                     dtype=dtype)
+        one = p.pool.window_attention(dev_bf16(q[-1:]), p.table(), p.lens_dev([n]), n, window, sinks, scale,
+                                      dtype=dtype)
+        torch.cuda.synchronize()
+        ref = np.stack([window_reference(ora, p.oracles[0], q[i], n - chunk + i, window, sinks, scale)
+                        for i in range(chunk)])
+        check_attention(some[0], ref, f"{dtype} chunk")
+        check_attention(one, ref[-1:], f"{dtype} token")
