@@ -349,7 +349,9 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
  * its workspace, so calls on several streams, and replays of graphs that
  * captured them, have to be ordered by the caller; a workspace that a later,
  * larger call outgrows stays until the pool is destroyed, so captured calls
- * stay valid. */
+ * stay valid. (A captured prefill call is split over its keys too, in that
+ * workspace, unlike fmkv_paged_prefill_step; an eager one uses the GPU's shared
+ * buffer.) */
 
 /* One token per sequence: fmkv_paged_decode_attention over a window. */
 int fmkv_paged_window_decode_attention(fmkv_pool* pool, const void* q_bf16,

@@ -63,8 +63,8 @@ def test_window_prefill_step(gpu, ora, mode, D, bits, Hkv, Hq):
 @pytest.mark.parametrize("mode,D,bits,Hkv,Hq", [CONFIGS[0], CONFIGS[1], CONFIGS[2], CONFIGS[4], CONFIGS[7], CONFIGS[9]])
 @pytest.mark.parametrize("start", [[3000], [2100, 40]])
 def test_window_prefill_split(gpu, ora, mode, D, bits, Hkv, Hq, start):
-    """Few queries over a long window: split over the keys (eager) and unsplit
-    (captured), the sinks' blocks in the first range."""
+    """Few queries over a long window: split over the keys, the sinks' blocks in
+    the first range, eager and (in the pool's workspace) captured."""
     import torch
 
     n, window, sinks = 5, 1500, 100
@@ -87,8 +87,9 @@ def test_window_prefill_split(gpu, ora, mode, D, bits, Hkv, Hq, start):
     for _ in range(3):
         held.zero_()
         graph.replay()
+        call(torch.empty_like(eager))
         torch.cuda.synchronize()
-        check(ora, p, held, q, start, window, sinks, D ** -0.5)
+        assert torch.equal(held, eager)
 
 
 def test_one_query_is_the_decode_call(gpu, ora):
@@ -110,8 +111,7 @@ def test_one_query_is_the_decode_call(gpu, ora):
 @pytest.mark.parametrize("mode,D,bits,Hkv,Hq,n", [(AFFINE, 512, 8, 2, 16, 333), (PLAIN, 128, 16, 4, 32, 600),
                                                   (CODEBOOK, 256, 3, 4, 32, 300), (AFFINE, 256, 4, 4, 32, 300)])
 def test_window_prefill_tail(gpu, ora, mode, D, bits, Hkv, Hq, n):
-    """More work-groups than run at once: the last ones' keys are split (eager
-    calls) or not (captured ones)."""
+    """More work-groups than run at once: the last ones' keys are split."""
     import torch
 
     start, window, sinks = [900, 1000, 40, 700], 1000, 21
@@ -131,6 +131,9 @@ def test_window_prefill_tail(gpu, ora, mode, D, bits, Hkv, Hq, n):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         call(held)
-    graph.replay()
-    torch.cuda.synchronize()
-    check_window(held, eager.double().cpu().numpy(), 12.0, "captured")
+    for _ in range(3):
+        held.zero_()
+        graph.replay()
+        call(again)
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager) and torch.equal(again, eager)
