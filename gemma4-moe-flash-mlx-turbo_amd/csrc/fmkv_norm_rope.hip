@@ -12,6 +12,9 @@
 // sum of squares crosses lanes. A lane's sines and cosines are those of its four
 // pairs, computed once per token and used for every head of it.
 //
+// 8192 tokens of 16 q, 2 k and 2 v rows of 512 dims, 128 of them rotated: 70 us for
+// 336 MB, 4.8 TB/s; 32 tokens of 32 rows of 256 dims: 3.9 us in a graph.
+//
 // Angles: the frequency in turns, theta^(-2i/r) / 2 pi, is held as a fraction
 // of 2^64; times the position modulo 2^64 it is the angle's fraction of a turn
 // to 2^-24 at any 32-bit position, where an angle in 32 bits loses all but a

@@ -60,7 +60,11 @@ __device__ inline T load_at(const uint8_t* block, int64_t at) {
 //   V: a piece holds several tokens of some dims, merged from their sources'.
 // A token that is not there (past the sequence's list, a position or page out of
 // range) leaves its slot as it was; its loads read the block written instead,
-// so that no load waits for a test of another.
+// so that no load waits for a test of another. Few registers (26 to 57) and no
+// loop over blocks: what is in flight comes from the many work-groups of a CU. 8
+// sequences of 3000 to 16000 tokens, every second kept, 8 bits, 2 heads of 512
+// dims: 52 us for 186 MB read (the sources' lines, nearly all) and 83 written, 5.1
+// TB/s; one of 3077 tokens, a third kept, bf16, 4 heads of 128 dims: 3.9 us in a graph.
 template <int MODE, int BITS, int D>
 __global__ __launch_bounds__(kCompactThreads) void compact_kernel(CompactArgs a) {
   constexpr BlockLayout L = make_layout(D, BITS, MODE);
