@@ -200,6 +200,11 @@ struct Workspace {
   // (allocating does not end a capture in this thread's relaxed mode)
   int grow(size_t need) {
     const size_t want = std::max(need, bytes + bytes / 2);
+    try {
+      kept.reserve(kept.size() + 1);
+    } catch (const std::exception&) {
+      return fail(FMKV_ERR_OOM, "no host memory for a workspace");
+    }
     float* p = nullptr;
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     (void)hipThreadExchangeStreamCaptureMode(&mode);
@@ -751,7 +756,10 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   if (win > 0) {
     if (n_seqs == 0) return FMKV_OK;
     int rc = check_attn_args(p->desc, q, n_q_heads, tau, out, out_dtype);
-    if (rc || (rc = check_device(p))) return rc;
+    if (rc) return rc;
+    // (a copy to LDS in pieces of 16 bytes, whose last address bits do not count)
+    if ((uintptr_t)q % 16 != 0) return fail(FMKV_ERR_UNSUPPORTED, "q must be 16-byte aligned");
+    if ((rc = check_device(p))) return rc;
   }
   a->win = win;
   a->sinks = sinks;

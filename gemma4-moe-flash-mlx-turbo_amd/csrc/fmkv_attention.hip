@@ -1281,33 +1281,28 @@ hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t 
   // a paged pool has per-sequence lengths; a cache has neither
   if ((a.st.block_table != nullptr) != (a.seq_lens != nullptr)) return hipErrorInvalidValue;
   if (MODE == kWindow && !a.st.block_table) return hipErrorInvalidValue;
+  // (kWindow is a paged pool's: it has no other instances)
   if constexpr (kSoloCapable<D, BITS>) {
     if (a.bps >= kSoloMinBlocks) {
       // head_dim 256 at 4 bits with at most 2 q heads per KV head (Gemma-4's
       // sliding layers): the packed-column form of the solo streams
-      if constexpr (MODE == kWindow) {
-        if constexpr (D == 256 && BITS == 4)
-          if (a.group <= 2)
-            return launch_kind<D, BITS, MODE, kPagedSoloWaves, true, true>(a, grid, s, ev0, ev1);
-        return launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1);
-      } else {
-      if constexpr (MODE == kDense && D == 256 && BITS == 4) {
+      constexpr bool kPacked = (MODE == kDense || MODE == kWindow) && D == 256 && BITS == 4;
+      if constexpr (MODE != kWindow) {
+        if (!a.st.block_table) {
+          if constexpr (kPacked)
+            if (a.group <= 2) return launch_kind<D, BITS, MODE, 12, false, true>(a, grid, s, ev0, ev1);
+          return launch_kind<D, BITS, MODE, 12, false>(a, grid, s, ev0, ev1);
+        }
+      }
+      if constexpr (kPacked)
         if (a.group <= 2)
-          return a.st.block_table
-                     ? launch_kind<D, BITS, MODE, kPagedSoloWaves, true, true>(a, grid, s, ev0, ev1)
-                     : launch_kind<D, BITS, MODE, 12, false, true>(a, grid, s, ev0, ev1);
-      }
-      return a.st.block_table ? launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1)
-                              : launch_kind<D, BITS, MODE, 12, false>(a, grid, s, ev0, ev1);
-      }
+          return launch_kind<D, BITS, MODE, kPagedSoloWaves, true, true>(a, grid, s, ev0, ev1);
+      return launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1);
     }
   }
-  if constexpr (MODE == kWindow) {
-    return launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1);
-  } else {
-  return a.st.block_table ? launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1)
-                          : launch_kind<D, BITS, MODE, 0, false>(a, grid, s, ev0, ev1);
-  }
+  if constexpr (MODE != kWindow)
+    if (!a.st.block_table) return launch_kind<D, BITS, MODE, 0, false>(a, grid, s, ev0, ev1);
+  return launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1);
 }
 
 template <int D, int BITS>

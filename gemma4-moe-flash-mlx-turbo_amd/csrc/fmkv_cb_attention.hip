@@ -294,9 +294,9 @@ __device__ void cb_new_token_column(const AttnArgs& a, uint8_t* tab, float2* rop
   }
 }
 
-// MODE: kDense, kWindow (dense over a paged window with sinks), or the statistics (kStats: keys only, split (m, l) and block
-// maxima) and gated (kGated) passes of sparse-V, as the affine kernel runs
-// them.
+// MODE: kDense, kWindow (dense over a paged window with sinks), or the
+// statistics (kStats: keys only, split (m, l) and block maxima) and gated
+// (kGated) passes of sparse-V, as the affine kernel runs them.
 template <int D, int BITS, int MODE>
 __global__ __launch_bounds__(kCbWaves * 64)
 __attribute__((amdgpu_waves_per_eu(2, 2)))

@@ -158,9 +158,9 @@ __device__ void plain_new_token_column(const AttnArgs& a, float2* rope, int64_t 
   }
 }
 
-// MODE: kDense, kWindow (dense over a paged window with sinks), or the statistics (kStats: keys only, split (m, l) and block
-// maxima) and gated (kGated) passes of sparse-V, as the affine kernel runs
-// them.
+// MODE: kDense, kWindow (dense over a paged window with sinks), or the
+// statistics (kStats: keys only, split (m, l) and block maxima) and gated
+// (kGated) passes of sparse-V, as the affine kernel runs them.
 template <int D, int MODE>
 __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   using P = PlainPlan<D>;

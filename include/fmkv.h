@@ -353,7 +353,8 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
  * workspace, unlike fmkv_paged_prefill_step; an eager one uses the GPU's shared
  * buffer.) */
 
-/* One token per sequence: fmkv_paged_decode_attention over a window. */
+/* One token per sequence: fmkv_paged_decode_attention over a window. q is
+ * 16-byte aligned (here and in the next call). */
 int fmkv_paged_window_decode_attention(fmkv_pool* pool, const void* q_bf16,
                                        const int32_t* block_tables, int32_t max_blocks,
                                        const int32_t* seq_lens, int32_t n_seqs,

@@ -70,3 +70,7 @@ def test_wrong_tensors_are_refused(gpu):
             pool.window_attention(*bad, 64, 16)
     with pytest.raises(ValueError):
         pool.window_attention(q, table, n, 64, 16, out=torch.zeros((1, 4, 64), device="cuda"))
+    off = torch.zeros(q.numel() + 8, dtype=torch.bfloat16, device="cuda")[1:1 + q.numel()].view(q.shape)
+    with pytest.raises(fmkv.Exception_) as e:
+        pool.window_attention(off, table, n, 64, 16)
+    assert e.value.code == fmkv.FMKV_ERR_UNSUPPORTED
