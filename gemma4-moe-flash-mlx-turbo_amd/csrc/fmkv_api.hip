@@ -343,13 +343,16 @@ fmkv::Store pool_store(const fmkv_pool* p, const int32_t* table, int32_t stride)
   return s;
 }
 
+constexpr size_t kOwnPartials = (size_t)8 << 20;
+
 // The prefill attention, split over its keys when the grid alone would leave
 // CUs idle. Not under stream capture (a replay would not be ordered with other
 // uses of the partials) and not when there is no memory for the partials: the
-// unsplit launch needs none. A captured call that has a workspace of its own
-// (own: a windowed call's pool, whose uses the caller orders) is split there:
-// 5 queries after 3000 positions, 8/4 heads of 128 dims, bf16, in a graph: 16.3 us,
-// unsplit 50.5.
+// unsplit launch needs none. A call that has a workspace of its own (own: a
+// windowed call's pool, whose uses the caller orders) is split there where it is
+// captured, or its partials are so few that every pool may hold them: 5
+// queries after 3000 positions, 8/4 heads of 128 dims, bf16, in a graph 16.3 us,
+// unsplit 50.5; eager 17.4, with the shared buffer's wait and event 20.2.
 hipError_t run_prefill(fmkv::PrefillArgs& pa, PrefillScratch* sc, int cus, int64_t max_steps,
                        hipStream_t s, Workspace* own = nullptr) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -361,15 +364,14 @@ hipError_t run_prefill(fmkv::PrefillArgs& pa, PrefillScratch* sc, int cus, int64
     pa.part_o = p;
     pa.part_ml = p + bytes / sizeof(float) / (D + 2) * D;
   };
-  if (captured && own) {
-    const size_t bytes = fmkv::prefill_plan(pa, cus, max_steps, true);
-    if (bytes > 0 && own->ensure(bytes) == FMKV_OK)
+  const size_t bytes = fmkv::prefill_plan(pa, cus, max_steps, own || (sc && !captured));
+  if (own && bytes > 0 && (captured || !sc || bytes <= kOwnPartials)) {
+    if (own->ensure(bytes) == FMKV_OK)
       place(own->ptr, bytes);
-    else if (bytes > 0)
+    else
       (void)fmkv::prefill_plan(pa, cus, max_steps, false);
     return fmkv::launch_prefill_attention(pa, s);
   }
-  const size_t bytes = fmkv::prefill_plan(pa, cus, max_steps, sc && !captured);
   if (bytes == 0) return fmkv::launch_prefill_attention(pa, s);
   std::lock_guard<std::mutex> lock(sc->mu);
   if (!sc->ready(cus) || bytes > sc->bytes) {

@@ -349,9 +349,9 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
  * its workspace, so calls on several streams, and replays of graphs that
  * captured them, have to be ordered by the caller; a workspace that a later,
  * larger call outgrows stays until the pool is destroyed, so captured calls
- * stay valid. (A captured prefill call is split over its keys too, in that
- * workspace, unlike fmkv_paged_prefill_step; an eager one uses the GPU's shared
- * buffer.) */
+ * stay valid. (A prefill call that is split over its keys holds its partial rows
+ * there, too, where it is captured or they take 8 MiB at most, and else in the
+ * GPU's shared buffer: see fmkv_prefill_step.) */
 
 /* One token per sequence: fmkv_paged_decode_attention over a window. q is
  * 16-byte aligned (here and in the next call). */
