@@ -1579,6 +1579,8 @@ int fmkv_paged_compact(fmkv_pool* p, const int32_t* block_tables, int32_t max_bl
   if (n_seqs == 0 || max_keep == 0) return FMKV_OK;
   if (!block_tables || !keep || !n_keep || !dst_tables)
     return fail(FMKV_ERR_INVALID_ARG, "block_tables/keep/n_keep/dst_tables are null");
+  // (a grid holds fewer than 2^32 threads in x, 256 a block)
+  if (max_keep > (1 << 28) - 16) return fail(FMKV_ERR_INVALID_ARG, "max_keep must be <= 2^28 - 16");
   if (max_keep > (int64_t)dst_max_blocks * fmkv::kBlockTokens)
     return fail(FMKV_ERR_INVALID_ARG, "max_keep exceeds dst_max_blocks * 16");
   const int rc = check_device(p);

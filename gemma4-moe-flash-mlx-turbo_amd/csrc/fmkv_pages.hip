@@ -192,7 +192,8 @@ hipError_t launch_copy_blocks(CopyArgs& a, int n_pools, int64_t n_pairs, hipStre
   int64_t most = 0;
   for (int i = 0; i < n_pools; i++) most = a.block_bytes[i] > most ? a.block_bytes[i] : most;
   a.parts = (int32_t)((most + kCopyBytes - 1) / kCopyBytes);
-  const int64_t per = INT32_MAX / a.parts;  // pairs of a launch (its grid's x)
+  // pairs of a launch: its grid's x holds fewer than 2^32 threads
+  const int64_t per = (int64_t)(UINT32_MAX / kCopyThreads) / a.parts;
   for (int64_t done = 0; done < n_pairs; done += per) {
     const int64_t n = n_pairs - done < per ? n_pairs - done : per;
     const dim3 grid((unsigned)(n * a.parts), n_pools);

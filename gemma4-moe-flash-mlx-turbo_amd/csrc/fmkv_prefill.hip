@@ -1458,7 +1458,7 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
     const BlockLayout& L = a.new_st.layout;
     const int64_t once =
         D == 128 && !a.share_rows && !(L.mode == kCodebook && L.bits == 3) ? 4 * (int64_t)cus : places;
-    if (total > once && total <= (1 << 24)) {
+    if (total > once && total <= (1 << 22)) {  // (a grid's x holds fewer than 2^32 threads)
       const int64_t rem = total % once;
       const int64_t ranges = rem > 0 ? std::min(places / rem, max_steps / (2 * kPfMinSteps)) : 0;
       if (ranges < 2 || max_steps - max_steps / ranges < (D == 512 ? 24 : 12)) return 0;

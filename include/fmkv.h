@@ -404,9 +404,9 @@ int fmkv_pools_copy_blocks(fmkv_pool* const* pools, int32_t n_pools, const int32
 
 /* The tokens that each sequence keeps, moved to the front of other blocks:
  * position keep[s][i] of sequence s (block_tables) becomes position i of its
- * row of dst_tables, i < n_keep[s] (at most max_keep). Codes, scales and norms
- * move as they are (a kept K keeps the rotation of the position it was computed
- * at). keep: int32 device [n_seqs][max_keep], in any order; n_keep: int32 device
+ * row of dst_tables, i < n_keep[s] (at most max_keep, which is at most 2^28 -
+ * 16). Codes, scales and norms move as they are (a kept K keeps the rotation of
+ * the position it was computed at). keep: int32 device [n_seqs][max_keep], in any order; n_keep: int32 device
  * [n_seqs]; dst_tables: int32 device [n_seqs][dst_max_blocks]. A token whose
  * position or blocks lie outside the tables or the pool is left out, and its
  * slot, like every slot behind the last kept token, stays as it was. The blocks

@@ -68,6 +68,35 @@ def test_copy_blocks_of_many_pools(gpu):
         assert torch.equal(p.storage(), w)
 
 
+def test_copy_blocks_of_more_threads_than_a_grid_holds(gpu):
+    """Blocks of 512 KB in a list of 131080 pairs, nearly all of which name no block:
+    over 2^32 threads."""
+    import torch
+
+    pool = filled(gpu, PLAIN, 512, 16, 16, 9)
+    n = 131080
+    src, dst = np.full(n, -1, np.int32), np.zeros(n, np.int32)
+    at = [0, 131070, 131071, n - 1]
+    src[at], dst[at] = [0, 1, 2, 3], [4, 5, 6, 7]
+    want = pool.storage().clone()
+    want[4:8] = want[0:4]
+    gpu.copy_blocks([pool], i32(src), i32(dst))
+    torch.cuda.synchronize()
+    assert torch.equal(pool.storage(), want)
+
+
+def test_compact_of_more_threads_than_a_grid_holds_is_refused(gpu):
+    import torch
+
+    pool = filled(gpu, *MODES[0], 8)
+    before = pool.storage().clone()
+    t, n = i32([[0, 1]]), i32([2])
+    assert gpu.load_library().fmkv_paged_compact(pool._h, t.data_ptr(), 2, t.data_ptr(), 1 << 28, n.data_ptr(),
+                                                 t.data_ptr(), 1 << 24, 1, None) == gpu.FMKV_ERR_INVALID_ARG
+    torch.cuda.synchronize()
+    assert torch.equal(pool.storage(), before)
+
+
 def test_copy_blocks_graph_and_stream(gpu):
     import torch
 
