@@ -702,6 +702,7 @@ class PagedPool:
         n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        _check_window(window, sinks)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_attention(
@@ -722,6 +723,7 @@ class PagedPool:
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        _check_window(window, sinks)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_step(
@@ -740,6 +742,7 @@ class PagedPool:
         n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        _check_window(window, sinks)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_attention(
@@ -758,6 +761,7 @@ class PagedPool:
         _check_tensor("values", values, torch.bfloat16, (n, n_new, self._H, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        _check_window(window, sinks)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_step(
@@ -897,7 +901,7 @@ class PageBook:
 
     def users(self, block: int) -> int:
         v = ctypes.c_int32()
-        _check(self._lib.fmkv_pages_users(self._h, block, ctypes.byref(v)))
+        _check(self._lib.fmkv_pages_users(self._h, _i32s([block])[0], ctypes.byref(v)))
         return v.value
 
     def alloc(self, n: int) -> list[int]:
@@ -931,12 +935,16 @@ class PageBook:
         blocks = list(blocks)
         if (n_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS > len(blocks):
             raise ValueError(f"{n_tokens} tokens need more than {len(blocks)} blocks")
+        _check_window(window, sinks)
         buf, n = _i32s(blocks), ctypes.c_int64()
         _check(self._lib.fmkv_pages_slide(self._h, buf, n_tokens, window, sinks, ctypes.byref(n)))
         return list(buf[:len(blocks)])
 
 
 def _i32s(values):
+    # (ctypes would keep the low 32 bits of a larger number, another block's)
+    if values and (min(values) < -2 ** 31 or max(values) >= 2 ** 31):
+        raise ValueError("a block does not fit 32 bits")
     return (ctypes.c_int32 * max(len(values), 1))(*values)
 
 
@@ -947,6 +955,12 @@ class _Storage:
         self.owner = owner
         self.__cuda_array_interface__ = {"data": (ptr, False), "shape": tuple(shape),
                                          "typestr": "|u1", "strides": None, "version": 2}
+
+
+def _check_window(window: int, sinks: int) -> None:
+    """Values whose low 32 bits ctypes would pass on (the library checks the rest)."""
+    if not (-2 ** 31 <= window < 2 ** 31 and -2 ** 31 <= sinks < 2 ** 31):
+        raise ValueError("window and sinks must be at most 2^30")
 
 
 def _check_tensor(name: str, t: torch.Tensor, dtype, shape):

@@ -154,3 +154,15 @@ def test_random_use_keeps_the_book():
         held = [sum(blocks.count(b) for blocks, _ in seqs) for b in range(64)]
         assert held == [book.users(b) for b in range(64)]
         assert book.free_count() == held.count(0)
+
+
+@pytest.mark.parametrize("wide", [2 ** 32, -2 ** 32 + 1, 2 ** 31])
+def test_numbers_past_32_bits_are_refused(wide):
+    book = fmkv.PageBook(8)
+    a = book.alloc(4)
+    for call in (lambda: book.release([a[0], wide]), lambda: book.users(wide), lambda: book.fork([wide], 5),
+                 lambda: book.slide(a, 64, wide + 16), lambda: book.slide(a, 64, 16, wide),
+                 lambda: book.slide([a[0], wide], 32, 16)):
+        with pytest.raises(ValueError):
+            call()
+    assert book.free_count() == 4 and [book.users(b) for b in a] == [1] * 4

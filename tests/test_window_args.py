@@ -70,6 +70,11 @@ def test_wrong_tensors_are_refused(gpu):
             pool.window_attention(*bad, 64, 16)
     with pytest.raises(ValueError):
         pool.window_attention(q, table, n, 64, 16, out=torch.zeros((1, 4, 64), device="cuda"))
+    for window, sinks in ((2 ** 32 + 16, 0), (16, 2 ** 32)):
+        for call in (lambda: pool.window_attention(q, table, n, 64, window, sinks),
+                     lambda: pool.window_prefill(q[:, None], table, n - 1, window, sinks)):
+            with pytest.raises(ValueError):
+                call()
     off = torch.zeros(q.numel() + 8, dtype=torch.bfloat16, device="cuda")[1:1 + q.numel()].view(q.shape)
     with pytest.raises(fmkv.Exception_) as e:
         pool.window_attention(off, table, n, 64, 16)
