@@ -1154,16 +1154,31 @@ void prefill_attn_kernel(PrefillArgs a) {
   lds_barrier();
   // an interval between two barriers: QK of step i + 1, softmax of step i, PV of
   // step i - 1; the last one has no QK (a tenth of a call of one or two steps)
+  // A wave in a product goes before a wave in its softmax, so that the matrix
+  // cores wait less for the vector work of the SIMD's other wave: it is of another
+  // work-group or, at head_dim 512, of the same one, where the two stay in step
+  // and the affine weights' conversion inside PV is better not preferred. (2048
+  // tokens, window 1024, 16 / 8 heads of 256 dims, 4 bits: 115.5 us, all waves
+  // alike 125.5; after 6000 positions, 8 bits: 645 and 718. 512 dims, 16 / 2 heads,
+  // after 6000, 8 bits: QK alone 1226, both 1249, neither 1248; bf16: 1127, 1099,
+  // 1128; 4-bit codebook, window: 405, 386, 406. 128 dims, after 6000, 8 bits: 358,
+  // 366, 366; bf16: 400, 405, 387; 3-bit codebook: 440, 462, 431.)
+  constexpr bool kQkFirst = D > 128 || MODE == kAffine;
+  constexpr bool kPvFirst = D == 256 || (D == 512 && MODE != kAffine);
 #pragma unroll 1
   for (int i = 0; i < n - 1; i++) {
     fresh_offsets();
     rescale((i - 1) & 1);
+    if constexpr (kQkFirst) __builtin_amdgcn_s_setprio(1);
     qk((i + 1) & 1);
+    if constexpr (kQkFirst) __builtin_amdgcn_s_setprio(0);
     load_k(after);
     softmax(i & 1, s_begin + i, mine, f_cur);
     keep_own();
     load_n(nxt);
+    if constexpr (kPvFirst) __builtin_amdgcn_s_setprio(2);
     pv((i - 1) & 1, std::false_type{});
+    if constexpr (kPvFirst) __builtin_amdgcn_s_setprio(0);
     load_v(cur);
     lds_barrier();
     advance(i + 1);
