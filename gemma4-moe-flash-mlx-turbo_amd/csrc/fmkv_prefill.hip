@@ -15,7 +15,7 @@
 // registers (no LDS staging), and is used for four 16-row tiles. (One pair of
 // waves per 16 rows, every pair decoding every block, took 7.78 ms for a
 // 2048-token chunk after 32768 positions, 16 q / 2 KV heads of 512 dims, 8
-// bits; this split takes 5.2 ms, and 0.147 against 0.227 ms for a 2048-token
+// bits; this split takes 5.04 ms, and 0.140 against 0.227 ms for a 2048-token
 // chunk on a 1024-position ring, 16 / 8 heads of 256 dims, 4 bits.) Small grids
 // at head_dim 128 and 256 share the rows among eight waves, RW = 4 and 2 per 64
 // dims (prefill_plan).
@@ -1464,8 +1464,8 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
   // split over their keys where that fills the chip, and the round ends sooner by
   // the steps saved (all tiles see about a window), less the rotations of the
   // ranges' rows and the merge: 12 steps, 24 of 512 dims. Four 333-token chunks
-  // (336 work-groups), window 2000, 8 bits, 512 dims: 241 us, unsplit 271; a
-  // 2500-token chunk, window 1024, 4 bits, 256 dims (632): 169, unsplit 198. At
+  // (336 work-groups), window 2000, 8 bits, 512 dims: 236 us, unsplit 267; a
+  // 2500-token chunk, window 1024, 4 bits, 256 dims (632): 160, unsplit 202. At
   // head_dim 128 four work-groups a CU do run unless their LDS is the 3-bit
   // codebook's (4 x 2048 tokens, 1024 work-groups, bf16: 135; counted as three a
   // CU and split 168).
