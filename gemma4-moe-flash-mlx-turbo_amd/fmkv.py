@@ -595,6 +595,7 @@ class PagedPool:
     """Pool of 16-token blocks shared by many sequences (batched decode)."""
 
     def __init__(self, desc: CacheDesc, n_blocks: int):
+        _check_bits("n_blocks", n_blocks, 64)
         self.desc = desc
         self.n_blocks = n_blocks
         self._D, self._H = desc.head_dim, desc.n_kv_heads  # (a struct's field takes longer to read)
@@ -877,6 +878,7 @@ class PageBook:
     lists of ints (-1: given back)."""
 
     def __init__(self, n_blocks: int):
+        _check_bits("n_blocks", n_blocks, 64)
         self.n_blocks = n_blocks
         self._lib = load_library()
         h = ctypes.c_void_p()
@@ -906,6 +908,7 @@ class PageBook:
 
     def alloc(self, n: int) -> list[int]:
         """n free blocks (an error, and none taken, when fewer are free)."""
+        _check_bits("n", n, 64)
         if n > self.n_blocks:
             raise Exception_(FMKV_ERR_CAPACITY, f"{n} blocks asked for of {self.n_blocks}")
         buf = (ctypes.c_int32 * max(n, 1))()
@@ -920,6 +923,7 @@ class PageBook:
     def fork(self, blocks, n_tokens: int):
         """(blocks of a second sequence that goes on from n_tokens of a first,
         the (src, dst) copy that copy_blocks has to make for it or None)."""
+        _check_bits("n_tokens", n_tokens, 64)
         blocks = list(blocks)
         n = (n_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS
         if n > len(blocks):
@@ -932,6 +936,7 @@ class PageBook:
     def slide(self, blocks, n_tokens: int, window: int, sinks: int = 0) -> list[int]:
         """The sequence's blocks after giving back those that no query at position
         n_tokens or later sees through the window and the sinks (-1 there)."""
+        _check_bits("n_tokens", n_tokens, 64)
         blocks = list(blocks)
         if (n_tokens + BLOCK_TOKENS - 1) // BLOCK_TOKENS > len(blocks):
             raise ValueError(f"{n_tokens} tokens need more than {len(blocks)} blocks")
@@ -939,6 +944,13 @@ class PageBook:
         buf, n = _i32s(blocks), ctypes.c_int64()
         _check(self._lib.fmkv_pages_slide(self._h, buf, n_tokens, window, sinks, ctypes.byref(n)))
         return list(buf[:len(blocks)])
+
+
+def _check_bits(name: str, value: int, bits: int) -> None:
+    """ctypes passes on the low bits of a number that is too wide for the
+    argument, another number, which the library cannot tell from a good one."""
+    if not -(1 << bits - 1) <= value < 1 << bits - 1:
+        raise ValueError(f"{name} does not fit {bits} bits")
 
 
 def _i32s(values):

@@ -166,3 +166,19 @@ def test_numbers_past_32_bits_are_refused(wide):
         with pytest.raises(ValueError):
             call()
     assert book.free_count() == 4 and [book.users(b) for b in a] == [1] * 4
+
+
+@pytest.mark.parametrize("low", [2, 16, 40, 1600])
+def test_counts_past_64_bits_are_refused(low):
+    """(Their low 64 bits would be counts that the buffers were not made for.)"""
+    book = fmkv.PageBook(64)
+    a = book.alloc(4)
+    for wide in (low - 2 ** 64, low + 2 ** 64, -2 ** 63 - 1, 2 ** 63):
+        for call in (lambda: fmkv.PageBook(wide), lambda: fmkv.PagedPool(fmkv.make_desc(2, 128, 4), wide),
+                     lambda: book.alloc(wide), lambda: book.fork(a, wide), lambda: book.slide(a, wide, 16)):
+            with pytest.raises((ValueError, fmkv.Exception_)):
+                call()
+    for call in (lambda: book.alloc(-5), lambda: book.fork(a, -5), lambda: book.slide(a, -5, 16)):
+        with pytest.raises(fmkv.Exception_):
+            call()
+    assert book.free_count() == 60 and [book.users(b) for b in a] == [1] * 4
