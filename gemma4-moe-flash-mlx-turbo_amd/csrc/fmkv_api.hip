@@ -1811,6 +1811,13 @@ int check_block(const fmkv_pages* p, int32_t block) {
   return FMKV_OK;
 }
 
+// A sequence's tokens: positions are 32-bit (start_pos, seq_lens).
+int check_tokens(int64_t n_tokens) {
+  if (n_tokens < 0 || n_tokens > INT32_MAX)
+    return fail(FMKV_ERR_INVALID_ARG, "n_tokens must be in [0, 2^31)");
+  return FMKV_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1893,8 +1900,9 @@ int fmkv_pages_release(fmkv_pages* p, const int32_t* blocks, int64_t n) {
 
 int fmkv_pages_fork(fmkv_pages* p, const int32_t* blocks, int64_t n_tokens, int32_t* child,
                     int32_t* copy_src, int32_t* copy_dst) {
-  if (!p || n_tokens < 0 || !copy_src || !copy_dst || (n_tokens > 0 && (!blocks || !child)))
-    return fail(FMKV_ERR_INVALID_ARG, "bad pages / blocks / n_tokens / child / copy_src / copy_dst");
+  if (int rc = check_tokens(n_tokens)) return rc;
+  if (!p || !copy_src || !copy_dst || (n_tokens > 0 && (!blocks || !child)))
+    return fail(FMKV_ERR_INVALID_ARG, "pages/blocks/child/copy_src/copy_dst are null");
   const int64_t n = (n_tokens + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
   const bool part = n_tokens % fmkv::kBlockTokens != 0 && blocks[n - 1] != -1;
   for (int64_t i = 0; i < n; i++) {
@@ -1920,10 +1928,11 @@ int fmkv_pages_fork(fmkv_pages* p, const int32_t* blocks, int64_t n_tokens, int3
 
 int fmkv_pages_slide(fmkv_pages* p, int32_t* blocks, int64_t n_tokens, int32_t window,
                      int32_t sinks, int64_t* n_freed) {
-  if (!p || n_tokens < 0 || (n_tokens > 0 && !blocks) || !n_freed)
-    return fail(FMKV_ERR_INVALID_ARG, "bad pages / blocks / n_tokens / n_freed");
-  int rc = check_window(window, sinks);
+  int rc = check_tokens(n_tokens);
   if (rc) return rc;
+  if (!p || (n_tokens > 0 && !blocks) || !n_freed)
+    return fail(FMKV_ERR_INVALID_ARG, "pages/blocks/n_freed are null");
+  if ((rc = check_window(window, sinks))) return rc;
   constexpr int64_t B = fmkv::kBlockTokens;
   // blocks [first, last) hold hidden positions alone: from the sinks' end to the
   // window of the next query, at position n_tokens

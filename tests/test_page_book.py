@@ -182,3 +182,18 @@ def test_counts_past_64_bits_are_refused(low):
         with pytest.raises(fmkv.Exception_):
             call()
     assert book.free_count() == 60 and [book.users(b) for b in a] == [1] * 4
+
+
+@pytest.mark.parametrize("n_tokens", [2 ** 63 - 1, 2 ** 63 - 14, 2 ** 40, 2 ** 31, -1, -2 ** 63])
+def test_sequences_past_32_bit_positions_are_refused(n_tokens):
+    import ctypes
+
+    lib, book = fmkv.load_library(), fmkv.PageBook(4)
+    book.alloc(2)
+    blocks, child = (ctypes.c_int32 * 2)(0, 1), (ctypes.c_int32 * 2)(7, 7)
+    src, dst, freed = ctypes.c_int32(5), ctypes.c_int32(5), ctypes.c_int64(5)
+    assert lib.fmkv_pages_fork(book._h, blocks, n_tokens, child, ctypes.byref(src),
+                               ctypes.byref(dst)) == fmkv.FMKV_ERR_INVALID_ARG
+    assert lib.fmkv_pages_slide(book._h, blocks, n_tokens, 16, 0, ctypes.byref(freed)) == fmkv.FMKV_ERR_INVALID_ARG
+    assert list(blocks) == [0, 1] and list(child) == [7, 7] and (src.value, dst.value, freed.value) == (5, 5, 5)
+    assert [book.users(b) for b in range(4)] == [1, 1, 0, 0] and book.free_count() == 2
