@@ -102,17 +102,22 @@ def make_prologue(k_norm_weight: torch.Tensor, eps: float, rope_dims: int, rope_
     (the C struct itself carries only the device address)."""
     if k_norm_weight.dtype != torch.bfloat16 or k_norm_weight.dim() != 1:
         raise ValueError("k_norm_weight must be bf16 [head_dim]")
-    if not k_norm_weight.is_contiguous():
-        raise ValueError("k_norm_weight must be contiguous")
+    if not k_norm_weight.is_contiguous() or not k_norm_weight.is_cuda:
+        raise ValueError("k_norm_weight must be contiguous and on the GPU")
     pro = KvPrologue(k_norm_weight.data_ptr(), eps, rope_dims, rope_theta, 1 if v_from_k else 0)
     pro.weight = k_norm_weight
     return pro
 
 
-def _check_prologue_weight(prologue: KvPrologue, head_dim: int) -> None:
+def _check_prologue_weight(prologue: KvPrologue, head_dim: int, keys: torch.Tensor) -> None:
+    """The weight is of the head's length and on the GPU of the rows."""
     w = getattr(prologue, "weight", None)
-    if w is not None and w.numel() != head_dim:
+    if w is None:
+        return
+    if w.numel() != head_dim:
         raise ValueError(f"k_norm_weight has {w.numel()} elements; head_dim is {head_dim}")
+    if w.get_device() != keys.get_device():
+        raise ValueError(f"k_norm_weight is on {w.device}, the rows are on {keys.device}")
 
 
 class QkvPrologue(ctypes.Structure):
@@ -137,8 +142,9 @@ def make_qkv_prologue(q_norm_weight, k_norm_weight, eps: float, rope_dims: int, 
     given); sections: pairs of each position axis (None: one axis). The struct
     keeps the weights alive, as make_prologue's does."""
     for w in (q_norm_weight, k_norm_weight):
-        if w is not None and (w.dtype != torch.bfloat16 or w.dim() != 1 or not w.is_contiguous()):
-            raise ValueError("norm weights must be contiguous bf16 [head_dim]")
+        if w is not None and (w.dtype != torch.bfloat16 or w.dim() != 1 or not w.is_contiguous() or
+                              not w.is_cuda):
+            raise ValueError("norm weights must be contiguous bf16 [head_dim] on the GPU")
     cut = tuple(sections) if sections is not None else (rope_dims // 2,)
     if not 1 <= len(cut) <= 4:
         raise ValueError("sections must be one to four counts of pairs")
@@ -402,7 +408,7 @@ class KVCache:
         if values is None:
             values = keys
         self._check_kv(keys, values)
-        _check_prologue_weight(prologue, self.desc.head_dim)
+        _check_prologue_weight(prologue, self.desc.head_dim, keys)
         _check(self._lib.fmkv_cache_append_projected(self._h, _ptr(keys), _ptr(values),
                                                      keys.shape[0], ctypes.byref(prologue),
                                                      _stream(stream)))
@@ -465,7 +471,7 @@ class KVCache:
         if values is None:
             values = keys
         self._check_kv(keys, values)
-        _check_prologue_weight(prologue, self.desc.head_dim)
+        _check_prologue_weight(prologue, self.desc.head_dim, keys)
         if q.dtype != torch.bfloat16 or q.dim() != 2 or q.shape[1] != self.desc.head_dim:
             raise ValueError("q must be bf16 [n_q_heads, head_dim]")
         if out is None:
@@ -630,7 +636,7 @@ class PagedPool:
         if values is None:
             values = keys
         n_seqs, n_new = keys.shape[0], keys.shape[1]
-        _check_prologue_weight(prologue, self.desc.head_dim)
+        _check_prologue_weight(prologue, self.desc.head_dim, keys)
         _check(self._lib.fmkv_paged_append_projected(
             self._h, _ptr(keys), _ptr(values), _ptr(block_tables), block_tables.shape[1],
             _ptr(start_pos), n_seqs, n_new, ctypes.byref(prologue), _stream(stream)))
@@ -684,7 +690,7 @@ class PagedPool:
         (RoPE positions from start_pos; values None with prologue.v_from_k)."""
         if values is None:
             values = keys
-        _check_prologue_weight(prologue, self.desc.head_dim)
+        _check_prologue_weight(prologue, self.desc.head_dim, keys)
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(self._lib.fmkv_paged_decode_step_projected(
@@ -829,8 +835,12 @@ def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=No
     dev = torch.cuda.current_device()
     n, _, D = (k if q is None else q).shape
     for w in getattr(prologue, "weights", ()):
-        if w is not None and w.shape[0] != D:
+        if w is None:
+            continue
+        if w.shape[0] != D:
             raise ValueError(f"a norm weight has {w.shape[0]} elements; head_dim is {D}")
+        if w.get_device() != dev:
+            raise ValueError(f"a norm weight is on {w.device}, not on the current GPU")
     q_heads, q_ptr, q_stride = _head_rows("q", q, n, D, dev)
     k_heads, k_ptr, k_stride = _head_rows("k", k, n, D, dev)
     v_heads, v_ptr, v_stride = _head_rows("v", v, n, D, dev)
