@@ -104,6 +104,7 @@ def make_prologue(k_norm_weight: torch.Tensor, eps: float, rope_dims: int, rope_
         raise ValueError("k_norm_weight must be bf16 [head_dim]")
     if not k_norm_weight.is_contiguous() or not k_norm_weight.is_cuda:
         raise ValueError("k_norm_weight must be contiguous and on the GPU")
+    _check_bits("rope_dims", rope_dims, 32)
     pro = KvPrologue(k_norm_weight.data_ptr(), eps, rope_dims, rope_theta, 1 if v_from_k else 0)
     pro.weight = k_norm_weight
     return pro
@@ -148,6 +149,8 @@ def make_qkv_prologue(q_norm_weight, k_norm_weight, eps: float, rope_dims: int, 
     cut = tuple(sections) if sections is not None else (rope_dims // 2,)
     if not 1 <= len(cut) <= 4:
         raise ValueError("sections must be one to four counts of pairs")
+    for name, value in (("rope_dims", rope_dims), *(("a section", x) for x in cut)):
+        _check_bits(name, value, 32)
     pro = QkvPrologue(None if q_norm_weight is None else q_norm_weight.data_ptr(),
                       None if k_norm_weight is None else k_norm_weight.data_ptr(), eps, rope_dims,
                       rope_theta, len(cut), (ctypes.c_int32 * 4)(*cut), int(v_norm), int(v_from_k))
@@ -292,6 +295,10 @@ def _stream(stream) -> int | None:
 
 def make_desc(n_kv_heads: int, head_dim: int, bits: int, window: int = 0, capacity: int = 0,
               mode: int = MODE_AFFINE, group_size: int = 64, sign_seed: int = 42) -> CacheDesc:
+    for name, value in (("n_kv_heads", n_kv_heads), ("head_dim", head_dim), ("bits", bits),
+                        ("group_size", group_size), ("mode", mode), ("window", window)):
+        _check_bits(name, value, 32)
+    _check_bits("capacity", capacity, 64)
     return CacheDesc(n_kv_heads, head_dim, bits, group_size, mode, window, capacity, sign_seed)
 
 
@@ -650,6 +657,7 @@ class PagedPool:
         speed only, on tables wider than that; 0: the table's width)."""
         if q.dim() != 4 or q.shape[:2] != keys.shape[:2]:
             raise ValueError("q must be bf16 [n_seqs, n_new, n_q_heads, head_dim]")
+        _check_bits("max_seq_len", max_seq_len, 32)
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(self._lib.fmkv_paged_prefill_step_bounded(
@@ -661,6 +669,7 @@ class PagedPool:
     def attention(self, q, block_tables, seq_lens, max_seq_len: int, scale: float = 1.0,
                   sparse_v_tau: float = 0.0, out=None, dtype=torch.bfloat16, stream=None):
         """q bf16 [n_seqs, n_q_heads, D]; seq_lens int32 [n_seqs]."""
+        _check_bits("max_seq_len", max_seq_len, 32)
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(self._lib.fmkv_paged_decode_attention(
@@ -674,6 +683,7 @@ class PagedPool:
                     stream=None):
         """append(keys, values, ...) at start_pos, then attention over seq_lens
         (= start_pos + n_new) in one call."""
+        _check_bits("max_seq_len", max_seq_len, 32)
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(self._lib.fmkv_paged_decode_step(
@@ -691,6 +701,7 @@ class PagedPool:
         if values is None:
             values = keys
         _check_prologue_weight(prologue, self.desc.head_dim, keys)
+        _check_bits("max_seq_len", max_seq_len, 32)
         if out is None:
             out = torch.empty(q.shape, dtype=dtype, device=q.device)
         _check(self._lib.fmkv_paged_decode_step_projected(
@@ -709,7 +720,7 @@ class PagedPool:
         n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
-        _check_window(window, sinks)
+        _check_window(window, sinks, max_seq_len)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_attention(
@@ -730,7 +741,7 @@ class PagedPool:
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
-        _check_window(window, sinks)
+        _check_window(window, sinks, max_seq_len)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_decode_step(
@@ -749,7 +760,7 @@ class PagedPool:
         n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
-        _check_window(window, sinks)
+        _check_window(window, sinks, max_seq_len)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_attention(
@@ -768,7 +779,7 @@ class PagedPool:
         _check_tensor("values", values, torch.bfloat16, (n, n_new, self._H, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("start_pos", start_pos, torch.int32, (n,))
-        _check_window(window, sinks)
+        _check_window(window, sinks, max_seq_len)
         dev = self._device
         out = _out(out, q, dtype, stream)
         _check(self._lib.fmkv_paged_window_prefill_step(
@@ -979,10 +990,11 @@ class _Storage:
                                          "typestr": "|u1", "strides": None, "version": 2}
 
 
-def _check_window(window: int, sinks: int) -> None:
+def _check_window(window: int, sinks: int, max_seq_len: int = 0) -> None:
     """Values whose low 32 bits ctypes would pass on (the library checks the rest)."""
     if not (-2 ** 31 <= window < 2 ** 31 and -2 ** 31 <= sinks < 2 ** 31):
         raise ValueError("window and sinks must be at most 2^30")
+    _check_bits("max_seq_len", max_seq_len, 32)
 
 
 def _check_tensor(name: str, t: torch.Tensor, dtype, shape):

@@ -79,3 +79,37 @@ def test_wrong_tensors_are_refused(gpu):
     with pytest.raises(fmkv.Exception_) as e:
         pool.window_attention(off, table, n, 64, 16)
     assert e.value.code == fmkv.FMKV_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("wide", [2 ** 32 + 16, 2 ** 31, -2 ** 31 - 1, 16 - 2 ** 32, 2 ** 64 + 16])
+def test_lengths_past_32_bits_are_refused(wide):
+    """A bound of 2^32 + 16 would arrive as 16, and decode leave out what splits for 16
+    positions do not cover. In every call that takes one, before any HIP call."""
+    import torch
+
+    pool = object.__new__(fmkv.PagedPool)
+    pool.desc, pool._lib, pool._h, pool._D, pool._H, pool._device = fmkv.make_desc(2, 128, 4), None, None, 128, 2, -1
+    q, kv = (torch.zeros((1, 1, h, 128), dtype=torch.bfloat16) for h in (4, 2))
+    table, n = torch.zeros((1, 4), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    pro = fmkv.KvPrologue()
+    for call in (lambda: pool.window_attention(q[0], table, n, wide, 16),
+                 lambda: pool.window_decode_step(kv, kv, table, n, n, wide, q[0], 16),
+                 lambda: pool.window_prefill(q, table, n, 16, max_seq_len=wide),
+                 lambda: pool.window_prefill_step(kv, kv, table, n, q, 16, max_seq_len=wide),
+                 lambda: pool.attention(q[0], table, n, wide),
+                 lambda: pool.decode_step(kv, kv, table, n, n, wide, q[0]),
+                 lambda: pool.decode_step_projected(kv, kv, table, n, n, wide, pro, q[0]),
+                 lambda: pool.prefill_step(kv, kv, table, n, q, max_seq_len=wide)):
+        with pytest.raises(ValueError, match="max_seq_len does not fit"):
+            call()
+
+
+@pytest.mark.parametrize("wide", [2 ** 32 + 16, -2 ** 32 + 16])
+def test_descriptions_and_prologues_past_32_bits_are_refused(wide):
+    for change in ("n_kv_heads", "head_dim", "bits", "window", "mode", "group_size"):
+        with pytest.raises(ValueError, match=change):
+            fmkv.make_desc(**{**dict(n_kv_heads=2, head_dim=128, bits=4), change: wide})
+    with pytest.raises(ValueError, match="rope_dims"):
+        fmkv.make_qkv_prologue(None, None, 1e-6, wide, 1e4)
+    with pytest.raises(ValueError, match="section"):
+        fmkv.make_qkv_prologue(None, None, 1e-6, 64, 1e4, sections=(16, wide))
