@@ -1666,9 +1666,22 @@ int fmkv_qkv_norm_rope(const fmkv_qkv_prologue* pro, int32_t head_dim, int32_t n
   auto span = [&](const void* p, int64_t bytes) {
     return std::pair<uintptr_t, uintptr_t>((uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes);
   };
+  // (nor over what every row reads: the weights and the positions)
+  const struct {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+  } shared[3] = {{"q_norm_weight", n_q_heads > 0 ? pro->q_norm_weight : nullptr, head_dim * 2},
+                 {"k_norm_weight", n_kv_heads > 0 ? pro->k_norm_weight : nullptr, head_dim * 2},
+                 {"positions", pro->rope_dims > 0 ? positions : nullptr, pro->n_axes * n_tokens * 4}};
   for (int i = 0; i < 3; i++) {
     if (!rows[i].there) continue;
     const auto o = span(rows[i].out, n_tokens * rows[i].heads * head_dim * 2);
+    for (const auto& x : shared) {
+      const auto in = span(x.at, x.bytes);
+      if (x.at && o.first < in.second && in.first < o.second)
+        return fail(FMKV_ERR_INVALID_ARG, std::string(rows[i].name) + "'s output overlaps " + x.name);
+    }
     for (int j = 0; j < 3; j++) {
       if (!rows[j].there) continue;
       const auto in = span(rows[j].in, ((n_tokens - 1) * rows[j].stride + rows[j].heads * head_dim) * 2);

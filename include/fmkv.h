@@ -476,7 +476,8 @@ typedef struct fmkv_qkv_prologue {
  * 128, 256 or 512. positions: int32 device [n_axes][n_tokens] (NULL with
  * rope_dims 0). Outputs are contiguous [n_tokens][heads][head_dim] bf16, the
  * inputs of the append, decode step and prefill calls. An output may be its own
- * input where that is contiguous; any other overlap is refused. */
+ * input where that is contiguous; any other overlap is refused, of the weights
+ * and the positions too. */
 int fmkv_qkv_norm_rope(const fmkv_qkv_prologue* prologue, int32_t head_dim, int32_t n_q_heads,
                        int32_t n_kv_heads, int64_t n_tokens, const void* q, int64_t q_stride,
                        const void* k, int64_t k_stride, const void* v, int64_t v_stride,

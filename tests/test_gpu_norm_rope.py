@@ -263,3 +263,43 @@ def test_bad_arguments_are_refused(gpu):
               lambda: gpu.qkv_norm_rope(q[..., :64].contiguous(), None, None, pos, pro)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_outputs_over_weights_or_positions_are_refused(gpu):
+    """Every row reads them, in no order: refused, and nothing is written."""
+    import torch
+
+    D, n = 128, 4
+    for which in ("q_norm_weight", "k_norm_weight", "positions", "last weight", "one axis off"):
+        flat = torch.ones(4 * n * 4 * D, dtype=torch.bfloat16, device="cuda")
+        q, k, v = rows(1, (n, 4, D)), rows(2, (n, 2, D)), rows(3, (n, 2, D))
+        w = torch.ones(D, dtype=torch.bfloat16, device="cuda")
+        pos = torch.zeros((2, n), dtype=torch.int32, device="cuda")
+        out = [torch.zeros_like(x) for x in (q, k, v)]
+        qw, kw = w, w
+        if which == "q_norm_weight":
+            out[0], qw = flat[:n * 4 * D].view(n, 4, D), flat[n * 4 * D - 1:n * 4 * D - 1 + D]
+        elif which == "k_norm_weight":
+            out[2], kw = flat[:n * 2 * D].view(n, 2, D), flat[:D]
+        elif which == "last weight":
+            out[0], kw = flat[D - 1:D - 1 + n * 4 * D].view(n, 4, D), flat[:D]
+        elif which == "positions":
+            out[1], pos = flat[:n * 2 * D].view(n, 2, D), flat[2:2 + 4 * n].view(torch.int32).view(2, n)
+        else:  # the second axis's last position
+            out[1] = flat[4 * n - 2:4 * n - 2 + n * 2 * D].view(n, 2, D)
+            pos = flat[:4 * n].view(torch.int32).view(2, n)
+        before = flat.clone()
+        pro = gpu.make_qkv_prologue(qw, kw, 1e-6, 64, 1e4, sections=(16, 16))
+        with pytest.raises(gpu.Exception_, match="overlaps") as e:
+            gpu.qkv_norm_rope(q, k, v, pos, pro, out=tuple(out))
+        torch.cuda.synchronize()
+        assert e.value.code == gpu.FMKV_ERR_INVALID_ARG and torch.equal(flat, before), which
+    # what is not read does not count, and neighbours are not overlaps
+    flat = torch.ones(n * 4 * D + 2 * D, dtype=torch.bfloat16, device="cuda")
+    pro = gpu.make_qkv_prologue(flat[:D], flat[-D:], 1e-6, 64, 1e4)
+    got = flat[D:-D].view(n, 4, D)
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    gpu.qkv_norm_rope(q, None, None, pos, pro, out=(got, None, None))
+    torch.cuda.synchronize()
+    check(got, reference(q, flat[:D], 1e-6, pos, 64, 1e4, (32,)), "q")
+    assert bool((flat[:D] == 1).all()) and bool((flat[-D:] == 1).all())
