@@ -197,9 +197,10 @@ struct Workspace {
     bytes = need;
     return FMKV_OK;
   }
-  // (allocating does not end a capture in this thread's relaxed mode)
+  // (allocating does not end a capture in this thread's relaxed mode; half as
+  // large again where memory allows, else what the call needs)
   int grow(size_t need) {
-    const size_t want = std::max(need, bytes + bytes / 2);
+    size_t want = std::max(need, bytes + bytes / 2);
     try {
       kept.reserve(kept.size() + 1);
     } catch (const std::exception&) {
@@ -208,7 +209,12 @@ struct Workspace {
     float* p = nullptr;
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     (void)hipThreadExchangeStreamCaptureMode(&mode);
-    const hipError_t e = hipMalloc(&p, want);
+    hipError_t e = hipMalloc(&p, want);
+    if (e != hipSuccess && want > need) {
+      (void)hipGetLastError();
+      want = need;
+      e = hipMalloc(&p, want);
+    }
     (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (e != hipSuccess) {
       (void)hipGetLastError();
