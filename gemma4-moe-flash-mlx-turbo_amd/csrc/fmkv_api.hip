@@ -172,24 +172,50 @@ struct ExtWorkspace {
   size_t bytes = 0;
 };
 
+// The call on stream s becomes part of a graph.
+bool is_captured(hipStream_t s) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  const bool captured = hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+  if (captured) (void)hipGetLastError();
+  return captured;
+}
+
+// Allocating does not end a capture in a thread's relaxed mode.
+struct RelaxedCapture {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
+
 struct Workspace {
   float* ptr = nullptr;
   size_t bytes = 0;
-  // a pool's: earlier, smaller buffers stay until the handle's end, since a
-  // captured graph may use them (each at least half as large again as the one
-  // before, so together they stay below twice the last)
-  bool keep = false;
+  // A pool's calls say whether they are captured. What a captured call uses stays
+  // until the handle's end, since its graph uses it at every replay; an outgrown
+  // buffer of eager calls alone is freed.
+  bool captured = false;  // the call being prepared
+  bool in_graph = false;  // ptr: an earlier one
   std::vector<float*> kept;
   // zero: a new allocation starts zeroed (head-block staging, whose
   // unwritten slots are read, masked, as the cache's own are)
   int ensure(size_t need, bool zero = false) {
-    if (need <= bytes) return FMKV_OK;
-    if (keep) return grow(need);
-    if (ptr) (void)hipFree(ptr);
+    if (need > bytes) {
+      const int rc = captured || in_graph ? grow(need) : replace(need, zero);
+      if (rc) return rc;
+    }
+    in_graph = in_graph || captured;
+    return FMKV_OK;
+  }
+  int replace(size_t need, bool zero) {
+    if (ptr) (void)hipFree(ptr);  // (waits for the calls that use it)
     ptr = nullptr;
     bytes = 0;
     hipError_t e = hipMalloc(&ptr, need);
-    if (e != hipSuccess) return fail(FMKV_ERR_OOM, "workspace allocation failed");
+    if (e != hipSuccess) {
+      ptr = nullptr;
+      (void)hipGetLastError();
+      return fail(FMKV_ERR_OOM, "workspace allocation failed");
+    }
     if (zero) {
       e = hipMemset(ptr, 0, need);
       if (e != hipSuccess) return hip_fail(e, "hipMemset(workspace)");
@@ -197,8 +223,8 @@ struct Workspace {
     bytes = need;
     return FMKV_OK;
   }
-  // (allocating does not end a capture in this thread's relaxed mode; half as
-  // large again where memory allows, else what the call needs)
+  // Half as large again where memory allows, so that the buffers kept together
+  // stay below twice the last; else what the call needs.
   int grow(size_t need) {
     size_t want = std::max(need, bytes + bytes / 2);
     try {
@@ -207,15 +233,12 @@ struct Workspace {
       return fail(FMKV_ERR_OOM, "no host memory for a workspace");
     }
     float* p = nullptr;
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    (void)hipThreadExchangeStreamCaptureMode(&mode);
     hipError_t e = hipMalloc(&p, want);
     if (e != hipSuccess && want > need) {
       (void)hipGetLastError();
       want = need;
       e = hipMalloc(&p, want);
     }
-    (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (e != hipSuccess) {
       (void)hipGetLastError();
       return fail(FMKV_ERR_OOM, "workspace allocation failed");
@@ -223,6 +246,7 @@ struct Workspace {
     if (ptr) kept.push_back(ptr);
     ptr = p;
     bytes = want;
+    in_graph = false;
     return FMKV_OK;
   }
   void release() {
@@ -255,15 +279,13 @@ struct PrefillScratch {
   // thread's relaxed mode.
   bool ready(int cus) {
     if (ptr) return true;
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    (void)hipThreadExchangeStreamCaptureMode(&mode);
+    RelaxedCapture relaxed;
     bytes = fmkv::prefill_scratch_bytes(cus);
     if (hipMalloc(&ptr, bytes) != hipSuccess) ptr = nullptr;
     if (ptr && hipEventCreateWithFlags(&used, hipEventDisableTiming) != hipSuccess) {
       (void)hipFree(ptr);
       ptr = nullptr;
     }
-    (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (!ptr) (void)hipGetLastError();
     return ptr != nullptr;
   }
@@ -361,9 +383,7 @@ constexpr size_t kOwnPartials = (size_t)8 << 20;
 // unsplit 50.5; eager 17.4, with the shared buffer's wait and event 20.2.
 hipError_t run_prefill(fmkv::PrefillArgs& pa, PrefillScratch* sc, int cus, int64_t max_steps,
                        hipStream_t s, Workspace* own = nullptr) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  const bool captured = hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
-  if (captured) (void)hipGetLastError();
+  const bool captured = is_captured(s);
   // (bytes = rows * (D + 2) floats)
   auto place = [&](float* p, size_t bytes) {
     const int D = pa.new_st.layout.head_dim;
@@ -372,6 +392,8 @@ hipError_t run_prefill(fmkv::PrefillArgs& pa, PrefillScratch* sc, int cus, int64
   };
   const size_t bytes = fmkv::prefill_plan(pa, cus, max_steps, own || (sc && !captured));
   if (own && bytes > 0 && (captured || !sc || bytes <= kOwnPartials)) {
+    RelaxedCapture relaxed;
+    own->captured = captured;
     if (own->ensure(bytes) == FMKV_OK)
       place(own->ptr, bytes);
     else
@@ -748,8 +770,8 @@ int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows
 int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
                             int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
                             int32_t max_seq_len, int32_t n_q_heads, float scale, float tau,
-                            void* out, int32_t out_dtype, int new_col, fmkv::AttnArgs* a,
-                            int32_t win = 0, int32_t sinks = 0) {
+                            void* out, int32_t out_dtype, int new_col, hipStream_t s,
+                            fmkv::AttnArgs* a, int32_t win = 0, int32_t sinks = 0) {
   if (n_seqs < 0 || max_seq_len < 0 || max_blocks < 1)
     return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / max_seq_len / max_blocks");
   if (n_seqs > 0 && (!block_tables || !seq_lens))
@@ -757,6 +779,8 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   if ((int64_t)max_seq_len > (int64_t)max_blocks * fmkv::kBlockTokens)
     return fail(FMKV_ERR_INVALID_ARG, "max_seq_len exceeds max_blocks * 16");
   if (n_seqs > 65535) return fail(FMKV_ERR_INVALID_ARG, "at most 65535 sequences per call");
+  RelaxedCapture relaxed;  // (the workspace may grow)
+  p->ws.captured = is_captured(s);
   a->seq_lens = seq_lens;
   a->seq_len = 0;
   a->window = 0;
@@ -1263,7 +1287,6 @@ int fmkv_pool_create(const fmkv_cache_desc* desc, int64_t n_blocks, fmkv_pool** 
   p->split = prefill_scratch_join();
   p->device = 0;
   (void)hipGetDevice(&p->device);
-  p->ws.keep = true;
   *out = p;
   return FMKV_OK;
 }
@@ -1400,14 +1423,14 @@ int fmkv_paged_window_decode_attention(fmkv_pool* p, const void* q, const int32_
   int rc = check_window(window, sinks);
   if (rc) return rc;
   if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   fmkv::AttnArgs a;
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
-                               n_q_heads, scale, 0.0f, out, out_dtype, 0, &a, window, sinks);
+                               n_q_heads, scale, 0.0f, out, out_dtype, 0, s, &a, window, sinks);
   if (rc || n_seqs == 0) return rc;
   hipEvent_t e0, e1;
   next_events(&e0, &e1);
-  hipError_t e = launch_attention(a, n_seqs, p->desc.n_kv_heads, static_cast<hipStream_t>(stream),
-                                  e0, e1);
+  hipError_t e = launch_attention(a, n_seqs, p->desc.n_kv_heads, s, e0, e1);
   if (e != hipSuccess) return hip_fail(e, "paged window attention launch");
   return FMKV_OK;
 }
@@ -1448,11 +1471,11 @@ int fmkv_paged_decode_attention(fmkv_pool* p, const void* q, const int32_t* bloc
                                 int32_t max_seq_len, int32_t n_q_heads, float scale, float tau,
                                 void* out, int32_t out_dtype, void* stream) {
   if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   fmkv::AttnArgs a;
   int rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
-                                   n_q_heads, scale, tau, out, out_dtype, 0, &a);
+                                   n_q_heads, scale, tau, out, out_dtype, 0, s, &a);
   if (rc || n_seqs == 0) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   hipEvent_t e0, e1;
   next_events(&e0, &e1);
   hipError_t e = launch_attention(a, n_seqs, p->desc.n_kv_heads, s, e0, e1);
@@ -1483,11 +1506,11 @@ int paged_decode_step_impl(fmkv_pool* p, const void* k, const void* v,
   // one new token per sequence: the attention launch appends it itself, at
   // position seq_lens[s] - 1 (= start_pos[s])
   const int fused = n_new == 1 ? 1 : 0;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
   fmkv::AttnArgs at;
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
-                               n_q_heads, scale, tau, out, out_dtype, fused, &at, win, sinks);
+                               n_q_heads, scale, tau, out, out_dtype, fused, s, &at, win, sinks);
   if (rc || n_seqs == 0) return rc;
-  const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e;
   if (fused) {
     at.k_new = ap.k;

@@ -347,9 +347,9 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
  * infinities and NaN included, does not reach an output. A sequence of length
  * 0 gets zeros. The current GPU has to be the pool's. Calls on one pool share
  * its workspace, so calls on several streams, and replays of graphs that
- * captured them, have to be ordered by the caller; a workspace that a later,
- * larger call outgrows stays until the pool is destroyed, so captured calls
- * stay valid. (A prefill call that is split over its keys holds its partial rows
+ * captured them, have to be ordered by the caller; a workspace that captured
+ * calls use stays until the pool is destroyed when a later, larger call outgrows
+ * it, so they stay valid. (A prefill call that is split over its keys holds its partial rows
  * there, too, where it is captured or they take 8 MiB at most, and else in the
  * GPU's shared buffer: see fmkv_prefill_step.) */
 

@@ -1,5 +1,6 @@
-"""The workspace of a pool's decode calls: growth takes no more than the call needs
-where memory is short."""
+"""The workspace of a pool's decode calls: what eager calls outgrow is freed, what
+captured calls use stays, and growth takes no more than the call needs where
+memory is short."""
 import pytest
 import torch
 
@@ -60,7 +61,66 @@ def free():
     return torch.cuda.mem_get_info()[0]
 
 
-@pytest.mark.parametrize("captured", [True])
+@pytest.mark.parametrize("windowed", [True, False])
+def test_eager_calls_keep_one_workspace(server, windowed):
+    """Batches that grow a little each time: the pool holds the last one's partials."""
+    sizes = [16, 18, 21, 24, 27, 31]
+    calls = [(a, server.q.new_empty(a[0].shape), server.alone(a, windowed)) for a in map(server.args, sizes)]
+    before = free()
+    for a, out, want in calls:
+        server.run(a, windowed, out=out)
+        assert before - free() <= a[0].shape[0] * server.PER + (24 << 20)
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("windowed", [True, False])
+def test_captured_calls_keep_theirs(server, windowed):
+    """Graphs of three sizes, each outgrown by the next and by eager calls: replays
+    stay right, and all buffers together stay below three times the last."""
+    sizes = (8, 9, 20)
+    calls = [(a, server.alone(a, windowed)) for a in map(server.args, sizes)]
+    eager = server.args(13)
+    eager_want = server.alone(eager, windowed)
+    before = free()
+    graphs = []
+    for n, (a, want) in zip(sizes, calls):
+        out = torch.zeros_like(a[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            server.run(a, windowed, out=out)
+        graphs.append((g, out, want))
+        server.run(server.args(n + 1), windowed)
+    server.run(server.args(40), windowed)
+    assert before - free() <= 3 * 40 * server.PER + (128 << 20)  # (torch's own besides)
+    for _ in range(3):
+        for g, out, want in graphs:
+            out.zero_()
+            g.replay()
+            assert torch.equal(server.run(eager, windowed), eager_want)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+
+
+def test_growth_while_another_stream_captures(server):
+    """An eager call outgrows the workspace inside another stream's capture: the
+    capture survives, and the call's result is the usual one."""
+    want = server.run(server.args(1), True)
+    small, large = server.args(3), server.args(11)
+    outs = [torch.zeros_like(a[0]) for a in (small, large)]
+    server.run(small, True, out=outs[0])
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    eager, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        server.pool.window_attention(*large, BLOCKS * 16, 0, 0.02, out=outs[1], stream=eager)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert bool((outs[1] == want).all()) and bool((outs[0] == want).all()) and x.tolist() == [3.0] * 4
+
+
+@pytest.mark.parametrize("captured", [False, True])
 def test_growth_where_memory_is_short(server, captured):
     """A call a tenth larger than the one before, on a card that has no room for half
     as much again: eager calls need room for one workspace, captured ones for both."""
