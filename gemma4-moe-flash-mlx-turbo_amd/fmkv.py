@@ -286,10 +286,16 @@ def _on(stream):
     return torch.cuda.stream(stream)
 
 
+# The current stream's handle alone: making a torch.cuda.Stream takes longer than a
+# launch. (Not a public name of torch's: where it is missing, the public way.)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream) -> int | None:
     if stream is None:
-        # (the handle alone: making a torch.cuda.Stream takes longer than a launch)
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        if _raw_stream is None:
+            return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
