@@ -93,8 +93,11 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(AppendArgs a) {
     if (bx >= count) return;
     lb = (first + bx) % nb_ring;
   } else {
-    const int64_t first = pos0 / kBlockTokens, last = (end - 1) / kBlockTokens;
-    if (bx > last - first) return;
+    // (positions below 0, a padded row's of a batch, are not stored: the table
+    // entries before a sequence's first are another's)
+    if (e0 < 0) e0 = 0;
+    const int64_t first = e0 / kBlockTokens, last = (end - 1) / kBlockTokens;
+    if (end <= e0 || bx > last - first) return;
     lb = first + bx;
   }
 

@@ -375,7 +375,9 @@ void prefill_attn_kernel(PrefillArgs a) {
   const int64_t wg_lo = lo_of(pA), wg_hi = pB;
   const int64_t b_lo = wg_lo / kBlockTokens, b_hi = wg_hi / kBlockTokens;
   const int64_t ps = a.p_split;
-  // (WIN: last block with keys < sinks; virtual block i < n_old is block i)
+  // (WIN: last block with keys < sinks; virtual block i < n_old is block i. A tile
+  // of negative positions, a padded row's, has n_old and nst of 0 or less: one step
+  // of keys from 0 on, past every row)
   int64_t old_last = ((WIN ? a.sinks : ps) + kBlockTokens - 1) / kBlockTokens - 1;  // last block with keys < ps
   if (old_last > b_hi) old_last = b_hi;
   const int64_t n_old = WIN ? old_last + 1 : old_last >= b_lo ? old_last - b_lo + 1 : 0;

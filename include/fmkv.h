@@ -261,7 +261,8 @@ int fmkv_pool_destroy(fmkv_pool* pool);
 /* Append n_new tokens to each of n_seqs sequences. k/v: bf16
  * [n_seqs][n_new][n_kv_heads][head_dim]. block_tables: int32 device
  * [n_seqs][max_blocks]; start_pos: int32 device [n_seqs], the position of
- * each sequence's first new token. */
+ * each sequence's first new token. Positions below 0 (a padded row's), past the
+ * table's width or of blocks outside the pool are not written. */
 int fmkv_paged_append(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
                       const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
                       int32_t n_seqs, int32_t n_new, void* stream);
@@ -345,7 +346,7 @@ int fmkv_paged_prefill_step_bounded(fmkv_pool* pool, const void* k_bf16, const v
  * pages between the sinks and the window of the earliest query can be given
  * to other sequences (entries -1, say). What hidden slots of a block hold,
  * infinities and NaN included, does not reach an output. A sequence of length
- * 0 gets zeros. The current GPU has to be the pool's. Calls on one pool share
+ * 0 gets zeros, as does a prefill query at a position below 0. The current GPU has to be the pool's. Calls on one pool share
  * its workspace, so calls on several streams, and replays of graphs that
  * captured them, have to be ordered by the caller; a workspace that captured
  * calls use stays until the pool is destroyed when a later, larger call outgrows
