@@ -1946,7 +1946,9 @@ int fmkv_pages_fork(fmkv_pages* p, const int32_t* blocks, int64_t n_tokens, int3
   if (!p || !copy_src || !copy_dst || (n_tokens > 0 && (!blocks || !child)))
     return fail(FMKV_ERR_INVALID_ARG, "pages/blocks/child/copy_src/copy_dst are null");
   const int64_t n = (n_tokens + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
-  const bool part = n_tokens % fmkv::kBlockTokens != 0 && blocks[n - 1] != -1;
+  const bool part = n_tokens % fmkv::kBlockTokens != 0;
+  if (part && blocks[n - 1] == -1)
+    return fail(FMKV_ERR_INVALID_ARG, "the block that the sequence would go on in was given back");
   for (int64_t i = 0; i < n; i++) {
     if (blocks[i] == -1) continue;
     const int rc = check_block(p, blocks[i]);

@@ -438,7 +438,7 @@ int fmkv_pages_release(fmkv_pages* pages, const int32_t* blocks, int64_t n);
  * blocks (ceil(n_tokens / 16) of them), whole ones shared, a partly filled last
  * one replaced by a free block. *copy_src and *copy_dst name the copy that
  * fmkv_pools_copy_blocks then has to make (-1: none). Entries of -1 (blocks
- * given back) stay -1. n_tokens is below 2^31 (here and in the next call). */
+ * given back) stay -1; a partly filled last one among them is refused. n_tokens is below 2^31 (here and in the next call). */
 int fmkv_pages_fork(fmkv_pages* pages, const int32_t* blocks, int64_t n_tokens, int32_t* child,
                     int32_t* copy_src, int32_t* copy_dst);
 /* Gives back the blocks of a sequence of n_tokens that no later query sees

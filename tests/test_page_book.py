@@ -197,3 +197,16 @@ def test_sequences_past_32_bit_positions_are_refused(n_tokens):
     assert lib.fmkv_pages_slide(book._h, blocks, n_tokens, 16, 0, ctypes.byref(freed)) == fmkv.FMKV_ERR_INVALID_ARG
     assert list(blocks) == [0, 1] and list(child) == [7, 7] and (src.value, dst.value, freed.value) == (5, 5, 5)
     assert [book.users(b) for b in range(4)] == [1, 1, 0, 0] and book.free_count() == 2
+
+
+def test_fork_behind_the_window_is_refused():
+    """A fork from a position in a block that was given back: its tokens are gone, and
+    the next one would be stored nowhere."""
+    book = fmkv.PageBook(8)
+    a = book.slide(book.alloc(4), 64, 17)
+    for n in (1, 17, 33, 47):
+        with pytest.raises(fmkv.Exception_) as e:
+            book.fork(a, n)
+        assert e.value.code == fmkv.FMKV_ERR_INVALID_ARG
+    assert book.free_count() == 7 and book.users(a[3]) == 1
+    assert book.fork(a, 48) == ([-1, -1, -1], None)
