@@ -729,8 +729,10 @@ int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
 // each number of rounds are as many as fit it, or as the combine allows, and
 // equal; the cheapest wins. (us per call, by blocks per split: one sequence,
 // 66 blocks of 4 bits, 256 dims, 8 heads: 1: 20.1, 2: 15.4, 3: 10.9, 8: 11.0, 16:
-// 13.0; seven of 254 blocks, 8 bits, 512 dims, 2 heads: 14, which leaves 10
-// work-groups to a second round: 28.6, 16: 22.8, 32: 27.1; 32 ragged ones of up
+// 13.0; seven of 254 blocks each, 8 bits, 512 dims, 2 heads: 14, which leaves 10
+// work-groups to a second round: 28.7, 15, what this comes to: 23.6, 16: 23.0, 32:
+// 27.1; seven ragged ones within that bound, whose short ones leave room in the
+// first round: 14: 21.2, 15: 21.9, 16: 21.4; 32 ragged ones of up
 // to 258 blocks, 4 bits: 64 (4 splits and one of 2 blocks): 60.2, 86: 51.4, 129:
 // 53.9; the same all at 258: 66.5, 65.7, 63.9; one of 254 blocks, 2 heads of 512
 // dims: 2: 17.0, 4: 15.5, 8: 16.8, 16: 19.6.)

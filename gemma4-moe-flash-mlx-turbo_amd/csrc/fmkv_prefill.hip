@@ -22,8 +22,12 @@
 //
 // What bounds it: the issue of matrix and vector instructions together. A
 // 16x16x32 MFMA alone takes 8.7 ns of a SIMD, with four independent FMAs after
-// it 12.4 ns (the FMAs alone: 5): they hardly overlap, also between the two
-// waves of a SIMD. Of the 2.5 us of a step of a SIMD (8 bits, head_dim 512)
+// it 12.4 ns (the FMAs alone: 5): in one wave they hardly overlap. One wave's
+// products and the other's vector work do in part, more where products go first
+// (the pipeline's priorities, up to 12%): of the busy cycles of a 2048-token
+// chunk after 32768 positions (8 bits, head_dim 512) the matrix cores' are 36%,
+// vector instructions at four cycles each 46%; on a window of 1024 (4 bits,
+// head_dim 256) 27 and 59%. Of the 2.5 us of a step of a SIMD (8 bits, 512)
 // its 128 MFMAs are 1.1 us, the conversion of codes and weights, the scales
 // and the softmax the rest. Hence the packed f16 arithmetic on the weights
 // (v_pk_* 1.9 ns for two elements; v_fma_mixlo_f16 3.7 ns for one).
@@ -1164,7 +1168,10 @@ void prefill_attn_kernel(PrefillArgs a) {
   // alike 125.5; after 6000 positions, 8 bits: 645 and 718. 512 dims, 16 / 2 heads,
   // after 6000, 8 bits: QK alone 1226, both 1249, neither 1248; bf16: 1127, 1099,
   // 1128; 4-bit codebook, window: 405, 386, 406. 128 dims, after 6000, 8 bits: 358,
-  // 366, 366; bf16: 400, 405, 387; 3-bit codebook: 440, 462, 431.)
+  // 366, 366; bf16: 400, 405, 387; 3-bit codebook: 440, 462, 431. The other caches of
+  // 256 dims, 2048 tokens after 6000 positions, these and none: 2-bit codebook 613 and
+  // 644, 3 bits 629 and 667, 4 bits 944 and 963, bf16 636 and 646; window 1024: 105 and
+  // 112, 110 and 114, 137 and 144, 106 and 107.)
   constexpr bool kQkFirst = D > 128 || MODE == kAffine;
   constexpr bool kPvFirst = D == 256 || (D == 512 && MODE != kAffine);
 #pragma unroll 1
