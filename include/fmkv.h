@@ -277,7 +277,11 @@ int fmkv_paged_append_projected(fmkv_pool* pool, const void* k_proj_bf16, const 
 /* Decode attention for n_seqs sequences; seq_lens: int32 device [n_seqs]
  * (positions visible, current token included); max_seq_len bounds them.
  * q: bf16 [n_seqs][n_q_heads][head_dim]; out: [n_seqs][n_q_heads][head_dim].
- * scale and sparse_v_tau as in fmkv_decode_attention. */
+ * scale and sparse_v_tau as in fmkv_decode_attention. The slots of a last block
+ * past its sequence's length count with weight 0 here and in the decode steps
+ * below, so what they hold (of a block's earlier owner, say) has to be finite, as
+ * appends of finite rows leave it; the prefill calls and the windowed ones
+ * (fmkv_paged_window_decode_attention) take anything there. */
 int fmkv_paged_decode_attention(fmkv_pool* pool, const void* q_bf16, const int32_t* block_tables,
                                 int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
                                 int32_t max_seq_len, int32_t n_q_heads, float scale,
