@@ -571,11 +571,11 @@ int prepare_attention_common(Owner* o, const fmkv::Store& st, int32_t n_seqs, in
   plan_splits(o->cus, H, n_seqs, nblk, wg_per_cu, min_bps, first_mult, new_col,
               st.block_table != nullptr, a);
   a->new_col = new_col;
-  a->part_stride = a->max_splits + new_col;
+  a->part_stride = a->prefix.slots + a->max_splits + new_col;
   // sparse-V (tau > 0) always goes through the split partials and the
   // combine, which normalises by the stats pass's full softmax sum
   a->tau = tau;
-  a->direct = a->max_splits == 1 && !new_col && tau == 0.0f;
+  a->direct = a->max_splits == 1 && !new_col && tau == 0.0f && !a->prefix.lens && a->score_blocks == 0;
   a->k_new = a->v_new = nullptr;
   a->out = out;
   a->out_f32 = out_dtype == FMKV_DTYPE_F32;
@@ -600,8 +600,10 @@ int prepare_attention_common(Owner* o, const fmkv::Store& st, int32_t n_seqs, in
   const size_t cnt_off = score_off + 16 * n_blk;
   const size_t need_gather = (cnt_off + (size_t)n_seqs * n_q_heads) * sizeof(float);
   if (gather && ext.ptr && need_gather > ext.bytes) gather = false;
-  const size_t need =
-      gather ? need_gather : (n_blk ? blk_off + n_blk : stat_off + n_stat_ml) * sizeof(float);
+  size_t need = gather ? need_gather : (n_blk ? blk_off + n_blk : stat_off + n_stat_ml) * sizeof(float);
+  // the scores whose weights are accumulated (without sparse-V), 16-byte aligned
+  if (a->score_blocks > 0)
+    need = (blk_off + (size_t)n_seqs * a->score_blocks * n_q_heads * fmkv::kBlockTokens) * sizeof(float);
   float* ws = ext.ptr;
   if (ws) {
     if (need > ext.bytes)
@@ -632,6 +634,7 @@ int prepare_attention_common(Owner* o, const fmkv::Store& st, int32_t n_seqs, in
   }
   a->part_o = n_rows ? ws : nullptr;
   a->part_ml = n_rows ? ws + n_rows * D : nullptr;
+  a->scores = a->score_blocks > 0 ? ws + blk_off : nullptr;
   a->tau_stats = n_stats ? ws + n_rows * (D + 2) : nullptr;
   a->stat_ml = n_stat_ml ? ws + stat_off : nullptr;
   a->blk_max = n_blk ? ws + blk_off : nullptr;
@@ -692,6 +695,25 @@ int check_device(const fmkv_pool* p) {
   if (dev != p->device)
     return fail(FMKV_ERR_INVALID_ARG, "the pool is on GPU " + std::to_string(p->device) +
                                           ", the current GPU is " + std::to_string(dev));
+  return FMKV_OK;
+}
+
+// [a, a + an) and [b, b + bn) have bytes in common.
+bool overlaps(const void* a, int64_t an, const void* b, int64_t bn) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + (uintptr_t)bn && y < x + (uintptr_t)an;
+}
+
+// The buffers of accumulated weights: one of them, or two apart.
+int check_weights(int32_t n_seqs, int32_t max_seq_len, const float* weights, const float* weights_out,
+                  int32_t weights_width) {
+  if (n_seqs <= 0) return FMKV_OK;
+  if (!weights_out) return fail(FMKV_ERR_INVALID_ARG, "weights_out is null");
+  if (weights_width < 1 || weights_width < max_seq_len)
+    return fail(FMKV_ERR_INVALID_ARG, "weights_width must be at least 1 and max_seq_len");
+  const int64_t bytes = (int64_t)n_seqs * weights_width * 4;
+  if (weights && weights != weights_out && overlaps(weights, bytes, weights_out, bytes))
+    return fail(FMKV_ERR_INVALID_ARG, "weights and weights_out overlap in part");
   return FMKV_OK;
 }
 
@@ -768,7 +790,12 @@ int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows
   return pairs < 8 && (nblk + pairs - 1) / pairs * rows <= cus ? pairs : best(3, 8);
 }
 
-// win > 0: over the last `win` positions and the first `sinks` ones.
+// Everything that a sequence holds, to the calls that run as windowed ones.
+constexpr int32_t kNoWindow = INT32_MAX;
+
+// win > 0: over the last `win` positions and the first `sinks` ones. a->prefix: what
+// lies behind a batch's shared prefixes, max_seq_len that part's bound;
+// a->score_blocks > 0: with the scores stored.
 int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
                             int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
                             int32_t max_seq_len, int32_t n_q_heads, float scale, float tau,
@@ -798,7 +825,7 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   a->win = win;
   a->sinks = sinks;
   int64_t nblk = ((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
-  if (win > 0) nblk = std::min(nblk, window_blocks(win, sinks));
+  if (win > 0 && win != kNoWindow) nblk = std::min(nblk, window_blocks(win, sinks));
   // Ragged lengths: the bound counts every sequence at max_seq_len, so the
   // plan aims at several work-groups per CU (the dispatcher balances their
   // uneven sizes), but at least 64 blocks each (a work-group's prologue and
@@ -1569,6 +1596,198 @@ int fmkv_paged_decode_step_projected(fmkv_pool* p, const void* k_proj, const voi
   return paged_decode_step_impl(p, k_proj, v_proj, block_tables, max_blocks, start_pos, seq_lens,
                                 n_seqs, n_new, max_seq_len, q, n_q_heads, scale, tau, out,
                                 out_dtype, stream, pro);
+}
+
+}  // extern "C"
+
+namespace {
+
+// Decode attention of a batch in groups that share prefixes: the prefixes' partials,
+// then what each sequence has behind its own, and the merge. step: with the append of one
+// new token per sequence.
+int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, const void* q,
+                       const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
+                       const int32_t* seq_lens, int32_t n_seqs, const int32_t* prefix_lens,
+                       const int32_t* group_starts, int32_t n_groups, int32_t max_prefix_len,
+                       int32_t max_rest_len, int32_t n_q_heads, float scale, void* out,
+                       int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  if (n_groups < 0 || n_groups > 65535 || max_prefix_len < 0)
+    return fail(FMKV_ERR_INVALID_ARG, "n_groups must be in [0, 65535] and max_prefix_len >= 0");
+  if (n_seqs > 0 && (!prefix_lens || !group_starts))
+    return fail(FMKV_ERR_INVALID_ARG, "prefix_lens/group_starts are null");
+  int rc;
+  fmkv::AppendArgs ap;
+  int tasks = 0;
+  if (step && (rc = prepare_paged_append(p, k, v, block_tables, max_blocks, start_pos, n_seqs, 1, &ap, &tasks)))
+    return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (n_seqs < 0 || max_blocks < 1) return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / max_blocks");
+  if (n_seqs == 0) return FMKV_OK;
+  if ((rc = check_attn_args(p->desc, q, n_q_heads, 0.0f, out, out_dtype))) return rc;
+  fmkv::PrefillArgs pa;
+  pa.old_st = pa.new_st = pool_store(p, block_tables, max_blocks);
+  pa.p0 = 0;
+  pa.start_pos = nullptr;
+  pa.n_seqs = n_seqs;
+  pa.n_q = 1;
+  pa.window = pa.ring_slots = pa.vis_begin = pa.p_split = pa.new_blk0 = 0;
+  pa.group = n_q_heads / p->desc.n_kv_heads;
+  pa.n_q_heads = n_q_heads;
+  pa.q = static_cast<const uint16_t*>(q);
+  pa.qscale = scale * 1.4426950408889634f;
+  std::memcpy(pa.sign_bits, p->sign_bits, sizeof(pa.sign_bits));
+  pa.c = p->c;
+  pa.out = nullptr;
+  pa.out_f32 = 0;
+  pa.seq_lens = seq_lens;
+  pa.new_col = step ? 1 : 0;
+  pa.prefix.lens = prefix_lens;
+  pa.prefix.starts = group_starts;
+  pa.prefix.n_groups = n_groups;
+  const int64_t most = std::min<int64_t>(max_prefix_len, (int64_t)max_blocks * fmkv::kBlockTokens);
+  if (n_groups > 0) fmkv::prefix_plan(pa, p->cus, most / 32 + 1);
+  fmkv::AttnArgs at;
+  at.prefix = pa.prefix;
+  rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_rest_len,
+                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
+  if (rc) return rc;
+  if (step) {
+    at.k_new = ap.k;
+    at.v_new = ap.v;
+  }
+  hipError_t e = hipSuccess;
+  if (n_groups > 0) {
+    pa.part_o = at.part_o;
+    pa.part_ml = at.part_ml;
+    pa.part_stride = at.part_stride;
+    e = fmkv::launch_prefix_attention(pa, s);
+    if (e != hipSuccess) return hip_fail(e, "prefix attention launch");
+  }
+  hipEvent_t e0, e1;
+  next_events(&e0, &e1);
+  e = launch_attention(at, n_seqs, p->desc.n_kv_heads, s, e0, e1);
+  if (e != hipSuccess) return hip_fail(e, "paged prefix attention launch");
+  return FMKV_OK;
+}
+
+// Decode attention with accumulated weights. step: with the append of one new
+// token per sequence.
+int weighing_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, const void* q,
+                         const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
+                         const int32_t* seq_lens, int32_t n_seqs, int32_t max_seq_len,
+                         const float* weights, float* weights_out, int32_t weights_width,
+                         int32_t n_q_heads, float scale, void* out, int32_t out_dtype, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  int rc = check_weights(n_seqs, max_seq_len, weights, weights_out, weights_width);
+  if (rc) return rc;
+  fmkv::AppendArgs ap;
+  int tasks = 0;
+  if (step && (rc = prepare_paged_append(p, k, v, block_tables, max_blocks, start_pos, n_seqs, 1, &ap, &tasks)))
+    return rc;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  fmkv::AttnArgs at;
+  at.score_blocks = std::max<int64_t>(((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens, 1);
+  rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
+                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
+  if (rc || n_seqs == 0) return rc;
+  at.weights_in = weights;
+  at.weights_out = weights_out;
+  at.weights_width = weights_width;
+  if (step) {
+    at.k_new = ap.k;
+    at.v_new = ap.v;
+  }
+  hipEvent_t e0, e1;
+  next_events(&e0, &e1);
+  const hipError_t e = launch_attention(at, n_seqs, p->desc.n_kv_heads, s, e0, e1);
+  if (e != hipSuccess) return hip_fail(e, "paged weighing attention launch");
+  return FMKV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fmkv_paged_prefix_decode_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
+                                       int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
+                                       const int32_t* prefix_lens, const int32_t* group_starts,
+                                       int32_t n_groups, int32_t max_prefix_len, int32_t max_rest_len,
+                                       int32_t n_q_heads, float scale, void* out, int32_t out_dtype,
+                                       void* stream) {
+  return prefix_decode_impl(p, false, nullptr, nullptr, q, block_tables, max_blocks, nullptr, seq_lens,
+                            n_seqs, prefix_lens, group_starts, n_groups, max_prefix_len, max_rest_len,
+                            n_q_heads, scale, out, out_dtype, stream);
+}
+
+int fmkv_paged_prefix_decode_step(fmkv_pool* p, const void* k, const void* v,
+                                  const int32_t* block_tables, int32_t max_blocks,
+                                  const int32_t* start_pos, const int32_t* seq_lens, int32_t n_seqs,
+                                  const int32_t* prefix_lens, const int32_t* group_starts,
+                                  int32_t n_groups, int32_t max_prefix_len, int32_t max_rest_len,
+                                  const void* q, int32_t n_q_heads, float scale, void* out,
+                                  int32_t out_dtype, void* stream) {
+  return prefix_decode_impl(p, true, k, v, q, block_tables, max_blocks, start_pos, seq_lens, n_seqs,
+                            prefix_lens, group_starts, n_groups, max_prefix_len, max_rest_len,
+                            n_q_heads, scale, out, out_dtype, stream);
+}
+
+int fmkv_paged_weighing_decode_attention(fmkv_pool* p, const void* q, const int32_t* block_tables,
+                                         int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
+                                         int32_t max_seq_len, const float* weights, float* weights_out,
+                                         int32_t weights_width, int32_t n_q_heads, float scale,
+                                         void* out, int32_t out_dtype, void* stream) {
+  return weighing_decode_impl(p, false, nullptr, nullptr, q, block_tables, max_blocks, nullptr, seq_lens,
+                              n_seqs, max_seq_len, weights, weights_out, weights_width, n_q_heads, scale,
+                              out, out_dtype, stream);
+}
+
+int fmkv_paged_weighing_decode_step(fmkv_pool* p, const void* k, const void* v,
+                                    const int32_t* block_tables, int32_t max_blocks,
+                                    const int32_t* start_pos, const int32_t* seq_lens, int32_t n_seqs,
+                                    int32_t max_seq_len, const void* q, const float* weights,
+                                    float* weights_out, int32_t weights_width, int32_t n_q_heads,
+                                    float scale, void* out, int32_t out_dtype, void* stream) {
+  return weighing_decode_impl(p, true, k, v, q, block_tables, max_blocks, start_pos, seq_lens, n_seqs,
+                              max_seq_len, weights, weights_out, weights_width, n_q_heads, scale, out,
+                              out_dtype, stream);
+}
+
+int fmkv_heaviest_tokens(const float* weights, int32_t weights_width, const int32_t* seq_lens,
+                         int32_t n_seqs, int32_t max_keep, int32_t sinks, int32_t recent,
+                         int32_t* keep, int32_t* n_keep, float* kept_weights, int32_t kept_width,
+                         void* stream) {
+  if (n_seqs < 0 || n_seqs > 65535) return fail(FMKV_ERR_INVALID_ARG, "n_seqs must be in [0, 65535]");
+  if (weights_width < 1 || weights_width > (1 << 30))
+    return fail(FMKV_ERR_INVALID_ARG, "weights_width must be in [1, 2^30]");
+  if (max_keep < 1 || max_keep > (1 << 28) - 16)
+    return fail(FMKV_ERR_INVALID_ARG, "max_keep must be in [1, 2^28 - 16]");
+  if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > max_keep)
+    return fail(FMKV_ERR_INVALID_ARG, "sinks and recent must be >= 0 and together at most max_keep");
+  if (n_seqs == 0) return FMKV_OK;
+  if (!weights || !seq_lens || !keep || !n_keep)
+    return fail(FMKV_ERR_INVALID_ARG, "weights/seq_lens/keep/n_keep are null");
+  if (kept_weights) {
+    if (kept_width < max_keep) return fail(FMKV_ERR_INVALID_ARG, "kept_width must be at least max_keep");
+    if (overlaps(weights, (int64_t)n_seqs * weights_width * 4, kept_weights, (int64_t)n_seqs * kept_width * 4))
+      return fail(FMKV_ERR_INVALID_ARG, "kept_weights overlaps weights");
+  }
+  fmkv::HeaviestArgs a;
+  a.weights = weights;
+  a.width = weights_width;
+  a.seq_lens = seq_lens;
+  a.max_keep = max_keep;
+  a.sinks = sinks;
+  a.recent = recent;
+  a.keep = keep;
+  a.n_keep = n_keep;
+  a.kept = kept_weights;
+  a.kept_width = kept_width;
+  const hipError_t e = fmkv::launch_heaviest(a, n_seqs, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return hip_fail(e, "heaviest tokens launch");
+  return FMKV_OK;
 }
 
 int fmkv_pools_copy_blocks(fmkv_pool* const* pools, int32_t n_pools, const int32_t* src,

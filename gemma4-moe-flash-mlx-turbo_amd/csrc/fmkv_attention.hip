@@ -63,6 +63,7 @@
 #include "fmkv_prologue.h"
 #include "fmkv_quant.h"
 #include "fmkv_attn_common.h"
+#include "fmkv_combine.h"
 
 namespace fmkv {
 namespace {
@@ -473,9 +474,9 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // per KV head -- the 16 matrix-core columns carry (group, head, high /
   // residual) instead of (head, high / residual), so each lane forms the
   // scores and P' of one group only (build_q_table)
-  static_assert(!PACK || ((MODE == kDense || MODE == kWindow) && P::kSolo && D == 256 && BITS == 4),
+  static_assert(!PACK || ((MODE == kDense || windowed(MODE)) && P::kSolo && D == 256 && BITS == 4),
                 "packed columns: dense solo streams, head_dim 256, 4 bits");
-  static_assert(MODE != kWindow || PAGED, "a window with sinks is a paged pool's");
+  static_assert(!windowed(MODE) || PAGED, "a window with sinks is a paged pool's");
   constexpr int E = D / 64;
   constexpr int QS = P::kQS;
   // copy instructions per wave per block (the stats pass copies no V codes)
@@ -523,11 +524,11 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // kWindow: blocks below are numbered over the visible ones, wg.block(v) is
   // the sequence's own number
   WinGeom wg{};
-  if constexpr (MODE == kWindow) {
-    wg = win_geometry(Tg, a.win, a.sinks, a.st.table_stride);
+  if constexpr (windowed(MODE)) {
+    wg = attn_window(a, seq, Tg);
     geo = wg.geo;
   }
-  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
+  auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   // one sequence: the host planned max_splits for exactly this block range
   // (no division before the first copies); paged: per sequence
   const int n_splits = PAGED ? n_splits_for(geo, bps0, bps, max_splits, skew_p) : max_splits;
@@ -577,7 +578,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   int tsh = 0;
   if constexpr (PAGED) {
     n_tbl = b_end - b_begin;
-    if constexpr (MODE == kWindow) {
+    if constexpr (windowed(MODE)) {
       const int64_t v0 = b_begin < wg.sink_blks ? wg.sink_blks : b_begin;
       tbl0 = v0 + wg.skip;
       n_tbl = b_end - v0;
@@ -863,7 +864,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
     // only at the edges of the visible range
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
@@ -874,21 +875,21 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
       uint8_t* const vmeta_c =
           const_cast<uint8_t*>(sp) + P::kMetaOff + half * 2 * MH + MH + c * 64 + j * 16;
       u32x4 m = (u32x4){0, 0, 0, 0};
-      if (MODE == kWindow && c < GH) m = lds16(vmeta_c);
+      if (windowed(MODE) && c < GH) m = lds16(vmeta_c);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int64_t slot = t0 + 4 * j + i;
-        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+        bool vis = (windowed(MODE) ? (slot >= wg.lo || slot < a.sinks) && slot < T
                                     : slot >= vis_lo && slot < vis_hi) &&
                    slot != ex_slot;
-        if (MODE != kWindow && ring_trim)
+        if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if (!vis) {
           s[i] = -INFINITY;
           m[i] = 0;
         }
       }
-      if constexpr (MODE == kWindow) {
+      if constexpr (windowed(MODE)) {
         if (c < GH) *reinterpret_cast<u32x4*>(vmeta_c) = m;
         vm = lds16(sp + P::kMetaOff + half * 2 * MH + MH + (PACK ? grp * 64 : 0) + j * 16);
       }
@@ -897,6 +898,9 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
 #pragma unroll
       for (int i = 0; i < 4; i++) s[i] = s[i] >= theta ? s[i] : -INFINITY;
     }
+    if constexpr (MODE == kWeigh)
+      if (half == 0 && hi && col_valid && (!PACK || grp == 0))
+        store_scores(a, seq, b, kvh * G + head, j, s);
     float mb = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     mb = xor16_max(mb);
     mb = xor32_max(mb);
@@ -1167,10 +1171,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   }
 }
 
-// out[seq][h][d] = sum_s 2^(m_s - M) O_s[d] / sum_s 2^(m_s - M) l_s.
-// One work-group per (64 dims, q head, sequence); thread (sl, dq) owns dims
-// d0 + 4*dq .. +3 and splits sl, sl + 16, ..., merged in one pass with a
-// running maximum; the 16 partial merges meet in LDS.
+// The split merge (combine_rows), grid (64 dims, q head, sequence).
 // Arguments: as the split kernel's, what the kernel needs first comes as
 // leading scalars (preloaded into SGPRs with the dispatch), the struct last.
 // n_cols: split partials per sequence (splits and new-token column), or -1
@@ -1181,79 +1182,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* part_o, const
                                                       void* out, int32_t n_cols,
                                                       int32_t part_stride, uint32_t flags,
                                                       AttnArgs a) {
-  __shared__ float4_t red_o[16][16];
-  __shared__ float red_m[16][16];
-  __shared__ float red_l[16][16];
-  const int seq = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-  const int dq = tid & 15, sl = tid >> 4;
-  const int d0 = blockIdx.x * 64 + dq * 4;
-  const int nqh = (int)(flags >> 8);
-  int n_splits = n_cols;
-  if (n_cols < 0) {
-    const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
-    const SeqGeom geo =
-        a.win > 0 ? win_geometry(T, a.win, a.sinks, a.st.table_stride).geo
-                  : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
-    n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p) + a.new_col;
-  }
-  const int64_t stride = (int64_t)nqh;
-  const int64_t base = (int64_t)seq * part_stride * stride + h;
-
-  // split maxima are finite (the split kernel starts from -1e30): the first
-  // merge scales the empty state by exp2(-inf) = 0
-  float M = -INFINITY, den = 0.0f;
-  float4_t acc = (float4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = sl; s < n_splits; s += 16) {
-    const int64_t r = base + s * stride;
-    const float2 ml = *reinterpret_cast<const float2*>(part_ml + r * 2);
-    const float4_t ov = *reinterpret_cast<const float4_t*>(part_o + r * D + d0);
-    const float mn = fmaxf(M, ml.x);
-    const float alpha = exp2f(M - mn);
-    const float w = exp2f(ml.x - mn);
-    den = fmaf(w, ml.y, den * alpha);
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = fmaf(w, ov[i], acc[i] * alpha);
-    M = mn;
-  }
-  red_o[sl][dq] = acc;
-  red_m[sl][dq] = M;
-  red_l[sl][dq] = den;
-  __syncthreads();
-  if (tid < 16) {
-    float Mx = red_m[0][tid];
-#pragma unroll
-    for (int k = 1; k < 16; k++) Mx = fmaxf(Mx, red_m[k][tid]);
-    float4_t s = (float4_t){0.f, 0.f, 0.f, 0.f};
-    float L = 0.0f;
-    if (Mx != -INFINITY) {
-#pragma unroll
-      for (int k = 0; k < 16; k++) {
-        const float w = exp2f(red_m[k][tid] - Mx);  // 0 for slots without splits (-inf)
-        s += w * red_o[k][tid];
-        L = fmaf(w, red_l[k][tid], L);
-      }
-    }
-    const int64_t o_idx = ((int64_t)seq * nqh + h) * D + blockIdx.x * 64 + tid * 4;
-    // sparse-V: the kept weights are normalised by the full sum L of the
-    // stats pass (no renormalisation, gemma4_attention.rs:226-232), taken at
-    // its max M
-    const bool sparse = (flags & 2u) != 0;
-    float gated = 0.0f;
-    if (sparse) {
-      const int64_t nh = (int64_t)gridDim.z * nqh, r = (int64_t)seq * nqh + h;
-      const float Mf = a.tau_stats[nh + r], Lf = a.tau_stats[2 * nh + r];
-      gated = (Lf > 0.0f && Mx != -INFINITY) ? exp2f(Mx - Mf) / Lf : 0.0f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float v = sparse ? s[i] * gated : (L > 0.0f ? s[i] / L : 0.0f);
-      if (flags & 1u)
-        reinterpret_cast<float*>(out)[o_idx + i] = v;
-      else
-        reinterpret_cast<uint16_t*>(out)[o_idx + i] = f32_to_bf16(v);
-    }
-  }
+  combine_rows<D>(part_o, part_ml, out, n_cols, part_stride, flags, a, blockIdx.x, blockIdx.y,
+                  blockIdx.z, gridDim.z);
 }
 
 // The split kernel of one mode; with events, they are recorded by the
@@ -1280,14 +1210,14 @@ template <int D, int BITS, int MODE>
 hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t ev0, hipEvent_t ev1) {
   // a paged pool has per-sequence lengths; a cache has neither
   if ((a.st.block_table != nullptr) != (a.seq_lens != nullptr)) return hipErrorInvalidValue;
-  if (MODE == kWindow && !a.st.block_table) return hipErrorInvalidValue;
+  if (windowed(MODE) && !a.st.block_table) return hipErrorInvalidValue;
   // (kWindow is a paged pool's: it has no other instances)
   if constexpr (kSoloCapable<D, BITS>) {
     if (a.bps >= kSoloMinBlocks) {
       // head_dim 256 at 4 bits with at most 2 q heads per KV head (Gemma-4's
       // sliding layers): the packed-column form of the solo streams
-      constexpr bool kPacked = (MODE == kDense || MODE == kWindow) && D == 256 && BITS == 4;
-      if constexpr (MODE != kWindow) {
+      constexpr bool kPacked = (MODE == kDense || windowed(MODE)) && D == 256 && BITS == 4;
+      if constexpr (!windowed(MODE)) {
         if (!a.st.block_table) {
           if constexpr (kPacked)
             if (a.group <= 2) return launch_kind<D, BITS, MODE, 12, false, true>(a, grid, s, ev0, ev1);
@@ -1300,7 +1230,7 @@ hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t 
       return launch_kind<D, BITS, MODE, kPagedSoloWaves, true>(a, grid, s, ev0, ev1);
     }
   }
-  if constexpr (MODE != kWindow)
+  if constexpr (!windowed(MODE))
     if (!a.st.block_table) return launch_kind<D, BITS, MODE, 0, false>(a, grid, s, ev0, ev1);
   return launch_kind<D, BITS, MODE, 0, true>(a, grid, s, ev0, ev1);
 }
@@ -1337,7 +1267,12 @@ hipError_t launch_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_t s
       return e;
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
-  e = a.win > 0 ? launch_split<D, BITS, kWindow>(a, grid, s, ev0, ev1)
+  if (a.scores) {
+    e = launch_split<D, BITS, kWeigh>(a, grid, s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  const AttnArgs own = behind_prefix(a);
+  e = a.win > 0 ? launch_split<D, BITS, kWindow>(own, grid, s, ev0, ev1)
                 : launch_split<D, BITS, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);

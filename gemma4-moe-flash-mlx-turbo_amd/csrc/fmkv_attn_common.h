@@ -28,8 +28,26 @@ constexpr float kRescaleSlack = 8.0f;
 // is the dense pass with every score below theta dropped; the combine
 // divides by the full L of the stats pass.
 // kWindow: softmax attention of a paged sequence over its last a.win positions
-// and its first a.sinks ones (WinGeom), tau 0.
-constexpr int kDense = 0, kStats = 1, kGated = 2, kWindow = 3;
+// and its first a.sinks ones, or what is its own behind a shared prefix (WinGeom),
+// tau 0. kWeigh: the same, with every score to a.scores.
+constexpr int kDense = 0, kStats = 1, kGated = 2, kWindow = 3, kWeigh = 4;
+constexpr bool windowed(int mode) { return mode == kWindow || mode == kWeigh; }
+
+// The visible blocks of sequence `seq`, of length T.
+__device__ inline WinGeom attn_window(const AttnArgs& a, int seq, int64_t T) {
+  if (!a.prefix.lens) return win_geometry(T, a.win, a.sinks, a.st.table_stride);
+  const int64_t first = a.prefix.end(seq, T - a.new_col, a.st.table_stride);
+  return win_geometry(T, T > first ? T - first : 0, 0, a.st.table_stride);
+}
+
+// kWeigh: the scores of tokens 4 j .. 4 j + 3 of block b (-inf where hidden)
+// with query head `qh`, [n_seqs][score_blocks][n_q_heads][16].
+__device__ inline void store_scores(const AttnArgs& a, int seq, int64_t b, int qh, int j,
+                                    const float (&s)[4]) {
+  if (b >= a.score_blocks) return;
+  float* p = a.scores + ((((int64_t)seq * a.score_blocks + b) * a.n_q_heads + qh) * kBlockTokens + 4 * j);
+  *reinterpret_cast<float4_t*>(p) = (float4_t){s[0], s[1], s[2], s[3]};
+}
 
 // A stream's visiting order in the gated pass: the set bits of `mask` in
 // increasing order, then next, next + 1, ... below n (scalar values).

@@ -336,10 +336,10 @@ void cb_decode_kernel(AttnArgs a) {
   // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
   // is the sequence's own number
   WinGeom wg{};
-  if constexpr (MODE == kWindow) wg = win_geometry(T, a.win, a.sinks, a.st.table_stride);
-  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
+  if constexpr (windowed(MODE)) wg = attn_window(a, seq, T);
+  auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   const SeqGeom geo =
-      MODE == kWindow
+      windowed(MODE)
           ? wg.geo
           : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
   const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
@@ -375,7 +375,7 @@ void cb_decode_kernel(AttnArgs a) {
   // sparse-V: this (sequence, KV head)'s row of block maxima; the gated pass
   // visits only the blocks holding a score at or above a head's threshold
   const int64_t blk_row =
-      MODE == kDense || MODE == kWindow ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
+      MODE == kDense || windowed(MODE) ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
   BlockList blist{0ull, 0, nb};
   int nbx = nb;  // blocks visited
   if constexpr (MODE == kGated) {
@@ -516,22 +516,22 @@ void cb_decode_kernel(AttnArgs a) {
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int64_t slot = t0 + 4 * j + i;
-        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+        bool vis = (windowed(MODE) ? (slot >= wg.lo || slot < a.sinks) && slot < T
                                     : slot >= vis_lo && slot < vis_hi) &&
                    slot != ex_slot;
-        if (MODE != kWindow && ring_trim)
+        if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if (!vis) {
           sc[i] = -INFINITY;
           // (a hidden token's norm may be anything, and 0 * inf is NaN)
-          if constexpr (MODE == kWindow) vscale[i] = 0.0f;
+          if constexpr (windowed(MODE)) vscale[i] = 0.0f;
         }
       }
     }
@@ -539,6 +539,8 @@ void cb_decode_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; i++) sc[i] = sc[i] >= theta ? sc[i] : -INFINITY;
     }
+    if constexpr (MODE == kWeigh)
+      if (half == 0 && hi && col_valid) store_scores(a, seq, b, kvh * G + head, j, sc);
     // online softmax in base 2 (the affine kernel's rule: the reference max
     // moves only on jumps above kRescaleSlack)
     float mb = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
@@ -755,7 +757,12 @@ hipError_t launch_cb_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
   if (a.win > 0 && !a.st.block_table) return hipErrorInvalidValue;
-  e = a.win > 0 ? launch_cb_mode<D, BITS, kWindow>(a, grid, s, ev0, ev1)
+  if (a.scores) {
+    e = launch_cb_mode<D, BITS, kWeigh>(a, grid, s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  const AttnArgs own = behind_prefix(a);
+  e = a.win > 0 ? launch_cb_mode<D, BITS, kWindow>(own, grid, s, ev0, ev1)
                 : launch_cb_mode<D, BITS, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);

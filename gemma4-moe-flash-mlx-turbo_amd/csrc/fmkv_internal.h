@@ -19,6 +19,24 @@ struct Store {
   BlockLayout layout;
 };
 
+// The shared prefixes of a batch: the sequences [starts[g], starts[g + 1]) of
+// group g hold the first lens[s] / 16 pages of the group's first one. Sequences
+// in no group share nothing.
+struct PrefixArgs {
+  const int32_t* lens = nullptr;    // [n_seqs], device; null: no prefixes
+  const int32_t* starts = nullptr;  // [n_groups + 1], device
+  int32_t n_groups = 0;
+  int32_t slots = 0;  // partials of a prefix, before a sequence's others
+  // Positions of sequence s that its group's prefix holds, of the T that are stored.
+  __device__ int64_t end(int s, int64_t T, int64_t table_stride) const {
+    if (s < starts[0] || s >= starts[n_groups]) return 0;
+    int64_t p = lens[s] & ~(int32_t)(kBlockTokens - 1);
+    if (p > table_stride * kBlockTokens) p = table_stride * kBlockTokens;
+    if (p > T) p = T;
+    return p > 0 ? p : 0;
+  }
+};
+
 // Decode split-K plan shared by the host and the kernels: wave pairs per
 // work-group (each pair streams whole head-blocks, one half of head_dim per
 // wave) and work-groups per CU the split count aims at (one: a work-group's
@@ -128,7 +146,32 @@ struct AttnArgs {
   // `sinks` ones (WinGeom, fmkv_device.h).
   int64_t win = 0;
   int64_t sinks = 0;
+  // A batch that shares prefixes (win > 0 too, whatever it is): the split columns see
+  // what lies behind a sequence's prefix, and the combine merges the prefix's
+  // partials, part_o and part_ml's first prefix.slots of a sequence, with theirs.
+  PrefixArgs prefix;
+  // Accumulated attention weights (win > 0 too): the split kernels store every
+  // score, base 2, [n_seqs][score_blocks][n_q_heads][16], and a launch that also is the
+  // combine adds the weights of a position, summed over the query heads, to
+  // weights_in (null: 0) and stores them, [n_seqs][weights_width] f32 each.
+  float* scores = nullptr;
+  int64_t score_blocks = 0;
+  const float* weights_in = nullptr;
+  float* weights_out = nullptr;
+  int64_t weights_width = 0;
 };
+
+// The split kernels' arguments of a batch that shares prefixes: their partials
+// come after the prefix's.
+inline AttnArgs behind_prefix(const AttnArgs& a) {
+  AttnArgs own = a;
+  if (a.prefix.lens) {
+    const int64_t rows = (int64_t)a.prefix.slots * a.n_q_heads;
+    own.part_o += rows * a.st.layout.head_dim;
+    own.part_ml += rows * 2;
+  }
+  return own;
+}
 
 // Prefill (chunked) attention: n_q queries at positions p0 .. p0 + n_q - 1,
 // query p attending to key positions [lo(p), p], lo(p) = max(vis_begin,
@@ -175,6 +218,16 @@ struct PrefillArgs {
   // keys each (0: none).
   int32_t tail_ranges = 0;
   uint32_t tail_from = 0;
+  // A batch's shared prefixes (launch_prefix_attention): the rows of a tile are
+  // those of 64 / group sequences of one group, each of which sees what the prefix
+  // holds of its seq_lens[s] - new_col positions. Grid z counts prefix.slots ranges of
+  // keys, whose partials go, rotated back, to slots 0 .. of part_o [n_seqs]
+  // [part_stride][n_q_heads][D] and part_ml [..][2], where the decode kernels' combine
+  // finds them.
+  PrefixArgs prefix;
+  const int32_t* seq_lens = nullptr;
+  int32_t new_col = 0;
+  int32_t part_stride = 0;
 };
 
 struct ReadArgs {
@@ -256,6 +309,18 @@ struct CompactArgs {
   const int32_t* n_keep;  // [n_seqs]
 };
 
+// The positions that sequences keep, by accumulated weight (fmkv_weights.hip).
+struct HeaviestArgs {
+  const float* weights;  // [n_seqs][width]
+  int64_t width;
+  const int32_t* seq_lens;
+  int32_t max_keep, sinks, recent;
+  int32_t* keep;    // [n_seqs][max_keep]
+  int32_t* n_keep;  // [n_seqs]
+  float* kept;      // [n_seqs][kept_width], or null
+  int64_t kept_width;
+};
+
 // Norms and rotation of projected rows (fmkv_norm_rope.hip).
 struct NormRopeArgs {
   const uint16_t *q, *k, *v;  // rows of a token: heads x D from its start
@@ -295,7 +360,17 @@ constexpr int kGatherMaxRows = 16384;
 hipError_t launch_sparse_gather(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The split merge of every decode kernel: out = LSE merge of the partials.
 hipError_t launch_combine(const AttnArgs& a, int n_seqs, hipStream_t s);
+// The same and the accumulated weights (a.scores), fmkv_weights.hip.
+hipError_t launch_combine_weigh(const AttnArgs& a, int n_seqs, hipStream_t s);
+// The kept positions of n_seqs sequences (fmkv_weights.hip).
+hipError_t launch_heaviest(const HeaviestArgs& a, int n_seqs, hipStream_t s);
 hipError_t launch_prefill_attention(const PrefillArgs& a, hipStream_t s);
+// The partials of a batch's shared prefixes (PrefillArgs::prefix): n_seqs, group,
+// q, qscale, new_st, part_o and part_ml and what stands with them.
+hipError_t launch_prefix_attention(const PrefillArgs& a, hipStream_t s);
+// How a batch's prefixes of at most max_steps steps of 32 keys are shared out on
+// `cus` CUs: prefix.slots and share_rows of a.
+void prefix_plan(PrefillArgs& a, int cus, int64_t max_steps);
 // How a prefill call runs on a GPU of `cus` CUs (share_rows, units and
 // min_split of a), no sequence having more than max_steps steps of 32 keys:
 // the bytes of its partials (part_o, then part_ml), 0 where it is not split.

@@ -183,10 +183,10 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
   // is the sequence's own number
   WinGeom wg{};
-  if constexpr (MODE == kWindow) wg = win_geometry(T, a.win, a.sinks, a.st.table_stride);
-  auto block_of = [&](int64_t v) { return MODE == kWindow ? wg.block(v) : v; };
+  if constexpr (windowed(MODE)) wg = attn_window(a, seq, T);
+  auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   const SeqGeom geo =
-      MODE == kWindow
+      windowed(MODE)
           ? wg.geo
           : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
   const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   // sparse-V: this (sequence, KV head)'s row of block maxima; the gated pass
   // visits only the blocks holding a score at or above a head's threshold
   const int64_t blk_row =
-      MODE == kDense || MODE == kWindow ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
+      MODE == kDense || windowed(MODE) ? 0 : ((int64_t)seq * a.st.n_kv_heads + kvh) * a.blk_stride;
   BlockList blist{0ull, 0, nb};
   int nbx = nb;  // blocks visited
   if constexpr (MODE == kGated) {
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (MODE == kWindow ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
@@ -303,16 +303,16 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int64_t slot = t0 + 4 * j + r;
-        bool vis = (MODE == kWindow ? (slot >= wg.lo || slot < a.sinks) && slot < T
+        bool vis = (windowed(MODE) ? (slot >= wg.lo || slot < a.sinks) && slot < T
                                     : slot >= vis_lo && slot < vis_hi) &&
                    slot != ex_slot;
-        if (MODE != kWindow && ring_trim)
+        if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if (!vis) s4[r] = -INFINITY;
         seen[r >> 1] |= vis ? 0xffffu << 16 * (r & 1) : 0u;
       }
       // a hidden token's weight is 0, but its V row may be anything, and 0 * inf is NaN
-      if constexpr (MODE == kWindow) {
+      if constexpr (windowed(MODE)) {
 #pragma unroll
         for (int t = 0; t < TW; t++) cur.v[t].x &= seen[0], cur.v[t].y &= seen[1];
       }
@@ -321,6 +321,8 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; r++) s4[r] = s4[r] >= theta ? s4[r] : -INFINITY;
     }
+    if constexpr (MODE == kWeigh)
+      if (wave == 0 && hi_col && head < G) store_scores(a, seq, b, kvh * G + head, j, s4);
     // -- online softmax in base 2 (as the affine kernel) --
     float mb = fmaxf(fmaxf(s4[0], s4[1]), fmaxf(s4[2], s4[3]));
     mb = xor16_max(mb);
@@ -466,7 +468,12 @@ hipError_t launch_plain_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStre
     return a.direct ? hipSuccess : launch_combine(g, n_seqs, s);
   }
   if (a.win > 0 && !a.st.block_table) return hipErrorInvalidValue;
-  e = a.win > 0 ? launch_plain_mode<D, kWindow>(a, grid, s, ev0, ev1)
+  if (a.scores) {
+    e = launch_plain_mode<D, kWeigh>(a, grid, s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  const AttnArgs own = behind_prefix(a);
+  e = a.win > 0 ? launch_plain_mode<D, kWindow>(own, grid, s, ev0, ev1)
                 : launch_plain_mode<D, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
   return launch_combine(a, n_seqs, s);

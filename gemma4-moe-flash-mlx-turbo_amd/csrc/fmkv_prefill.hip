@@ -310,11 +310,55 @@ __device__ inline PrefillUnit prefill_unit(const PrefillArgs& a, int u, int seq,
   return r;
 }
 
-// WIN: a paged pool's window with sinks (a.window, a.sinks): position p sees j
-// <= p with j > p - window or j < sinks. The sinks' blocks take the place of
+// The largest value of a wave's lanes.
+__device__ inline int wave_max(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_xor(v, d);
+    v = v > o ? v : o;
+  }
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Tile `tile` of a batch's groups, QP sequences a tile: its first sequence, how
+// many it has, and the group's first one (n 0: a tile that nothing needs). Lane l
+// looks at group g0 + l; every wave that asks gets the same answer.
+struct PrefixTile {
+  int s0, n, leader;
+};
+__device__ inline PrefixTile prefix_tile(const PrefixArgs& p, int n_seqs, int QP, int tile, int lane) {
+  for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
+    const int g = g0 + lane;
+    int a = 0, b = 0;
+    if (g < p.n_groups) a = p.starts[g], b = p.starts[g + 1];
+    a = a < 0 ? 0 : a;
+    b = b > n_seqs ? n_seqs : b;
+    const int count = b > a ? (b - a + QP - 1) / QP : 0;
+    const int upto = scan_add(count), total = __builtin_amdgcn_readlane(upto, 63);
+    if (tile < total) {
+      const int l = __builtin_ctzll(__ballot(upto > tile));
+      const int t = tile - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
+      PrefixTile r;
+      r.leader = __builtin_amdgcn_readlane(a, l);
+      r.s0 = r.leader + t * QP;
+      r.n = __builtin_amdgcn_readlane(b, l) - r.s0;
+      if (r.n > QP) r.n = QP;
+      return r;
+    }
+    tile -= total;
+  }
+  return PrefixTile{0, 0, 0};
+}
+
+// KIND of a call. kCausal: a chunk's queries, the sequence's positions up to their
+// own. kBand: a paged pool's window with sinks (a.window, a.sinks): position p
+// sees j <= p with j > p - window or j < sinks. The sinks' blocks take the place of
 // the old store's, in the pool itself, and the blocks between them and the
-// window, whose pages a server may have given back, are never looked up.
-template <int D, int BITS, int MODE, int RW, bool WIN>
+// window, whose pages a server may have given back, are never looked up. kShared:
+// the prefix of a group of sequences (a.prefix), one query each: the row of
+// sequence s "at" the last of the prefix's positions that s sees.
+constexpr int kCausal = 0, kBand = 1, kShared = 2;
+template <int D, int BITS, int MODE, int RW, int KIND>
 __global__ __launch_bounds__(D * RW)  // RW waves per 64 dims
 __attribute__((amdgpu_waves_per_eu(RW == 4 ? 4 : 2, RW == 4 ? 4 : 2)))
 void prefill_attn_kernel(PrefillArgs a) {
@@ -326,10 +370,12 @@ void prefill_attn_kernel(PrefillArgs a) {
   constexpr int QS = P::kQStride, RS = P::kRStride;
   // codebook index width (the template's BITS; other modes never use it)
   constexpr int CB = MODE == kCodebook ? BITS : 2;
+  constexpr bool WIN = KIND == kBand, PFX = KIND == kShared;
 
   __shared__ __align__(16) uint8_t region[P::kRegion];
   __shared__ float lrow[kPfRows], mrow[kPfRows];
   __shared__ int not_finite;
+  __shared__ int row_end[PFX ? kPfRows : 1];  // PFX: positions that a sequence's rows see
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -360,11 +406,26 @@ void prefill_attn_kernel(PrefillArgs a) {
     if (un.seq < 0) return;
     seq = un.seq, range = (int)blockIdx.z - un.first, ranges = un.ranges;
   }
-  const int qi0 = tile * QP;
+  PrefixTile pt{};
+  int p_min = 0, p_max = 0;  // PFX: fewest and most positions that a row sees, less one
+  if constexpr (PFX) {
+    pt = prefix_tile(a.prefix, a.n_seqs, QP, tile, lane);
+    if (pt.n <= 0) return;
+    seq = pt.leader, range = blockIdx.z, ranges = a.prefix.slots;
+    const int s = pt.s0 + (lane < pt.n ? lane : pt.n - 1);
+    const int end = (int)a.prefix.end(s, (int64_t)a.seq_lens[s] - a.new_col, a.new_st.table_stride);
+    if (wave == 0) row_end[lane] = end;  // (barriers follow)
+    p_max = wave_max(end) - 1;
+    p_min = -wave_max(-end) - 1;
+    if (p_max < 0) return;  // (the combine looks for no partials of such sequences)
+  }
+  const int qi0 = PFX ? 0 : tile * QP;
   // paged: the sequence's start, through a scalar load (everything derived
   // from it stays in scalar registers)
-  const int64_t p0 = a.start_pos ? (int64_t)((cint_ptr)(uintptr_t)a.start_pos)[seq] : a.p0;
-  const int nq = a.n_q - qi0 < QP ? a.n_q - qi0 : QP;  // valid positions of the tile
+  const int64_t p0 = PFX ? 0 : a.start_pos ? (int64_t)((cint_ptr)(uintptr_t)a.start_pos)[seq] : a.p0;
+  // valid positions of the tile (PFX: sequences)
+  const int nq = PFX ? pt.n : a.n_q - qi0 < QP ? a.n_q - qi0 : QP;
+  const int64_t q_row0 = PFX ? (int64_t)pt.s0 : (int64_t)seq * a.n_q + qi0;
 
   // visible keys of position p: [lo(p), p]
   auto lo_of = [&](int64_t p) -> int64_t {
@@ -375,7 +436,7 @@ void prefill_attn_kernel(PrefillArgs a) {
 
   // ---- virtual blocks of the work-group: [lo(first), last] in 16-key
   // blocks, the part below p_split from old_st, the rest from new_st ----
-  const int64_t pA = p0 + qi0, pB = p0 + qi0 + nq - 1;
+  const int64_t pA = PFX ? p_min : p0 + qi0, pB = PFX ? p_max : p0 + qi0 + nq - 1;
   const int64_t wg_lo = lo_of(pA), wg_hi = pB;
   const int64_t b_lo = wg_lo / kBlockTokens, b_hi = wg_hi / kBlockTokens;
   const int64_t ps = a.p_split;
@@ -599,7 +660,11 @@ void prefill_attn_kernel(PrefillArgs a) {
   _Float16* const qlo = qhi + kPfRows * QS;
   float* const qsum = reinterpret_cast<float*>(qlo + kPfRows * QS);  // [row][NG] (affine)
   if (tid == 0) not_finite = 0;
-  const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
+  uint32_t words[16];
+#pragma unroll
+  for (int k = 0; k < 16; k++)  // (PFX: the compiler would hold some in vector registers)
+    words[k] = PFX ? __builtin_amdgcn_readfirstlane(a.sign_bits[k]) : a.sign_bits[k];
+  const uint32_t sbits = lane_sign_bits<D>(words, lane);
   const float cs_lane = fwht_lane_sign(lane) * a.c;
   const int rows = nq * G;  // of the chunk
   // Two rows at a time, the next two on their way meanwhile. (One at a time,
@@ -610,7 +675,7 @@ void prefill_attn_kernel(PrefillArgs a) {
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const int rr = wave + NW * (k0 + k), r = rr < rows ? rr : rows - 1, rq = pos_of(r);
-      const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
+      const int64_t row = (q_row0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
       load_words<E / 2>(a.q + row * D + lane * E, ahead[k]);
     }
   };
@@ -721,6 +786,7 @@ void prefill_attn_kernel(PrefillArgs a) {
   // no row does)
   auto pos_at = [&](int r) __attribute__((always_inline)) {
     const int rq = pos_of(r);
+    if constexpr (PFX) return row_end[rq < nq ? rq : nq - 1] - 1;  // (b_lo is 0)
     return pA_r + (rq < nq ? rq : nq - 1);
   };
   int p_row[NRS];
@@ -1267,7 +1333,7 @@ void prefill_attn_kernel(PrefillArgs a) {
                               : o[rt][ct];
   }
   __syncthreads();
-  if (ranges > 1) {  // partial rows, as accumulated, with their (m, l)
+  if (!PFX && ranges > 1) {  // partial rows, as accumulated, with their (m, l)
     const int64_t slot =
         (WIN && a.tail_ranges > 0 ? (int64_t)(blockIdx.x - a.tail_from)
                                   : ((int64_t)blockIdx.z * gridDim.y + kvh) * gridDim.x + blockIdx.x) *
@@ -1303,6 +1369,16 @@ void prefill_attn_kernel(PrefillArgs a) {
       const int rq_ = pos_of(r), rh_ = r - rq_ * G;
       if (rq_ >= nq) continue;
       const float l = lrow[r];
+      if constexpr (PFX) {  // partial rows, rotated back
+        const int64_t row = ((q_row0 + rq_) * a.part_stride + range) * a.n_q_heads + (int64_t)kvh * G + rh_;
+        typedef float vec __attribute__((ext_vector_type(E)));
+        vec o;
+#pragma unroll
+        for (int i = 0; i < E; i++) o[i] = x[k][i] * (MODE == kPlain ? 1.0f : cs_lane);
+        *reinterpret_cast<vec*>(a.part_o + row * D + lane * E) = o;
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(mrow[r], l);
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < E; i++)
         x[k][i] = l > 0.0f ? (x[k][i] * (MODE == kPlain ? 1.0f : cs_lane)) / l : 0.0f;
@@ -1380,14 +1456,14 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int t
                       lane * E, x);
 }
 
-template <int D, int BITS, int MODE, int RW, bool WIN>
+template <int D, int BITS, int MODE, int RW, int KIND>
 hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   const int qp = kPfRows / a.group;
   const int tiles = (a.n_q + qp - 1) / qp, H = a.new_st.n_kv_heads;
   const unsigned split = a.tail_ranges > 0 ? (unsigned)tiles * H * a.n_seqs - a.tail_from : 0;
   dim3 grid(tiles, H, a.units > 0 ? a.units : a.n_seqs);
   if (split) grid = dim3(a.tail_from + split * a.tail_ranges);
-  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, WIN>), grid, dim3(D * RW), 0, s, a);
+  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, KIND>), grid, dim3(D * RW), 0, s, a);
   if (a.units > 0 || split) {
     dim3 mgrid(tiles * (kPfRows / kPfMergeRows), H, a.n_seqs);
     if (split) mgrid = dim3(split * (kPfRows / kPfMergeRows));
@@ -1395,15 +1471,32 @@ hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   }
   return hipGetLastError();
 }
+// Tiles that a batch's groups have at most.
+int64_t prefix_tiles(const PrefillArgs& a) {
+  const int qp = kPfRows / a.group;
+  return a.n_seqs / qp + std::min<int64_t>(a.prefix.n_groups, a.n_seqs);
+}
+template <int D, int BITS, int MODE, int RW>
+hipError_t launch_shared(const PrefillArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)prefix_tiles(a), a.new_st.n_kv_heads, a.prefix.slots);
+  hipLaunchKernelGGL((prefill_attn_kernel<D, BITS, MODE, RW, kShared>), grid, dim3(D * RW), 0, s, a);
+  return hipGetLastError();
+}
 template <int D, int BITS, int MODE>
 hipError_t launch_t(const PrefillArgs& a, hipStream_t s) {
   // (a window without a ring is a paged pool's)
   const bool win = a.window > 0 && a.ring_slots == 0;
   if (win && !a.new_st.block_table) return hipErrorInvalidValue;
+  if (a.prefix.lens) {
+    if constexpr (D < 512)
+      if (a.share_rows) return launch_shared<D, BITS, MODE, 512 / D>(a, s);
+    return launch_shared<D, BITS, MODE, 1>(a, s);
+  }
   if constexpr (D < 512)
     if (a.share_rows)
-      return win ? launch_rw<D, BITS, MODE, 512 / D, true>(a, s) : launch_rw<D, BITS, MODE, 512 / D, false>(a, s);
-  return win ? launch_rw<D, BITS, MODE, 1, true>(a, s) : launch_rw<D, BITS, MODE, 1, false>(a, s);
+      return win ? launch_rw<D, BITS, MODE, 512 / D, kBand>(a, s)
+                 : launch_rw<D, BITS, MODE, 512 / D, kCausal>(a, s);
+  return win ? launch_rw<D, BITS, MODE, 1, kBand>(a, s) : launch_rw<D, BITS, MODE, 1, kCausal>(a, s);
 }
 
 }  // namespace
@@ -1498,6 +1591,18 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
   if (2 * units < 3 * a.n_seqs) return 0;
   a.units = (int)units;
   return prefill_part_bytes(units * wgs, D);
+}
+
+void prefix_plan(PrefillArgs& a, int cus, int64_t max_steps) {
+  const int D = a.new_st.layout.head_dim;
+  const int64_t wgs = prefix_tiles(a) * a.new_st.n_kv_heads;
+  a.share_rows = D < 512 && wgs <= cus / 4;
+  const int64_t most = std::max<int64_t>((max_steps + kPfMinSteps - 1) / kPfMinSteps, 1);
+  a.prefix.slots = (int32_t)std::clamp<int64_t>(prefill_places(D, a.share_rows, cus) / wgs, 1, most);
+}
+
+hipError_t launch_prefix_attention(const PrefillArgs& a, hipStream_t s) {
+  return launch_prefill_attention(a, s);
 }
 
 hipError_t launch_prefill_attention(const PrefillArgs& a, hipStream_t s) {

@@ -57,6 +57,9 @@ EXPORTED = (
     "fmkv_paged_window_decode_attention", "fmkv_paged_window_decode_step",
     "fmkv_paged_window_prefill_attention", "fmkv_paged_window_prefill_step", "fmkv_pool_storage",
     "fmkv_pools_copy_blocks", "fmkv_paged_compact", "fmkv_qkv_norm_rope",
+    "fmkv_paged_prefix_decode_attention", "fmkv_paged_prefix_decode_step",
+    "fmkv_paged_weighing_decode_attention", "fmkv_paged_weighing_decode_step",
+    "fmkv_heaviest_tokens",
     "fmkv_pages_create", "fmkv_pages_destroy", "fmkv_pages_free_count", "fmkv_pages_users",
     "fmkv_pages_alloc", "fmkv_pages_release", "fmkv_pages_fork", "fmkv_pages_slide",
 )
@@ -231,6 +234,16 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         "fmkv_paged_compact": ([vp, vp, i32, vp, i32, vp, vp, i32, i32, vp], ctypes.c_int),
         "fmkv_qkv_norm_rope": ([P(QkvPrologue), i32, i32, i32, i64, vp, i64, vp, i64, vp, i64, vp,
                                 vp, vp, vp, vp], ctypes.c_int),
+        "fmkv_paged_prefix_decode_attention": ([vp, vp, vp, i32, vp, i32, vp, vp, i32, i32, i32, i32,
+                                                ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_prefix_decode_step": ([vp, vp, vp, vp, i32, vp, vp, i32, vp, vp, i32, i32, i32,
+                                           vp, i32, ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_weighing_decode_attention": ([vp, vp, vp, i32, vp, i32, i32, vp, vp, i32, i32,
+                                                  ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_weighing_decode_step": ([vp, vp, vp, vp, i32, vp, vp, i32, i32, vp, vp, vp, i32,
+                                             i32, ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_heaviest_tokens": ([vp, i32, vp, i32, i32, i32, i32, vp, vp, vp, i32, vp],
+                                 ctypes.c_int),
         "fmkv_pages_create": ([i64, P(vp)], ctypes.c_int),
         "fmkv_pages_destroy": ([vp], ctypes.c_int),
         "fmkv_pages_free_count": ([vp, P(i64)], ctypes.c_int),
@@ -794,6 +807,91 @@ class PagedPool:
             _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
         return out
 
+    def prefix_attention(self, q, block_tables, seq_lens, prefix_lens, group_starts,
+                         max_prefix_len: int, max_rest_len: int, scale: float = 1.0, out=None,
+                         dtype=torch.bfloat16, stream=None):
+        """attention() of a batch in groups that share prefixes, each prefix read
+        once for its group: the sequences group_starts[g] .. group_starts[g + 1] - 1
+        have the whole blocks of their first prefix_lens[s] positions in common. q bf16
+        [n_seqs, n_q_heads, D]; seq_lens, prefix_lens int32 [n_seqs]; group_starts
+        int32 [n_groups + 1]. max_rest_len bounds what a sequence holds behind its
+        shared blocks; max_prefix_len, the longest prefix, is for speed."""
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        groups = _check_groups(prefix_lens, group_starts, n, max_prefix_len, max_rest_len)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
+        _check(self._lib.fmkv_paged_prefix_decode_attention(
+            self._h, _here(q, dev), _here(block_tables, dev), width, _here(seq_lens, dev), n,
+            _here(prefix_lens, dev), _here(group_starts, dev), groups, max_prefix_len, max_rest_len,
+            heads, scale, _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
+        return out
+
+    def prefix_decode_step(self, keys, values, block_tables, start_pos, seq_lens, prefix_lens,
+                           group_starts, max_prefix_len: int, max_rest_len: int, q,
+                           scale: float = 1.0, out=None, dtype=torch.bfloat16, stream=None):
+        """append(keys, values, ...) of one token per sequence at start_pos
+        (= seq_lens - 1, behind the shared blocks), then prefix_attention, in one
+        call. keys/values bf16 [n_seqs, 1, n_kv_heads, D]."""
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        _check_tensor("keys", keys, torch.bfloat16, (n, 1, self._H, self._D))
+        _check_tensor("values", values, torch.bfloat16, (n, 1, self._H, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        groups = _check_groups(prefix_lens, group_starts, n, max_prefix_len, max_rest_len)
+        dev = self._device
+        out = _out(out, q, dtype, stream)
+        _check(self._lib.fmkv_paged_prefix_decode_step(
+            self._h, _here(keys, dev), _here(values, dev), _here(block_tables, dev), width,
+            _here(start_pos, dev), _here(seq_lens, dev), n, _here(prefix_lens, dev),
+            _here(group_starts, dev), groups, max_prefix_len, max_rest_len, _here(q, dev), heads, scale,
+            _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
+        return out
+
+    def weighing_attention(self, q, block_tables, seq_lens, max_seq_len: int, weights=None,
+                           weights_out=None, scale: float = 1.0, out=None, dtype=torch.bfloat16,
+                           stream=None):
+        """(attention(), accumulated weights): each position's softmax weights,
+        summed over the query heads, added to `weights` (None: zeros), f32 [n_seqs,
+        at least max_seq_len]. weights_out: a buffer of that shape for the sums (None:
+        weights itself, or a new one of max_seq_len); its entries from seq_lens[s]
+        on stay as they were (0 in a new one)."""
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        dev = self._device
+        weights_out = _sums(weights, weights_out, n, max_seq_len, q, stream)
+        out = _out(out, q, dtype, stream)
+        _check(self._lib.fmkv_paged_weighing_decode_attention(
+            self._h, _here(q, dev), _here(block_tables, dev), width, _here(seq_lens, dev), n,
+            max_seq_len, _here(weights, dev), _here(weights_out, dev), weights_out.shape[1], heads,
+            scale, _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
+        return out, weights_out
+
+    def weighing_decode_step(self, keys, values, block_tables, start_pos, seq_lens,
+                             max_seq_len: int, q, weights=None, weights_out=None,
+                             scale: float = 1.0, out=None, dtype=torch.bfloat16, stream=None):
+        """append(keys, values, ...) of one token per sequence at start_pos
+        (= seq_lens - 1), then weighing_attention, in one call. keys/values bf16
+        [n_seqs, 1, n_kv_heads, D]."""
+        n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
+        _check_tensor("keys", keys, torch.bfloat16, (n, 1, self._H, self._D))
+        _check_tensor("values", values, torch.bfloat16, (n, 1, self._H, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+        dev = self._device
+        weights_out = _sums(weights, weights_out, n, max_seq_len, q, stream)
+        out = _out(out, q, dtype, stream)
+        _check(self._lib.fmkv_paged_weighing_decode_step(
+            self._h, _here(keys, dev), _here(values, dev), _here(block_tables, dev), width,
+            _here(start_pos, dev), _here(seq_lens, dev), n, max_seq_len, _here(q, dev),
+            _here(weights, dev), _here(weights_out, dev), weights_out.shape[1], heads, scale,
+            _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
+        return out, weights_out
+
     def compact(self, block_tables, keep, n_keep, dst_tables, stream=None) -> None:
         """Moves the tokens that sequences keep to the front of other blocks:
         position keep[s, i] becomes position i of dst_tables' row s, i <
@@ -836,6 +934,40 @@ def copy_blocks(pools, src, dst, stream=None) -> None:
     handles = (ctypes.c_void_p * max(len(pools), 1))(*[p._h for p in pools])
     _check(load_library().fmkv_pools_copy_blocks(handles, len(pools), _here(src, dev),
                                                  _here(dst, dev), src.shape[0], _stream(stream)))
+
+
+def heaviest_tokens(weights, seq_lens, max_keep: int, sinks: int = 0, recent: int = 0, keep=None,
+                    n_keep=None, weights_out=None, stream=None):
+    """(keep, n_keep, weights_out): the positions that each sequence keeps, in
+    order, as PagedPool.compact takes them. Of more than max_keep the first `sinks`
+    and the last `recent` ones and the heaviest of the others by `weights` (f32
+    [n_seqs, width]; equal ones: the lower position); of at most max_keep all.
+    weights_out f32 [n_seqs, at least max_keep]: their weights, 0 behind them. keep
+    int32 [n_seqs, max_keep] stays as it was behind n_keep[s] (0 in a new one)."""
+    n, width = _check_tensor("weights", weights, torch.float32, (None, None))
+    _check_tensor("seq_lens", seq_lens, torch.int32, (n,))
+    for name, value in (("max_keep", max_keep), ("sinks", sinks), ("recent", recent),
+                        ("the width of weights", width)):
+        _check_bits(name, value, 32)
+    if not 1 <= max_keep <= 2 ** 28 - 16:
+        raise ValueError("max_keep must be in [1, 2^28 - 16]")
+    dev = torch.cuda.current_device()
+    _here(weights, dev)
+    with _on(stream):
+        if keep is None:
+            keep = torch.zeros((n, max_keep), dtype=torch.int32, device=weights.device)
+        if n_keep is None:
+            n_keep = torch.empty(n, dtype=torch.int32, device=weights.device)
+        if weights_out is None:
+            weights_out = torch.empty((n, max_keep), dtype=torch.float32, device=weights.device)
+    _check_tensor("keep", keep, torch.int32, (n, max_keep))
+    _check_tensor("n_keep", n_keep, torch.int32, (n,))
+    kept_width = _check_tensor("weights_out", weights_out, torch.float32, (n, None))[1]
+    _check_bits("the width of weights_out", kept_width, 32)
+    _check(load_library().fmkv_heaviest_tokens(
+        _here(weights, dev), width, _here(seq_lens, dev), n, max_keep, sinks, recent,
+        _here(keep, dev), _here(n_keep, dev), _here(weights_out, dev), kept_width, _stream(stream)))
+    return keep, n_keep, weights_out
 
 
 def qkv_norm_rope(q, k, v, positions, prologue: QkvPrologue, out=None, stream=None):
@@ -1001,6 +1133,33 @@ def _check_window(window: int, sinks: int, max_seq_len: int = 0) -> None:
     if not (-2 ** 31 <= window < 2 ** 31 and -2 ** 31 <= sinks < 2 ** 31):
         raise ValueError("window and sinks must be at most 2^30")
     _check_bits("max_seq_len", max_seq_len, 32)
+
+
+def _check_groups(prefix_lens, group_starts, n: int, max_prefix_len: int, max_rest_len: int) -> int:
+    """Number of groups of a batch that shares prefixes."""
+    _check_tensor("prefix_lens", prefix_lens, torch.int32, (n,))
+    ends = _check_tensor("group_starts", group_starts, torch.int32, (None,))[0]
+    if ends < 1:
+        raise ValueError("group_starts must have n_groups + 1 entries")
+    _check_bits("max_prefix_len", max_prefix_len, 32)
+    _check_bits("max_rest_len", max_rest_len, 32)
+    return ends - 1
+
+
+def _sums(weights, weights_out, n: int, max_seq_len: int, like: torch.Tensor, stream):
+    """Where accumulated weights go: weights_out, weights itself, or a new buffer."""
+    _check_bits("max_seq_len", max_seq_len, 32)
+    if weights is not None:
+        width = _check_tensor("weights", weights, torch.float32, (n, None))[1]
+        if weights_out is None:
+            weights_out = weights
+        _check_tensor("weights_out", weights_out, torch.float32, (n, width))
+    elif weights_out is None:
+        with _on(stream):
+            weights_out = torch.zeros((n, max(max_seq_len, 1)), dtype=torch.float32, device=like.device)
+    _check_bits("the width of weights_out", _check_tensor("weights_out", weights_out, torch.float32,
+                                                          (n, None))[1], 32)
+    return weights_out
 
 
 def _check_tensor(name: str, t: torch.Tensor, dtype, shape):

@@ -396,6 +396,93 @@ int fmkv_paged_window_prefill_step(fmkv_pool* pool, const void* k_bf16, const vo
                                    float scale, int32_t window, int32_t sinks, void* out,
                                    int32_t out_dtype, void* stream);
 
+/* Decode attention of a batch whose sequences share prefixes (fmkv_pages_fork's
+ * whole blocks: one system prompt, the beams of one conversation): what
+ * fmkv_paged_decode_attention gives, a prefix read once for its group and not once
+ * for each sequence. Group g is the sequences group_starts[g] .. group_starts[g + 1]
+ * - 1, whose block tables begin with the same blocks: those of the group's first
+ * sequence are read for the positions below prefix_lens[s], rounded down to whole
+ * blocks (a sequence may share less than its group's first one does; what it
+ * holds behind that is its own). Sequences in no group share nothing. prefix_lens: int32
+ * device [n_seqs]; group_starts: int32 device [n_groups + 1], in order.
+ * max_prefix_len is the longest of prefix_lens, for speed only (a wrong one gives right
+ * results). max_rest_len bounds what sequences have behind their shared blocks
+ * (seq_lens[s] less prefix_lens[s] rounded down; all of seq_lens[s] in no group), as
+ * max_seq_len bounds the lengths of the other calls. What slots past a sequence's
+ * length hold does not reach an output; a sequence of length 0 gets zeros. q
+ * is 16-byte aligned. Every cache mode, at most 8 query heads per KV head. The
+ * order of sums, and so an output's last bits, depends on the bounds and on the batch.
+ * The current GPU has to be the pool's; for calls on several streams, and graphs, see
+ * the windowed calls above. */
+int fmkv_paged_prefix_decode_attention(fmkv_pool* pool, const void* q_bf16,
+                                       const int32_t* block_tables, int32_t max_blocks,
+                                       const int32_t* seq_lens, int32_t n_seqs,
+                                       const int32_t* prefix_lens, const int32_t* group_starts,
+                                       int32_t n_groups, int32_t max_prefix_len,
+                                       int32_t max_rest_len, int32_t n_q_heads, float scale,
+                                       void* out, int32_t out_dtype, void* stream);
+
+/* fmkv_paged_decode_step of one new token per sequence (at seq_lens - 1 =
+ * start_pos, behind its shared blocks) for such a batch; the attention launch
+ * appends the tokens. */
+int fmkv_paged_prefix_decode_step(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
+                                  const int32_t* block_tables, int32_t max_blocks,
+                                  const int32_t* start_pos, const int32_t* seq_lens,
+                                  int32_t n_seqs, const int32_t* prefix_lens,
+                                  const int32_t* group_starts, int32_t n_groups,
+                                  int32_t max_prefix_len, int32_t max_rest_len,
+                                  const void* q_bf16, int32_t n_q_heads, float scale, void* out,
+                                  int32_t out_dtype, void* stream);
+
+/* Accumulated attention weights, by which a cache is cut to the tokens that
+ * matter: how much softmax weight each position of a sequence has got, summed over
+ * the query heads and over the calls that accumulate. weights and weights_out: f32
+ * device [n_seqs][weights_width], weights_width >= max_seq_len. A call stores
+ *   weights_out[s][j] = weights[s][j] + sum of the weights of position j
+ * for the positions j < seq_lens[s] (and below weights_width); the others' entries
+ * of weights_out stay as they were. weights NULL: zeros. The two are one buffer
+ * or do not overlap. f32 sums in a fixed order: the same call gives the same bits. */
+
+/* fmkv_paged_decode_attention with the accumulated weights of its softmax. What
+ * slots past a sequence's length hold does not reach an output; a sequence of
+ * length 0 gets zeros. q is 16-byte aligned. Needs 4 bytes of the pool's
+ * workspace per query head and position of n_seqs sequences of max_seq_len. The
+ * current GPU has to be the pool's; for calls on several streams, and graphs, see
+ * the windowed calls above. */
+int fmkv_paged_weighing_decode_attention(fmkv_pool* pool, const void* q_bf16,
+                                         const int32_t* block_tables, int32_t max_blocks,
+                                         const int32_t* seq_lens, int32_t n_seqs,
+                                         int32_t max_seq_len, const float* weights,
+                                         float* weights_out, int32_t weights_width,
+                                         int32_t n_q_heads, float scale, void* out,
+                                         int32_t out_dtype, void* stream);
+
+/* fmkv_paged_decode_step of one new token per sequence (at seq_lens - 1 =
+ * start_pos), with the accumulated weights, the new token's among them. */
+int fmkv_paged_weighing_decode_step(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
+                                    const int32_t* block_tables, int32_t max_blocks,
+                                    const int32_t* start_pos, const int32_t* seq_lens,
+                                    int32_t n_seqs, int32_t max_seq_len, const void* q_bf16,
+                                    const float* weights, float* weights_out,
+                                    int32_t weights_width, int32_t n_q_heads, float scale,
+                                    void* out, int32_t out_dtype, void* stream);
+
+/* The positions that each sequence keeps: of more than max_keep its first
+ * `sinks` and last `recent` ones and the heaviest of the others, max_keep in all
+ * (equal weights: the lower position first; a NaN is lighter than any weight); of
+ * at most max_keep all. They come in ascending order, as fmkv_paged_compact takes them:
+ * keep int32 device [n_seqs][max_keep] (entries behind the kept ones stay as they
+ * were), n_keep int32 device [n_seqs]. kept_weights (or NULL): f32 device
+ * [n_seqs][kept_width], the kept positions' weights in that order, the entries behind
+ * them 0: the weights of the compacted sequences, to accumulate on. weights: f32
+ * device [n_seqs][weights_width]; weights_width and kept_width are at most 2^30,
+ * max_keep at most 2^28 - 16 and kept_width; seq_lens past weights_width count as
+ * that. Outputs do not overlap the inputs or one another. */
+int fmkv_heaviest_tokens(const float* weights, int32_t weights_width, const int32_t* seq_lens,
+                         int32_t n_seqs, int32_t max_keep, int32_t sinks, int32_t recent,
+                         int32_t* keep, int32_t* n_keep, float* kept_weights,
+                         int32_t kept_width, void* stream);
+
 /* Blocks src[i] copied to dst[i], i < n_pairs, in every one of n_pools pools (the
  * layers of a model that share their block tables), all KV heads: a forked
  * sequence's partly filled last block, blocks moved together. src, dst: int32

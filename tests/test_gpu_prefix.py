@@ -1,0 +1,178 @@
+"""Decode attention of batches that share prefixes, against 64-bit references
+over each sequence's own rows."""
+import numpy as np
+import pytest
+
+from gpu_util import check_codes, dev_bf16, fast_kv
+from shared_util import Shared, attend_reference, poison_from
+from window_util import AFFINE, CODEBOOK, PLAIN, TOKENS, check_window, queries
+
+pytestmark = pytest.mark.gpu
+
+# mode, bits, D, Hkv, Hq
+FORMS = [(AFFINE, 4, 256, 8, 16), (AFFINE, 8, 512, 2, 16), (PLAIN, 16, 128, 4, 8), (AFFINE, 4, 128, 2, 2),
+         (AFFINE, 8, 256, 1, 5), (AFFINE, 4, 512, 1, 8), (AFFINE, 8, 128, 3, 9), (CODEBOOK, 2, 128, 2, 4),
+         (CODEBOOK, 3, 256, 2, 12), (CODEBOOK, 4, 512, 1, 7), (CODEBOOK, 3, 512, 2, 2), (PLAIN, 16, 512, 1, 8),
+         (PLAIN, 16, 256, 2, 6), (CODEBOOK, 4, 256, 1, 1), (CODEBOOK, 3, 128, 2, 16)]
+
+# groups of (prefix, lengths), the sequences of no group before and after
+BATCHES = {
+    "pair": ([(160, [171, 200])], ((), ())),
+    # a prefix that ends inside a block, members at its very end, inside it, of no length
+    "edges": ([(77, [77, 64, 90, 0, 79, 17, 1, 80, 100])], ((5,), (33, 0))),
+    # lone sequences as groups, one shorter than a block, an empty group, a prefix of nothing
+    "lone": ([(40, [55]), (9, [25, 26]), (300, [300]), (0, [31]), (48, [])], ((), (1,))),
+    # more sequences than a tile holds at any number of heads, uneven groups
+    "many": ([(513, list(range(514, 514 + 70))), (35, [36] * 3), (128, [129 + 7 * i for i in range(20)])], ((), ())),
+    "long": ([(3001, [3010, 3500, 3001]), (1600, [1601, 1700])], ((), (700,))),
+}
+
+
+def reference(ora, b, q, scale):
+    return np.stack([attend_reference(ora, oc, q[s], n, scale)[0] for s, (oc, n) in enumerate(zip(b.oracles, b.lens))])
+
+
+def vmax(b):
+    return max(float(np.abs(oc.dequant_kv(np.arange(n))[1]).max()) for oc, n in zip(b.oracles, b.lens) if n)
+
+
+@pytest.mark.parametrize("batch", BATCHES)
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", FORMS)
+def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch):
+    import torch
+
+    groups, alone = BATCHES[batch]
+    b = Shared(gpu, ora, mode, D, bits, Hkv, groups, alone, seed=3)
+    q = queries(11, len(b.lens), Hq, Hkv, D)
+    want = reference(ora, b, q, D ** -0.5)
+    big = vmax(b)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = b.pool.prefix_attention(dev_bf16(q), *b.args(), scale=D ** -0.5, dtype=dtype)
+        check_window(out, want, big, f"{batch} {dtype}")
+    # only speed follows from the longest prefix that the caller names
+    tables, lens, prefix, starts, _, rest = b.args()
+    for bound in (0, 2 ** 31 - 1):
+        out = b.pool.prefix_attention(dev_bf16(q), tables, lens, prefix, starts, bound, rest, scale=D ** -0.5,
+                                      dtype=torch.float32)
+        check_window(out, want, big, f"{batch} bound {bound}")
+
+
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", FORMS)
+def test_step(gpu, ora, mode, bits, D, Hkv, Hq):
+    """Three steps of one token per sequence, a padded row among them; stored codes
+    bit for bit; the shared blocks as they were."""
+    import torch
+
+    b = Shared(gpu, ora, mode, D, bits, Hkv, [(77, [77, 80, 95, 101]), (32, [32, 47])], ((6,), (0,)), seed=5, room=4)
+    n = len(b.lens)
+    padded = 3  # a row of no sequence: length 0, position -1
+    for step in range(3):
+        k, v = (fast_kv(500 + 10 * step + i, n, Hkv, D, outliers=False) for i in (0, 1))
+        q = queries(60 + step, n, Hq, Hkv, D)
+        shared = b.pool.storage()[torch.from_numpy(b.tables[1, :4]).long().cuda()].clone()
+        lens = [t + 1 for t in b.lens]
+        lens[padded] = 0
+        start = [t - 1 for t in lens]
+        for s in range(n):
+            if s != padded:
+                b.oracles[s].append(k[s:s + 1], v[s:s + 1])
+                b.lens[s] += 1
+        rest = max(t - min(p, t) // TOKENS * TOKENS if b.starts[0] <= s < b.starts[-1] else t
+                   for s, (t, p) in enumerate(zip(b.lens, b.prefix)))
+        out = b.pool.prefix_decode_step(
+            dev_bf16(k[:, None]), dev_bf16(v[:, None]), b.table(), b.ints(start), b.ints(lens), b.ints(b.prefix),
+            b.ints(b.starts), max(b.prefix), rest, dev_bf16(q), scale=D ** -0.5, dtype=torch.float32)
+        want = reference(ora, b, q, D ** -0.5)
+        want[padded] = 0.0
+        check_window(out, want, vmax(b), f"step {step}")
+        assert not out[padded].any()
+        assert torch.equal(b.pool.storage()[torch.from_numpy(b.tables[1, :4]).long().cuda()], shared)
+    codes, meta = b.pool.read_codes()
+    for s in range(n):
+        at = np.arange(b.lens[s])
+        slots = torch.from_numpy(b.tables[s, at // TOKENS] * TOKENS + at % TOKENS).long().cuda()
+        check_codes(codes[slots], meta[slots], b.oracles[s], slots=at, what=f"sequence {s}")
+
+
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[1], FORMS[2], FORMS[8]])
+def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq):
+    """What lies past a sequence's length, in its blocks and in the shared ones, does
+    not reach its output."""
+    import torch
+
+    b = Shared(gpu, ora, mode, D, bits, Hkv, [(160, [180, 175, 160])], ((), (20,)), seed=7)
+    q = queries(13, 4, Hq, Hkv, D)
+    tables, lens, prefix, starts, longest, rest = b.args()
+    # a member that sees 37 of the shared positions, where the others' rows are infinite
+    short = b.ints([180, 37, 160, 20])
+    before = b.pool.prefix_attention(dev_bf16(q), tables, short, prefix, starts, longest, rest, scale=D ** -0.5,
+                                     dtype=torch.float32)
+    poison_from(b, 0, 40)
+    after = b.pool.prefix_attention(dev_bf16(q), tables, short, prefix, starts, longest, rest, scale=D ** -0.5,
+                                    dtype=torch.float32)
+    want = attend_reference(ora, b.oracles[1], q[1], 37, D ** -0.5)[0]
+    check_window(after[1:2], want[None], vmax(b), "the short member")
+    assert torch.equal(after[3], before[3])
+    assert not torch.equal(after[0], before[0])  # (which sees them)
+
+
+def test_graph_and_streams(gpu, ora):
+    """A captured step replayed with eager calls between, on tensors of another
+    stream; the same bits each time."""
+    import torch
+
+    D, Hkv, Hq = 256, 8, 16
+    b = Shared(gpu, ora, AFFINE, D, 4, Hkv, [(400, [410 + i for i in range(9)])], seed=9)
+    q = dev_bf16(queries(17, 9, Hq, Hkv, D))
+    args = b.args()
+    want = b.pool.prefix_attention(q, *args, scale=D ** -0.5)
+    other = torch.cuda.Stream()
+    out = torch.zeros_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.pool.prefix_attention(q, *args, scale=D ** -0.5, out=out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert torch.equal(b.pool.prefix_attention(q, *args, scale=D ** -0.5), want)
+        torch.cuda.synchronize()
+    got = b.pool.prefix_attention(q, *args, scale=D ** -0.5, stream=other)
+    other.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_forked_book(gpu, ora):
+    """The blocks that PageBook.fork shares, as a server uses them: the same
+    attention as over each sequence's whole table."""
+    import torch
+
+    D, Hkv, Hq, bits, prompt = 512, 2, 16, 8, 203
+    book = gpu.PageBook(64)
+    pool = gpu.PagedPool(gpu.make_desc(Hkv, D, bits), 64)
+    parent = book.alloc(-(-prompt // TOKENS))
+    k, v = (dev_bf16(fast_kv(i, prompt, Hkv, D, outliers=False)[None]) for i in (1, 2))
+    table = torch.tensor([parent], dtype=torch.int32, device="cuda")
+    pool.append(k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    rows, copies = [parent], []
+    for _ in range(4):
+        child, copy = book.fork(parent, prompt)
+        rows.append(child)
+        copies.append(copy)
+    src, dst = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in zip(*copies))
+    gpu.copy_blocks([pool], src, dst)
+    rows = [r + book.alloc(1) for r in rows]
+    tables = torch.tensor(rows, dtype=torch.int32, device="cuda")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    n = len(rows)
+    for step in range(8):
+        kn, vn = (dev_bf16(fast_kv(40 + 2 * step + i, n, Hkv, D, outliers=False)[:, None]) for i in (0, 1))
+        q = dev_bf16(queries(80 + step, n, Hq, Hkv, D))
+        t = prompt + step + 1
+        out = pool.prefix_decode_step(kn, vn, tables, ints([t - 1] * n), ints([t] * n), ints([prompt] * n),
+                                      ints([0, n]), prompt, t - prompt // TOKENS * TOKENS, q, scale=D ** -0.5,
+                                      dtype=torch.float32)
+        want = pool.window_attention(q, tables, ints([t] * n), t, window=2 ** 30, scale=D ** -0.5,
+                                     dtype=torch.float32)
+        check_window(out, want.double().cpu().numpy(), 2 * float(vn.abs().max() + v.abs().max()), f"step {step}")
