@@ -1755,6 +1755,52 @@ int fmkv_paged_weighing_decode_step(fmkv_pool* p, const void* k, const void* v,
                               out_dtype, stream);
 }
 
+int fmkv_paged_attention_weights(fmkv_pool* p, const void* q, const int32_t* block_tables,
+                                 int32_t max_blocks, const int32_t* start_pos, int32_t n_seqs,
+                                 int32_t n_new, int32_t max_seq_len, const float* weights,
+                                 float* weights_out, int32_t weights_width, int32_t n_q_heads,
+                                 float scale, void* stream) {
+  if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
+  if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
+  if (n_seqs < 0 || n_seqs > 65535 || n_new < 0 || max_seq_len < 0 || max_blocks < 1)
+    return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / n_new / max_seq_len / max_blocks");
+  if ((int64_t)max_seq_len > (int64_t)max_blocks * fmkv::kBlockTokens)
+    return fail(FMKV_ERR_INVALID_ARG, "max_seq_len exceeds max_blocks * 16");
+  int rc = check_weights(n_seqs, max_seq_len, weights, weights_out, weights_width);
+  if (rc) return rc;
+  if (n_seqs == 0 || n_new == 0) return FMKV_OK;
+  // (the output's place is taken by the weights)
+  if ((rc = check_attn_args(p->desc, q, n_q_heads, 0.0f, weights_out, FMKV_DTYPE_F32))) return rc;
+  if (!block_tables || !start_pos) return fail(FMKV_ERR_INVALID_ARG, "block_tables/start_pos are null");
+  if ((uintptr_t)q % 2 != 0) return fail(FMKV_ERR_UNSUPPORTED, "q must be 2-byte aligned");
+  if ((rc = check_device(p))) return rc;
+  fmkv::ObserveArgs a;
+  a.st = pool_store(p, block_tables, max_blocks);
+  a.start_pos = start_pos;
+  a.n_seqs = n_seqs;
+  a.n_q = n_new;
+  a.group = n_q_heads / p->desc.n_kv_heads;
+  a.n_q_heads = n_q_heads;
+  a.q = static_cast<const uint16_t*>(q);
+  a.qscale = scale * 1.4426950408889634f;
+  std::memcpy(a.sign_bits, p->sign_bits, sizeof(a.sign_bits));
+  a.c = p->c;
+  a.blocks = (int32_t)std::max<int64_t>(((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens, 1);
+  const size_t floats = fmkv::observe_plan(a, p->cus);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  RelaxedCapture relaxed;  // (the workspace may grow)
+  p->ws.captured = is_captured(s);
+  if ((rc = p->ws.ensure(floats * sizeof(float)))) return rc;
+  a.ml = p->ws.ptr;
+  a.part = a.ml + floats - (size_t)n_seqs * p->desc.n_kv_heads * a.sharers * a.part_width;
+  a.weights_in = weights;
+  a.weights_out = weights_out;
+  a.weights_width = weights_width;
+  const hipError_t e = fmkv::launch_observe(a, s);
+  if (e != hipSuccess) return hip_fail(e, "attention weights launch");
+  return FMKV_OK;
+}
+
 int fmkv_heaviest_tokens(const float* weights, int32_t weights_width, const int32_t* seq_lens,
                          int32_t n_seqs, int32_t max_keep, int32_t sinks, int32_t recent,
                          int32_t* keep, int32_t* n_keep, float* kept_weights, int32_t kept_width,

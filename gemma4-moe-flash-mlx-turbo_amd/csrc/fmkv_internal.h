@@ -321,6 +321,29 @@ struct HeaviestArgs {
   int64_t kept_width;
 };
 
+// Accumulated weights of n_q queries per sequence (fmkv_observe.hip), whose keys
+// are in the pool. A tile is 64 rows, 64 / group queries of a KV head's heads.
+struct ObserveArgs {
+  Store st;
+  const int32_t* start_pos;  // [n_seqs]
+  int32_t n_seqs, n_q;
+  int32_t group, n_q_heads;
+  const uint16_t* q;  // bf16 [n_seqs][n_q][n_q_heads][D]
+  float qscale;       // softmax scale * log2(e)
+  uint32_t sign_bits[16];
+  float c;            // 1/sqrt(D)
+  int32_t blocks;     // the longest sequence's blocks
+  // the plan: blocks of a wave's step, ranges of keys, tiles of a KV head, the
+  // work-groups that share them
+  int32_t step_blocks, ranges, tiles, sharers;
+  float* ml;    // [n_seqs][n_kv_heads][tiles][ranges][64] (m, l)
+  float* part;  // [n_seqs][n_kv_heads * sharers][part_width] sums of weights
+  int64_t part_width;
+  const float* weights_in;
+  float* weights_out;
+  int64_t weights_width;
+};
+
 // Norms and rotation of projected rows (fmkv_norm_rope.hip).
 struct NormRopeArgs {
   const uint16_t *q, *k, *v;  // rows of a token: heads x D from its start
@@ -362,6 +385,10 @@ hipError_t launch_sparse_gather(const AttnArgs& a, int n_seqs, hipStream_t s);
 hipError_t launch_combine(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The same and the accumulated weights (a.scores), fmkv_weights.hip.
 hipError_t launch_combine_weigh(const AttnArgs& a, int n_seqs, hipStream_t s);
+// The plan of an ObserveArgs on a GPU of `cus` CUs, and the floats of its
+// workspace (ml, then part).
+size_t observe_plan(ObserveArgs& a, int cus);
+hipError_t launch_observe(const ObserveArgs& a, hipStream_t s);
 // The kept positions of n_seqs sequences (fmkv_weights.hip).
 hipError_t launch_heaviest(const HeaviestArgs& a, int n_seqs, hipStream_t s);
 hipError_t launch_prefill_attention(const PrefillArgs& a, hipStream_t s);

@@ -1,0 +1,555 @@
+// Accumulated attention weights of a prompt's queries: weight[s][j] of position j
+// is the sum, over the queries of sequence s at positions p >= j and over the query
+// heads h, of 2^(s_ph(j) - M_ph) / L_ph, where s are the base-2 scores q . k, M_ph and
+// L_ph the maximum and the sum of a query's softmax. V is not read.
+//
+// M and L are known only when a row has seen all its keys, and the scores of all rows
+// with all keys are too many to keep (4 bytes for each pair: 268 MB for 128 queries of
+// 16 heads over 32768 keys), so the products are formed twice: a launch for each
+// range of keys' (m, l), one for the weights with M and 1 / L merged from those, and
+// one that adds up what KV heads and tiles of rows have given a position.
+//
+// A work-group holds 64 rows (64 / G consecutive queries of a KV head's G heads) as
+// matrix-core operands in LDS; its waves take different keys, NB blocks of 16 a step,
+// straight from memory to registers, where a code is turned into an operand once
+// for all rows. Nothing is exchanged between the waves while they run. Over the
+// 64-dim groups of a step the scores of the 64 rows with the step's keys stay in
+// registers; an operand of the rows is read from LDS once for NB products.
+//
+// Operands as in prefill (fmkv_prefill.hip): K codes (or centroids) exact, q_rot as
+// an f16 high part and residual; plain caches bf16 as stored.
+//
+// In the second launch a lane's sums over its rows of the weights of its keys stay in
+// registers until all rows are done; 16 lanes meet at the end. Every sum has one
+// order: no atomics.
+#include <algorithm>
+
+#include "fmkv_device.h"
+#include "fmkv_internal.h"
+#include "fmkv_rows_common.h"
+#include "fmkv_cb_common.h"
+
+namespace fmkv {
+namespace {
+
+constexpr int kObRows = 64;
+constexpr int kObTiles = kObRows / 16;
+constexpr float kObSlack = 8.0f;  // (base 2) a score may exceed its row's reference by
+
+template <int D, int BITS, int MODE>
+struct ObPlan {
+  static constexpr BlockLayout L = make_layout(D, BITS, MODE);
+  static constexpr int NG = D / 64, E = D / 64;
+  static constexpr int NW = D == 512 ? 8 : 4;  // waves (512 dims' rows fill a CU's LDS)
+  static constexpr int kParts = MODE == kPlain ? 1 : 2;  // high parts, residuals
+  static constexpr int kRows = kObTiles * 2 * NG * kParts * 1024;
+  static constexpr int KW = MODE == kAffine ? BITS / 2 : MODE == kPlain ? 8 : BITS == 3 ? 4 : 2;
+  static constexpr int kLut = MODE == kCodebook ? CbLut<BITS == 16 ? 2 : BITS>::kBytes : 16;
+};
+
+// Sequence s of a call: its positions, its keys' blocks, and the WG-steps (NW waves'
+// NB blocks) of a range.
+struct ObSeq {
+  int64_t p0, T;
+  int blocks, per;
+};
+template <int NW, int NB>
+__device__ inline ObSeq ob_seq(const ObserveArgs& a, int seq) {
+  ObSeq r;
+  r.p0 = ((cint_ptr)(uintptr_t)a.start_pos)[seq];
+  r.T = r.p0 + a.n_q;
+  int64_t b = r.T > 0 ? (r.T + kBlockTokens - 1) / kBlockTokens : 0;
+  if (b > a.blocks) b = a.blocks;
+  r.blocks = (int)b;
+  const int steps = (r.blocks + NW * NB - 1) / (NW * NB);
+  r.per = (steps + a.ranges - 1) / a.ranges;
+  return r;
+}
+
+// SUMS: the second launch. Grid (range of keys, KV head and sharer of its tiles, sequence).
+template <int D, int BITS, int MODE, int NB, bool SUMS>
+__global__ __launch_bounds__((ObPlan<D, BITS, MODE>::NW * 64))
+__attribute__((amdgpu_waves_per_eu(2, 2)))
+void observe_kernel(ObserveArgs a) {
+  using P = ObPlan<D, BITS, MODE>;
+  constexpr BlockLayout L = P::L;
+  constexpr int NG = P::NG, NW = P::NW, E = P::E, KW = P::KW, LPG = 64 / E, RT = kObTiles;
+  constexpr int CB = MODE == kCodebook ? BITS : 2;
+  __shared__ __align__(16) uint8_t rows_s[P::kRows];
+  __shared__ __align__(16) uint8_t lut[P::kLut];
+  __shared__ float qsum[kObRows][NG];
+  __shared__ int row_pos[kObRows];
+  __shared__ float2 stat[SUMS ? 1 : NW][kObRows];  // (m, l) of the waves; SUMS: M, 1 / L
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane >> 4, c = lane & 15;
+  const int seq = blockIdx.z, range = blockIdx.x;
+  const int kvh = blockIdx.y / a.sharers, sharer = blockIdx.y - kvh * a.sharers;
+  const ObSeq q = ob_seq<NW, NB>(a, seq);
+  const int s_begin = range * q.per;
+  const int n_steps = (q.blocks + NW * NB - 1) / (NW * NB);
+  const int s_end = s_begin + q.per < n_steps ? s_begin + q.per : n_steps;
+  if (s_begin >= s_end) return;
+  const int ranges = (n_steps + q.per - 1) / q.per;  // of this sequence
+  const int G = a.group, QP = kObRows / G;
+
+  const uint64_t base = reinterpret_cast<uint64_t>(a.st.base) + kvh * a.st.head_stride;
+  const cint_ptr table = (cint_ptr)(uintptr_t)(a.st.block_table + (int64_t)seq * a.st.table_stride);
+  const int32_t n_pool = (int32_t)(a.st.n_blocks < INT32_MAX ? a.st.n_blocks : INT32_MAX);
+  auto blk_ptr = [&](int b) __attribute__((always_inline)) -> gptr_t {
+    // (past the last block: that one, whose keys are masked; an entry outside the
+    // pool reads a valid block rather than faulting)
+    const int32_t e = table[b < q.blocks ? b : q.blocks - 1];
+    const uint32_t phys = (uint32_t)(e < 0 ? 0 : (e >= n_pool ? n_pool - 1 : e));
+    return (gptr_t)(base + (uint64_t)phys * (uint64_t)a.st.block_stride);
+  };
+
+  const int kbit = (c * (D / 2) + 8 * j) * CB;
+  const uint32_t ksh = kbit & 31;
+  const uint32_t k_off = (uint32_t)L.k_codes + (MODE == kAffine     ? lane * 16
+                                                : MODE == kCodebook ? (kbit >> 5) * 4
+                                                                    : (c * D + 8 * j) * 2);
+  const uint32_t km_off = (uint32_t)L.k_meta + j * 16;
+  struct Stage {
+    uint32_t kr[NB][KW];
+    u32x4 km[NB];
+  };
+  auto load = [&](const gptr_t (&bp)[NB], int g, Stage& st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      if constexpr (MODE == kAffine) {
+        if constexpr (BITS == 8) {
+          const u32x4 w = load_at<u32x4>(bp[b], k_off, g * 1024);
+#pragma unroll
+          for (int i = 0; i < 4; i++) st.kr[b][i] = w[i];
+        } else {
+          const u32x2 w = load_at<u32x2>(bp[b], k_off, (g >> 1) * 1024 + (g & 1) * 8);
+          st.kr[b][0] = w[0];
+          st.kr[b][1] = w[1];
+        }
+        st.km[b] = load_at<u32x4>(bp[b], km_off, g * 64);
+      } else if constexpr (MODE == kCodebook) {
+        const int off = (g / (NG / 2)) * (D * CB) + (g % (NG / 2)) * 8 * CB;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          if constexpr (CB == 3) {
+            const u32x2 w = load_at<u32x2_a4>(bp[b], k_off, off + s * 4 * CB);
+            st.kr[b][2 * s] = w[0];
+            st.kr[b][2 * s + 1] = w[1];
+          } else {
+            st.kr[b][s] = load_at<uint32_t>(bp[b], k_off, off + s * 4 * CB);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          const u32x4 w = load_at<u32x4>(bp[b], k_off, g * 128 + s * 64);
+#pragma unroll
+          for (int i = 0; i < 4; i++) st.kr[b][4 * s + i] = w[i];
+        }
+      }
+    }
+  };
+
+  const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
+  const float cs_lane = fwht_lane_sign(lane) * a.c;
+  const uint32_t lut_l = lds_addr(lut) + (lane & (kLutCopies - 1)) * 4;
+  if constexpr (MODE == kCodebook) cb_fill_lut<CB>(lut, tid, NW * 64);
+
+  bool first = true;  // of this work-group's tiles
+  // (the last tile first: it sees the most keys, so every later one's steps have a
+  // partial to add to)
+#pragma unroll 1
+  for (int tile = a.tiles - 1 - sharer; tile >= 0; tile -= a.sharers) {
+    const int qi0 = tile * QP;
+    const int nq = a.n_q - qi0 < QP ? a.n_q - qi0 : QP;
+    const int rows = nq * G, nt = (rows + 15) / 16;
+    const int64_t p_last = q.p0 + qi0 + nq - 1, p_first = q.p0 + qi0;
+    const int64_t ml_row = (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * a.ranges;
+
+    // ---- the rows as operands: row r by wave r % NW ----
+    for (int r = tid; r < kObRows; r += NW * 64) {
+      const int rq = r / G;
+      // (a row past the chunk, or a padded one before position 0, sees nothing)
+      const int64_t p = r < rows ? q.p0 + qi0 + rq : -1;
+      row_pos[r] = (int)(p < 0 ? -1 : p);
+      if constexpr (SUMS) {
+        float M = -1e30f, l = 0.0f;
+        for (int k = 0; k < ranges; k++) {
+          const float2 x = *reinterpret_cast<const float2*>(a.ml + ((ml_row + k) * kObRows + r) * 2);
+          const float mn = fmaxf(M, x.x);
+          l = fmaf(l, exp2f(M - mn), x.y * exp2f(x.x - mn));
+          M = mn;
+        }
+        stat[0][r] = make_float2(M, l > 0.0f ? 1.0f / l : 0.0f);
+      }
+    }
+#pragma unroll 1
+    for (int r = wave; r < nt * 16; r += NW) {
+      float x[E];
+#pragma unroll
+      for (int i = 0; i < E; i++) x[i] = 0.0f;
+      uint32_t raw[E / 2];
+#pragma unroll
+      for (int i = 0; i < E / 2; i++) raw[i] = 0;
+      if (r < rows) {
+        const int rq = r / G;
+        const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
+        load_words<E / 2>(a.q + row * D + lane * E, raw);
+      }
+      const int rt = r >> 4, rc = r & 15, d0 = lane * E, o = d0 & 63;
+      if constexpr (MODE == kPlain) {
+        uint8_t* p = rows_s + (rt * 2 * NG + (d0 >> 5)) * 1024 + (((o & 31) >> 3) * 16 + rc) * 16 + (o & 7) * 2;
+#pragma unroll
+        for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < E / 2; i++) {
+          x[2 * i] = __uint_as_float(raw[i] << 16) * a.qscale;
+          x[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u) * a.qscale;
+        }
+        wave_fwht_signed<E>(x, lane);
+        float gs = 0.0f;
+        _Float16 hv[E], lv[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const float v = apply_sign(x[i] * cs_lane, sbits, i);
+          gs += v;
+          hv[i] = (_Float16)v;
+          lv[i] = (_Float16)(v - (float)hv[i]);
+        }
+        // (K's operand places: QSlot for affine caches, dims in order for codebooks)
+        const int g = d0 >> 6;
+        const int s = MODE == kAffine && BITS == 8 ? (o >> 3) & 1 : o >> 5;
+        const int jj = MODE == kAffine && BITS == 8 ? o >> 4 : (o >> 3) & 3;
+        uint8_t* p = rows_s + ((rt * 2 * NG + 2 * g + s) * 2) * 1024 + (jj * 16 + rc) * 16 + (o & 7) * 2;
+        store_halves<E>(p, hv);
+        store_halves<E>(p + 1024, lv);
+        if constexpr (MODE == kAffine) {
+          gs = group_sum<LPG>(gs, lane);
+          if ((lane & (LPG - 1)) == 0) qsum[r][g] = gs;
+        }
+      }
+    }
+    __syncthreads();
+
+    int p_row[RT];
+    float m_run[RT], l_run[RT];  // SUMS: M and 1 / L of the lane's rows
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+      p_row[rt] = rt < nt ? row_pos[rt * 16 + c] : -1;
+      m_run[rt] = -1e30f;
+      l_run[rt] = 0.0f;
+      if constexpr (SUMS) {
+        const float2 x = stat[0][rt * 16 + c];
+        m_run[rt] = x.x;
+        l_run[rt] = rt < nt ? x.y : 0.0f;
+      }
+    }
+
+    // ---- the steps: NB blocks of keys a wave ----
+    auto blocks_of = [&](int step, gptr_t (&bp)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) bp[b] = blk_ptr((step * NW + wave) * NB + b);
+    };
+    gptr_t bp[NB], bn[NB];
+    Stage cur, nxt;
+    blocks_of(s_begin, bp);
+    load(bp, 0, cur);
+#pragma unroll 1
+    for (int step = s_begin; step < s_end; step++) {
+      const int64_t key0 = (int64_t)(step * NW + wave) * NB * kBlockTokens;
+      float* part = nullptr;
+      if constexpr (SUMS)
+        part = a.part + ((int64_t)seq * a.st.n_kv_heads * a.sharers + blockIdx.y) * a.part_width + key0;
+      if (key0 > p_last) {  // nothing of this tile sees these keys, or later ones
+        if constexpr (SUMS) {
+          if (first)
+            for (int i = lane; i < NB * kBlockTokens && key0 + i < a.part_width; i += 64) part[i] = 0.0f;
+        }
+        continue;
+      }
+      blocks_of(step + 1 < s_end ? step + 1 : step, bn);
+      u32x2 kn[MODE == kCodebook ? NB : 1];
+      if constexpr (MODE == kCodebook) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) kn[b] = load_at<u32x2>(bp[b], (uint32_t)L.k_meta + 8 * j);
+      }
+      float4_t s[RT][NB];
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) s[rt][b] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        if (g + 1 < NG)
+          load(bp, g + 1, nxt);
+        else
+          load(bn, 0, nxt);
+        half8_t ah[NB][2], al[MODE == kCodebook && !kCbExact<CB> ? NB : 1][2];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            if constexpr (MODE == kAffine) {
+              ah[b][t] = k_operand_plain<BITS>(cur.kr[b], t);
+            } else if constexpr (MODE == kPlain) {
+              ah[b][t] = __builtin_bit_cast(half8_t, (u32x4){cur.kr[b][4 * t], cur.kr[b][4 * t + 1],
+                                                             cur.kr[b][4 * t + 2], cur.kr[b][4 * t + 3]});
+            } else {
+              uint32_t f;
+              if constexpr (CB == 3)
+                f = __builtin_amdgcn_alignbit(cur.kr[b][2 * t + 1], cur.kr[b][2 * t], ksh);
+              else
+                f = cur.kr[b][t] >> ksh;
+              if constexpr (kCbExact<CB>) {
+                ah[b][t] = __builtin_bit_cast(
+                    half8_t, (u32x4){cb_pair_exact<CB, 0>(lut_l, f), cb_pair_exact<CB, 1>(lut_l, f),
+                                     cb_pair_exact<CB, 2>(lut_l, f), cb_pair_exact<CB, 3>(lut_l, f)});
+              } else {
+                uint32_t h4[4], l4[4];
+                cb_pair_hl4<0>(lut_l, f, h4[0], l4[0]);
+                cb_pair_hl4<1>(lut_l, f, h4[1], l4[1]);
+                cb_pair_hl4<2>(lut_l, f, h4[2], l4[2]);
+                cb_pair_hl4<3>(lut_l, f, h4[3], l4[3]);
+                ah[b][t] = __builtin_bit_cast(half8_t, (u32x4){h4[0], h4[1], h4[2], h4[3]});
+                al[b][t] = __builtin_bit_cast(half8_t, (u32x4){l4[0], l4[1], l4[2], l4[3]});
+              }
+            }
+          }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+          if (rt >= nt) continue;  // (uniform)
+          half8_t bh[2], bl[2];
+#pragma unroll
+          for (int t = 0; t < 2; t++) {
+            const uint8_t* p = rows_s + ((rt * 2 * NG + 2 * g + t) * P::kParts) * 1024 + lane * 16;
+            bh[t] = *reinterpret_cast<const half8_t*>(p);
+            if constexpr (MODE != kPlain) bl[t] = *reinterpret_cast<const half8_t*>(p + 1024);
+          }
+          float4_t acc[NB];
+#pragma unroll
+          for (int b = 0; b < NB; b++) acc[b] = MODE == kAffine ? (float4_t){0.f, 0.f, 0.f, 0.f} : s[rt][b];
+          if constexpr (MODE == kPlain) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+              for (int b = 0; b < NB; b++)
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ah[b][t]),
+                                                                 __builtin_bit_cast(bf16x8_t, bh[t]), acc[b], 0, 0, 0);
+          } else {
+            // the residuals' products first
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+              for (int b = 0; b < NB; b++)
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b][t], bl[t], acc[b], 0, 0, 0);
+            if constexpr (MODE == kCodebook && !kCbExact<CB>) {
+#pragma unroll
+              for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                  acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[b][t], bh[t], acc[b], 0, 0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+              for (int b = 0; b < NB; b++)
+                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b][t], bh[t], acc[b], 0, 0, 0);
+          }
+          if constexpr (MODE == kAffine) {
+            const float qs = qsum[rt * 16 + c][g];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+              for (int i = 0; i < 4; i++)
+                s[rt][b][i] = fmaf(lo16(cur.km[b][i]), acc[b][i], fmaf(hi16(cur.km[b][i]), qs, s[rt][b][i]));
+          } else {
+#pragma unroll
+            for (int b = 0; b < NB; b++) s[rt][b] = acc[b];
+          }
+        }
+        cur = nxt;
+      }
+#pragma unroll
+      for (int b = 0; b < NB; b++) bp[b] = bn[b];
+
+      // ---- softmax: lane (j, c) has keys 16 b + 4 j + i of rows 16 rt + c ----
+      const bool full = key0 + NB * kBlockTokens - 1 <= p_first && rows == nt * 16 && p_first >= 0;
+      float4_t w[SUMS ? NB : 1];
+      if constexpr (SUMS) {
+#pragma unroll
+        for (int b = 0; b < NB; b++) w[b] = (float4_t){0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) {
+        if (rt >= nt) continue;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if constexpr (MODE == kCodebook) {
+              const uint32_t n = kn[b][i >> 1];
+              s[rt][b][i] *= (i & 1 ? hi16(n) : lo16(n)) * (a.c * kCbOperandScale<CB>);
+            }
+            if constexpr (MODE == kPlain) s[rt][b][i] *= a.qscale;
+          }
+        if (!full) {
+          const int rel = p_row[rt] - (int)key0 - 4 * j;  // (key0 <= p_last: both fit)
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (16 * b + i > rel) s[rt][b][i] = -INFINITY;
+        }
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              w[b][i] = fmaf(__builtin_amdgcn_exp2f(s[rt][b][i] - m_run[rt]), l_run[rt], w[b][i]);
+        } else {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+            mx = fmaxf(mx, fmaxf(fmaxf(s[rt][b][0], s[rt][b][1]), fmaxf(s[rt][b][2], s[rt][b][3])));
+          if (__any(mx > m_run[rt] + kObSlack)) {
+            const float m_new = fmaxf(m_run[rt], mx);
+            l_run[rt] *= __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+            m_run[rt] = m_new;
+          }
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = __builtin_amdgcn_exp2f(s[rt][b][i] - m_run[rt]);
+            l_run[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+          }
+        }
+      }
+      if constexpr (SUMS) {  // the sixteen lanes of a key meet; lane c < NB stores block c's
+        float4_t mine = w[0];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) w[b][i] = group_sum<16>(w[b][i], lane);
+          if (c == b) mine = w[b];
+        }
+        const int64_t at = 16 * c + 4 * j;
+        if (c < NB && key0 + at < a.part_width) {
+          float4_t* p = reinterpret_cast<float4_t*>(part + at);
+          *p = first ? mine : *p + mine;
+        }
+      }
+    }
+    first = false;
+    if constexpr (!SUMS) {
+      // (m, l) of the lanes' key quarters, then of the waves
+#pragma unroll
+      for (int rt = 0; rt < RT; rt++) {
+        const float M = xor32_max(xor16_max(m_run[rt]));
+        const float l = xor32_sum(xor16_sum(l_run[rt] * __builtin_amdgcn_exp2f(m_run[rt] - M)));
+        if (j == 0) stat[wave][rt * 16 + c] = make_float2(M, l);
+      }
+      __syncthreads();
+      if (tid < kObRows) {
+        float M = stat[0][tid].x, l = 0.0f;
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, stat[w][tid].x);
+#pragma unroll
+        for (int w = 0; w < NW; w++) l = fmaf(stat[w][tid].y, exp2f(stat[w][tid].x - M), l);
+        *reinterpret_cast<float2*>(a.ml + ((ml_row + range) * kObRows + tid) * 2) = make_float2(M, l);
+      }
+    }
+    __syncthreads();  // the rows and their statistics are done with
+  }
+}
+
+// weights_out[s][j] = weights_in[s][j] + the partials of position j, in order.
+__global__ __launch_bounds__(256) void observe_sum_kernel(ObserveArgs a) {
+  const int seq = blockIdx.y;
+  int64_t T = (int64_t)a.start_pos[seq] + a.n_q;
+  if (T > a.weights_width) T = a.weights_width;
+  const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (p >= T) return;
+  const int n = a.st.n_kv_heads * a.sharers;
+  float sum = 0.0f;
+  if (p < (int64_t)a.blocks * kBlockTokens) {
+    const float* src = a.part + (int64_t)seq * n * a.part_width + p;
+#pragma unroll 8
+    for (int i = 0; i < n; i++) sum += src[(int64_t)i * a.part_width];
+  }
+  const int64_t at = (int64_t)seq * a.weights_width + p;
+  a.weights_out[at] = (a.weights_in ? a.weights_in[at] : 0.0f) + sum;
+}
+
+template <int D, int BITS, int MODE, int NB>
+hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
+  const dim3 grid(a.ranges, a.st.n_kv_heads * a.sharers, a.n_seqs), block(ObPlan<D, BITS, MODE>::NW * 64);
+  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, NB, false>), grid, block, 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, NB, true>), grid, block, 0, s, a);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const int64_t keys = (int64_t)a.blocks * kBlockTokens;
+  hipLaunchKernelGGL(observe_sum_kernel, dim3((unsigned)((keys + 255) / 256), a.n_seqs), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+template <int D, int BITS, int MODE>
+hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
+  return a.step_blocks == 4 ? launch_ob<D, BITS, MODE, 4>(a, s) : launch_ob<D, BITS, MODE, 1>(a, s);
+}
+
+}  // namespace
+
+size_t observe_plan(ObserveArgs& a, int cus) {
+  const int D = a.st.layout.head_dim, waves = D == 512 ? 8 : 4;
+  const int64_t places = (int64_t)cus * (D == 512 ? 1 : 2);  // work-groups that run at once
+  const int qp = kObRows / a.group;
+  a.tiles = (a.n_q + qp - 1) / qp;
+  const int64_t per_tile = (int64_t)a.st.n_kv_heads * a.n_seqs;
+  const int64_t rows = per_tile * a.tiles;
+  a.step_blocks = rows * ((a.blocks + 4 * waves - 1) / (4 * waves)) >= places ? 4 : 1;
+  const int64_t steps = (a.blocks + waves * a.step_blocks - 1) / (waves * a.step_blocks);
+  // as many work-groups as run at once, several tiles one after the other where there are more
+  a.sharers = (int32_t)std::clamp<int64_t>(2 * places / per_tile, 1, a.tiles);
+  a.ranges = (int32_t)std::clamp<int64_t>(places / (per_tile * a.sharers), 1, steps);
+  a.part_width = (int64_t)a.blocks * kBlockTokens;
+  return (size_t)(rows * a.ranges * kObRows * 2 + per_tile * a.sharers * a.part_width);
+}
+
+hipError_t launch_observe(const ObserveArgs& a, hipStream_t s) {
+  const BlockLayout& L = a.st.layout;
+  if (L.mode == kAffine) {
+    switch (L.head_dim * 16 + L.bits) {
+      case 128 * 16 + 4: return launch_ob<128, 4, kAffine>(a, s);
+      case 128 * 16 + 8: return launch_ob<128, 8, kAffine>(a, s);
+      case 256 * 16 + 4: return launch_ob<256, 4, kAffine>(a, s);
+      case 256 * 16 + 8: return launch_ob<256, 8, kAffine>(a, s);
+      case 512 * 16 + 4: return launch_ob<512, 4, kAffine>(a, s);
+      case 512 * 16 + 8: return launch_ob<512, 8, kAffine>(a, s);
+    }
+  } else if (L.mode == kCodebook) {
+    switch (L.head_dim * 16 + L.bits) {
+      case 128 * 16 + 2: return launch_ob<128, 2, kCodebook>(a, s);
+      case 128 * 16 + 3: return launch_ob<128, 3, kCodebook>(a, s);
+      case 128 * 16 + 4: return launch_ob<128, 4, kCodebook>(a, s);
+      case 256 * 16 + 2: return launch_ob<256, 2, kCodebook>(a, s);
+      case 256 * 16 + 3: return launch_ob<256, 3, kCodebook>(a, s);
+      case 256 * 16 + 4: return launch_ob<256, 4, kCodebook>(a, s);
+      case 512 * 16 + 2: return launch_ob<512, 2, kCodebook>(a, s);
+      case 512 * 16 + 3: return launch_ob<512, 3, kCodebook>(a, s);
+      case 512 * 16 + 4: return launch_ob<512, 4, kCodebook>(a, s);
+    }
+  } else if (L.mode == kPlain) {
+    switch (L.head_dim) {
+      case 128: return launch_ob<128, 16, kPlain>(a, s);
+      case 256: return launch_ob<256, 16, kPlain>(a, s);
+      case 512: return launch_ob<512, 16, kPlain>(a, s);
+    }
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace fmkv

@@ -59,7 +59,7 @@ EXPORTED = (
     "fmkv_pools_copy_blocks", "fmkv_paged_compact", "fmkv_qkv_norm_rope",
     "fmkv_paged_prefix_decode_attention", "fmkv_paged_prefix_decode_step",
     "fmkv_paged_weighing_decode_attention", "fmkv_paged_weighing_decode_step",
-    "fmkv_heaviest_tokens",
+    "fmkv_paged_attention_weights", "fmkv_heaviest_tokens",
     "fmkv_pages_create", "fmkv_pages_destroy", "fmkv_pages_free_count", "fmkv_pages_users",
     "fmkv_pages_alloc", "fmkv_pages_release", "fmkv_pages_fork", "fmkv_pages_slide",
 )
@@ -242,6 +242,8 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
                                                   ctypes.c_float, vp, i32, vp], ctypes.c_int),
         "fmkv_paged_weighing_decode_step": ([vp, vp, vp, vp, i32, vp, vp, i32, i32, vp, vp, vp, i32,
                                              i32, ctypes.c_float, vp, i32, vp], ctypes.c_int),
+        "fmkv_paged_attention_weights": ([vp, vp, vp, i32, vp, i32, i32, i32, vp, vp, i32, i32,
+                                          ctypes.c_float, vp], ctypes.c_int),
         "fmkv_heaviest_tokens": ([vp, i32, vp, i32, i32, i32, i32, vp, vp, vp, i32, vp],
                                  ctypes.c_int),
         "fmkv_pages_create": ([i64, P(vp)], ctypes.c_int),
@@ -891,6 +893,23 @@ class PagedPool:
             _here(weights, dev), _here(weights_out, dev), weights_out.shape[1], heads, scale,
             _here(out, dev), _dtype_code(out.dtype), _stream(stream)))
         return out, weights_out
+
+    def attention_weights(self, q, block_tables, start_pos, max_seq_len: int, weights=None,
+                          weights_out=None, scale: float = 1.0, stream=None):
+        """The accumulated weights alone, of q bf16 [n_seqs, n_new, n_q_heads, D] at
+        positions start_pos .. start_pos + n_new - 1, whose keys were appended
+        before, each over the positions up to its own; max_seq_len bounds start_pos + n_new.
+        weights, weights_out: see weighing_attention. Returns weights_out."""
+        n, n_new, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, None, self._D))
+        width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
+        _check_tensor("start_pos", start_pos, torch.int32, (n,))
+        dev = self._device
+        weights_out = _sums(weights, weights_out, n, max_seq_len, q, stream)
+        _check(self._lib.fmkv_paged_attention_weights(
+            self._h, _here(q, dev), _here(block_tables, dev), width, _here(start_pos, dev), n, n_new,
+            max_seq_len, _here(weights, dev), _here(weights_out, dev), weights_out.shape[1], heads,
+            scale, _stream(stream)))
+        return weights_out
 
     def compact(self, block_tables, keep, n_keep, dst_tables, stream=None) -> None:
         """Moves the tokens that sequences keep to the front of other blocks:

@@ -467,6 +467,20 @@ int fmkv_paged_weighing_decode_step(fmkv_pool* pool, const void* k_bf16, const v
                                     int32_t weights_width, int32_t n_q_heads, float scale,
                                     void* out, int32_t out_dtype, void* stream);
 
+/* The accumulated weights of n_new consecutive queries per sequence at start_pos ..
+ * start_pos + n_new - 1 (a prompt's last ones, say; the softmax of query p is over
+ * the positions j <= p), whose keys are in the pool already. V is not read, and no
+ * attention is returned (fmkv_paged_prefill_step and the windowed calls give it).
+ * q: bf16 [n_seqs][n_new][n_q_heads][head_dim]. max_seq_len bounds start_pos + n_new.
+ * Queries at positions below 0 (a padded row's) add nothing. At most 8 query heads per KV
+ * head, every cache mode. The current GPU has to be the pool's; for calls on several
+ * streams, and graphs, see the windowed calls above. */
+int fmkv_paged_attention_weights(fmkv_pool* pool, const void* q_bf16, const int32_t* block_tables,
+                                 int32_t max_blocks, const int32_t* start_pos, int32_t n_seqs,
+                                 int32_t n_new, int32_t max_seq_len, const float* weights,
+                                 float* weights_out, int32_t weights_width, int32_t n_q_heads,
+                                 float scale, void* stream);
+
 /* The positions that each sequence keeps: of more than max_keep its first
  * `sinks` and last `recent` ones and the heaviest of the others, max_keep in all
  * (equal weights: the lower position first; a NaN is lighter than any weight); of
