@@ -853,6 +853,22 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   const int64_t share = (total + n_slots - 1) / n_slots;
   const int min_bps = (int)std::min<int64_t>(64, std::max<int64_t>(share, 1));
   const int wg_per_cu = 6 * slots * fmkv::kAttnWgPerCu;
+  if (win == kNoWindow) {
+    // Lengths that no window makes alike: sequences count half of the longest, at most
+    // 64 blocks a split, and first splits of four times that as above. (Seven of 65 ..
+    // 20011 tokens, 8 bits, 2 heads of 512 dims: 35 blocks 33.5 us, the longest's
+    // plan, 68 and 64 blocks, 42.5 and 40.6, 24: 44.3; 32 of 512 .. 16384, 4 bits, 8
+    // heads of 256 dims: 64 blocks, first splits four times that, 106; 171: 163. What 41 sequences have behind
+    // their prefixes, 32 blocks at most, bf16, 4 heads of 128 dims: 4 blocks 40.9 us the call, 8 with first
+    // splits of 32: 60.4.)
+    const int64_t rows = (int64_t)p->desc.n_kv_heads * n_s;
+    int64_t b = window_bps(p->desc, p->cus, nblk, n_s > 1 ? (rows + 1) / 2 : rows, new_col);
+    if (n_s > 1) b = std::min<int64_t>(b, 64);
+    const int mult = b >= 64 && total >= 4 * n_slots * b ? 4 : 1;
+    return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,
+                                    max_blocks, q, n_q_heads, scale, tau, out, out_dtype,
+                                    1 << 20 /* b is the blocks per split */, (int)b, mult, new_col, a);
+  }
   if (win > 0) {
     const int64_t b = window_bps(p->desc, p->cus, nblk, (int64_t)p->desc.n_kv_heads * n_s, new_col);
     return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,

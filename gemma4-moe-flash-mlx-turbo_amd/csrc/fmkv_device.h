@@ -309,6 +309,18 @@ __device__ inline void wave_fwht(float (&x)[E], int lane) {
   fwht_lane_stage<32>(x, lane);
 }
 
+// The sums of lanes 0 .. l, in every lane l: DPP row shifts, then the last
+// lanes of rows broadcast over the rows after them.
+__device__ inline int scan_add(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+  return v;
+}
+
 // Visible-position test shared by the attention and combine kernels.
 struct SeqGeom {
   int64_t blk_lo, blk_hi;  // logical blocks to scan

@@ -336,7 +336,7 @@ struct ObserveArgs {
   // the plan: blocks of a wave's step, ranges of keys, tiles of a KV head, the
   // work-groups that share them
   int32_t step_blocks, ranges, tiles, sharers;
-  float* ml;    // [n_seqs][n_kv_heads][tiles][ranges][64] (m, l)
+  float* ml;    // [n_seqs][n_kv_heads][tiles][64][ranges] (m, l)
   float* part;  // [n_seqs][n_kv_heads * sharers][part_width] sums of weights
   int64_t part_width;
   const float* weights_in;

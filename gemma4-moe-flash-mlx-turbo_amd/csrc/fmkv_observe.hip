@@ -23,6 +23,7 @@
 // registers until all rows are done; 16 lanes meet at the end. Every sum has one
 // order: no atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "fmkv_device.h"
 #include "fmkv_internal.h"
@@ -33,16 +34,29 @@ namespace fmkv {
 namespace {
 
 constexpr int kObRows = 64;
-constexpr int kObTiles = kObRows / 16;
 constexpr float kObSlack = 8.0f;  // (base 2) a score may exceed its row's reference by
 
-template <int D, int BITS, int MODE>
+// A power of 2 of the codes' offset that goes to the scales it is multiplied with,
+// so that neither that nor the sums of q times the rest leave f16.
+template <int BITS>
+constexpr float kScaleUp = BITS == 8 ? 64.0f : 1.0f;
+
+// Blocks of a wave's step in calls of many keys: what the registers hold.
+constexpr int many_blocks(int mode) { return mode == kAffine ? 3 : 4; }
+
+template <int D, int BITS, int MODE, int RT>
 struct ObPlan {
   static constexpr BlockLayout L = make_layout(D, BITS, MODE);
   static constexpr int NG = D / 64, E = D / 64;
-  static constexpr int NW = D == 512 ? 8 : 4;  // waves (512 dims' rows fill a CU's LDS)
+  static constexpr int NW = 8;  // waves: two a SIMD, what their registers allow
   static constexpr int kParts = MODE == kPlain ? 1 : 2;  // high parts, residuals
-  static constexpr int kRows = kObTiles * 2 * NG * kParts * 1024;
+  // An operand's place: part, tile of rows, 32 dims. 16 bytes more than its 1 KiB: the
+  // lanes that write a row, whose pieces lie in as many operands, then take all banks
+  // and not the same few (512 dims, a
+  // work-group's 64 rows and one step of keys: 28.0 -> 26.3 us).
+  static constexpr int operand(int part, int rt, int e) { return ((part * RT + rt) * 2 * NG + e) * 1040; }
+  static constexpr int kSums = operand(kParts, 0, 0);  // the operands of the biases
+  static constexpr int kRows = kSums + (MODE == kAffine ? RT * 1024 : 0);
   static constexpr int KW = MODE == kAffine ? BITS / 2 : MODE == kPlain ? 8 : BITS == 3 ? 4 : 2;
   static constexpr int kLut = MODE == kCodebook ? CbLut<BITS == 16 ? 2 : BITS>::kBytes : 16;
 };
@@ -67,19 +81,20 @@ __device__ inline ObSeq ob_seq(const ObserveArgs& a, int seq) {
 }
 
 // SUMS: the second launch. Grid (range of keys, KV head and sharer of its tiles, sequence).
-template <int D, int BITS, int MODE, int NB, bool SUMS>
-__global__ __launch_bounds__((ObPlan<D, BITS, MODE>::NW * 64))
+// RT: matrix-core tiles of the rows, 4, or 1 where all calls' tiles have 16 rows at most.
+template <int D, int BITS, int MODE, int RT, int NB, bool SUMS>
+__global__ __launch_bounds__((ObPlan<D, BITS, MODE, RT>::NW * 64))
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 void observe_kernel(ObserveArgs a) {
-  using P = ObPlan<D, BITS, MODE>;
+  using P = ObPlan<D, BITS, MODE, RT>;
   constexpr BlockLayout L = P::L;
-  constexpr int NG = P::NG, NW = P::NW, E = P::E, KW = P::KW, LPG = 64 / E, RT = kObTiles;
+  constexpr int NG = P::NG, NW = P::NW, E = P::E, KW = P::KW;
+  constexpr int LPG = 64 / E;  // lanes of a 64-dim group
   constexpr int CB = MODE == kCodebook ? BITS : 2;
   __shared__ __align__(16) uint8_t rows_s[P::kRows];
   __shared__ __align__(16) uint8_t lut[P::kLut];
-  __shared__ float qsum[kObRows][NG];
-  __shared__ int row_pos[kObRows];
-  __shared__ float2 stat[SUMS ? 1 : NW][kObRows];  // (m, l) of the waves; SUMS: M, 1 / L
+  __shared__ int row_pos[RT * 16];
+  __shared__ float2 stat[SUMS ? 1 : NW][RT * 16];  // (m, l) of the waves; SUMS: M, 1 / L
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -111,9 +126,22 @@ void observe_kernel(ObserveArgs a) {
                                                 : MODE == kCodebook ? (kbit >> 5) * 4
                                                                     : (c * D + 8 * j) * 2);
   const uint32_t km_off = (uint32_t)L.k_meta + j * 16;
+  const uint32_t kb_off = (uint32_t)L.k_meta + c * 4 + (j < 2 ? 2 : 0);
+  const U4Consts u4;
   struct Stage {
     uint32_t kr[NB][KW];
     u32x4 km[NB];
+  };
+  // affine: the biases (lanes (0, c), (1, c)) or scales of key c of each block, by group
+  auto load_bias = [&](const gptr_t (&bp)[NB], half8_t (&x)[NB]) __attribute__((always_inline)) {
+    if constexpr (MODE == kAffine) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        x[b] = half8_t{};
+#pragma unroll
+        for (int g = 0; g < NG; g++) x[b][g] = load_at<_Float16>(bp[b], kb_off, g * 64);
+      }
+    }
   };
   auto load = [&](const gptr_t (&bp)[NB], int g, Stage& st) __attribute__((always_inline)) {
 #pragma unroll
@@ -156,6 +184,11 @@ void observe_kernel(ObserveArgs a) {
   const float cs_lane = fwht_lane_sign(lane) * a.c;
   const uint32_t lut_l = lds_addr(lut) + (lane & (kLutCopies - 1)) * 4;
   if constexpr (MODE == kCodebook) cb_fill_lut<CB>(lut, tid, NW * 64);
+  if constexpr (MODE == kAffine) {  // (what of the biases' operands no group fills is 0)
+    for (int i = tid; i < RT * 64; i += NW * 64)
+      reinterpret_cast<u32x4*>(rows_s + P::kSums)[i] = (u32x4){0, 0, 0, 0};
+    __syncthreads();
+  }
 
   bool first = true;  // of this work-group's tiles
   // (the last tile first: it sees the most keys, so every later one's steps have a
@@ -164,71 +197,119 @@ void observe_kernel(ObserveArgs a) {
   for (int tile = a.tiles - 1 - sharer; tile >= 0; tile -= a.sharers) {
     const int qi0 = tile * QP;
     const int nq = a.n_q - qi0 < QP ? a.n_q - qi0 : QP;
-    const int rows = nq * G, nt = (rows + 15) / 16;
+    const int rows = nq * G;
     const int64_t p_last = q.p0 + qi0 + nq - 1, p_first = q.p0 + qi0;
-    const int64_t ml_row = (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * a.ranges;
+    const int64_t ml_row = (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * kObRows;
+
+    auto blocks_of = [&](int step, gptr_t (&bp)[NB]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++) bp[b] = blk_ptr((step * NW + wave) * NB + b);
+    };
+    gptr_t bp[NB], bn[NB];
+    Stage cur, nxt;
+    half8_t bias[NB];
+    blocks_of(s_begin, bp);
+    load(bp, 0, cur);
+    load_bias(bp, bias);
 
     // ---- the rows as operands: row r by wave r % NW ----
-    for (int r = tid; r < kObRows; r += NW * 64) {
+    for (int r = tid; r < RT * 16; r += NW * 64) {
       const int rq = r / G;
       // (a row past the chunk, or a padded one before position 0, sees nothing)
       const int64_t p = r < rows ? q.p0 + qi0 + rq : -1;
       row_pos[r] = (int)(p < 0 ? -1 : p);
-      if constexpr (SUMS) {
+    }
+    if constexpr (SUMS) {  // sixteen lanes a row: each merges every sixteenth range, then they meet
+#pragma unroll 2
+      for (int r = tid >> 4; r < RT * 16; r += NW * 4) {
+        const float2* x = reinterpret_cast<const float2*>(a.ml) + (ml_row + r) * a.ranges;
         float M = -1e30f, l = 0.0f;
-        for (int k = 0; k < ranges; k++) {
-          const float2 x = *reinterpret_cast<const float2*>(a.ml + ((ml_row + k) * kObRows + r) * 2);
-          const float mn = fmaxf(M, x.x);
-          l = fmaf(l, exp2f(M - mn), x.y * exp2f(x.x - mn));
+#pragma unroll 4
+        for (int k = tid & 15; k < ranges; k += 16) {
+          const float mn = fmaxf(M, x[k].x);
+          l = fmaf(l, exp2f(M - mn), x[k].y * exp2f(x[k].x - mn));
           M = mn;
         }
-        stat[0][r] = make_float2(M, l > 0.0f ? 1.0f / l : 0.0f);
+        const float Mx = group_max<16>(M, lane);
+        l = group_sum<16>(l * exp2f(M - Mx), lane);
+        if ((tid & 15) == 0) stat[0][r] = make_float2(Mx, l > 0.0f ? 1.0f / l : 0.0f);
       }
     }
-#pragma unroll 1
-    for (int r = wave; r < nt * 16; r += NW) {
-      float x[E];
+    // Four rows of a wave at a time, the next four on their way meanwhile
+    uint32_t raw[4][E / 2], ahead[4][E / 2];
+    auto load_rows = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < E; i++) x[i] = 0.0f;
-      uint32_t raw[E / 2];
-#pragma unroll
-      for (int i = 0; i < E / 2; i++) raw[i] = 0;
-      if (r < rows) {
-        const int rq = r / G;
+      for (int k = 0; k < 4; k++) {
+        const int rr = r0 + k * NW, r = rr < rows ? rr : rows - 1, rq = r / G;
         const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
-        load_words<E / 2>(a.q + row * D + lane * E, raw);
+        load_words<E / 2>(a.q + row * D + lane * E, ahead[k]);
       }
-      const int rt = r >> 4, rc = r & 15, d0 = lane * E, o = d0 & 63;
-      if constexpr (MODE == kPlain) {
-        uint8_t* p = rows_s + (rt * 2 * NG + (d0 >> 5)) * 1024 + (((o & 31) >> 3) * 16 + rc) * 16 + (o & 7) * 2;
+    };
+    load_rows(wave);
+#pragma unroll 1
+    for (int r0 = wave; r0 < RT * 16; r0 += 4 * NW) {
 #pragma unroll
-        for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[i];
-      } else {
+      for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int i = 0; i < E / 2; i++) {
-          x[2 * i] = __uint_as_float(raw[i] << 16) * a.qscale;
-          x[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u) * a.qscale;
+        for (int i = 0; i < E / 2; i++) raw[k][i] = r0 + k * NW < rows ? ahead[k][i] : 0u;
+      if (r0 + 4 * NW < RT * 16) load_rows(r0 + 4 * NW);
+      const int d0 = lane * E, o = d0 & 63;
+      float x[4][E];
+      if constexpr (MODE != kPlain) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+#pragma unroll
+          for (int i = 0; i < E / 2; i++) {
+            x[k][2 * i] = __uint_as_float(raw[k][i] << 16) * a.qscale;
+            x[k][2 * i + 1] = __uint_as_float(raw[k][i] & 0xffff0000u) * a.qscale;
+          }
+          wave_fwht_signed<E>(x[k], lane);
         }
-        wave_fwht_signed<E>(x, lane);
-        float gs = 0.0f;
-        _Float16 hv[E], lv[E];
+      }
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-          const float v = apply_sign(x[i] * cs_lane, sbits, i);
-          gs += v;
-          hv[i] = (_Float16)v;
-          lv[i] = (_Float16)(v - (float)hv[i]);
-        }
-        // (K's operand places: QSlot for affine caches, dims in order for codebooks)
-        const int g = d0 >> 6;
-        const int s = MODE == kAffine && BITS == 8 ? (o >> 3) & 1 : o >> 5;
-        const int jj = MODE == kAffine && BITS == 8 ? o >> 4 : (o >> 3) & 3;
-        uint8_t* p = rows_s + ((rt * 2 * NG + 2 * g + s) * 2) * 1024 + (jj * 16 + rc) * 16 + (o & 7) * 2;
-        store_halves<E>(p, hv);
-        store_halves<E>(p + 1024, lv);
-        if constexpr (MODE == kAffine) {
-          gs = group_sum<LPG>(gs, lane);
-          if ((lane & (LPG - 1)) == 0) qsum[r][g] = gs;
+      for (int k = 0; k < 4; k++) {
+        const int r = r0 + k * NW, rt = r >> 4, rc = r & 15;
+        if (r >= RT * 16) continue;
+        if constexpr (MODE == kPlain) {
+          const int e = d0 >> 5;
+          uint8_t* p = rows_s + P::operand(0, rt, e) + (((o & 31) >> 3) * 16 + rc) * 16 + (o & 7) * 2;
+#pragma unroll
+          for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[k][i];
+        } else {
+          float gs = 0.0f;
+          _Float16 hv[E], lv[E];
+#pragma unroll
+          for (int i = 0; i < E; i++) {
+            const float v = apply_sign(x[k][i] * cs_lane, sbits, i);
+            gs += v;
+            hv[i] = (_Float16)v;
+            lv[i] = (_Float16)(v - (float)hv[i]);
+            if constexpr (MODE == kAffine) {  // (exact)
+              hv[i] = hv[i] * (_Float16)kCodeScale<BITS>;
+              lv[i] = lv[i] * (_Float16)kCodeScale<BITS>;
+            }
+          }
+          // (K's operand places: QSlot for affine caches, dims in order for codebooks)
+          const int g = d0 >> 6;
+          const int s = MODE == kAffine && BITS == 8 ? (o >> 3) & 1 : o >> 5;
+          const int jj = MODE == kAffine && BITS == 8 ? o >> 4 : (o >> 3) & 3;
+          uint8_t* p = rows_s + (jj * 16 + rc) * 16 + (o & 7) * 2;
+          store_halves<E>(p + P::operand(0, rt, 2 * g + s), hv);
+          store_halves<E>(p + P::operand(1, rt, 2 * g + s), lv);
+          if constexpr (MODE == kAffine) {
+            gs = group_sum<LPG>(gs, lane);
+            if ((lane & (LPG - 1)) == 0) {
+              // sums of 64 dims, high parts and residuals, against the biases; and
+              // the sums that the codes' offset adds, against the scales
+              _Float16* q = reinterpret_cast<_Float16*>(rows_s + P::kSums + rt * 1024) + rc * 8 + g;
+              const float off = gs * (-kCodeOffset<BITS> / kScaleUp<BITS>);
+              const _Float16 h = (_Float16)gs, ho = (_Float16)off;
+              q[0] = h;
+              q[16 * 8] = (_Float16)(gs - (float)h);
+              q[32 * 8] = ho;
+              q[48 * 8] = (_Float16)(off - (float)ho);
+            }
+          }
         }
       }
     }
@@ -238,25 +319,27 @@ void observe_kernel(ObserveArgs a) {
     float m_run[RT], l_run[RT];  // SUMS: M and 1 / L of the lane's rows
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-      p_row[rt] = rt < nt ? row_pos[rt * 16 + c] : -1;
+      p_row[rt] = row_pos[rt * 16 + c];
       m_run[rt] = -1e30f;
       l_run[rt] = 0.0f;
       if constexpr (SUMS) {
         const float2 x = stat[0][rt * 16 + c];
         m_run[rt] = x.x;
-        l_run[rt] = rt < nt ? x.y : 0.0f;
+        l_run[rt] = x.y;
       }
     }
 
     // ---- the steps: NB blocks of keys a wave ----
-    auto blocks_of = [&](int step, gptr_t (&bp)[NB]) __attribute__((always_inline)) {
+    // the next products' operands, rows of a tile and 64 dims: residuals, high parts
+    half8_t rows_l[2], rows_h[2];
+    auto load_tile = [&](half8_t (&x)[2], int part, int rt, int g) __attribute__((always_inline)) {
 #pragma unroll
-      for (int b = 0; b < NB; b++) bp[b] = blk_ptr((step * NW + wave) * NB + b);
+      for (int t = 0; t < 2; t++)
+        x[t] = *reinterpret_cast<const half8_t*>(
+            rows_s + P::operand(part, rt, 2 * g + t) + lane * 16);
     };
-    gptr_t bp[NB], bn[NB];
-    Stage cur, nxt;
-    blocks_of(s_begin, bp);
-    load(bp, 0, cur);
+    if constexpr (MODE != kPlain) load_tile(rows_l, 1, 0, 0);
+    load_tile(rows_h, 0, 0, 0);
 #pragma unroll 1
     for (int step = s_begin; step < s_end; step++) {
       const int64_t key0 = (int64_t)(step * NW + wave) * NB * kBlockTokens;
@@ -276,24 +359,49 @@ void observe_kernel(ObserveArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; b++) kn[b] = load_at<u32x2>(bp[b], (uint32_t)L.k_meta + 8 * j);
       }
+      // The scores start at -M (SUMS, affine), and at the biases' and the codes' offset's part, one
+      // product of 16 keys' biases and scales (lanes (0, c) and (1, c): key c's biases of groups
+      // 0 .. 7, the others its scales) with the rows' sums
       float4_t s[RT][NB];
 #pragma unroll
-      for (int rt = 0; rt < RT; rt++)
+      for (int b = 0; b < NB; b++) {
+        half8_t kb{};
+        if constexpr (MODE == kAffine) {
 #pragma unroll
-        for (int b = 0; b < NB; b++) s[rt][b] = (float4_t){0.f, 0.f, 0.f, 0.f};
+          for (int g = 0; g < 8; g++) kb[g] = bias[b][g] * (j < 2 ? (_Float16)1.0f : (_Float16)kScaleUp<BITS>);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+          const float z = SUMS && MODE == kAffine ? -m_run[rt] : 0.0f;
+          s[rt][b] = (float4_t){z, z, z, z};
+          if constexpr (MODE == kAffine) {
+            const half8_t qb = *reinterpret_cast<const half8_t*>(rows_s + P::kSums + rt * 1024 + lane * 16);
+            s[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, s[rt][b], 0, 0, 0);
+              __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         if (g + 1 < NG)
           load(bp, g + 1, nxt);
         else
           load(bn, 0, nxt);
-        half8_t ah[NB][2], al[MODE == kCodebook && !kCbExact<CB> ? NB : 1][2];
+        half8_t ah[NB][2], al[NB][2];  // (al: 4-bit codebooks)
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
           for (int t = 0; t < 2; t++) {
             if constexpr (MODE == kAffine) {
-              ah[b][t] = k_operand_plain<BITS>(cur.kr[b], t);
+              if constexpr (BITS == 8) {
+                const uint32_t w0 = cur.kr[b][2 * t], w1 = cur.kr[b][2 * t + 1];
+                ah[b][t] = cat8(u8x2_to_h2_biased(w0, 0x04010400u), u8x2_to_h2_biased(w0, 0x04030402u),
+                                u8x2_to_h2_biased(w1, 0x04010400u), u8x2_to_h2_biased(w1, 0x04030402u));
+              } else {
+                const uint32_t x = cur.kr[b][t];
+                ah[b][t] = cat8(u4x2_to_h2_unit(x, 0, u4), u4x2_to_h2_unit(x, 1, u4),
+                                u4x2_to_h2_unit(x, 2, u4), u4x2_to_h2_unit(x, 3, u4));
+              }
             } else if constexpr (MODE == kPlain) {
               ah[b][t] = __builtin_bit_cast(half8_t, (u32x4){cur.kr[b][4 * t], cur.kr[b][4 * t + 1],
                                                              cur.kr[b][4 * t + 2], cur.kr[b][4 * t + 3]});
@@ -320,63 +428,54 @@ void observe_kernel(ObserveArgs a) {
           }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-          if (rt >= nt) continue;  // (uniform)
-          half8_t bh[2], bl[2];
-#pragma unroll
-          for (int t = 0; t < 2; t++) {
-            const uint8_t* p = rows_s + ((rt * 2 * NG + 2 * g + t) * P::kParts) * 1024 + lane * 16;
-            bh[t] = *reinterpret_cast<const half8_t*>(p);
-            if constexpr (MODE != kPlain) bl[t] = *reinterpret_cast<const half8_t*>(p + 1024);
-          }
           float4_t acc[NB];
 #pragma unroll
           for (int b = 0; b < NB; b++) acc[b] = MODE == kAffine ? (float4_t){0.f, 0.f, 0.f, 0.f} : s[rt][b];
-          if constexpr (MODE == kPlain) {
+          // The residuals' products first; a part's operands of the next tile come as soon
+          // as this one's products are under way. (The barriers keep the compiler from
+          // starting all tiles of a step at once, which no registers hold.)
+          const int rn = rt + 1 < RT ? rt + 1 : 0, gn = rn ? g : g + 1 < NG ? g + 1 : 0;
+          auto products = [&](const half8_t (&k)[NB][2], const half8_t (&x)[2]) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
-              for (int b = 0; b < NB; b++)
-                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ah[b][t]),
-                                                                 __builtin_bit_cast(bf16x8_t, bh[t]), acc[b], 0, 0, 0);
-          } else {
-            // the residuals' products first
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-              for (int b = 0; b < NB; b++)
-                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b][t], bl[t], acc[b], 0, 0, 0);
-            if constexpr (MODE == kCodebook && !kCbExact<CB>) {
-#pragma unroll
-              for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-                  acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[b][t], bh[t], acc[b], 0, 0, 0);
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-              for (int b = 0; b < NB; b++)
-                acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[b][t], bh[t], acc[b], 0, 0, 0);
+              for (int b = 0; b < NB; b++) {
+                if constexpr (MODE == kPlain)
+                  acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      __builtin_bit_cast(bf16x8_t, k[b][t]), __builtin_bit_cast(bf16x8_t, x[t]), acc[b], 0, 0, 0);
+                else
+                  acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[b][t], x[t], acc[b], 0, 0, 0);
+              }
+          };
+          if constexpr (MODE != kPlain) {
+            products(ah, rows_l);
+            load_tile(rows_l, 1, rn, gn);
           }
+          if constexpr (MODE == kCodebook && !kCbExact<CB>) products(al, rows_h);
+          products(ah, rows_h);
+          load_tile(rows_h, 0, rn, gn);
           if constexpr (MODE == kAffine) {
-            const float qs = qsum[rt * 16 + c][g];
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-              for (int i = 0; i < 4; i++)
-                s[rt][b][i] = fmaf(lo16(cur.km[b][i]), acc[b][i], fmaf(hi16(cur.km[b][i]), qs, s[rt][b][i]));
+              for (int i = 0; i < 4; i++) s[rt][b][i] = fmaf(lo16(cur.km[b][i]), acc[b][i], s[rt][b][i]);
+            // (here, not sunk to the softmax with every group's products kept for it)
+#pragma unroll
+            for (int b = 0; b < NB; b++) asm volatile("" : "+v"(s[rt][b]));
           } else {
 #pragma unroll
             for (int b = 0; b < NB; b++) s[rt][b] = acc[b];
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
         cur = nxt;
       }
 #pragma unroll
       for (int b = 0; b < NB; b++) bp[b] = bn[b];
+      load_bias(bp, bias);
 
       // ---- softmax: lane (j, c) has keys 16 b + 4 j + i of rows 16 rt + c ----
-      const bool full = key0 + NB * kBlockTokens - 1 <= p_first && rows == nt * 16 && p_first >= 0;
+      const bool full = key0 + NB * kBlockTokens - 1 <= p_first && rows == RT * 16 && p_first >= 0;
       float4_t w[SUMS ? NB : 1];
       if constexpr (SUMS) {
 #pragma unroll
@@ -384,7 +483,6 @@ void observe_kernel(ObserveArgs a) {
       }
 #pragma unroll
       for (int rt = 0; rt < RT; rt++) {
-        if (rt >= nt) continue;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -408,7 +506,8 @@ void observe_kernel(ObserveArgs a) {
           for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-              w[b][i] = fmaf(__builtin_amdgcn_exp2f(s[rt][b][i] - m_run[rt]), l_run[rt], w[b][i]);
+              w[b][i] = fmaf(__builtin_amdgcn_exp2f(MODE == kAffine ? s[rt][b][i] : s[rt][b][i] - m_run[rt]),
+                             l_run[rt], w[b][i]);
         } else {
           float mx = -INFINITY;
 #pragma unroll
@@ -427,6 +526,7 @@ void observe_kernel(ObserveArgs a) {
             l_run[rt] += (p[0] + p[1]) + (p[2] + p[3]);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);  // (nor all tiles' weights at once)
       }
       if constexpr (SUMS) {  // the sixteen lanes of a key meet; lane c < NB stores block c's
         float4_t mine = w[0];
@@ -453,13 +553,13 @@ void observe_kernel(ObserveArgs a) {
         if (j == 0) stat[wave][rt * 16 + c] = make_float2(M, l);
       }
       __syncthreads();
-      if (tid < kObRows) {
+      if (tid < RT * 16) {
         float M = stat[0][tid].x, l = 0.0f;
 #pragma unroll
         for (int w = 1; w < NW; w++) M = fmaxf(M, stat[w][tid].x);
 #pragma unroll
         for (int w = 0; w < NW; w++) l = fmaf(stat[w][tid].y, exp2f(stat[w][tid].x - M), l);
-        *reinterpret_cast<float2*>(a.ml + ((ml_row + range) * kObRows + tid) * 2) = make_float2(M, l);
+        reinterpret_cast<float2*>(a.ml)[(ml_row + tid) * a.ranges + range] = make_float2(M, l);
       }
     }
     __syncthreads();  // the rows and their statistics are done with
@@ -484,13 +584,13 @@ __global__ __launch_bounds__(256) void observe_sum_kernel(ObserveArgs a) {
   a.weights_out[at] = (a.weights_in ? a.weights_in[at] : 0.0f) + sum;
 }
 
-template <int D, int BITS, int MODE, int NB>
+template <int D, int BITS, int MODE, int RT, int NB>
 hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
-  const dim3 grid(a.ranges, a.st.n_kv_heads * a.sharers, a.n_seqs), block(ObPlan<D, BITS, MODE>::NW * 64);
-  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, NB, false>), grid, block, 0, s, a);
+  const dim3 grid(a.ranges, a.st.n_kv_heads * a.sharers, a.n_seqs), block(ObPlan<D, BITS, MODE, RT>::NW * 64);
+  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, RT, NB, false>), grid, block, 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, NB, true>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, RT, NB, true>), grid, block, 0, s, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int64_t keys = (int64_t)a.blocks * kBlockTokens;
   hipLaunchKernelGGL(observe_sum_kernel, dim3((unsigned)((keys + 255) / 256), a.n_seqs), dim3(256), 0, s, a);
@@ -498,23 +598,28 @@ hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
 }
 template <int D, int BITS, int MODE>
 hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
-  return a.step_blocks == 4 ? launch_ob<D, BITS, MODE, 4>(a, s) : launch_ob<D, BITS, MODE, 1>(a, s);
+  constexpr int kMany = many_blocks(MODE);
+  if (a.n_q * a.group <= 16)
+    return a.step_blocks > 1 ? launch_ob<D, BITS, MODE, 1, kMany>(a, s) : launch_ob<D, BITS, MODE, 1, 1>(a, s);
+  return a.step_blocks > 1 ? launch_ob<D, BITS, MODE, 4, kMany>(a, s) : launch_ob<D, BITS, MODE, 4, 1>(a, s);
 }
 
 }  // namespace
 
 size_t observe_plan(ObserveArgs& a, int cus) {
-  const int D = a.st.layout.head_dim, waves = D == 512 ? 8 : 4;
-  const int64_t places = (int64_t)cus * (D == 512 ? 1 : 2);  // work-groups that run at once
+  constexpr int waves = 8;
+  const int64_t places = cus;  // work-groups that run at once
   const int qp = kObRows / a.group;
   a.tiles = (a.n_q + qp - 1) / qp;
   const int64_t per_tile = (int64_t)a.st.n_kv_heads * a.n_seqs;
   const int64_t rows = per_tile * a.tiles;
-  a.step_blocks = rows * ((a.blocks + 4 * waves - 1) / (4 * waves)) >= places ? 4 : 1;
+  const int many = many_blocks(a.st.layout.mode);
+  a.step_blocks = rows * ((a.blocks + many * waves - 1) / (many * waves)) >= places ? many : 1;
   const int64_t steps = (a.blocks + waves * a.step_blocks - 1) / (waves * a.step_blocks);
   // as many work-groups as run at once, several tiles one after the other where there are more
   a.sharers = (int32_t)std::clamp<int64_t>(2 * places / per_tile, 1, a.tiles);
-  a.ranges = (int32_t)std::clamp<int64_t>(places / (per_tile * a.sharers), 1, steps);
+  const int ragged = a.n_seqs > 1 ? 2 : 1;
+  a.ranges = (int32_t)std::clamp<int64_t>(ragged * places / (per_tile * a.sharers), 1, steps);
   a.part_width = (int64_t)a.blocks * kBlockTokens;
   return (size_t)(rows * a.ranges * kObRows * 2 + per_tile * a.sharers * a.part_width);
 }

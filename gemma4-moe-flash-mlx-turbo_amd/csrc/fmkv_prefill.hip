@@ -200,18 +200,6 @@ __device__ inline int prefill_steps(const PrefillArgs& a, int64_t p0) {
   return (int)((keys > 0 ? keys : 0) / kPfKeys) + 2;
 }
 
-// The sums of lanes 0 .. l, in every lane l: DPP row shifts, then the last
-// lanes of rows broadcast over the rows after them.
-__device__ inline int scan_add(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
-  return v;
-}
-
 // What unit u of the grid is: its sequence, the sequence's first unit and its
 // number of key ranges. The range length c is the smallest (to a sixteenth)
 // for which all sequences' ranges fit the units: the longest work-group, and

@@ -89,7 +89,9 @@ __global__ __launch_bounds__(kWeighThreads) void combine_weigh_kernel(AttnArgs a
 
 constexpr int kKeepThreads = 1024;
 constexpr int kKeepWaves = kKeepThreads / 64;
-constexpr int kKeepCopies = 16;  // of the histogram, by lane
+constexpr int kKeepDigit = 12, kKeepBins = 1 << kKeepDigit;  // the first digit of a key
+constexpr int kKeepLast = (32 - kKeepDigit) / 2;             // the other two
+constexpr int kKeepRanked = 1024;  // keys that one wave can part, sixteen a lane
 
 // Weights as unsigned numbers of the same order, equal for equal weights (both
 // zeros are one); a NaN is below every weight.
@@ -99,17 +101,204 @@ __device__ inline uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+struct KeepShared {
+  uint32_t hist[kKeepBins];
+  uint32_t key[kKeepRanked], at[kKeepRanked];  // of a bin: keys, positions
+  uint32_t sum[3][kKeepWaves];
+  uint32_t bin, above, count, n_ranked;
+  uint32_t last_key, last_at;  // of the positions that are kept, the last in order of (weight, position)
+};
+
+// Sums of the waves before this one; every thread calls it (one barrier).
+__device__ inline uint32_t waves_before(uint32_t mine, uint32_t* sum, int wave, int lane) {
+  if (lane == 0) sum[wave] = mine;
+  __syncthreads();
+  uint32_t before = 0;
+#pragma unroll
+  for (int w = 0; w < kKeepWaves; w++) before += w < wave ? sum[w] : 0u;
+  return before;
+}
+
+// One wave, `count` keys and positions of sh (V * 64 at most) that share the key's
+// bits above `bits`: the need-th in order of falling key, then rising position. The bits
+// of it are found from the top, each by how many of the keys left have it set.
+template <int V>
+__device__ __noinline__ void part_bin(KeepShared& sh, uint32_t count, uint32_t need, int bits, int lane) {
+  uint32_t key[V], at[V], left = 0;  // bit v: the lane's v-th is left
+#pragma unroll
+  for (int v = 0; v < V; v++) {
+    const uint32_t e = v * 64 + lane;
+    const bool in = e < count;
+    key[v] = in ? sh.key[e] : 0u;
+    at[v] = in ? ~sh.at[e] : 0u;  // (the larger the earlier)
+    left |= (uint32_t)in << v;
+  }
+  uint32_t n_left = count;
+  auto part = [&](const uint32_t (&x)[V], int from) {
+#pragma unroll 1
+    for (int bit = from; bit >= 0 && n_left > need; bit--) {
+      uint32_t set = 0;
+      uint32_t n = 0;
+#pragma unroll
+      for (int v = 0; v < V; v++) {
+        const bool b = (left >> v & 1u) && (x[v] >> bit & 1u);
+        set |= (uint32_t)b << v;
+        n += (uint32_t)__popcll(__ballot(b));
+      }
+      if (n >= need) {
+        left = set;
+        n_left = n;
+      } else {
+        need -= n;
+        left &= ~set;
+        n_left -= n;
+      }
+    }
+  };
+  part(key, bits - 1);
+  part(at, 31);
+  // all that are left are kept: the least of them in that order
+  uint32_t k = 0xffffffffu, a = 0;
+#pragma unroll
+  for (int v = 0; v < V; v++)
+    if (left >> v & 1u) {
+      const uint32_t p = ~at[v];
+      if (key[v] < k || (key[v] == k && p > a)) k = key[v], a = p;
+    }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t ok = (uint32_t)__shfl_xor((int)k, d), oa = (uint32_t)__shfl_xor((int)a, d);
+    if (ok < k || (ok == k && oa > a)) k = ok, a = oa;
+  }
+  if (lane == 0) sh.last_key = k, sh.last_at = a;
+}
+
+// Of the n weights w[0 .. n) the heaviest `need` (0 < need < n), equal ones in
+// order of position, to put(rank in order of position, position, weight). A wave
+// takes a run of positions, a lane every 64th of it: KPT of them at most, in
+// registers (0: any number, read again whenever they are looked at).
+//   1. The need-th largest key's first 12 bits, from a histogram of all keys' (the
+//      next 10 and the last 10 where the bin still holds more than a wave parts).
+//   2. One wave finds the last one kept among the keys of that bin (part_bin).
+//   3. Each wave writes its own, behind those of the waves before it.
+template <int KPT, class Put>
+__device__ inline void keep_heaviest(const float* w, int64_t n, uint32_t need, KeepShared& sh, Put put) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t run = (n + kKeepThreads - 1) / kKeepThreads * 64, r0 = wave * run + lane;
+  const int kpt = (int)(run / 64);
+  const uint64_t below = (1ull << lane) - 1ull;
+  float held[KPT ? KPT : 1];
+  if constexpr (KPT > 0) {
+#pragma unroll
+    for (int t = 0; t < KPT; t++) {
+      const int64_t i = r0 + t * 64;
+      held[t] = t < kpt && i < n ? w[i] : 0.0f;
+    }
+  }
+  // f(weight, position, there is one) of the thread's positions
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (KPT > 0) {
+#pragma unroll
+      for (int t = 0; t < KPT; t++) {
+        const int64_t i = r0 + t * 64;
+        if (t < kpt) f(held[t], i, i < n);  // (uniform)
+      }
+    } else {
+#pragma unroll 4
+      for (int t = 0; t < kpt; t++) {
+        const int64_t i = r0 + (int64_t)t * 64;
+        f(i < n ? w[i] : 0.0f, i, i < n);
+      }
+    }
+  };
+  uint32_t prefix = 0, mask = 0, count = 0;
+  int shift = 32 - kKeepDigit;
+#pragma unroll 1
+  for (int digit = 0;; digit++) {
+    const uint32_t bins = digit == 0 ? kKeepBins : 1u << kKeepLast;
+#pragma unroll
+    for (int i = 0; i < kKeepBins / kKeepThreads; i++) sh.hist[i * kKeepThreads + tid] = 0;
+    __syncthreads();
+    each([&](float x, int64_t, bool in) {
+      const uint32_t k = weight_key(x);
+      if (in && (k & mask) == prefix) atomicAdd(&sh.hist[k >> shift & (bins - 1u)], 1u);
+    });
+    __syncthreads();
+    // thread t: four bins from 4095 - 4 t down, the heaviest first
+    constexpr int kPer = kKeepBins / kKeepThreads;
+    uint32_t c[kPer], sum = 0;
+    const int top = kKeepBins - 1 - kPer * tid;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) c[i] = sh.hist[top - i], sum += c[i];
+    const uint32_t upto = (uint32_t)scan_add((int)sum);
+    uint32_t above =
+        waves_before((uint32_t)__builtin_amdgcn_readlane((int)upto, 63), sh.sum[0], wave, lane) + upto - sum;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      if (above < need && above + c[i] >= need) sh.bin = top - i, sh.above = above, sh.count = c[i];
+      above += c[i];
+    }
+    if (tid == 0) sh.n_ranked = 0;
+    __syncthreads();
+    prefix |= sh.bin << shift;
+    mask |= (bins - 1u) << shift;
+    need -= sh.above;
+    count = sh.count;
+    if (count <= kKeepRanked || shift == 0) break;
+    shift -= kKeepLast;
+  }
+  if (count <= kKeepRanked) {
+    each([&](float x, int64_t i, bool in) {
+      const uint32_t k = weight_key(x);
+      const bool mine = in && (k & mask) == prefix;
+      const uint64_t m = __ballot(mine);
+      if (m) {
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&sh.n_ranked, (uint32_t)__popcll(m));
+        at = (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + (uint32_t)__popcll(m & below);
+        if (mine) sh.key[at] = k, sh.at[at] = (uint32_t)i;
+      }
+    });
+    __syncthreads();
+    if (wave == 0) {
+      if (count <= 256)
+        part_bin<4>(sh, count, need, shift, lane);
+      else
+        part_bin<kKeepRanked / 64>(sh, count, need, shift, lane);
+    }
+  } else {  // more equal keys than a wave parts: the need-th of them in order
+    uint32_t equal = 0;
+    each([&](float x, int64_t, bool in) { equal += (uint32_t)__popcll(__ballot(in && weight_key(x) == prefix)); });
+    uint32_t before = waves_before(equal, sh.sum[1], wave, lane);
+    each([&](float x, int64_t i, bool in) {
+      const bool eq = in && weight_key(x) == prefix;
+      const uint64_t m = __ballot(eq);
+      if (eq && before + (uint32_t)__popcll(m & below) == need - 1u) sh.last_key = prefix, sh.last_at = (uint32_t)i;
+      before += (uint32_t)__popcll(m);
+    });
+  }
+  __syncthreads();
+  const uint32_t last_key = sh.last_key, last_at = sh.last_at;
+  auto taken = [&](float x, int64_t i, bool in) __attribute__((always_inline)) {
+    const uint32_t k = weight_key(x);
+    return in && (k > last_key || (k == last_key && (uint32_t)i <= last_at));
+  };
+  uint32_t mine = 0;
+  each([&](float x, int64_t i, bool in) { mine += (uint32_t)__popcll(__ballot(taken(x, i, in))); });
+  uint32_t at = waves_before(mine, sh.sum[2], wave, lane);
+  each([&](float x, int64_t i, bool in) {
+    const bool take = taken(x, i, in);
+    const uint64_t m = __ballot(take);
+    if (take) put((int)(at + (uint32_t)__popcll(m & below)), i, x);
+    at += (uint32_t)__popcll(m);
+  });
+}
+
 // One work-group per sequence. Of T > max_keep positions the first `sinks` and the
-// last `recent` stay, and as many of the others, the heaviest, as make max_keep:
-// the B-th largest key digit by digit (8 bits, from the top: a histogram of the
-// keys that share the digits found so far), then every larger one and the first of
-// the equal ones, written in the order of the positions.
+// last `recent` stay, and as many of the others, the heaviest, as make max_keep.
 __global__ __launch_bounds__(kKeepThreads) void heaviest_kernel(HeaviestArgs a) {
-  __shared__ uint32_t hist[256 * kKeepCopies];
-  __shared__ uint32_t counts[256];
-  __shared__ uint32_t found[2];  // the digit, keys above it
-  __shared__ int wave_above[kKeepWaves], wave_equal[kKeepWaves];
-  const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ KeepShared sh;
+  const int seq = blockIdx.x, tid = threadIdx.x;
   int64_t T = a.seq_lens[seq];
   T = T < 0 ? 0 : T > a.width ? a.width : T;
   const float* w = a.weights + (int64_t)seq * a.width;
@@ -119,85 +308,31 @@ __global__ __launch_bounds__(kKeepThreads) void heaviest_kernel(HeaviestArgs a) 
   if (tid == 0) a.n_keep[seq] = n;
   if (kept)
     for (int64_t i = n + tid; i < a.kept_width; i += kKeepThreads) kept[i] = 0.0f;
-  auto put = [&](int at, int64_t i) {
+  auto put = [&](int at, int64_t i, float x) __attribute__((always_inline)) {
     keep[at] = (int32_t)i;
-    if (kept) kept[at] = w[i];
+    if (kept) kept[at] = x;
+  };
+  // positions first .. first + count - 1 to places at ..
+  auto put_run = [&](int at, int64_t first, int count) __attribute__((always_inline)) {
+#pragma unroll 4
+    for (int i = tid; i < count; i += kKeepThreads) put(at + i, first + i, w[first + i]);
   };
   if (T <= a.max_keep) {
-    for (int64_t i = tid; i < T; i += kKeepThreads) put((int)i, i);
+    put_run(0, 0, n);
     return;
   }
   const int64_t lo = a.sinks, hi = T - a.recent;  // the positions between
-  for (int i = tid; i < a.sinks; i += kKeepThreads) put(i, i);
-  for (int i = tid; i < a.recent; i += kKeepThreads) put(n - a.recent + i, hi + i);
-  uint32_t need = (uint32_t)(n - a.sinks - a.recent);
+  put_run(0, 0, a.sinks);
+  put_run(n - a.recent, hi, a.recent);
+  const uint32_t need = (uint32_t)(n - a.sinks - a.recent);
   if (need == 0) return;
-
-  uint32_t prefix = 0, mask = 0;  // the digits found
-#pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256 * kKeepCopies; i += kKeepThreads) hist[i] = 0;
-    __syncthreads();
-    for (int64_t i = lo + tid; i < hi; i += kKeepThreads) {
-      const uint32_t k = weight_key(w[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift & 255u) * kKeepCopies + (lane & (kKeepCopies - 1))], 1u);
-    }
-    __syncthreads();
-    if (tid < 256) {
-      uint32_t c = 0;
-      for (int i = 0; i < kKeepCopies; i++) c += hist[tid * kKeepCopies + ((tid + i) & (kKeepCopies - 1))];
-      counts[tid] = c;
-    }
-    __syncthreads();
-    if (wave == 0) {  // lane l: digits 255 - 4 l .. 252 - 4 l
-      uint32_t c[4], sum = 0;
-      for (int i = 0; i < 4; i++) c[i] = counts[255 - 4 * lane - i], sum += c[i];
-      uint32_t upto = sum;  // keys of the lanes 0 .. l
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)upto, d);
-        if (lane >= d) upto += o;
-      }
-      uint32_t above = upto - sum;
-      for (int i = 0; i < 4; i++) {
-        if (above < need && above + c[i] >= need) found[0] = 255 - 4 * lane - i, found[1] = above;
-        above += c[i];
-      }
-    }
-    __syncthreads();
-    prefix |= found[0] << shift;
-    mask |= 255u << shift;
-    need -= found[1];
-    __syncthreads();
-  }
-  // `need` of the keys equal to prefix, the first ones, and all above it. A
-  // wave takes a run of positions; what the waves before it keep gives its place.
-  const int64_t run = (hi - lo + kKeepWaves - 1) / kKeepWaves;
-  const int64_t r0 = lo + wave * run < hi ? lo + wave * run : hi, r1 = r0 + run < hi ? r0 + run : hi;
-  int above = 0, equal = 0;
-  for (int64_t i = r0 + lane; i < r1; i += 64) {
-    const uint32_t k = weight_key(w[i]);
-    above += k > prefix;
-    equal += k == prefix;
-  }
-  for (int d = 1; d < 64; d <<= 1) above += __shfl_xor(above, d), equal += __shfl_xor(equal, d);
-  if (lane == 0) wave_above[wave] = above, wave_equal[wave] = equal;
-  __syncthreads();
-  above = equal = 0;
-  for (int i = 0; i < wave; i++) above += wave_above[i], equal += wave_equal[i];
-  int equal_left = (int)need - equal;  // of this wave's equal keys
-  int at = a.sinks + above + (equal < (int)need ? equal : (int)need);
-  for (int64_t i0 = r0; i0 < r1; i0 += 64) {
-    const int64_t i = i0 + lane;
-    const uint32_t k = i < r1 ? weight_key(w[i]) : 0u;
-    const bool eq = i < r1 && k == prefix;
-    const uint64_t below = (1ull << lane) - 1ull;
-    const uint64_t eqs = __ballot(eq);
-    const bool take = i < r1 && (k > prefix || (eq && (int)__popcll(eqs & below) < equal_left));
-    const uint64_t takes = __ballot(take);
-    if (take) put(at + (int)__popcll(takes & below), i);
-    at += (int)__popcll(takes);
-    equal_left -= (int)__popcll(eqs);
-  }
+  auto put_mid = [&](int at, int64_t i, float x) __attribute__((always_inline)) { put(a.sinks + at, lo + i, x); };
+  if (hi - lo <= 8 * kKeepThreads)
+    keep_heaviest<8>(w + lo, hi - lo, need, sh, put_mid);
+  else if (hi - lo <= 16 * kKeepThreads)
+    keep_heaviest<16>(w + lo, hi - lo, need, sh, put_mid);
+  else
+    keep_heaviest<0>(w + lo, hi - lo, need, sh, put_mid);
 }
 
 }  // namespace
