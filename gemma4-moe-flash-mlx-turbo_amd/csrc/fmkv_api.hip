@@ -854,16 +854,18 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   const int min_bps = (int)std::min<int64_t>(64, std::max<int64_t>(share, 1));
   const int wg_per_cu = 6 * slots * fmkv::kAttnWgPerCu;
   if (win == kNoWindow) {
-    // Lengths that no window makes alike: sequences count half of the longest, at most
-    // 64 blocks a split, and first splits of four times that as above. (Seven of 65 ..
+    // Lengths that nothing makes alike (those behind a shared prefix, or with it, are
+    // much the same): where splits come out long, sequences count half of the longest, at most 64 blocks a split, and first splits of four times that as above. (Seven of 65 ..
     // 20011 tokens, 8 bits, 2 heads of 512 dims: 35 blocks 33.5 us, the longest's
     // plan, 68 and 64 blocks, 42.5 and 40.6, 24: 44.3; 32 of 512 .. 16384, 4 bits, 8
     // heads of 256 dims: 64 blocks, first splits four times that, 106; 171: 163. What 41 sequences have behind
     // their prefixes, 32 blocks at most, bf16, 4 heads of 128 dims: 4 blocks 40.9 us the call, 8 with first
-    // splits of 32: 60.4.)
+    // splits of 32: 60.4; 32 sequences' 64 blocks at most, 8 bits, 2 heads of 512 dims: 17 blocks 17.4
+    // us of the call, 8: 26.)
     const int64_t rows = (int64_t)p->desc.n_kv_heads * n_s;
-    int64_t b = window_bps(p->desc, p->cus, nblk, n_s > 1 ? (rows + 1) / 2 : rows, new_col);
-    if (n_s > 1) b = std::min<int64_t>(b, 64);
+    int64_t b = window_bps(p->desc, p->cus, nblk, rows, new_col);
+    if (a->score_blocks > 0 && n_s > 1 && b > 32)
+      b = std::clamp<int64_t>(window_bps(p->desc, p->cus, nblk, (rows + 1) / 2, new_col), 32, 64);
     const int mult = b >= 64 && total >= 4 * n_slots * b ? 4 : 1;
     return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,
                                     max_blocks, q, n_q_heads, scale, tau, out, out_dtype,
@@ -1629,8 +1631,10 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
                        int32_t out_dtype, void* stream) {
   if (!p) return fail(FMKV_ERR_INVALID_ARG, "pool is null");
   if (!std::isfinite(scale)) return fail(FMKV_ERR_INVALID_ARG, "scale must be finite");
-  if (n_groups < 0 || n_groups > 65535 || max_prefix_len < 0)
-    return fail(FMKV_ERR_INVALID_ARG, "n_groups must be in [0, 65535] and max_prefix_len >= 0");
+  if (n_groups < 0 || n_groups > 65535 || max_prefix_len < 0 || max_rest_len < 0)
+    return fail(FMKV_ERR_INVALID_ARG, "n_groups must be in [0, 65535], max_prefix_len and max_rest_len >= 0");
+  if (max_rest_len > (int64_t)max_blocks * fmkv::kBlockTokens)
+    return fail(FMKV_ERR_INVALID_ARG, "max_rest_len exceeds max_blocks * 16");
   if (n_seqs > 0 && (!prefix_lens || !group_starts))
     return fail(FMKV_ERR_INVALID_ARG, "prefix_lens/group_starts are null");
   int rc;
@@ -1662,11 +1666,12 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
   pa.prefix.lens = prefix_lens;
   pa.prefix.starts = group_starts;
   pa.prefix.n_groups = n_groups;
-  const int64_t most = std::min<int64_t>(max_prefix_len, (int64_t)max_blocks * fmkv::kBlockTokens);
-  if (n_groups > 0) fmkv::prefix_plan(pa, p->cus, most / 32 + 1);
+  const int64_t width = (int64_t)max_blocks * fmkv::kBlockTokens;
+  const bool shared = fmkv::prefix_plan(pa, p->cus, max_prefix_len, max_rest_len);
   fmkv::AttnArgs at;
-  at.prefix = pa.prefix;
-  rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_rest_len,
+  if (shared) at.prefix = pa.prefix;
+  const int32_t bound = shared ? max_rest_len : (int32_t)std::min<int64_t>((int64_t)max_prefix_len + max_rest_len, width);
+  rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, bound,
                                n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
   if (rc) return rc;
   if (step) {
@@ -1674,7 +1679,7 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
     at.v_new = ap.v;
   }
   hipError_t e = hipSuccess;
-  if (n_groups > 0) {
+  if (shared) {
     pa.part_o = at.part_o;
     pa.part_ml = at.part_ml;
     pa.part_stride = at.part_stride;

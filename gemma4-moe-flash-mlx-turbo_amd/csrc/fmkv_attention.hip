@@ -1275,6 +1275,7 @@ hipError_t launch_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_t s
   e = a.win > 0 ? launch_split<D, BITS, kWindow>(own, grid, s, ev0, ev1)
                 : launch_split<D, BITS, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
+  if (a.prefix.lens) return launch_shared_merge(a, n_seqs, s);
   return launch_combine(a, n_seqs, s);
 }
 

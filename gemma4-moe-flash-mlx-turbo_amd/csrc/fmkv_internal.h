@@ -147,7 +147,7 @@ struct AttnArgs {
   int64_t win = 0;
   int64_t sinks = 0;
   // A batch that shares prefixes (win > 0 too, whatever it is): the split columns see
-  // what lies behind a sequence's prefix, and the combine merges the prefix's
+  // what lies behind a sequence's prefix, and launch_shared_merge merges the prefix's
   // partials, part_o and part_ml's first prefix.slots of a sequence, with theirs.
   PrefixArgs prefix;
   // Accumulated attention weights (win > 0 too): the split kernels store every
@@ -221,9 +221,9 @@ struct PrefillArgs {
   // A batch's shared prefixes (launch_prefix_attention): the rows of a tile are
   // those of 64 / group sequences of one group, each of which sees what the prefix
   // holds of its seq_lens[s] - new_col positions. Grid z counts prefix.slots ranges of
-  // keys, whose partials go, rotated back, to slots 0 .. of part_o [n_seqs]
-  // [part_stride][n_q_heads][D] and part_ml [..][2], where the decode kernels' combine
-  // finds them.
+  // keys, whose partials go, in the rotated domain, to slots 0 .. of part_o [n_seqs]
+  // [part_stride][n_q_heads][D] and part_ml [..][2], where launch_shared_merge finds
+  // them.
   PrefixArgs prefix;
   const int32_t* seq_lens = nullptr;
   int32_t new_col = 0;
@@ -383,6 +383,8 @@ constexpr int kGatherMaxRows = 16384;
 hipError_t launch_sparse_gather(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The split merge of every decode kernel: out = LSE merge of the partials.
 hipError_t launch_combine(const AttnArgs& a, int n_seqs, hipStream_t s);
+// The same of a batch that shares prefixes (a.prefix), fmkv_prefill.hip.
+hipError_t launch_shared_merge(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The same and the accumulated weights (a.scores), fmkv_weights.hip.
 hipError_t launch_combine_weigh(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The plan of an ObserveArgs on a GPU of `cus` CUs, and the floats of its
@@ -395,9 +397,10 @@ hipError_t launch_prefill_attention(const PrefillArgs& a, hipStream_t s);
 // The partials of a batch's shared prefixes (PrefillArgs::prefix): n_seqs, group,
 // q, qscale, new_st, part_o and part_ml and what stands with them.
 hipError_t launch_prefix_attention(const PrefillArgs& a, hipStream_t s);
-// How a batch's prefixes of at most max_steps steps of 32 keys are shared out on
-// `cus` CUs: prefix.slots and share_rows of a.
-void prefix_plan(PrefillArgs& a, int cus, int64_t max_steps);
+// How a batch's prefixes are shared out on `cus` CUs (prefix.slots and share_rows of
+// a), none longer than max_prefix, with at most max_rest positions behind them; false
+// where every sequence had better attend its prefix by itself.
+bool prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix, int64_t max_rest);
 // How a prefill call runs on a GPU of `cus` CUs (share_rows, units and
 // min_split of a), no sequence having more than max_steps steps of 32 keys:
 // the bytes of its partials (part_o, then part_ml), 0 where it is not split.

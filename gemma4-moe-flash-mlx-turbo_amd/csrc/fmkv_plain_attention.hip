@@ -476,6 +476,7 @@ hipError_t launch_plain_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStre
   e = a.win > 0 ? launch_plain_mode<D, kWindow>(own, grid, s, ev0, ev1)
                 : launch_plain_mode<D, kDense>(a, grid, s, ev0, ev1);
   if (e != hipSuccess || a.direct) return e;
+  if (a.prefix.lens) return launch_shared_merge(a, n_seqs, s);
   return launch_combine(a, n_seqs, s);
 }
 

@@ -1257,6 +1257,33 @@ void prefill_attn_kernel(PrefillArgs a) {
     l_run[u] = xor32_sum(l_run[u]);
     if (kOwn ? j == 0 : lane < 8) lrow[sm_row(u)] = l_run[u], mrow[sm_row(u)] = m_run[u];
   }
+  if constexpr (PFX) {
+    // The partials as accumulated (shared_merge_kernel rotates a row back once for all
+    // of them), straight from the accumulators
+    auto row_at = [&](int r) __attribute__((always_inline)) -> int64_t {
+      const int rq = pos_of(r);
+      return rq < nq ? ((q_row0 + rq) * a.part_stride + range) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G) : -1;
+    };
+#pragma unroll
+    for (int u = 0; u < NRS; u++) {
+      const int64_t row = row_at(sm_row(u));
+      if ((kOwn ? j == 0 : lane < 8) && row >= 0)
+        *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m_run[u], l_run[u]);
+    }
+#pragma unroll
+    for (int rt = 0; rt < PT; rt++) {
+      const int64_t row = row_at((rt0 + rt) * 16 + c);
+      if constexpr (MODE == kAffine) bacc[rt] = xor32_sum(xor16_sum(bacc[rt]));
+      if (row < 0) continue;
+#pragma unroll
+      for (int ct = 0; ct < 4; ct++)
+        *reinterpret_cast<float4_t*>(a.part_o + row * D + dg * 64 + ct * 16 + 4 * j) =
+            MODE == kAffine     ? o[rt][ct] + bacc[rt]
+            : MODE == kCodebook ? o[rt][ct] * (1.0f / kPvScale<CB>)
+                                : o[rt][ct];
+    }
+    return;
+  }
   float* const Rr = reinterpret_cast<float*>(region);
 #pragma unroll
   for (int rt = 0; rt < PT; rt++) {
@@ -1269,7 +1296,7 @@ void prefill_attn_kernel(PrefillArgs a) {
                               : o[rt][ct];
   }
   __syncthreads();
-  if (!PFX && ranges > 1) {  // partial rows, as accumulated, with their (m, l)
+  if (ranges > 1) {  // partial rows, as accumulated, with their (m, l)
     const int64_t slot =
         (WIN && a.tail_ranges > 0 ? (int64_t)(blockIdx.x - a.tail_from)
                                   : ((int64_t)blockIdx.z * gridDim.y + kvh) * gridDim.x + blockIdx.x) *
@@ -1305,16 +1332,6 @@ void prefill_attn_kernel(PrefillArgs a) {
       const int rq_ = pos_of(r), rh_ = r - rq_ * G;
       if (rq_ >= nq) continue;
       const float l = lrow[r];
-      if constexpr (PFX) {  // partial rows, rotated back
-        const int64_t row = ((q_row0 + rq_) * a.part_stride + range) * a.n_q_heads + (int64_t)kvh * G + rh_;
-        typedef float vec __attribute__((ext_vector_type(E)));
-        vec o;
-#pragma unroll
-        for (int i = 0; i < E; i++) o[i] = x[k][i] * (MODE == kPlain ? 1.0f : cs_lane);
-        *reinterpret_cast<vec*>(a.part_o + row * D + lane * E) = o;
-        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(mrow[r], l);
-        continue;
-      }
 #pragma unroll
       for (int i = 0; i < E; i++)
         x[k][i] = l > 0.0f ? (x[k][i] * (MODE == kPlain ? 1.0f : cs_lane)) / l : 0.0f;
@@ -1392,6 +1409,83 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int t
                       lane * E, x);
 }
 
+// The last launch of a batch that shares prefixes: a work-group per (sequence, q
+// head), out = sum_k 2^(m_k - M) O_k / sum_k 2^(m_k - M) l_k over the prefix's
+// partials, which are in the cache's rotated domain, and the sequence's own, which are not:
+// the sum of the first is rotated back and the others' added. Its four waves take every
+// fourth partial, lane l dims E l ..; bound by reading them.
+constexpr int kMergeWaves = 4;
+template <int D, bool ROT>
+__global__ __launch_bounds__(kMergeWaves * 64) void shared_merge_kernel(AttnArgs a) {
+  constexpr int E = D / 64;
+  __shared__ float sums[2][kMergeWaves][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = blockIdx.x, seq = blockIdx.y, Hq = a.n_q_heads;
+  const int64_t T = a.seq_lens[seq];
+  const int n_own =
+      n_splits_for(attn_window(a, seq, T).geo, a.bps0, a.bps, a.max_splits, a.skew_p) + a.new_col;
+  const int s0 = a.prefix.end(seq, T - a.new_col, a.st.table_stride) > 0 ? 0 : a.prefix.slots;
+  const int n = a.prefix.slots + n_own;
+  const int64_t row0 = (int64_t)seq * a.part_stride * Hq + h;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row0;
+  // (every wave merges all (m, l): fewer waits than a meeting of four)
+  float M = -1e30f, l = 0.0f;
+#pragma unroll 2
+  for (int k = s0 + lane; k < n; k += 64) {
+    const float2 x = ml[(int64_t)k * Hq];
+    const float mn = fmaxf(M, x.x);
+    l = fmaf(l, exp2f(M - mn), x.y * exp2f(x.x - mn));
+    M = mn;
+  }
+  const float Mx = group_max<64>(M, lane);
+  l = group_sum<64>(l * exp2f(M - Mx), lane);
+  float x[2][E];
+#pragma unroll
+  for (int p = 0; p < 2; p++) {
+#pragma unroll
+    for (int i = 0; i < E; i++) x[p][i] = 0.0f;
+    const int end = p ? n : a.prefix.slots;
+#pragma unroll 4
+    for (int k = (p ? a.prefix.slots : s0) + wave; k < end; k += kMergeWaves) {
+      const float w = exp2f(ml[(int64_t)k * Hq].x - Mx);
+      typedef float vec __attribute__((ext_vector_type(E)));
+      const vec v = *reinterpret_cast<const vec*>(a.part_o + (row0 + (int64_t)k * Hq) * D + lane * E);
+#pragma unroll
+      for (int i = 0; i < E; i++) x[p][i] = fmaf(w, v[i], x[p][i]);
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++) sums[p][wave][lane * E + i] = x[p][i];
+  }
+  __syncthreads();
+  if (wave > 0) return;
+#pragma unroll
+  for (int p = 0; p < 2; p++)
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      x[p][i] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kMergeWaves; w++) x[p][i] += sums[p][w][lane * E + i];
+    }
+  if constexpr (ROT) {
+    const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
+    const float cs = fwht_lane_sign(lane) * a.c;
+#pragma unroll
+    for (int i = 0; i < E; i++) x[0][i] = apply_sign(x[0][i], sbits, i);
+    wave_fwht_signed<E>(x[0], lane);
+#pragma unroll
+    for (int i = 0; i < E; i++) x[0][i] *= cs;
+  }
+  const int64_t at = ((int64_t)seq * Hq + h) * D + lane * E;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const float v = l > 0.0f ? (x[0][i] + x[1][i]) / l : 0.0f;
+    if (a.out_f32)
+      reinterpret_cast<float*>(a.out)[at + i] = v;
+    else
+      reinterpret_cast<uint16_t*>(a.out)[at + i] = f32_to_bf16(v);
+  }
+}
+
 template <int D, int BITS, int MODE, int RW, int KIND>
 hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
   const int qp = kPfRows / a.group;
@@ -1410,7 +1504,8 @@ hipError_t launch_rw(const PrefillArgs& a, hipStream_t s) {
 // Tiles that a batch's groups have at most.
 int64_t prefix_tiles(const PrefillArgs& a) {
   const int qp = kPfRows / a.group;
-  return a.n_seqs / qp + std::min<int64_t>(a.prefix.n_groups, a.n_seqs);
+  const int64_t groups = std::min<int64_t>(a.prefix.n_groups, a.n_seqs);
+  return (a.n_seqs + groups * (qp - 1)) / qp;
 }
 template <int D, int BITS, int MODE, int RW>
 hipError_t launch_shared(const PrefillArgs& a, hipStream_t s) {
@@ -1529,12 +1624,39 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
   return prefill_part_bytes(units * wgs, D);
 }
 
-void prefix_plan(PrefillArgs& a, int cus, int64_t max_steps) {
-  const int D = a.new_st.layout.head_dim;
-  const int64_t wgs = prefix_tiles(a) * a.new_st.n_kv_heads;
+// Where few sequences or short prefixes are shared, every sequence for itself is
+// faster: the pages that the others read too come from the caches. Estimated in us (a
+// call's fixed part; a step of 32 keys, all work-groups side by side; partials written
+// and read at 5 TB/s; alone, the pages at 9 TB/s), and measured, shared and alone: 2
+// sequences behind 992 tokens, 4 bits, 8 heads of 256 dims: 27.1 and 17.2; 9 behind 8000, 8
+// bits, 2 heads of 512 dims: 48.9 and 40.5; 32 behind 32768: 120 and 274; 41 in five
+// groups behind 700 .. 6000, bf16, 4 heads of 128 dims: 40.5 and 52.6.
+bool prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix, int64_t max_rest) {
+  const BlockLayout& L = a.new_st.layout;
+  const int D = L.head_dim, H = a.new_st.n_kv_heads;
+  if (a.prefix.n_groups <= 0 || a.prefix.n_groups >= a.n_seqs) return false;
+  const int64_t wgs = prefix_tiles(a) * H, steps = max_prefix / kPfKeys;
+  if (steps < 1) return false;
   a.share_rows = D < 512 && wgs <= cus / 4;
-  const int64_t most = std::max<int64_t>((max_steps + kPfMinSteps - 1) / kPfMinSteps, 1);
-  a.prefix.slots = (int32_t)std::clamp<int64_t>(prefill_places(D, a.share_rows, cus) / wgs, 1, most);
+  const int64_t most = (steps + kPfMinSteps - 1) / kPfMinSteps, places = prefill_places(D, a.share_rows, cus);
+  a.prefix.slots = (int32_t)std::clamp<int64_t>(places / wgs, 1, most);
+  const double fixed = D == 128 ? 26.0 : D == 256 ? 20.0 : 32.0, step = D == 128 ? 0.75 : D == 256 ? 1.7 : 2.3;
+  const int64_t rounds = (wgs * a.prefix.slots + places - 1) / places;
+  const double shared = fixed + step * (double)((steps + a.prefix.slots - 1) / a.prefix.slots * rounds) +
+                        (double)a.n_seqs * a.n_q_heads * a.prefix.slots * D * 8 / 5e6;
+  const double alone = 16.0 + (double)(max_prefix + max_rest) / kBlockTokens * a.n_seqs * H * L.block_bytes / 9e6;
+  return shared < alone;
+}
+
+hipError_t launch_shared_merge(const AttnArgs& a, int n_seqs, hipStream_t s) {
+  const dim3 grid(a.n_q_heads, n_seqs);
+  const bool rot = a.st.layout.mode != kPlain;
+  const int D = a.st.layout.head_dim;
+  const auto kernel = D == 128   ? (rot ? shared_merge_kernel<128, true> : shared_merge_kernel<128, false>)
+                      : D == 256 ? (rot ? shared_merge_kernel<256, true> : shared_merge_kernel<256, false>)
+                                 : (rot ? shared_merge_kernel<512, true> : shared_merge_kernel<512, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kMergeWaves * 64), 0, s, a);
+  return hipGetLastError();
 }
 
 hipError_t launch_prefix_attention(const PrefillArgs& a, hipStream_t s) {

@@ -91,7 +91,7 @@ constexpr int kKeepThreads = 1024;
 constexpr int kKeepWaves = kKeepThreads / 64;
 constexpr int kKeepDigit = 12, kKeepBins = 1 << kKeepDigit;  // the first digit of a key
 constexpr int kKeepLast = (32 - kKeepDigit) / 2;             // the other two
-constexpr int kKeepRanked = 1024;  // keys that one wave can part, sixteen a lane
+constexpr int kKeepRanked = 256;  // keys that one wave parts, four a lane
 
 // Weights as unsigned numbers of the same order, equal for equal weights (both
 // zeros are one); a NaN is below every weight.
@@ -119,11 +119,12 @@ __device__ inline uint32_t waves_before(uint32_t mine, uint32_t* sum, int wave, 
   return before;
 }
 
-// One wave, `count` keys and positions of sh (V * 64 at most) that share the key's
-// bits above `bits`: the need-th in order of falling key, then rising position. The bits
-// of it are found from the top, each by how many of the keys left have it set.
-template <int V>
-__device__ __noinline__ void part_bin(KeepShared& sh, uint32_t count, uint32_t need, int bits, int lane) {
+// One wave, `count` keys and positions of sh that share the key's bits above `bits`, the
+// positions below n: the need-th in order of falling key, then rising position. The bits
+// of it are found from the top, each by how many of the keys left have it set. (Sixteen keys
+// a lane instead of another digit of all keys took 10 us of 16384.)
+__device__ inline void part_bin(KeepShared& sh, uint32_t count, uint32_t need, int bits, int64_t n, int lane) {
+  constexpr int V = kKeepRanked / 64;
   uint32_t key[V], at[V], left = 0;  // bit v: the lane's v-th is left
 #pragma unroll
   for (int v = 0; v < V; v++) {
@@ -156,7 +157,7 @@ __device__ __noinline__ void part_bin(KeepShared& sh, uint32_t count, uint32_t n
     }
   };
   part(key, bits - 1);
-  part(at, 31);
+  part(at, 31 - __builtin_clz((uint32_t)n));  // (higher bits are all alike)
   // all that are left are kept: the least of them in that order
   uint32_t k = 0xffffffffu, a = 0;
 #pragma unroll
@@ -260,12 +261,7 @@ __device__ inline void keep_heaviest(const float* w, int64_t n, uint32_t need, K
       }
     });
     __syncthreads();
-    if (wave == 0) {
-      if (count <= 256)
-        part_bin<4>(sh, count, need, shift, lane);
-      else
-        part_bin<kKeepRanked / 64>(sh, count, need, shift, lane);
-    }
+    if (wave == 0) part_bin(sh, count, need, shift, n, lane);
   } else {  // more equal keys than a wave parts: the need-th of them in order
     uint32_t equal = 0;
     each([&](float x, int64_t, bool in) { equal += (uint32_t)__popcll(__ballot(in && weight_key(x) == prefix)); });

@@ -816,8 +816,8 @@ class PagedPool:
         once for its group: the sequences group_starts[g] .. group_starts[g + 1] - 1
         have the whole blocks of their first prefix_lens[s] positions in common. q bf16
         [n_seqs, n_q_heads, D]; seq_lens, prefix_lens int32 [n_seqs]; group_starts
-        int32 [n_groups + 1]. max_rest_len bounds what a sequence holds behind its
-        shared blocks; max_prefix_len, the longest prefix, is for speed."""
+        int32 [n_groups + 1]. max_prefix_len bounds the prefixes, max_rest_len what a
+        sequence holds behind its shared blocks."""
         n, heads, _ = _check_tensor("q", q, torch.bfloat16, (None, None, self._D))
         width = _check_tensor("block_tables", block_tables, torch.int32, (n, None))[1]
         _check_tensor("seq_lens", seq_lens, torch.int32, (n,))

@@ -405,10 +405,11 @@ int fmkv_paged_window_prefill_step(fmkv_pool* pool, const void* k_bf16, const vo
  * blocks (a sequence may share less than its group's first one does; what it
  * holds behind that is its own). Sequences in no group share nothing. prefix_lens: int32
  * device [n_seqs]; group_starts: int32 device [n_groups + 1], in order.
- * max_prefix_len is the longest of prefix_lens, for speed only (a wrong one gives right
- * results). max_rest_len bounds what sequences have behind their shared blocks
- * (seq_lens[s] less prefix_lens[s] rounded down; all of seq_lens[s] in no group), as
- * max_seq_len bounds the lengths of the other calls. What slots past a sequence's
+ * max_prefix_len bounds prefix_lens, and max_rest_len what sequences have behind
+ * their shared blocks (seq_lens[s] less prefix_lens[s] rounded down; all of
+ * seq_lens[s] in no group), as max_seq_len bounds the lengths of the other calls.
+ * Where they say that sharing would cost more than it saves (few sequences, short
+ * prefixes), each sequence reads its own table's blocks instead. What slots past a sequence's
  * length hold does not reach an output; a sequence of length 0 gets zeros. q
  * is 16-byte aligned. Every cache mode, at most 8 query heads per KV head. The
  * order of sums, and so an output's last bits, depends on the bounds and on the batch.
