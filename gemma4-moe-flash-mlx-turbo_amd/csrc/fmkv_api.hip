@@ -31,6 +31,8 @@ int32_t g_bps_override = 0;
 // sparse-V after the statistics pass: 1 the gather, 0 the gated pass and the
 // combine (fmkv_set_sparse_v_gather)
 int32_t g_sparse_gather = 1;
+// how batches that share prefixes run (fmkv_set_prefix_sharing)
+int32_t g_prefix_way = FMKV_PREFIX_AUTO;
 
 // Kernel-timing records (fmkv_profile_enable / fmkv_profile_collect).
 struct Profiler {
@@ -1620,6 +1622,48 @@ int fmkv_paged_decode_step_projected(fmkv_pool* p, const void* k_proj, const voi
 
 namespace {
 
+// How a batch that shares prefixes runs. Alone: every sequence reads its own table's
+// blocks; those that others read too come from the caches. Rows: eight rows of a
+// group's sequences at a time in the decode kernels' matrix-core columns (kTiles), beside what
+// each has behind its prefix; without gain from five q heads per KV head on, where a
+// sequence fills the columns. Tiles: 64 rows at a time in the prefill kernel, then what each
+// has behind its prefix. Chosen by estimates in us: blocks at 10 and 8 TB/s (most from the
+// caches) and the fixed parts; measured alone / rows / tiles: 2 sequences behind 992 tokens, 4
+// bits, 8 heads of 256 dims: 13.3 / 16.4 / 27.1; 9 behind 8000, 8 bits, 2 heads of 512 dims, 8 q heads each:
+// 30.2 / 52.8 / 48.7; 41 in five groups behind 700 .. 6000, bf16, 4 heads of 128 dims:
+// 71.3 / 39.3 / 40.4; 32 behind 32768, 8 bits, 2 heads of 512 dims: 220 / 268 / 121.
+int32_t prefix_way(const fmkv_pool* p, fmkv::PrefillArgs& pa, int64_t max_prefix, int64_t max_rest,
+                   int64_t width) {
+  if (pa.prefix.n_groups <= 0 || max_prefix < fmkv::kBlockTokens) return FMKV_PREFIX_ALONE;
+  const int64_t H = p->desc.n_kv_heads, n = pa.n_seqs;
+  const double tiles_us = fmkv::prefix_plan(pa, p->cus, max_prefix);
+  // rows of eight: their plan, as of equal sequences of the prefixes' length
+  const int64_t qp = 8 / pa.group, groups = std::min<int64_t>(pa.prefix.n_groups, n);
+  const int64_t rows = (n + groups * (qp - 1)) / qp;
+  auto blocks_us = [&](double blocks, double rate) {
+    return blocks / fmkv::kBlockTokens * (double)(H * p->layout.block_bytes) / rate;
+  };
+  const double alone_us = 16.0 + blocks_us((double)n * (double)(max_prefix + max_rest), 1e7);
+  const double rows_us = 18.0 + blocks_us((double)rows * (double)max_prefix + (double)n * (double)max_rest, 8e6);
+  int32_t way = g_prefix_way;
+  if (way == FMKV_PREFIX_ROWS && n + rows > 65535) way = FMKV_PREFIX_ALONE;  // (the grid's y)
+  if (way == FMKV_PREFIX_AUTO) {
+    way = groups >= n ? FMKV_PREFIX_ALONE : FMKV_PREFIX_TILES;
+    double best = groups >= n ? 0.0 : tiles_us;
+    if (groups < n && qp > 1 && n + rows <= 65535 && rows_us < best) way = FMKV_PREFIX_ROWS, best = rows_us;
+    if (alone_us < best) way = FMKV_PREFIX_ALONE;
+  }
+  if (way == FMKV_PREFIX_ROWS) {
+    const int64_t blocks = (std::min(max_prefix, width) + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
+    int64_t b = std::max<int64_t>(window_bps(p->desc, p->cus, blocks, rows * H, 0), 1);
+    b = std::max(b, (blocks + 65534) / 65535);  // (the grid's z)
+    pa.prefix.tiles = (int32_t)rows;
+    pa.prefix.slots = (int32_t)((blocks + b - 1) / b);
+    pa.prefix.long_splits = b >= 8;
+  }
+  return way;
+}
+
 // Decode attention of a batch in groups that share prefixes: the prefixes' partials,
 // then what each sequence has behind its own, and the merge. step: with the append of one
 // new token per sequence.
@@ -1667,9 +1711,11 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
   pa.prefix.starts = group_starts;
   pa.prefix.n_groups = n_groups;
   const int64_t width = (int64_t)max_blocks * fmkv::kBlockTokens;
-  const bool shared = fmkv::prefix_plan(pa, p->cus, max_prefix_len, max_rest_len);
+  const int32_t way = prefix_way(p, pa, max_prefix_len, max_rest_len, width);
+  const bool shared = way != FMKV_PREFIX_ALONE;
   fmkv::AttnArgs at;
   if (shared) at.prefix = pa.prefix;
+  at.n_seqs = n_seqs;
   const int32_t bound = shared ? max_rest_len : (int32_t)std::min<int64_t>((int64_t)max_prefix_len + max_rest_len, width);
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, bound,
                                n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
@@ -1679,7 +1725,7 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
     at.v_new = ap.v;
   }
   hipError_t e = hipSuccess;
-  if (shared) {
+  if (way == FMKV_PREFIX_TILES) {
     pa.part_o = at.part_o;
     pa.part_ml = at.part_ml;
     pa.part_stride = at.part_stride;
@@ -2062,6 +2108,13 @@ int fmkv_pool_read_codes(const fmkv_pool* p, void* codes, void* meta, void* stre
 int fmkv_set_sparse_v_gather(int32_t on) {
   if (on != 0 && on != 1) return fail(FMKV_ERR_INVALID_ARG, "sparse_v_gather must be 0 or 1");
   g_sparse_gather = on;
+  return FMKV_OK;
+}
+
+int fmkv_set_prefix_sharing(int32_t way) {
+  if (way < FMKV_PREFIX_AUTO || way > FMKV_PREFIX_TILES)
+    return fail(FMKV_ERR_INVALID_ARG, "prefix sharing must be one of FMKV_PREFIX_*");
+  g_prefix_way = way;
   return FMKV_OK;
 }
 

@@ -180,7 +180,9 @@ __device__ inline void copy_q_row(const AttnArgs& a, uint8_t* dst, int seq, int 
 // residual if odd), zero unless c >> 2 == g -- each lane of the packed
 // kernel then serves one group of one head.
 template <int D, int BITS, int NW, bool PACK = false>
-__device__ void build_q_table(const AttnArgs& a, uint8_t* tab, int wave, int lane, uint32_t sbits) {
+__device__ void build_q_table(const AttnArgs& a, uint8_t* tab, int wave, int lane, uint32_t sbits,
+                              int rows = -1) {
+  const int group = rows < 0 ? a.group : rows;
   constexpr int E = D / 64, NG = D / 64, LPG = 64 / E;
   constexpr int HPW = (8 + NW - 1) / NW;  // table columns (heads) per wave
   const QSlot<E, BITS> qs(lane);
@@ -189,7 +191,7 @@ __device__ void build_q_table(const AttnArgs& a, uint8_t* tab, int wave, int lan
 #pragma unroll
   for (int k = 0; k < HPW; k++) {
     const int h = wave + k * NW;
-    const bool hv = h < a.group;
+    const bool hv = h < group;
     float x[E];
 #pragma unroll
     for (int i = 0; i < E; i++) x[i] = 0.0f;
@@ -502,20 +504,25 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   const int head = PACK ? (c >> 1) & 1 : c & 7;
   const bool hi = PACK ? (c & 1) == 0 : c < 8;
   const int grp = c >> 2;  // PACK: this lane's 64-dim group
-  const int G = (int)((flags >> 4) & 15u);
+  constexpr bool TILES = MODE == kTiles;
+  TileRows tr{};
+  if constexpr (TILES) {
+    if (!tile_rows(a, blockIdx.y, head, lane, tr)) return;
+  }
+  const int G = TILES ? tr.rows : (int)((flags >> 4) & 15u);  // query rows
   const bool col_valid = head < G;
   const int skew_p = (int)(skew & 255u), skew_extra = (int)(skew >> 8);
   // grid (KV head, sequence, split column): consecutive work-groups, which
   // the dispatcher deals round-robin to the XCDs, are the KV heads of one
   // split and then the sequences, so each XCD gets a like share of the work;
   // the new-token column comes last
-  const int kvh = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x, seq = TILES ? tr.seq : (int)blockIdx.y, split = blockIdx.z;
   const int g0 = half * GH;  // this wave's first group
 
   // the block range from the preloaded arguments (paged: the sequence's
   // length, bounded by the table width)
   int64_t Tg = geo_len;
-  if constexpr (PAGED) Tg = a.seq_lens[seq];
+  if constexpr (PAGED) Tg = TILES ? tr.T : (int64_t)a.seq_lens[seq];
   SeqGeom geo = seq_geometry(Tg, window, geo_vis_begin);
   if constexpr (PAGED) {
     if (geo.blk_hi > a.st.table_stride) geo.blk_hi = a.st.table_stride;
@@ -525,22 +532,26 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // the sequence's own number
   WinGeom wg{};
   if constexpr (windowed(MODE)) {
-    wg = attn_window(a, seq, Tg);
+    wg = TILES ? tile_window(a, tr) : attn_window(a, seq, Tg);
     geo = wg.geo;
   }
   auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   // one sequence: the host planned max_splits for exactly this block range
   // (no division before the first copies); paged: per sequence
-  const int n_splits = PAGED ? n_splits_for(geo, bps0, bps, max_splits, skew_p) : max_splits;
+  if (TILES && tr.tile) bps0 = bps = tile_bps(a, geo);
+  const int n_splits = TILES && tr.tile ? a.prefix.slots
+                       : PAGED          ? n_splits_for(geo, bps0, bps, max_splits, skew_p)
+                                        : max_splits;
   static_assert(P::kStageRegion >= D / 2 * (int)sizeof(float2), "rope table fits the staging");
   // decode step: the new token's column (dense mode, or the statistics pass
   // of a sparse-V step, whose gated pass then reads the stored token), the
   // grid's last split column
   if constexpr (MODE != kGated) {
-    if ((flags & 4u) && split == max_splits) {
+    if ((flags & 4u) && split == max_splits && !(TILES && tr.tile)) {
       new_token_column<D, BITS, P::kWaves * 64, PACK>(a, scratch, reinterpret_cast<float2*>(stage),
-                                                PAGED ? Tg : a.seq_len, n_splits, kvh, seq, wave,
-                                                lane);
+                                                PAGED ? Tg : a.seq_len,
+                                                TILES ? n_splits + a.prefix.slots : n_splits, kvh, seq,
+                                                wave, lane);
       return;
     }
   }
@@ -668,7 +679,14 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
       for (int k = 0; k < nk; k++) dma16(lds_addr(tbl_s) + k * kChunk, k * kChunk + lane * 16, trs);
     }
   }
-  copy_q_row<D, P::kWaves>(q, (int)(flags >> 8), G, scratch, seq, kvh, wave, lane);
+  if constexpr (TILES) {
+    for (int h = wave; h < G; h += P::kWaves)
+      if (lane < D / 8)
+        dma16(lds_addr(scratch + h * D * 2), lane * 16,
+              buffer_rsrc(q + tile_q_row(a, tr, kvh, h) * D, (uint32_t)(D * 2)));
+  } else {
+    copy_q_row<D, P::kWaves>(q, (int)(flags >> 8), G, scratch, seq, kvh, wave, lane);
+  }
 #pragma unroll
   for (int s = 0; s < NQ; s++)
     if (s < nbx) copy_block(s, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : s), false);
@@ -677,7 +695,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   wait_copies<CP, NQ>(nbx < NQ ? nbx : NQ);  // the q copy preceded every block
   // this lane's RHT signs, for the q rotation and the inverse rotation
   const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
-  build_q_table<D, BITS, P::kWaves, PACK>(a, scratch, wave, lane, sbits);
+  build_q_table<D, BITS, P::kWaves, PACK>(a, scratch, wave, lane, sbits, TILES ? G : -1);
 #pragma unroll
   for (int s = NQ; s < NST; s++)
     if (s < nbx) copy_block(s, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : s), false);
@@ -753,7 +771,7 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
   // a decode step's new token is the new-token column's (its slot may still
   // hold the position it replaces, or be written meanwhile)
   int64_t ex_slot = -1;
-  if (a.new_col && T > 0) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
+  if (a.new_col && T > 0 && !(TILES && tr.tile)) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
   // sparse-V: this column's score threshold
   float theta = -INFINITY;
   if constexpr (MODE == kGated) theta = col_valid ? th_s[head] : -INFINITY;
@@ -864,7 +882,8 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
     // only at the edges of the visible range
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) &&
+                              t0 + kBlockTokens <= (TILES ? (int64_t)tr.min_end : T)
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
@@ -874,8 +893,9 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
       // lane (j, c < GH) clearing group c's of tokens 4j .. 4j + 3.
       uint8_t* const vmeta_c =
           const_cast<uint8_t*>(sp) + P::kMetaOff + half * 2 * MH + MH + c * 64 + j * 16;
+      // (kTiles: rows differ in what they see; see `edge` below.)
       u32x4 m = (u32x4){0, 0, 0, 0};
-      if (windowed(MODE) && c < GH) m = lds16(vmeta_c);
+      if (windowed(MODE) && !TILES && c < GH) m = lds16(vmeta_c);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const int64_t slot = t0 + 4 * j + i;
@@ -884,16 +904,18 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
                    slot != ex_slot;
         if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
+        if constexpr (TILES) vis = tile_sees(tr, wg, a.sinks, ex_slot, slot);
         if (!vis) {
           s[i] = -INFINITY;
           m[i] = 0;
         }
       }
-      if constexpr (windowed(MODE)) {
+      if constexpr (windowed(MODE) && !TILES) {
         if (c < GH) *reinterpret_cast<u32x4*>(vmeta_c) = m;
         vm = lds16(sp + P::kMetaOff + half * 2 * MH + MH + (PACK ? grp * 64 : 0) + j * 16);
       }
     }
+    const bool edge = !full;
     if constexpr (MODE == kGated) {
 #pragma unroll
       for (int i = 0; i < 4; i++) s[i] = s[i] >= theta ? s[i] : -INFINITY;
@@ -987,11 +1009,18 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
         if (BITS == 8 || ((g0 + gi + 1) & 1) == 0) vw = codes(sp, 1, gi + 1);
         vm = vmeta(sp, gi + 1);
       }
+      u32x4 vm_u = vm_g;
+      if constexpr (TILES) {  // a hidden token's scale and bias may be anything, and 0 * inf is NaN
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) vm_u[i] = p[i] > 0.0f ? vm_u[i] : 0u;
+        }
+      }
       float x[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        x[i] = fmaf(p[i], lo16(vm_g[i]), 0.0f);  // one v_fma_mix; = the rounded product
-        bacc[gi] = fmaf(p[i], hi16(vm_g[i]), bacc[gi]);
+        x[i] = fmaf(p[i], lo16(vm_u[i]), 0.0f);  // one v_fma_mix; = the rounded product
+        bacc[gi] = fmaf(p[i], hi16(vm_u[i]), bacc[gi]);
       }
       const half2_t h01 = pkrtz(x[0], x[1]);
       const half2_t h23 = pkrtz(x[2], x[3]);
@@ -1151,9 +1180,10 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
           reinterpret_cast<uint16_t*>(a.out)[o_idx + i] = f32_to_bf16(v);
       }
     } else {
-      const int64_t pbase =
-          ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G;
-      float* dst = a.part_o + (pbase + hh) * D + lane * E;
+      const int64_t prow =
+          TILES ? tile_part_row(a, tr, kvh, hh, split)
+                : ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G + hh;
+      float* dst = a.part_o + prow * D + lane * E;
       if constexpr (E % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < E; i += 4)
@@ -1164,8 +1194,8 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
         for (int i = 0; i < E; i++) dst[i] = x[i] * cs;
       }
       if (lane == 0) {
-        a.part_ml[(pbase + hh) * 2 + 0] = M;
-        a.part_ml[(pbase + hh) * 2 + 1] = Lsum;
+        a.part_ml[prow * 2 + 0] = M;
+        a.part_ml[prow * 2 + 1] = Lsum;
       }
     }
   }
@@ -1213,10 +1243,10 @@ hipError_t launch_split(const AttnArgs& a, dim3 grid, hipStream_t s, hipEvent_t 
   if (windowed(MODE) && !a.st.block_table) return hipErrorInvalidValue;
   // (kWindow is a paged pool's: it has no other instances)
   if constexpr (kSoloCapable<D, BITS>) {
-    if (a.bps >= kSoloMinBlocks) {
+    if (MODE == kTiles ? a.prefix.long_splits != 0 : a.bps >= kSoloMinBlocks) {
       // head_dim 256 at 4 bits with at most 2 q heads per KV head (Gemma-4's
       // sliding layers): the packed-column form of the solo streams
-      constexpr bool kPacked = (MODE == kDense || windowed(MODE)) && D == 256 && BITS == 4;
+      constexpr bool kPacked = (MODE == kDense || windowed(MODE)) && MODE != kTiles && D == 256 && BITS == 4;
       if constexpr (!windowed(MODE)) {
         if (!a.st.block_table) {
           if constexpr (kPacked)
@@ -1270,6 +1300,10 @@ hipError_t launch_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_t s
   if (a.scores) {
     e = launch_split<D, BITS, kWeigh>(a, grid, s, ev0, ev1);
     return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  if (a.prefix.tiles > 0) {
+    e = launch_split<D, BITS, kTiles>(a, tiles_grid(a, n_kv_heads), s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine(a, n_seqs, s);
   }
   const AttnArgs own = behind_prefix(a);
   e = a.win > 0 ? launch_split<D, BITS, kWindow>(own, grid, s, ev0, ev1)

@@ -29,15 +29,117 @@ constexpr float kRescaleSlack = 8.0f;
 // divides by the full L of the stats pass.
 // kWindow: softmax attention of a paged sequence over its last a.win positions
 // and its first a.sinks ones, or what is its own behind a shared prefix (WinGeom),
-// tau 0. kWeigh: the same, with every score to a.scores.
-constexpr int kDense = 0, kStats = 1, kGated = 2, kWindow = 3, kWeigh = 4;
-constexpr bool windowed(int mode) { return mode == kWindow || mode == kWeigh; }
+// tau 0. kWeigh: the same, with every score to a.scores. kTiles: the same for a
+// batch that shares prefixes, whose grid has tiles of their rows besides (TileRows).
+constexpr int kDense = 0, kStats = 1, kGated = 2, kWindow = 3, kWeigh = 4, kTiles = 5;
+constexpr bool windowed(int mode) { return mode == kWindow || mode == kWeigh || mode == kTiles; }
 
 // The visible blocks of sequence `seq`, of length T.
 __device__ inline WinGeom attn_window(const AttnArgs& a, int seq, int64_t T) {
   if (!a.prefix.lens) return win_geometry(T, a.win, a.sinks, a.st.table_stride);
   const int64_t first = a.prefix.end(seq, T - a.new_col, a.st.table_stride);
   return win_geometry(T, T > first ? T - first : 0, 0, a.st.table_stride);
+}
+
+// The largest value of a wave's lanes.
+__device__ inline int wave_max(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_xor(v, d);
+    v = v > o ? v : o;
+  }
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Tile `tile` of a batch's groups, QP sequences a tile: its first sequence, how
+// many it has, and the group's first one (n 0: a tile that nothing needs). Lane l
+// looks at group g0 + l; every wave that asks gets the same answer.
+struct PrefixTile {
+  int s0, n, leader;
+};
+__device__ inline PrefixTile prefix_tile(const PrefixArgs& p, int n_seqs, int QP, int tile, int lane) {
+  for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
+    const int g = g0 + lane;
+    int a = 0, b = 0;
+    if (g < p.n_groups) a = p.starts[g], b = p.starts[g + 1];
+    a = a < 0 ? 0 : a;
+    b = b > n_seqs ? n_seqs : b;
+    const int count = b > a ? (b - a + QP - 1) / QP : 0;
+    const int upto = scan_add(count), total = __builtin_amdgcn_readlane(upto, 63);
+    if (tile < total) {
+      const int l = __builtin_ctzll(__ballot(upto > tile));
+      const int t = tile - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
+      PrefixTile r;
+      r.leader = __builtin_amdgcn_readlane(a, l);
+      r.s0 = r.leader + t * QP;
+      r.n = __builtin_amdgcn_readlane(b, l) - r.s0;
+      if (r.n > QP) r.n = QP;
+      return r;
+    }
+    tile -= total;
+  }
+  return PrefixTile{0, 0, 0};
+}
+
+// kTiles: what a work-group attends. Grid y counts the sequences, each with what
+// it has behind its prefix, then tiles of up to eight rows of a group's sequences (row r:
+// sequence s0 + r / G, head r % G of the KV head's G), which attend the group's prefix: the
+// matrix-core columns that one sequence's few heads would leave empty, and the pages
+// read once for all of them.
+struct TileRows {
+  bool tile;
+  int seq, s0, rows;  // whose block table; the first sequence; query rows
+  int64_t T;          // positions that some row sees
+  int row_end;        // of the lane's row `head`
+  int min_end;        // that every row sees
+};
+// false: nothing to do.
+__device__ inline bool tile_rows(const AttnArgs& a, int y, int head, int lane, TileRows& r) {
+  r.tile = y >= a.n_seqs;
+  if (!r.tile) {
+    r.seq = r.s0 = y;
+    r.rows = a.group;
+    r.T = a.seq_lens[y];
+    r.row_end = r.min_end = (int)r.T;
+    return true;
+  }
+  const PrefixTile t = prefix_tile(a.prefix, a.n_seqs, 8 / a.group, y - a.n_seqs, lane);
+  if (t.n <= 0) return false;
+  r.seq = t.leader;
+  r.s0 = t.s0;
+  r.rows = t.n * a.group;
+  const int s = t.s0 + (head < r.rows ? head : r.rows - 1) / a.group;
+  r.row_end = (int)a.prefix.end(s, (int64_t)a.seq_lens[s] - a.new_col, a.st.table_stride);
+  const int most = wave_max(r.row_end);
+  r.T = most;
+  r.min_end = -wave_max(-r.row_end);
+  return most > 0;
+}
+// Row h's place among the queries, and its partial `split`, a prefix's before the others.
+__device__ inline int64_t tile_q_row(const AttnArgs& a, const TileRows& r, int kvh, int h) {
+  const int s = r.s0 + h / a.group;
+  return (int64_t)s * a.n_q_heads + kvh * a.group + h % a.group;
+}
+__device__ inline int64_t tile_part_row(const AttnArgs& a, const TileRows& r, int kvh, int h, int split) {
+  const int s = r.s0 + h / a.group;
+  return ((int64_t)s * a.part_stride + (r.tile ? split : a.prefix.slots + split)) * a.n_q_heads +
+         kvh * a.group + h % a.group;
+}
+__device__ inline WinGeom tile_window(const AttnArgs& a, const TileRows& r) {
+  return r.tile ? win_geometry(r.T, r.T, 0, a.st.table_stride) : attn_window(a, r.seq, r.T);
+}
+// Whether the lane's row sees `slot`, without a branch: where the lanes of a
+// wave differ, `if (!vis) { s[i] = -inf; v[i] = 0; }` after short-circuit tests
+// was compiled to an empty branch (the hidden value lost) in the codebook
+// kernel's 2- and 3-bit forms; selects on this are not.
+__device__ inline bool tile_sees(const TileRows& r, const WinGeom& g, int64_t sinks, int64_t ex_slot,
+                                 int64_t slot) {
+  return ((slot >= g.lo) | (slot < sinks)) & (slot < r.row_end) & (slot != ex_slot);
+}
+// Blocks of each of a prefix's `slots` splits.
+__device__ inline int tile_bps(const AttnArgs& a, const SeqGeom& g) {
+  const int n = (int)(g.blk_hi - g.blk_lo);
+  return (n + a.prefix.slots - 1) / a.prefix.slots;
 }
 
 // kWeigh: the scores of tokens 4 j .. 4 j + 3 of block b (-inf where hidden)

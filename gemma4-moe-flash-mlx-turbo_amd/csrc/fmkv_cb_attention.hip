@@ -95,10 +95,11 @@ struct CbPlan {
 // by that wave (lanes < D / 8).
 template <int D>
 __device__ inline void cb_copy_q_row(const AttnArgs& a, uint8_t* dst, int seq, int kvh, int wave,
-                                     int lane) {
-  if (wave < a.group && lane < D / 8) {
+                                     int lane, const TileRows* tr = nullptr) {
+  if (wave < (tr ? tr->rows : a.group) && lane < D / 8) {
     const uint16_t* qh =
-        a.q + ((int64_t)seq * a.n_q_heads + (int64_t)kvh * a.group + wave) * D;
+        a.q + (tr ? tile_q_row(a, *tr, kvh, wave)
+                  : (int64_t)seq * a.n_q_heads + (int64_t)kvh * a.group + wave) * D;
     dma16(lds_addr(dst + wave * D * 2), lane * 16, buffer_rsrc(qh, (uint32_t)(D * 2)));
   }
 }
@@ -111,12 +112,12 @@ __device__ inline void cb_copy_q_row(const AttnArgs& a, uint8_t* dst, int seq, i
 // the work-group calls it (it holds two barriers).
 template <int D>
 __device__ void cb_build_q_table(const AttnArgs& a, uint8_t* tab, int wave, int lane,
-                                 uint32_t sbits) {
+                                 uint32_t sbits, int rows = -1) {
   constexpr int E = D / 64;
   float x[E];
 #pragma unroll
   for (int i = 0; i < E; i++) x[i] = 0.0f;
-  if (wave < a.group) {
+  if (wave < (rows < 0 ? a.group : rows)) {
     const uint32_t* raw = reinterpret_cast<const uint32_t*>(tab + (wave * D + lane * E) * 2);
 #pragma unroll
     for (int k = 0; k < E / 2; k++) {
@@ -325,35 +326,42 @@ void cb_decode_kernel(AttnArgs a) {
   const int j = lane >> 4, c = lane & 15;
   const int head = c & 7;
   const bool hi = c < 8;
-  const int G = a.group;
+  constexpr bool TILES = MODE == kTiles;
+  TileRows tr{};
+  if constexpr (TILES) {
+    if (!tile_rows(a, blockIdx.y, head, lane, tr)) return;
+  }
+  const int G = TILES ? tr.rows : a.group;  // query rows
   const bool col_valid = head < G;
   // this lane's copy of the tables
   const uint32_t lut_l = lds_addr(lut) + (lane & (kLutCopies - 1)) * 4;
   // grid (KV head, sequence, split column), as the affine kernel
-  const int kvh = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
+  const int kvh = blockIdx.x, seq = TILES ? tr.seq : (int)blockIdx.y, split = blockIdx.z;
 
-  const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
+  const int64_t T = TILES ? tr.T : a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
   // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
   // is the sequence's own number
   WinGeom wg{};
-  if constexpr (windowed(MODE)) wg = attn_window(a, seq, T);
+  if constexpr (windowed(MODE)) wg = TILES ? tile_window(a, tr) : attn_window(a, seq, T);
   auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   const SeqGeom geo =
       windowed(MODE)
           ? wg.geo
           : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
-  const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
+  const int per = TILES && tr.tile ? tile_bps(a, geo) : 0;
+  const int n_splits =
+      TILES && tr.tile ? a.prefix.slots : n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
   if constexpr (MODE != kGated) {
-    if (a.new_col && split == (int)gridDim.z - 1) {
+    if (a.new_col && split == a.max_splits && !(TILES && tr.tile)) {
       static_assert(P::kStageRegion >= D / 2 * (int)sizeof(float2), "rope table fits the staging");
-      cb_new_token_column<D, BITS>(a, scratch, reinterpret_cast<float2*>(stage), T, n_splits, kvh,
-                                   seq, wave, lane);
+      cb_new_token_column<D, BITS>(a, scratch, reinterpret_cast<float2*>(stage), T,
+                                   TILES ? n_splits + a.prefix.slots : n_splits, kvh, seq, wave, lane);
       return;
     }
   }
   if (split >= n_splits) return;
   int64_t b_begin, b_end;
-  split_range(geo, split, a.bps0, a.bps, a.skew_p, a.skew_extra, &b_begin, &b_end);
+  split_range(geo, split, per ? per : a.bps0, per ? per : a.bps, a.skew_p, a.skew_extra, &b_begin, &b_end);
 
   // table entries through the constant address space: a uniform index then
   // becomes a scalar load, which never waits for the copies in flight
@@ -412,13 +420,13 @@ void cb_decode_kernel(AttnArgs a) {
   cb_fill_lut<BITS>(lut, tid, kCbWaves * 64);
   if (lane == 0) xflag[wave] = 0;
   constexpr int NQ = (NST + 1) / 2;
-  cb_copy_q_row<D>(a, scratch, seq, kvh, wave, lane);
+  cb_copy_q_row<D>(a, scratch, seq, kvh, wave, lane, TILES ? &tr : nullptr);
 #pragma unroll
   for (int s = 0; s < NQ; s++)
     if (s < nbx) copy_block(s, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : s));
   wait_copies<CP, NQ>(nbx < NQ ? nbx : NQ);  // the q copy preceded every block
   const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
-  cb_build_q_table<D>(a, scratch, wave, lane, sbits);
+  cb_build_q_table<D>(a, scratch, wave, lane, sbits, TILES ? G : -1);
 #pragma unroll
   for (int s = NQ; s < NST; s++)
     if (s < nbx) copy_block(s, pb0 + (int64_t)NS * (MODE == kGated ? bcopy.pop() : s));
@@ -445,7 +453,7 @@ void cb_decode_kernel(AttnArgs a) {
   // a decode step's new token is the new-token column's (its slot may still
   // hold the position it replaces, or be written meanwhile)
   int64_t ex_slot = -1;
-  if (a.new_col && T > 0) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
+  if (a.new_col && T > 0 && !(TILES && tr.tile)) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
   // sparse-V: this column's score threshold
   float theta = -INFINITY;
   if constexpr (MODE == kGated) theta = col_valid ? th_s[head] : -INFINITY;
@@ -516,7 +524,8 @@ void cb_decode_kernel(AttnArgs a) {
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) &&
+                              t0 + kBlockTokens <= (TILES ? (int64_t)tr.min_end : T)
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
@@ -528,9 +537,13 @@ void cb_decode_kernel(AttnArgs a) {
                    slot != ex_slot;
         if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
-        if (!vis) {
+        if constexpr (TILES) vis = tile_sees(tr, wg, a.sinks, ex_slot, slot);
+        // (a hidden token's norm may be anything, and 0 * inf is NaN)
+        if constexpr (TILES) {
+          sc[i] = vis ? sc[i] : -INFINITY;
+          vscale[i] = vis ? vscale[i] : 0.0f;
+        } else if (!vis) {
           sc[i] = -INFINITY;
-          // (a hidden token's norm may be anything, and 0 * inf is NaN)
           if constexpr (windowed(MODE)) vscale[i] = 0.0f;
         }
       }
@@ -704,13 +717,15 @@ void cb_decode_kernel(AttnArgs a) {
           reinterpret_cast<uint16_t*>(a.out)[o_idx + i] = f32_to_bf16(v);
       }
     } else {
-      const int64_t pbase = ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G;
-      float* dst = a.part_o + (pbase + hh) * D + lane * E;
+      const int64_t prow =
+          TILES ? tile_part_row(a, tr, kvh, hh, split)
+                : ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G + hh;
+      float* dst = a.part_o + prow * D + lane * E;
 #pragma unroll
       for (int i = 0; i < E; i++) dst[i] = x[i] * cs;
       if (lane == 0) {
-        a.part_ml[(pbase + hh) * 2 + 0] = M;
-        a.part_ml[(pbase + hh) * 2 + 1] = Lsum;
+        a.part_ml[prow * 2 + 0] = M;
+        a.part_ml[prow * 2 + 1] = Lsum;
       }
     }
   }
@@ -760,6 +775,10 @@ hipError_t launch_cb_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStream_
   if (a.scores) {
     e = launch_cb_mode<D, BITS, kWeigh>(a, grid, s, ev0, ev1);
     return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  if (a.prefix.tiles > 0) {
+    e = launch_cb_mode<D, BITS, kTiles>(a, tiles_grid(a, n_kv_heads), s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine(a, n_seqs, s);
   }
   const AttnArgs own = behind_prefix(a);
   e = a.win > 0 ? launch_cb_mode<D, BITS, kWindow>(own, grid, s, ev0, ev1)

@@ -11,7 +11,8 @@ namespace {
 // d0 + 4*dq .. +3 and splits sl, sl + 16, ..., merged in one pass with a
 // running maximum; the 16 partial merges meet in LDS.
 // `dims`: which 64 of head_dim. n_cols: split partials per sequence (splits and
-// new-token column), or -1 for per-sequence counts from the struct (a paged batch); flags: bit 0 f32 output, bit 1 sparse-V,
+// new-token column), or -1 for per-sequence counts from the struct (a paged batch),
+// a shared prefix's partials among them (kTiles); flags: bit 0 f32 output, bit 1 sparse-V,
 // bits 8-31 q heads.
 template <int D>
 __device__ inline void combine_rows(const float* part_o, const float* part_ml, void* out,
@@ -24,13 +25,17 @@ __device__ inline void combine_rows(const float* part_o, const float* part_ml, v
   const int dq = tid & 15, sl = tid >> 4;
   const int d0 = dims * 64 + dq * 4;
   const int nqh = (int)(flags >> 8);
-  int n_splits = n_cols;
+  int n_splits = n_cols, s0 = 0;
   if (n_cols < 0) {
     const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
     const SeqGeom geo =
         a.win > 0 ? attn_window(a, seq, T).geo
                   : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
     n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p) + a.new_col;
+    if (a.prefix.lens) {
+      n_splits += a.prefix.slots;
+      if (a.prefix.end(seq, T - a.new_col, a.st.table_stride) == 0) s0 = a.prefix.slots;
+    }
   }
   const int64_t stride = (int64_t)nqh;
   const int64_t base = (int64_t)seq * part_stride * stride + h;
@@ -40,7 +45,7 @@ __device__ inline void combine_rows(const float* part_o, const float* part_ml, v
   float M = -INFINITY, den = 0.0f;
   float4_t acc = (float4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = sl; s < n_splits; s += 16) {
+  for (int s = s0 + sl; s < n_splits; s += 16) {
     const int64_t r = base + s * stride;
     const float2 ml = *reinterpret_cast<const float2*>(part_ml + r * 2);
     const float4_t ov = *reinterpret_cast<const float4_t*>(part_o + r * D + d0);

@@ -27,6 +27,10 @@ struct PrefixArgs {
   const int32_t* starts = nullptr;  // [n_groups + 1], device
   int32_t n_groups = 0;
   int32_t slots = 0;  // partials of a prefix, before a sequence's others
+  // Few rows share a prefix: the decode kernels attend it too, in so many tiles of
+  // eight rows (kTiles), of 8 blocks a split and more (long_splits) or fewer.
+  int32_t tiles = 0;
+  int32_t long_splits = 0;
   // Positions of sequence s that its group's prefix holds, of the T that are stored.
   __device__ int64_t end(int s, int64_t T, int64_t table_stride) const {
     if (s < starts[0] || s >= starts[n_groups]) return 0;
@@ -150,6 +154,7 @@ struct AttnArgs {
   // what lies behind a sequence's prefix, and launch_shared_merge merges the prefix's
   // partials, part_o and part_ml's first prefix.slots of a sequence, with theirs.
   PrefixArgs prefix;
+  int32_t n_seqs = 0;  // (with prefixes)
   // Accumulated attention weights (win > 0 too): the split kernels store every
   // score, base 2, [n_seqs][score_blocks][n_q_heads][16], and a launch that also is the
   // combine adds the weights of a position, summed over the query heads, to
@@ -160,6 +165,12 @@ struct AttnArgs {
   float* weights_out = nullptr;
   int64_t weights_width = 0;
 };
+
+// The grid of a batch that shares prefixes in tiles of few rows (kTiles).
+inline dim3 tiles_grid(const AttnArgs& a, int n_kv_heads) {
+  const int cols = a.max_splits + a.new_col;
+  return dim3(n_kv_heads, a.n_seqs + a.prefix.tiles, a.prefix.slots > cols ? a.prefix.slots : cols);
+}
 
 // The split kernels' arguments of a batch that shares prefixes: their partials
 // come after the prefix's.
@@ -397,10 +408,10 @@ hipError_t launch_prefill_attention(const PrefillArgs& a, hipStream_t s);
 // The partials of a batch's shared prefixes (PrefillArgs::prefix): n_seqs, group,
 // q, qscale, new_st, part_o and part_ml and what stands with them.
 hipError_t launch_prefix_attention(const PrefillArgs& a, hipStream_t s);
-// How a batch's prefixes are shared out on `cus` CUs (prefix.slots and share_rows of
-// a), none longer than max_prefix, with at most max_rest positions behind them; false
-// where every sequence had better attend its prefix by itself.
-bool prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix, int64_t max_rest);
+// How a batch's prefixes, none longer than max_prefix, are shared out on `cus` CUs
+// (prefix.slots and share_rows of a), and about how many us a call takes then: its
+// fixed part, the steps of 32 keys of a work-group, the partials written and read.
+double prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix);
 // How a prefill call runs on a GPU of `cus` CUs (share_rows, units and
 // min_split of a), no sequence having more than max_steps steps of 32 keys:
 // the bytes of its partials (part_o, then part_ml), 0 where it is not split.

@@ -176,31 +176,38 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int j = lane >> 4, c = lane & 15, head = c & 7;
   const bool hi_col = c < 8;
-  const int G = a.group;
-  const int kvh = blockIdx.x, seq = blockIdx.y, split = blockIdx.z;
+  constexpr bool TILES = MODE == kTiles;
+  TileRows tr{};
+  if constexpr (TILES) {
+    if (!tile_rows(a, blockIdx.y, head, lane, tr)) return;
+  }
+  const int G = TILES ? tr.rows : a.group;  // query rows
+  const int kvh = blockIdx.x, seq = TILES ? tr.seq : (int)blockIdx.y, split = blockIdx.z;
 
-  const int64_t T = a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
+  const int64_t T = TILES ? tr.T : a.seq_lens ? (int64_t)a.seq_lens[seq] : a.seq_len;
   // kWindow: blocks are numbered over the visible ones (WinGeom), wg.block(v)
   // is the sequence's own number
   WinGeom wg{};
-  if constexpr (windowed(MODE)) wg = attn_window(a, seq, T);
+  if constexpr (windowed(MODE)) wg = TILES ? tile_window(a, tr) : attn_window(a, seq, T);
   auto block_of = [&](int64_t v) { return windowed(MODE) ? wg.block(v) : v; };
   const SeqGeom geo =
       windowed(MODE)
           ? wg.geo
           : seq_geometry(T, a.window, a.vis_begin, a.st.table_stride, a.st.block_table != nullptr);
-  const int n_splits = n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
+  const int per = TILES && tr.tile ? tile_bps(a, geo) : 0;
+  const int n_splits =
+      TILES && tr.tile ? a.prefix.slots : n_splits_for(geo, a.bps0, a.bps, a.max_splits, a.skew_p);
   if constexpr (MODE != kGated) {
-    if (a.new_col && split == (int)gridDim.z - 1) {
+    if (a.new_col && split == a.max_splits && !(TILES && tr.tile)) {
       static_assert(sizeof(rows) >= D / 2 * sizeof(float2), "rope table fits the row area");
-      plain_new_token_column<D>(a, reinterpret_cast<float2*>(rows), T, n_splits, kvh, seq, wave,
-                                lane);
+      plain_new_token_column<D>(a, reinterpret_cast<float2*>(rows), T,
+                                TILES ? n_splits + a.prefix.slots : n_splits, kvh, seq, wave, lane);
       return;
     }
   }
   if (split >= n_splits) return;
   int64_t b_begin, b_end;
-  split_range(geo, split, a.bps0, a.bps, a.skew_p, a.skew_extra, &b_begin, &b_end);
+  split_range(geo, split, per ? per : a.bps0, per ? per : a.bps, a.skew_p, a.skew_extra, &b_begin, &b_end);
   const int nb = (int)(b_end - b_begin);
   // sparse-V: this (sequence, KV head)'s row of block maxima; the gated pass
   // visits only the blocks holding a score at or above a head's threshold
@@ -246,7 +253,8 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   // wave's slices (zero past the group)
   u32x4 bq[SW];
   {
-    const uint16_t* qh = a.q + ((int64_t)seq * a.n_q_heads + (int64_t)kvh * G + head) * D;
+    const uint16_t* qh = a.q + (TILES ? tile_q_row(a, tr, kvh, head < G ? head : 0)
+                                      : (int64_t)seq * a.n_q_heads + (int64_t)kvh * G + head) * D;
 #pragma unroll
     for (int s = 0; s < SW; s++)
       bq[s] = head < G ? *reinterpret_cast<const u32x4*>(qh + (wave * SW + s) * 32 + 8 * j)
@@ -260,7 +268,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
   const bool ring_trim = a.window > 0 && a.vis_begin > T - a.window;
   // a decode step's new token is the new-token column's
   int64_t ex_slot = -1;
-  if (a.new_col && T > 0) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
+  if (a.new_col && T > 0 && !(TILES && tr.tile)) ex_slot = a.window > 0 ? (T - 1) % a.window : T - 1;
 
   // sparse-V: this column's score threshold
   float theta = -INFINITY;
@@ -295,7 +303,8 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
     // visibility: whole block in the common case, per token at the edges
     const int64_t t0 = b * kBlockTokens;
     const bool full =
-        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) && t0 + kBlockTokens <= T
+        (windowed(MODE) ? (t0 >= wg.lo || t0 + kBlockTokens <= a.sinks) &&
+                              t0 + kBlockTokens <= (TILES ? (int64_t)tr.min_end : T)
                          : t0 >= vis_lo && t0 + kBlockTokens <= vis_hi && !ring_trim) &&
         (uint64_t)(ex_slot - t0) >= (uint64_t)kBlockTokens;
     if (!full) {
@@ -308,13 +317,33 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
                    slot != ex_slot;
         if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
+        if constexpr (TILES) vis = tile_sees(tr, wg, a.sinks, ex_slot, slot);
         if (!vis) s4[r] = -INFINITY;
         seen[r >> 1] |= vis ? 0xffffu << 16 * (r & 1) : 0u;
       }
       // a hidden token's weight is 0, but its V row may be anything, and 0 * inf is NaN
-      if constexpr (windowed(MODE)) {
+      if constexpr (windowed(MODE) && !TILES) {
 #pragma unroll
         for (int t = 0; t < TW; t++) cur.v[t].x &= seen[0], cur.v[t].y &= seen[1];
+      }
+      // kTiles: rows differ in what they see. Values that are not finite become 0, and
+      // infinite the accumulators of the rows that do see them: a product of ones
+      // counts how many of them a row sees, per dim.
+      if constexpr (TILES) {
+        auto bad_of = [](uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u; };
+#pragma unroll
+        for (int t = 0; t < TW; t++) {
+          const uint32_t b0 = bad_of(cur.v[t].x), b1 = bad_of(cur.v[t].y);
+          if (!__any((b0 | b1) != 0u)) continue;
+          const float4_t n = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+              __builtin_bit_cast(short4_t, make_uint2(b0 * 0x3f80u, b1 * 0x3f80u)),
+              __builtin_bit_cast(short4_t, make_uint2(seen[0] & 0x3f803f80u, seen[1] & 0x3f803f80u)),
+              (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[t][r] = fmaf(n[r] * 0x1p127f, 0x1p127f, o[t][r]);
+          cur.v[t].x &= ~(b0 * 0xffffu);
+          cur.v[t].y &= ~(b1 * 0xffffu);
+        }
       }
     }
     if constexpr (MODE == kGated) {
@@ -416,7 +445,9 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
           reinterpret_cast<uint16_t*>(a.out)[o_idx + e] = f32_to_bf16(v);
       }
     } else {
-      const int64_t pb = ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G + hh;
+      const int64_t pb =
+          TILES ? tile_part_row(a, tr, kvh, hh, split)
+                : ((int64_t)seq * a.part_stride + split) * a.n_q_heads + (int64_t)kvh * G + hh;
 #pragma unroll
       for (int e = 0; e < E; e++) a.part_o[pb * D + lane * E + e] = rows[hh][lane * E + e];
       if (lane == 0) {
@@ -471,6 +502,10 @@ hipError_t launch_plain_t(const AttnArgs& a, int n_seqs, int n_kv_heads, hipStre
   if (a.scores) {
     e = launch_plain_mode<D, kWeigh>(a, grid, s, ev0, ev1);
     return e != hipSuccess ? e : launch_combine_weigh(a, n_seqs, s);
+  }
+  if (a.prefix.tiles > 0) {
+    e = launch_plain_mode<D, kTiles>(a, tiles_grid(a, n_kv_heads), s, ev0, ev1);
+    return e != hipSuccess ? e : launch_combine(a, n_seqs, s);
   }
   const AttnArgs own = behind_prefix(a);
   e = a.win > 0 ? launch_plain_mode<D, kWindow>(own, grid, s, ev0, ev1)

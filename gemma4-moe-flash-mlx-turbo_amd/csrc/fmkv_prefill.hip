@@ -246,46 +246,6 @@ __device__ inline PrefillUnit prefill_unit(const PrefillArgs& a, int u, int seq,
   return r;
 }
 
-// The largest value of a wave's lanes.
-__device__ inline int wave_max(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_xor(v, d);
-    v = v > o ? v : o;
-  }
-  return __builtin_amdgcn_readfirstlane(v);
-}
-
-// Tile `tile` of a batch's groups, QP sequences a tile: its first sequence, how
-// many it has, and the group's first one (n 0: a tile that nothing needs). Lane l
-// looks at group g0 + l; every wave that asks gets the same answer.
-struct PrefixTile {
-  int s0, n, leader;
-};
-__device__ inline PrefixTile prefix_tile(const PrefixArgs& p, int n_seqs, int QP, int tile, int lane) {
-  for (int g0 = 0; g0 < p.n_groups; g0 += 64) {
-    const int g = g0 + lane;
-    int a = 0, b = 0;
-    if (g < p.n_groups) a = p.starts[g], b = p.starts[g + 1];
-    a = a < 0 ? 0 : a;
-    b = b > n_seqs ? n_seqs : b;
-    const int count = b > a ? (b - a + QP - 1) / QP : 0;
-    const int upto = scan_add(count), total = __builtin_amdgcn_readlane(upto, 63);
-    if (tile < total) {
-      const int l = __builtin_ctzll(__ballot(upto > tile));
-      const int t = tile - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(count, l));
-      PrefixTile r;
-      r.leader = __builtin_amdgcn_readlane(a, l);
-      r.s0 = r.leader + t * QP;
-      r.n = __builtin_amdgcn_readlane(b, l) - r.s0;
-      if (r.n > QP) r.n = QP;
-      return r;
-    }
-    tile -= total;
-  }
-  return PrefixTile{0, 0, 0};
-}
-
 // KIND of a call. kCausal: a chunk's queries, the sequence's positions up to their
 // own. kBand: a paged pool's window with sinks (a.window, a.sinks): position p
 // sees j <= p with j > p - window or j < sinks. The sinks' blocks take the place of
@@ -1624,28 +1584,17 @@ size_t prefill_plan(PrefillArgs& a, int cus, int64_t max_steps, bool may_split) 
   return prefill_part_bytes(units * wgs, D);
 }
 
-// Where few sequences or short prefixes are shared, every sequence for itself is
-// faster: the pages that the others read too come from the caches. Estimated in us (a
-// call's fixed part; a step of 32 keys, all work-groups side by side; partials written
-// and read at 5 TB/s; alone, the pages at 9 TB/s), and measured, shared and alone: 2
-// sequences behind 992 tokens, 4 bits, 8 heads of 256 dims: 27.1 and 17.2; 9 behind 8000, 8
-// bits, 2 heads of 512 dims: 48.9 and 40.5; 32 behind 32768: 120 and 274; 41 in five
-// groups behind 700 .. 6000, bf16, 4 heads of 128 dims: 40.5 and 52.6.
-bool prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix, int64_t max_rest) {
-  const BlockLayout& L = a.new_st.layout;
-  const int D = L.head_dim, H = a.new_st.n_kv_heads;
-  if (a.prefix.n_groups <= 0 || a.prefix.n_groups >= a.n_seqs) return false;
-  const int64_t wgs = prefix_tiles(a) * H, steps = max_prefix / kPfKeys;
-  if (steps < 1) return false;
+double prefix_plan(PrefillArgs& a, int cus, int64_t max_prefix) {
+  const int D = a.new_st.layout.head_dim;
+  const int64_t wgs = prefix_tiles(a) * a.new_st.n_kv_heads;
+  const int64_t steps = std::max<int64_t>(max_prefix / kPfKeys, 1);
   a.share_rows = D < 512 && wgs <= cus / 4;
   const int64_t most = (steps + kPfMinSteps - 1) / kPfMinSteps, places = prefill_places(D, a.share_rows, cus);
   a.prefix.slots = (int32_t)std::clamp<int64_t>(places / wgs, 1, most);
   const double fixed = D == 128 ? 26.0 : D == 256 ? 20.0 : 32.0, step = D == 128 ? 0.75 : D == 256 ? 1.7 : 2.3;
   const int64_t rounds = (wgs * a.prefix.slots + places - 1) / places;
-  const double shared = fixed + step * (double)((steps + a.prefix.slots - 1) / a.prefix.slots * rounds) +
-                        (double)a.n_seqs * a.n_q_heads * a.prefix.slots * D * 8 / 5e6;
-  const double alone = 16.0 + (double)(max_prefix + max_rest) / kBlockTokens * a.n_seqs * H * L.block_bytes / 9e6;
-  return shared < alone;
+  return fixed + step * (double)((steps + a.prefix.slots - 1) / a.prefix.slots * rounds) +
+         (double)a.n_seqs * a.n_q_heads * a.prefix.slots * D * 8 / 5e6;
 }
 
 hipError_t launch_shared_merge(const AttnArgs& a, int n_seqs, hipStream_t s) {

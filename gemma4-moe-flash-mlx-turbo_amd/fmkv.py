@@ -37,6 +37,7 @@ MODE_AFFINE = 0
 MODE_CODEBOOK = 1
 MODE_PLAIN = 2  # unquantized bf16 rows (bits 16): KVCacheInner::Plain, src/cache.rs:174-178
 PLAIN_BITS = 16
+PREFIX_AUTO, PREFIX_ALONE, PREFIX_ROWS, PREFIX_TILES = 0, 1, 2, 3  # see set_prefix_sharing
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 BLOCK_TOKENS = 16
@@ -59,7 +60,7 @@ EXPORTED = (
     "fmkv_pools_copy_blocks", "fmkv_paged_compact", "fmkv_qkv_norm_rope",
     "fmkv_paged_prefix_decode_attention", "fmkv_paged_prefix_decode_step",
     "fmkv_paged_weighing_decode_attention", "fmkv_paged_weighing_decode_step",
-    "fmkv_paged_attention_weights", "fmkv_heaviest_tokens",
+    "fmkv_paged_attention_weights", "fmkv_heaviest_tokens", "fmkv_set_prefix_sharing",
     "fmkv_pages_create", "fmkv_pages_destroy", "fmkv_pages_free_count", "fmkv_pages_users",
     "fmkv_pages_alloc", "fmkv_pages_release", "fmkv_pages_fork", "fmkv_pages_slide",
 )
@@ -200,6 +201,7 @@ def load_library(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         "fmkv_pool_read_codes": ([vp, vp, vp, vp], ctypes.c_int),
         "fmkv_set_blocks_per_split": ([i32], ctypes.c_int),
         "fmkv_set_sparse_v_gather": ([i32], ctypes.c_int),
+        "fmkv_set_prefix_sharing": ([i32], ctypes.c_int),
         "fmkv_cache_decode_splits": ([vp, P(i32)], ctypes.c_int),
         "fmkv_profile_enable": ([i32], ctypes.c_int),
         "fmkv_profile_collect": ([P(ctypes.c_double), P(i32)], ctypes.c_int),
@@ -344,6 +346,12 @@ def set_sparse_v_gather(on: bool) -> None:
     """Sparse-V after its statistics pass: the gather of the kept V rows
     (True, the default) or the gated pass and the split merge (False)."""
     _check(load_library().fmkv_set_sparse_v_gather(1 if on else 0))
+
+
+def set_prefix_sharing(way: int) -> None:
+    """How batches that share prefixes run: PREFIX_AUTO (by a call's sizes), or always
+    each sequence alone, eight rows at a time, or 64 (for tuning and tests)."""
+    _check(load_library().fmkv_set_prefix_sharing(way))
 
 
 def profile_enable(max_records: int) -> None:

@@ -620,6 +620,17 @@ int fmkv_set_blocks_per_split(int32_t blocks_per_split);
  * counterpart (a tuning and test switch). */
 int fmkv_set_sparse_v_gather(int32_t on);
 
+/* How batches that share prefixes run (fmkv_paged_prefix_decode_attention and its
+ * step): AUTO (the default) by estimates from a call's sizes; ALONE: every sequence
+ * reads its own table's blocks; ROWS: eight rows (sequences times q heads per KV
+ * head) at a time read a prefix once; TILES: 64 rows. Each gives the same
+ * attention. No reference counterpart (a tuning and test switch). */
+#define FMKV_PREFIX_AUTO 0
+#define FMKV_PREFIX_ALONE 1
+#define FMKV_PREFIX_ROWS 2
+#define FMKV_PREFIX_TILES 3
+int fmkv_set_prefix_sharing(int32_t way);
+
 /* Kernel timing (profiling aid, no reference counterpart): while enabled,
  * each decode attention call records a pair of HIP events around its split-K
  * kernel on the caller's stream, up to max_records pairs (0 disables and

@@ -9,7 +9,17 @@ from window_util import AFFINE, CODEBOOK, PLAIN, TOKENS, check_window, queries
 
 pytestmark = pytest.mark.gpu
 
-LOOSE = 2 ** 31 - 1  # a bound of the prefixes with which they are always shared
+WAYS = ["alone", "rows", "tiles"]
+
+
+@pytest.fixture
+def way(request, gpu):
+    gpu.set_prefix_sharing(1 + WAYS.index(request.param))
+    yield request.param
+    gpu.set_prefix_sharing(gpu.PREFIX_AUTO)
+
+
+every_way = pytest.mark.parametrize("way", WAYS, indirect=True)
 
 # mode, bits, D, Hkv, Hq
 FORMS = [(AFFINE, 4, 256, 8, 16), (AFFINE, 8, 512, 2, 16), (PLAIN, 16, 128, 4, 8), (AFFINE, 4, 128, 2, 2),
@@ -38,9 +48,10 @@ def vmax(b):
     return max(float(np.abs(oc.dequant_kv(np.arange(n))[1]).max()) for oc, n in zip(b.oracles, b.lens) if n)
 
 
+@every_way
 @pytest.mark.parametrize("batch", BATCHES)
 @pytest.mark.parametrize("mode,bits,D,Hkv,Hq", FORMS)
-def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch):
+def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch, way):
     import torch
 
     groups, alone = BATCHES[batch]
@@ -48,21 +59,33 @@ def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch):
     q = queries(11, len(b.lens), Hq, Hkv, D)
     want = reference(ora, b, q, D ** -0.5)
     big = vmax(b)
-    for dtype in (torch.float32, torch.bfloat16):
-        out = b.pool.prefix_attention(dev_bf16(q), *b.args(), scale=D ** -0.5, dtype=dtype)
-        check_window(out, want, big, f"{batch} {dtype}")
-    # looser bounds: the prefixes shared where the tight ones say that it does not pay, in
-    # some ranges of keys and in as many as the chip takes, most of them of none
     tables, lens, prefix, starts, longest, rest = b.args()
-    for bound in (longest + 30000, 2 ** 31 - 1):
+    # the tight bounds, and looser ones: more ranges of keys, most of them of none
+    for dtype, bound in ((torch.float32, longest), (torch.bfloat16, longest), (torch.float32, longest + 9000),
+                         (torch.float32, 2 ** 31 - 1)):
         out = b.pool.prefix_attention(dev_bf16(q), tables, lens, prefix, starts, bound, rest, scale=D ** -0.5,
-                                      dtype=torch.float32)
-        check_window(out, want, big, f"{batch} bound {bound}")
+                                      dtype=dtype)
+        check_window(out, want, big, f"{batch} {dtype} {bound}")
 
 
-@pytest.mark.parametrize("loose", [False, True])
+def test_automatic(gpu, ora):
+    """The choice by sizes, from two sequences to many behind a long prefix."""
+    import torch
+
+    for Hkv, Hq, D in ((8, 16, 256), (2, 16, 512)):
+        for prefix, n in ((20, 2), (640, 3), (640, 40), (5000, 4), (5000, 33)):
+            b = Shared(gpu, ora, AFFINE, D, 4, Hkv, [(prefix, [prefix + 1 + 3 * i for i in range(n)])], seed=15)
+            q = dev_bf16(queries(23, n, Hq, Hkv, D))
+            got = b.pool.prefix_attention(q, *b.args(), scale=D ** -0.5, dtype=torch.float32)
+            want = b.pool.window_attention(q, b.table(), b.ints(b.lens), max(b.lens), window=2 ** 30, scale=D ** -0.5,
+                                           dtype=torch.float32)
+            # (two results, each within the bound of check_window)
+            check_window(got, want.double().cpu().numpy(), 2 * vmax(b), f"{n} behind {prefix}")
+
+
+@every_way
 @pytest.mark.parametrize("mode,bits,D,Hkv,Hq", FORMS)
-def test_step(gpu, ora, mode, bits, D, Hkv, Hq, loose):
+def test_step(gpu, ora, mode, bits, D, Hkv, Hq, way):
     """Three steps of one token per sequence, a padded row among them; stored codes
     bit for bit; the shared blocks as they were."""
     import torch
@@ -85,7 +108,7 @@ def test_step(gpu, ora, mode, bits, D, Hkv, Hq, loose):
                    for s, (t, p) in enumerate(zip(b.lens, b.prefix)))
         out = b.pool.prefix_decode_step(
             dev_bf16(k[:, None]), dev_bf16(v[:, None]), b.table(), b.ints(start), b.ints(lens), b.ints(b.prefix),
-            b.ints(b.starts), LOOSE if loose else max(b.prefix), rest, dev_bf16(q), scale=D ** -0.5, dtype=torch.float32)
+            b.ints(b.starts), max(b.prefix), rest, dev_bf16(q), scale=D ** -0.5, dtype=torch.float32)
         want = reference(ora, b, q, D ** -0.5)
         want[padded] = 0.0
         check_window(out, want, vmax(b), f"step {step}")
@@ -98,9 +121,9 @@ def test_step(gpu, ora, mode, bits, D, Hkv, Hq, loose):
         check_codes(codes[slots], meta[slots], b.oracles[s], slots=at, what=f"sequence {s}")
 
 
-@pytest.mark.parametrize("loose", [False, True])
+@every_way
 @pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[1], FORMS[2], FORMS[8]])
-def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, loose):
+def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, way):
     """What lies past a sequence's length, in its blocks and in the shared ones, does
     not reach its output."""
     import torch
@@ -108,7 +131,6 @@ def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, loose):
     b = Shared(gpu, ora, mode, D, bits, Hkv, [(160, [180, 175, 160])], ((), (20,)), seed=7)
     q = queries(13, 4, Hq, Hkv, D)
     tables, lens, prefix, starts, longest, rest = b.args()
-    longest = LOOSE if loose else longest
     # a member that sees 37 of the shared positions, where the others' rows are infinite
     short = b.ints([180, 37, 160, 20])
     before = b.pool.prefix_attention(dev_bf16(q), tables, short, prefix, starts, longest, rest, scale=D ** -0.5,
@@ -122,8 +144,8 @@ def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, loose):
     assert not torch.equal(after[0], before[0])  # (which sees them)
 
 
-@pytest.mark.parametrize("loose", [False, True])
-def test_graph_and_streams(gpu, ora, loose):
+@every_way
+def test_graph_and_streams(gpu, ora, way):
     """A captured step replayed with eager calls between, on tensors of another
     stream; the same bits each time."""
     import torch
@@ -131,9 +153,7 @@ def test_graph_and_streams(gpu, ora, loose):
     D, Hkv, Hq = 256, 8, 16
     b = Shared(gpu, ora, AFFINE, D, 4, Hkv, [(400, [410 + i for i in range(9)])], seed=9)
     q = dev_bf16(queries(17, 9, Hq, Hkv, D))
-    args = list(b.args())
-    if loose:
-        args[4] = LOOSE
+    args = b.args()
     want = b.pool.prefix_attention(q, *args, scale=D ** -0.5)
     other = torch.cuda.Stream()
     out = torch.zeros_like(want)
@@ -152,8 +172,8 @@ def test_graph_and_streams(gpu, ora, loose):
     assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("loose", [False, True])
-def test_forked_book(gpu, ora, loose):
+@every_way
+def test_forked_book(gpu, ora, way):
     """The blocks that PageBook.fork shares, as a server uses them: the same
     attention as over each sequence's whole table."""
     import torch
@@ -181,7 +201,7 @@ def test_forked_book(gpu, ora, loose):
         q = dev_bf16(queries(80 + step, n, Hq, Hkv, D))
         t = prompt + step + 1
         out = pool.prefix_decode_step(kn, vn, tables, ints([t - 1] * n), ints([t] * n), ints([prompt] * n),
-                                      ints([0, n]), LOOSE if loose else prompt, t - prompt // TOKENS * TOKENS, q, scale=D ** -0.5,
+                                      ints([0, n]), prompt, t - prompt // TOKENS * TOKENS, q, scale=D ** -0.5,
                                       dtype=torch.float32)
         want = pool.window_attention(q, tables, ints([t] * n), t, window=2 ** 30, scale=D ** -0.5,
                                      dtype=torch.float32)
