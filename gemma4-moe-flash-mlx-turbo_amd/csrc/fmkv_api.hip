@@ -1838,6 +1838,8 @@ int fmkv_paged_attention_weights(fmkv_pool* p, const void* q, const int32_t* blo
   if (n_seqs == 0 || n_new == 0) return FMKV_OK;
   // (the output's place is taken by the weights)
   if ((rc = check_attn_args(p->desc, q, n_q_heads, 0.0f, weights_out, FMKV_DTYPE_F32))) return rc;
+  if ((int64_t)n_new > (int64_t)65535 * (64 / (n_q_heads / p->desc.n_kv_heads)))
+    return fail(FMKV_ERR_INVALID_ARG, "n_new must be at most 65535 * (64 / query heads per KV head)");
   if (!block_tables || !start_pos) return fail(FMKV_ERR_INVALID_ARG, "block_tables/start_pos are null");
   if ((uintptr_t)q % 2 != 0) return fail(FMKV_ERR_UNSUPPORTED, "q must be 2-byte aligned");
   if ((rc = check_device(p))) return rc;
@@ -1858,8 +1860,9 @@ int fmkv_paged_attention_weights(fmkv_pool* p, const void* q, const int32_t* blo
   RelaxedCapture relaxed;  // (the workspace may grow)
   p->ws.captured = is_captured(s);
   if ((rc = p->ws.ensure(floats * sizeof(float)))) return rc;
-  a.ml = p->ws.ptr;
-  a.part = a.ml + floats - (size_t)n_seqs * p->desc.n_kv_heads * a.sharers * a.part_width;
+  a.rows = reinterpret_cast<uint8_t*>(p->ws.ptr);
+  a.ml = p->ws.ptr + a.images;
+  a.part = p->ws.ptr + floats - (size_t)n_seqs * p->desc.n_kv_heads * a.sharers * a.part_width;
   a.weights_in = weights;
   a.weights_out = weights_out;
   a.weights_width = weights_width;

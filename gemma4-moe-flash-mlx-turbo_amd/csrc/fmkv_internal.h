@@ -347,6 +347,8 @@ struct ObserveArgs {
   // the plan: blocks of a wave's step, ranges of keys, tiles of a KV head, the
   // work-groups that share them
   int32_t step_blocks, ranges, tiles, sharers;
+  int64_t images;  // floats of the rows' operands where they get a launch of their own
+  uint8_t* rows;   // those, [n_seqs][n_kv_heads][tiles]
   float* ml;    // [n_seqs][n_kv_heads][tiles][64][ranges] (m, l)
   float* part;  // [n_seqs][n_kv_heads * sharers][part_width] sums of weights
   int64_t part_width;

@@ -10,7 +10,9 @@
 // one that adds up what KV heads and tiles of rows have given a position.
 //
 // A work-group holds 64 rows (64 / G consecutive queries of a KV head's G heads) as
-// matrix-core operands in LDS; its waves take different keys, NB blocks of 16 a step,
+// matrix-core operands in LDS, rotated in a launch of their own where they are many (four
+// prompts of 700 .. 8000 positions, 33 queries, 8 bits, 2 heads of 512 dims: 99.8 us a call with the
+// rotation in each work-group, 78.7 without); its waves take different keys, NB blocks of 16 a step,
 // straight from memory to registers, where a code is turned into an operand once
 // for all rows. Nothing is exchanged between the waves while they run. Over the
 // 64-dim groups of a step the scores of the 64 rows with the step's keys stay in
@@ -54,12 +56,23 @@ struct ObPlan {
   // lanes that write a row, whose pieces lie in as many operands, then take all banks
   // and not the same few (512 dims, a
   // work-group's 64 rows and one step of keys: 28.0 -> 26.3 us).
-  static constexpr int operand(int part, int rt, int e) { return ((part * RT + rt) * 2 * NG + e) * 1040; }
-  static constexpr int kSums = operand(kParts, 0, 0);  // the operands of the biases
+  static constexpr int kOperands = kParts * RT * 2 * NG;
+  static constexpr int kStride = 1040;
+  static constexpr int index(int part, int rt, int e) { return (part * RT + rt) * 2 * NG + e; }
+  static constexpr int operand(int part, int rt, int e) { return index(part, rt, e) * kStride; }
+  static constexpr int kSums = kOperands * kStride;  // the operands of the biases
   static constexpr int kRows = kSums + (MODE == kAffine ? RT * 1024 : 0);
   static constexpr int KW = MODE == kAffine ? BITS / 2 : MODE == kPlain ? 8 : BITS == 3 ? 4 : 2;
   static constexpr int kLut = MODE == kCodebook ? CbLut<BITS == 16 ? 2 : BITS>::kBytes : 16;
+  // A tile's operands in memory, as a launch of their own leaves them: 1 KiB each, the biases' last.
+  static constexpr int kPieces = kOperands + (MODE == kAffine ? RT : 0);
 };
+
+// Calls of more than 16 rows rotate them in a launch of their own, which every range
+// of keys of both launches then copies to LDS; where 16 rows are all, or none is rotated
+// (plain caches), each work-group prepares them itself.
+template <int MODE, int RT>
+constexpr bool kObRotated = MODE != kPlain && RT > 1;
 
 // Sequence s of a call: its positions, its keys' blocks, and the WG-steps (NW waves'
 // NB blocks) of a range.
@@ -78,6 +91,91 @@ __device__ inline ObSeq ob_seq(const ObserveArgs& a, int seq) {
   const int steps = (r.blocks + NW * NB - 1) / (NW * NB);
   r.per = (steps + a.ranges - 1) / a.ranges;
   return r;
+}
+
+// Row r of a tile, rotated but for the signs (x: the lane's D / 64 dims), as its places
+// in the operands: at `ops`, OP bytes apart, and `sums`.
+template <int D, int BITS, int MODE, int RT, int OP>
+__device__ inline void store_row(const float (&x)[D / 64], uint8_t* ops, uint8_t* sums, int r, int lane,
+                                 uint32_t sbits, float cs_lane) {
+  using P = ObPlan<D, BITS, MODE, RT>;
+  constexpr int E = P::E, LPG = 64 / E;  // lanes of a 64-dim group
+  const int rt = r >> 4, rc = r & 15, d0 = lane * E, o = d0 & 63;
+  float gs = 0.0f;
+  _Float16 hv[E], lv[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    const float v = apply_sign(x[i] * cs_lane, sbits, i);
+    gs += v;
+    hv[i] = (_Float16)v;
+    lv[i] = (_Float16)(v - (float)hv[i]);
+    if constexpr (MODE == kAffine) {  // (exact)
+      hv[i] = hv[i] * (_Float16)kCodeScale<BITS>;
+      lv[i] = lv[i] * (_Float16)kCodeScale<BITS>;
+    }
+  }
+  // (K's operand places: QSlot for affine caches, dims in order for codebooks)
+  const int g = d0 >> 6;
+  const int s = MODE == kAffine && BITS == 8 ? (o >> 3) & 1 : o >> 5;
+  const int jj = MODE == kAffine && BITS == 8 ? o >> 4 : (o >> 3) & 3;
+  uint8_t* p = ops + (jj * 16 + rc) * 16 + (o & 7) * 2;
+  store_halves<E>(p + P::index(0, rt, 2 * g + s) * OP, hv);
+  store_halves<E>(p + P::index(1, rt, 2 * g + s) * OP, lv);
+  if constexpr (MODE == kAffine) {
+    gs = group_sum<LPG>(gs, lane);
+    if ((lane & (LPG - 1)) == 0) {
+      // sums of 64 dims, high parts and residuals, against the biases; and
+      // the sums that the codes' offset adds, against the scales
+      _Float16* q = reinterpret_cast<_Float16*>(sums + rt * 1024) + rc * 8 + g;
+      const float off = gs * (-kCodeOffset<BITS> / kScaleUp<BITS>);
+      const _Float16 h = (_Float16)gs, ho = (_Float16)off;
+      q[0] = h;
+      q[16 * 8] = (_Float16)(gs - (float)h);
+      q[32 * 8] = ho;
+      q[48 * 8] = (_Float16)(off - (float)ho);
+    }
+  }
+}
+
+// A tile's rows as operands (kObRotated), 16 rows a work-group, four of its waves' four at a
+// time. Grid (tile and 16 rows, KV head, sequence).
+template <int D, int BITS, int MODE>
+__global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
+  constexpr int RT = kObRows / 16;
+  using P = ObPlan<D, BITS, MODE, RT>;
+  constexpr int E = P::E, NG = P::NG;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x / RT, rt = blockIdx.x % RT, kvh = blockIdx.y, seq = blockIdx.z;
+  const int G = a.group, QP = kObRows / G, qi0 = tile * QP;
+  const int rows = (a.n_q - qi0 < QP ? a.n_q - qi0 : QP) * G;
+  uint8_t* const ops = a.rows + (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * (P::kPieces * 1024);
+  uint8_t* const sums = ops + P::kOperands * 1024;
+  const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
+  const float cs_lane = fwht_lane_sign(lane) * a.c;
+  const int r0 = rt * 16 + wave * 4;
+  uint32_t raw[4][E / 2];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int r = r0 + k < rows ? r0 + k : rows - 1, rq = r / G;
+    const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
+    load_words<E / 2>(a.q + row * D + lane * E, raw[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) {
+      const uint32_t w = r0 + k < rows ? raw[k][i] : 0u;
+      x[2 * i] = __uint_as_float(w << 16) * a.qscale;
+      x[2 * i + 1] = __uint_as_float(w & 0xffff0000u) * a.qscale;
+    }
+    wave_fwht_signed<E>(x, lane);
+    store_row<D, BITS, MODE, RT, 1024>(x, ops, sums, r0 + k, lane, sbits, cs_lane);
+    if (MODE == kAffine && NG < 8 && lane < 4 * (8 - NG))  // (groups that the dims do not have)
+      reinterpret_cast<_Float16*>(sums + rt * 1024)[(lane & 3) * 128 + ((r0 + k) & 15) * 8 + NG + (lane >> 2)] =
+          (_Float16)0.0f;
+  }
 }
 
 // SUMS: the second launch. Grid (range of keys, KV head and sharer of its tiles, sequence).
@@ -184,7 +282,7 @@ void observe_kernel(ObserveArgs a) {
   const float cs_lane = fwht_lane_sign(lane) * a.c;
   const uint32_t lut_l = lds_addr(lut) + (lane & (kLutCopies - 1)) * 4;
   if constexpr (MODE == kCodebook) cb_fill_lut<CB>(lut, tid, NW * 64);
-  if constexpr (MODE == kAffine) {  // (what of the biases' operands no group fills is 0)
+  if constexpr (MODE == kAffine && !kObRotated<MODE, RT>) {  // (what of the biases' operands no group fills is 0)
     for (int i = tid; i < RT * 64; i += NW * 64)
       reinterpret_cast<u32x4*>(rows_s + P::kSums)[i] = (u32x4){0, 0, 0, 0};
     __syncthreads();
@@ -212,6 +310,15 @@ void observe_kernel(ObserveArgs a) {
     load(bp, 0, cur);
     load_bias(bp, bias);
 
+    if constexpr (kObRotated<MODE, RT>) {
+      const u32x4 rs = buffer_rsrc(a.rows + ml_row / kObRows * (P::kPieces * 1024), P::kPieces * 1024);
+      const uint32_t to = lds_addr(rows_s);
+#pragma unroll 1
+      for (int o = wave; o < P::kPieces; o += NW)
+        dma16(to + (o < P::kOperands ? o * P::kStride : P::kSums + (o - P::kOperands) * 1024),
+              o * 1024 + lane * 16, rs);
+    }
+
     // ---- the rows as operands: row r by wave r % NW ----
     for (int r = tid; r < RT * 16; r += NW * 64) {
       const int rq = r / G;
@@ -220,11 +327,9 @@ void observe_kernel(ObserveArgs a) {
       row_pos[r] = (int)(p < 0 ? -1 : p);
     }
     if constexpr (SUMS) {  // sixteen lanes a row: each merges every sixteenth range, then they meet
-#pragma unroll 2
       for (int r = tid >> 4; r < RT * 16; r += NW * 4) {
         const float2* x = reinterpret_cast<const float2*>(a.ml) + (ml_row + r) * a.ranges;
         float M = -1e30f, l = 0.0f;
-#pragma unroll 4
         for (int k = tid & 15; k < ranges; k += 16) {
           const float mn = fmaxf(M, x[k].x);
           l = fmaf(l, exp2f(M - mn), x[k].y * exp2f(x[k].x - mn));
@@ -235,84 +340,55 @@ void observe_kernel(ObserveArgs a) {
         if ((tid & 15) == 0) stat[0][r] = make_float2(Mx, l > 0.0f ? 1.0f / l : 0.0f);
       }
     }
-    // Four rows of a wave at a time, the next four on their way meanwhile
-    uint32_t raw[4][E / 2], ahead[4][E / 2];
-    auto load_rows = [&](int r0) __attribute__((always_inline)) {
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int rr = r0 + k * NW, r = rr < rows ? rr : rows - 1, rq = r / G;
-        const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
-        load_words<E / 2>(a.q + row * D + lane * E, ahead[k]);
-      }
-    };
-    load_rows(wave);
-#pragma unroll 1
-    for (int r0 = wave; r0 < RT * 16; r0 += 4 * NW) {
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-#pragma unroll
-        for (int i = 0; i < E / 2; i++) raw[k][i] = r0 + k * NW < rows ? ahead[k][i] : 0u;
-      if (r0 + 4 * NW < RT * 16) load_rows(r0 + 4 * NW);
-      const int d0 = lane * E, o = d0 & 63;
-      float x[4][E];
-      if constexpr (MODE != kPlain) {
+    if constexpr (kObRotated<MODE, RT>) {
+      wait_vmcnt<0>();
+    } else {
+      // Four rows of a wave at a time, the next four on their way meanwhile
+      uint32_t raw[4][E / 2], ahead[4][E / 2];
+      auto load_rows = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-#pragma unroll
-          for (int i = 0; i < E / 2; i++) {
-            x[k][2 * i] = __uint_as_float(raw[k][i] << 16) * a.qscale;
-            x[k][2 * i + 1] = __uint_as_float(raw[k][i] & 0xffff0000u) * a.qscale;
-          }
-          wave_fwht_signed<E>(x[k], lane);
+          const int rr = r0 + k * NW, r = rr < rows ? rr : rows - 1, rq = r / G;
+          const int64_t row = ((int64_t)seq * a.n_q + qi0 + rq) * a.n_q_heads + (int64_t)kvh * G + (r - rq * G);
+          load_words<E / 2>(a.q + row * D + lane * E, ahead[k]);
         }
-      }
+      };
+      load_rows(wave);
+#pragma unroll 1
+      for (int r0 = wave; r0 < RT * 16; r0 += 4 * NW) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int r = r0 + k * NW, rt = r >> 4, rc = r & 15;
-        if (r >= RT * 16) continue;
-        if constexpr (MODE == kPlain) {
-          const int e = d0 >> 5;
-          uint8_t* p = rows_s + P::operand(0, rt, e) + (((o & 31) >> 3) * 16 + rc) * 16 + (o & 7) * 2;
+        for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[k][i];
-        } else {
-          float gs = 0.0f;
-          _Float16 hv[E], lv[E];
+          for (int i = 0; i < E / 2; i++) raw[k][i] = r0 + k * NW < rows ? ahead[k][i] : 0u;
+        if (r0 + 4 * NW < RT * 16) load_rows(r0 + 4 * NW);
+        const int d0 = lane * E, o = d0 & 63;
+        float x[4][E];
+        if constexpr (MODE != kPlain) {
 #pragma unroll
-          for (int i = 0; i < E; i++) {
-            const float v = apply_sign(x[k][i] * cs_lane, sbits, i);
-            gs += v;
-            hv[i] = (_Float16)v;
-            lv[i] = (_Float16)(v - (float)hv[i]);
-            if constexpr (MODE == kAffine) {  // (exact)
-              hv[i] = hv[i] * (_Float16)kCodeScale<BITS>;
-              lv[i] = lv[i] * (_Float16)kCodeScale<BITS>;
+          for (int k = 0; k < 4; k++) {
+#pragma unroll
+            for (int i = 0; i < E / 2; i++) {
+              x[k][2 * i] = __uint_as_float(raw[k][i] << 16) * a.qscale;
+              x[k][2 * i + 1] = __uint_as_float(raw[k][i] & 0xffff0000u) * a.qscale;
             }
+            wave_fwht_signed<E>(x[k], lane);
           }
-          // (K's operand places: QSlot for affine caches, dims in order for codebooks)
-          const int g = d0 >> 6;
-          const int s = MODE == kAffine && BITS == 8 ? (o >> 3) & 1 : o >> 5;
-          const int jj = MODE == kAffine && BITS == 8 ? o >> 4 : (o >> 3) & 3;
-          uint8_t* p = rows_s + (jj * 16 + rc) * 16 + (o & 7) * 2;
-          store_halves<E>(p + P::operand(0, rt, 2 * g + s), hv);
-          store_halves<E>(p + P::operand(1, rt, 2 * g + s), lv);
-          if constexpr (MODE == kAffine) {
-            gs = group_sum<LPG>(gs, lane);
-            if ((lane & (LPG - 1)) == 0) {
-              // sums of 64 dims, high parts and residuals, against the biases; and
-              // the sums that the codes' offset adds, against the scales
-              _Float16* q = reinterpret_cast<_Float16*>(rows_s + P::kSums + rt * 1024) + rc * 8 + g;
-              const float off = gs * (-kCodeOffset<BITS> / kScaleUp<BITS>);
-              const _Float16 h = (_Float16)gs, ho = (_Float16)off;
-              q[0] = h;
-              q[16 * 8] = (_Float16)(gs - (float)h);
-              q[32 * 8] = ho;
-              q[48 * 8] = (_Float16)(off - (float)ho);
-            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int r = r0 + k * NW, rt = r >> 4, rc = r & 15;
+          if (r >= RT * 16) continue;
+          if constexpr (MODE == kPlain) {
+            const int e = d0 >> 5;
+            uint8_t* p = rows_s + P::operand(0, rt, e) + (((o & 31) >> 3) * 16 + rc) * 16 + (o & 7) * 2;
+#pragma unroll
+            for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[k][i];
+          } else {
+            store_row<D, BITS, MODE, RT, P::kStride>(x[k], rows_s, rows_s + P::kSums, r, lane, sbits, cs_lane);
           }
         }
       }
-    }
+      }
     __syncthreads();
 
     int p_row[RT];
@@ -587,8 +663,14 @@ __global__ __launch_bounds__(256) void observe_sum_kernel(ObserveArgs a) {
 template <int D, int BITS, int MODE, int RT, int NB>
 hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
   const dim3 grid(a.ranges, a.st.n_kv_heads * a.sharers, a.n_seqs), block(ObPlan<D, BITS, MODE, RT>::NW * 64);
+  hipError_t e = hipSuccess;
+  if constexpr (kObRotated<MODE, RT>) {
+    hipLaunchKernelGGL((observe_rows_kernel<D, BITS, MODE>),
+                       dim3(a.tiles * RT, a.st.n_kv_heads, a.n_seqs), dim3(256), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, RT, NB, false>), grid, block, 0, s, a);
-  hipError_t e = hipGetLastError();
+  e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, RT, NB, true>), grid, block, 0, s, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -618,10 +700,17 @@ size_t observe_plan(ObserveArgs& a, int cus) {
   const int64_t steps = (a.blocks + waves * a.step_blocks - 1) / (waves * a.step_blocks);
   // as many work-groups as run at once, several tiles one after the other where there are more
   a.sharers = (int32_t)std::clamp<int64_t>(2 * places / per_tile, 1, a.tiles);
-  const int ragged = a.n_seqs > 1 ? 2 : 1;
+  // More ranges than places where sequences are likely ragged: eight of 600 .. 6000
+  // positions, 4 bits, 8 heads of 256 dims, 32 queries: 62.7 us with as many, 53.7 with three
+  // times as many (two of 3000 .. 9000: 30.0 and 36.9; four of 12000 each, 512 dims: 140 and 160).
+  const int ragged = a.n_seqs > 2 ? 3 : 1;
   a.ranges = (int32_t)std::clamp<int64_t>(ragged * places / (per_tile * a.sharers), 1, steps);
   a.part_width = (int64_t)a.blocks * kBlockTokens;
-  return (size_t)(rows * a.ranges * kObRows * 2 + per_tile * a.sharers * a.part_width);
+  // operands of a tile: high parts and residuals of 64 rows, and 4 KiB for the biases
+  a.images = a.st.layout.mode == kPlain || a.n_q * a.group <= 16
+                 ? 0
+                 : rows * (kObRows * a.st.layout.head_dim + (a.st.layout.mode == kAffine ? 1024 : 0));
+  return (size_t)(a.images + rows * a.ranges * kObRows * 2 + per_tile * a.sharers * a.part_width);
 }
 
 hipError_t launch_observe(const ObserveArgs& a, hipStream_t s) {

@@ -205,7 +205,6 @@ __device__ inline void keep_heaviest(const float* w, int64_t n, uint32_t need, K
         if (t < kpt) f(held[t], i, i < n);  // (uniform)
       }
     } else {
-#pragma unroll 4
       for (int t = 0; t < kpt; t++) {
         const int64_t i = r0 + (int64_t)t * 64;
         f(i < n ? w[i] : 0.0f, i, i < n);

@@ -351,6 +351,7 @@ def set_sparse_v_gather(on: bool) -> None:
 def set_prefix_sharing(way: int) -> None:
     """How batches that share prefixes run: PREFIX_AUTO (by a call's sizes), or always
     each sequence alone, eight rows at a time, or 64 (for tuning and tests)."""
+    _check_bits("way", way, 32)
     _check(load_library().fmkv_set_prefix_sharing(way))
 
 
