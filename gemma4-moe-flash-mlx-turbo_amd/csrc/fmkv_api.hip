@@ -760,7 +760,9 @@ int prepare_paged_append(const fmkv_pool* p, const void* k, const void* v,
 // to 258 blocks, 4 bits: 64 (4 splits and one of 2 blocks): 60.2, 86: 51.4, 129:
 // 53.9; the same all at 258: 66.5, 65.7, 63.9; one of 254 blocks, 2 heads of 512
 // dims: 2: 17.0, 4: 15.5, 8: 16.8, 16: 19.6.)
-int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows, int new_col) {
+// beside: work-groups of the same launch that are not among these rows'.
+int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows, int new_col,
+                   int64_t beside = 0) {
   if (nblk < 1) return 1;
   const bool plain = d.mode == FMKV_MODE_PLAIN;
   const double fixed = plain ? 3.0 : 12.0;
@@ -768,6 +770,7 @@ int64_t window_bps(const fmkv_cache_desc& d, int cus, int64_t nblk, int64_t rows
   auto best = [&](int64_t per_cu, int64_t min_bps) {
     int64_t slots = per_cu * cus;
     if (new_col && rows <= slots / 2) slots -= rows;  // the new-token column's work-groups
+    if (beside <= slots / 2) slots -= beside;
     int64_t bps = 0;
     double cost = 0.0;
     const int64_t r0 = (rows + slots - 1) / slots;
@@ -1629,9 +1632,9 @@ namespace {
 // sequence fills the columns. Tiles: 64 rows at a time in the prefill kernel, then what each
 // has behind its prefix. Chosen by estimates in us: blocks at 10 and 8 TB/s (most from the
 // caches) and the fixed parts; measured alone / rows / tiles: 2 sequences behind 992 tokens, 4
-// bits, 8 heads of 256 dims: 13.3 / 16.4 / 27.1; 9 behind 8000, 8 bits, 2 heads of 512 dims, 8 q heads each:
-// 30.2 / 52.8 / 48.7; 41 in five groups behind 700 .. 6000, bf16, 4 heads of 128 dims:
-// 71.3 / 39.3 / 40.4; 32 behind 32768, 8 bits, 2 heads of 512 dims: 220 / 268 / 121.
+// bits, 8 heads of 256 dims: 13.6 / 16.6 / 27.2; 9 behind 8000, 8 bits, 2 heads of 512 dims, 8 q heads each:
+// 30.6 / 56.6 / 48.6; 41 in five groups behind 700 .. 6000, bf16, 4 heads of 128 dims:
+// 71.6 / 40.5 / 40.4; 32 behind 32768, 8 bits, 2 heads of 512 dims: 222 / 310 / 121.
 int32_t prefix_way(const fmkv_pool* p, fmkv::PrefillArgs& pa, int64_t max_prefix, int64_t max_rest,
                    int64_t width) {
   if (pa.prefix.n_groups <= 0 || max_prefix < fmkv::kBlockTokens) return FMKV_PREFIX_ALONE;
@@ -1643,8 +1646,8 @@ int32_t prefix_way(const fmkv_pool* p, fmkv::PrefillArgs& pa, int64_t max_prefix
   auto blocks_us = [&](double blocks, double rate) {
     return blocks / fmkv::kBlockTokens * (double)(H * p->layout.block_bytes) / rate;
   };
-  const double alone_us = 16.0 + blocks_us((double)n * (double)(max_prefix + max_rest), 1e7);
-  const double rows_us = 18.0 + blocks_us((double)rows * (double)max_prefix + (double)n * (double)max_rest, 8e6);
+  const double alone_us = 14.0 + blocks_us((double)n * (double)(max_prefix + max_rest), 1e7);
+  const double rows_us = 20.0 + blocks_us((double)rows * (double)max_prefix + (double)n * (double)max_rest, 8e6);
   int32_t way = g_prefix_way;
   if (way == FMKV_PREFIX_ROWS && n + rows > 65535) way = FMKV_PREFIX_ALONE;  // (the grid's y)
   if (way == FMKV_PREFIX_AUTO) {
@@ -1655,7 +1658,9 @@ int32_t prefix_way(const fmkv_pool* p, fmkv::PrefillArgs& pa, int64_t max_prefix
   }
   if (way == FMKV_PREFIX_ROWS) {
     const int64_t blocks = (std::min(max_prefix, width) + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens;
-    int64_t b = std::max<int64_t>(window_bps(p->desc, p->cus, blocks, rows * H, 0), 1);
+    // (one work-group at least for what each sequence has behind its prefix: 4 behind 12000
+    // tokens, 8 bits, 8 heads of 256 dims: 33.1 us without room for those, 31.1 with)
+    int64_t b = std::max<int64_t>(window_bps(p->desc, p->cus, blocks, rows * H, 0, n * H), 1);
     b = std::max(b, (blocks + 65534) / 65535);  // (the grid's z)
     pa.prefix.tiles = (int32_t)rows;
     pa.prefix.slots = (int32_t)((blocks + b - 1) / b);
@@ -1760,6 +1765,9 @@ int weighing_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, 
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
                                n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
   if (rc || n_seqs == 0) return rc;
+  // (before anything is launched: the merge's work-groups and the weights', in one grid)
+  if (((int64_t)(p->desc.head_dim / 64) * n_q_heads + (at.score_blocks + 15) / 16) * n_seqs > (1 << 24) - 1)
+    return fail(FMKV_ERR_INVALID_ARG, "n_seqs times max_seq_len is too large for one call");
   at.weights_in = weights;
   at.weights_out = weights_out;
   at.weights_width = weights_width;

@@ -68,6 +68,19 @@ def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch, way):
         check_window(out, want, big, f"{batch} {dtype} {bound}")
 
 
+@every_way
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[2], FORMS[7]])
+def test_more_groups_than_lanes(gpu, ora, mode, bits, D, Hkv, Hq, way):
+    """Groups are looked through 64 at a time."""
+    import torch
+
+    groups = [(33 + i % 3 * 16, [50 + i % 3 * 16 + j for j in range(1 + i % 4)]) for i in range(131)]
+    b = Shared(gpu, ora, mode, D, bits, Hkv, groups, ((20,), (9,)), seed=21)
+    q = queries(41, len(b.lens), Hq, Hkv, D)
+    out = b.pool.prefix_attention(dev_bf16(q), *b.args(), scale=D ** -0.5, dtype=torch.float32)
+    check_window(out, reference(ora, b, q, D ** -0.5), vmax(b), "many groups")
+
+
 def test_automatic(gpu, ora):
     """The choice by sizes, from two sequences to many behind a long prefix."""
     import torch
