@@ -805,7 +805,8 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
                             int32_t max_blocks, const int32_t* seq_lens, int32_t n_seqs,
                             int32_t max_seq_len, int32_t n_q_heads, float scale, float tau,
                             void* out, int32_t out_dtype, int new_col, hipStream_t s,
-                            fmkv::AttnArgs* a, int32_t win = 0, int32_t sinks = 0) {
+                            fmkv::AttnArgs* a, int32_t win = 0, int32_t sinks = 0,
+                            bool ragged = false) {
   if (n_seqs < 0 || max_seq_len < 0 || max_blocks < 1)
     return fail(FMKV_ERR_INVALID_ARG, "bad n_seqs / max_seq_len / max_blocks");
   if (n_seqs > 0 && (!block_tables || !seq_lens))
@@ -859,17 +860,20 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   const int min_bps = (int)std::min<int64_t>(64, std::max<int64_t>(share, 1));
   const int wg_per_cu = 6 * slots * fmkv::kAttnWgPerCu;
   if (win == kNoWindow) {
-    // Lengths that nothing makes alike (those behind a shared prefix, or with it, are
-    // much the same): where splits come out long, sequences count half of the longest, at most 64 blocks a split, and first splits of four times that as above. (Seven of 65 ..
+    // Lengths that nothing makes alike (`ragged`: not those of sequences that mostly read a
+    // common prefix): where splits come out long, sequences count half of the longest, at most
+    // 64 blocks a split, and first splits of four times that as above. (Scores stored, seven of 65 ..
     // 20011 tokens, 8 bits, 2 heads of 512 dims: 35 blocks 33.5 us, the longest's
     // plan, 68 and 64 blocks, 42.5 and 40.6, 24: 44.3; 32 of 512 .. 16384, 4 bits, 8
-    // heads of 256 dims: 64 blocks, first splits four times that, 106; 171: 163. What 41 sequences have behind
+    // heads of 256 dims: 64 blocks, first splits four times that, 106; 171: 163. In groups of
+    // one, 32 of up to 16000: 76 so, 145 as of equal ones; 16 of 1000 .. 13000, 8 bits, 2
+    // heads of 512 dims: 62 and 53. What 41 sequences have behind
     // their prefixes, 32 blocks at most, bf16, 4 heads of 128 dims: 4 blocks 40.9 us the call, 8 with first
     // splits of 32: 60.4; 32 sequences' 64 blocks at most, 8 bits, 2 heads of 512 dims: 17 blocks 17.4
     // us of the call, 8: 26.)
     const int64_t rows = (int64_t)p->desc.n_kv_heads * n_s;
     int64_t b = window_bps(p->desc, p->cus, nblk, rows, new_col);
-    if (a->score_blocks > 0 && n_s > 1 && b > 32)
+    if (ragged && n_s > 1 && b > 32)
       b = std::clamp<int64_t>(window_bps(p->desc, p->cus, nblk, (rows + 1) / 2, new_col), 32, 64);
     const int mult = b >= 64 && total >= 4 * n_slots * b ? 4 : 1;
     return prepare_attention_common(p, pool_store(p, block_tables, max_blocks), n_s, nblk,
@@ -1639,14 +1643,18 @@ int32_t prefix_way(const fmkv_pool* p, fmkv::PrefillArgs& pa, int64_t max_prefix
                    int64_t width) {
   if (pa.prefix.n_groups <= 0 || max_prefix < fmkv::kBlockTokens) return FMKV_PREFIX_ALONE;
   const int64_t H = p->desc.n_kv_heads, n = pa.n_seqs;
-  const double tiles_us = fmkv::prefix_plan(pa, p->cus, max_prefix);
+  double tiles_us = fmkv::prefix_plan(pa, p->cus, max_prefix);
   // rows of eight: their plan, as of equal sequences of the prefixes' length
   const int64_t qp = 8 / pa.group, groups = std::min<int64_t>(pa.prefix.n_groups, n);
   const int64_t rows = (n + groups * (qp - 1)) / qp;
   auto blocks_us = [&](double blocks, double rate) {
     return blocks / fmkv::kBlockTokens * (double)(H * p->layout.block_bytes) / rate;
   };
-  const double alone_us = 14.0 + blocks_us((double)n * (double)(max_prefix + max_rest), 1e7);
+  // (its fixed part is of calls with few tokens behind the prefixes)
+  tiles_us += blocks_us((double)n * (double)std::max<int64_t>(max_rest - 320, 0), 8e6);
+  // (a head-block takes what its products do where it has few bytes)
+  const double alone_rate = std::min(1e7, (double)p->layout.block_bytes / (2.6e-6 * p->desc.head_dim));
+  const double alone_us = 14.0 + blocks_us((double)n * (double)(max_prefix + max_rest), alone_rate);
   const double rows_us = 20.0 + blocks_us((double)rows * (double)max_prefix + (double)n * (double)max_rest, 8e6);
   int32_t way = g_prefix_way;
   if (way == FMKV_PREFIX_ROWS && n + rows > 65535) way = FMKV_PREFIX_ALONE;  // (the grid's y)
@@ -1721,9 +1729,11 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
   fmkv::AttnArgs at;
   if (shared) at.prefix = pa.prefix;
   at.n_seqs = n_seqs;
+  // (sequences that mostly read a common prefix are much alike)
+  const bool ragged = shared || n_groups >= n_seqs || n_groups == 0 || max_rest_len > max_prefix_len / 2;
   const int32_t bound = shared ? max_rest_len : (int32_t)std::min<int64_t>((int64_t)max_prefix_len + max_rest_len, width);
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, bound,
-                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
+                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0, ragged);
   if (rc) return rc;
   if (step) {
     at.k_new = ap.k;
@@ -1763,7 +1773,7 @@ int weighing_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, 
   fmkv::AttnArgs at;
   at.score_blocks = std::max<int64_t>(((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens, 1);
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, max_seq_len,
-                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0);
+                               n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0, true);
   if (rc || n_seqs == 0) return rc;
   // (before anything is launched: the merge's work-groups and the weights', in one grid)
   if (((int64_t)(p->desc.head_dim / 64) * n_q_heads + (at.score_blocks + 15) / 16) * n_seqs > (1 << 24) - 1)
