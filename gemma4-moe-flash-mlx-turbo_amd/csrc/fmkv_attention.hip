@@ -905,7 +905,9 @@ void decode_attn_kernel(const uint8_t* base, const uint16_t* q, int32_t geo_len,
         if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if constexpr (TILES) vis = tile_sees(tr, wg, a.sinks, ex_slot, slot);
-        if (!vis) {
+        if constexpr (TILES) {
+          s[i] = vis ? s[i] : -INFINITY;
+        } else if (!vis) {
           s[i] = -INFINITY;
           m[i] = 0;
         }

@@ -12,7 +12,7 @@
 // A work-group holds 64 rows (64 / G consecutive queries of a KV head's G heads) as
 // matrix-core operands in LDS, rotated in a launch of their own where they are many (four
 // prompts of 700 .. 8000 positions, 33 queries, 8 bits, 2 heads of 512 dims: 99.8 us a call with the
-// rotation in each work-group, 78.7 without); its waves take different keys, NB blocks of 16 a step,
+// rotation in each work-group, 77.6 without); its waves take different keys, NB blocks of 16 a step,
 // straight from memory to registers, where a code is turned into an operand once
 // for all rows. Nothing is exchanged between the waves while they run. Over the
 // 64-dim groups of a step the scores of the 64 rows with the step's keys stay in
@@ -20,6 +20,12 @@
 //
 // Operands as in prefill (fmkv_prefill.hip): K codes (or centroids) exact, q_rot as
 // an f16 high part and residual; plain caches bf16 as stored.
+//
+// Bound by the issue of matrix and vector instructions, which hardly overlap in two waves a
+// SIMD (128 queries of 16 heads over 32768 keys, 4 bits, 8 heads of 256 dims: 79.5 us a launch, 0.86
+// PFLOP/s on the matrix cores, busy 48% of the cycles, vector issue about 38%); calls of few steps by their first
+// loads and last merges. Priorities of waves, a later start for half of them, and one tile's products
+// under the scales of the one before changed nothing.
 //
 // In the second launch a lane's sums over its rows of the weights of its keys stay in
 // registers until all rows are done; 16 lanes meet at the end. Every sum has one

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
         if (!windowed(MODE) && ring_trim)
           vis = vis && slot_position(slot, T, a.window) >= a.vis_begin;
         if constexpr (TILES) vis = tile_sees(tr, wg, a.sinks, ex_slot, slot);
-        if (!vis) s4[r] = -INFINITY;
+        s4[r] = vis ? s4[r] : -INFINITY;
         seen[r >> 1] |= vis ? 0xffffu << 16 * (r & 1) : 0u;
       }
       // a hidden token's weight is 0, but its V row may be anything, and 0 * inf is NaN

@@ -19,6 +19,8 @@ constexpr int kWeighHeads = 64;     // query heads whose M and 1 / L are held at
 // The split merge, and the weights: grid x counts the merge's work-groups (64
 // dims, q head, sequence), then n_parts of 256 positions for each sequence. A position is
 // one thread's, which adds its heads up in order: no atomics, the same sum each time.
+// (32 sequences of 512 .. 16384 positions, 16 heads of 256 dims: 10.2 us, where the merge alone
+// takes 5; the stores of the scores cost the split kernel 10 us of its 100.)
 template <int D>
 __global__ __launch_bounds__(kWeighThreads) void combine_weigh_kernel(AttnArgs a, uint32_t flags,
                                                                       int n_seqs, int n_parts) {
@@ -289,7 +291,8 @@ __device__ inline void keep_heaviest(const float* w, int64_t n, uint32_t need, K
   });
 }
 
-// One work-group per sequence. Of T > max_keep positions the first `sinks` and the
+// One work-group per sequence: bound by its chain of loads, histogram, parting and
+// barriers (one of 5003 positions 8.8 us, 32 of 512 .. 16384 15.2). Of T > max_keep positions the first `sinks` and the
 // last `recent` stay, and as many of the others, the heaviest, as make max_keep.
 __global__ __launch_bounds__(kKeepThreads) void heaviest_kernel(HeaviestArgs a) {
   __shared__ KeepShared sh;
