@@ -474,8 +474,10 @@ int fmkv_paged_weighing_decode_step(fmkv_pool* pool, const void* k_bf16, const v
  * attention is returned (fmkv_paged_prefill_step and the windowed calls give it).
  * q: bf16 [n_seqs][n_new][n_q_heads][head_dim]. max_seq_len bounds start_pos + n_new.
  * Queries at positions below 0 (a padded row's) add nothing. At most 8 query heads per KV
- * head, every cache mode. The current GPU has to be the pool's; for calls on several
- * streams, and graphs, see the windowed calls above. */
+ * head, every cache mode. Needs the pool's workspace: 4 bytes for each element of q
+ * (quantized caches), and up to 2 KiB for each position of max_seq_len (4 bytes per
+ * sequence and KV head where those are more than 512). The current GPU has to be the
+ * pool's; for calls on several streams, and graphs, see the windowed calls above. */
 int fmkv_paged_attention_weights(fmkv_pool* pool, const void* q_bf16, const int32_t* block_tables,
                                  int32_t max_blocks, const int32_t* start_pos, int32_t n_seqs,
                                  int32_t n_new, int32_t max_seq_len, const float* weights,
