@@ -1853,14 +1853,16 @@ int fmkv_paged_attention_weights(fmkv_pool* p, const void* q, const int32_t* blo
     return fail(FMKV_ERR_INVALID_ARG, "max_seq_len exceeds max_blocks * 16");
   int rc = check_weights(n_seqs, max_seq_len, weights, weights_out, weights_width);
   if (rc) return rc;
-  if (n_seqs == 0 || n_new == 0) return FMKV_OK;
-  // (the output's place is taken by the weights)
-  if ((rc = check_attn_args(p->desc, q, n_q_heads, 0.0f, weights_out, FMKV_DTYPE_F32))) return rc;
+  if (n_seqs == 0) return FMKV_OK;
+  // (the output's place is taken by the weights; no queries need no address)
+  if ((rc = check_attn_args(p->desc, n_new == 0 ? weights_out : q, n_q_heads, 0.0f, weights_out, FMKV_DTYPE_F32)))
+    return rc;
   if ((int64_t)n_new > (int64_t)65535 * (64 / (n_q_heads / p->desc.n_kv_heads)))
     return fail(FMKV_ERR_INVALID_ARG, "n_new must be at most 65535 * (64 / query heads per KV head)");
   if (!block_tables || !start_pos) return fail(FMKV_ERR_INVALID_ARG, "block_tables/start_pos are null");
   if ((uintptr_t)q % 2 != 0) return fail(FMKV_ERR_UNSUPPORTED, "q must be 2-byte aligned");
   if ((rc = check_device(p))) return rc;
+  if (n_new == 0 && weights == weights_out) return FMKV_OK;  // (nothing is added)
   fmkv::ObserveArgs a;
   a.st = pool_store(p, block_tables, max_blocks);
   a.start_pos = start_pos;
@@ -1873,14 +1875,16 @@ int fmkv_paged_attention_weights(fmkv_pool* p, const void* q, const int32_t* blo
   std::memcpy(a.sign_bits, p->sign_bits, sizeof(a.sign_bits));
   a.c = p->c;
   a.blocks = (int32_t)std::max<int64_t>(((int64_t)max_seq_len + fmkv::kBlockTokens - 1) / fmkv::kBlockTokens, 1);
-  const size_t floats = fmkv::observe_plan(a, p->cus);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  RelaxedCapture relaxed;  // (the workspace may grow)
-  p->ws.captured = is_captured(s);
-  if ((rc = p->ws.ensure(floats * sizeof(float)))) return rc;
-  a.rows = reinterpret_cast<uint8_t*>(p->ws.ptr);
-  a.ml = p->ws.ptr + a.images;
-  a.part = p->ws.ptr + floats - (size_t)n_seqs * p->desc.n_kv_heads * a.sharers * a.part_width;
+  if (n_new > 0) {
+    const size_t floats = fmkv::observe_plan(a, p->cus);
+    RelaxedCapture relaxed;  // (the workspace may grow)
+    p->ws.captured = is_captured(s);
+    if ((rc = p->ws.ensure(floats * sizeof(float)))) return rc;
+    a.rows = reinterpret_cast<uint8_t*>(p->ws.ptr);
+    a.ml = p->ws.ptr + a.images;
+    a.part = p->ws.ptr + floats - (size_t)n_seqs * p->desc.n_kv_heads * a.sharers * a.part_width;
+  }
   a.weights_in = weights;
   a.weights_out = weights_out;
   a.weights_width = weights_width;

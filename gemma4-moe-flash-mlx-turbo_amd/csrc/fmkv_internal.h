@@ -346,12 +346,13 @@ struct ObserveArgs {
   int32_t blocks;     // the longest sequence's blocks
   // the plan: blocks of a wave's step, ranges of keys, tiles of a KV head, the
   // work-groups that share them
-  int32_t step_blocks, ranges, tiles, sharers;
-  int64_t images;  // floats of the rows' operands where they get a launch of their own
-  uint8_t* rows;   // those, [n_seqs][n_kv_heads][tiles]
-  float* ml;    // [n_seqs][n_kv_heads][tiles][64][ranges] (m, l)
-  float* part;  // [n_seqs][n_kv_heads * sharers][part_width] sums of weights
-  int64_t part_width;
+  // (no queries: none of it, and no partials to add)
+  int32_t step_blocks = 0, ranges = 0, tiles = 0, sharers = 0;
+  int64_t images = 0;       // floats of the rows' operands where they get a launch of their own
+  uint8_t* rows = nullptr;  // those, [n_seqs][n_kv_heads][tiles]
+  float* ml = nullptr;      // [n_seqs][n_kv_heads][tiles][64][ranges] (m, l)
+  float* part = nullptr;    // [n_seqs][n_kv_heads * sharers][part_width] sums of weights
+  int64_t part_width = 0;
   const float* weights_in;
   float* weights_out;
   int64_t weights_width;
@@ -401,7 +402,7 @@ hipError_t launch_shared_merge(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The same and the accumulated weights (a.scores), fmkv_weights.hip.
 hipError_t launch_combine_weigh(const AttnArgs& a, int n_seqs, hipStream_t s);
 // The plan of an ObserveArgs on a GPU of `cus` CUs, and the floats of its
-// workspace (ml, then part).
+// workspace (the rows' operands, ml, then part).
 size_t observe_plan(ObserveArgs& a, int cus);
 hipError_t launch_observe(const ObserveArgs& a, hipStream_t s);
 // The kept positions of n_seqs sequences (fmkv_weights.hip).

@@ -666,6 +666,12 @@ __global__ __launch_bounds__(256) void observe_sum_kernel(ObserveArgs a) {
   a.weights_out[at] = (a.weights_in ? a.weights_in[at] : 0.0f) + sum;
 }
 
+hipError_t launch_sum(const ObserveArgs& a, hipStream_t s) {
+  const int64_t keys = (int64_t)a.blocks * kBlockTokens;
+  hipLaunchKernelGGL(observe_sum_kernel, dim3((unsigned)((keys + 255) / 256), a.n_seqs), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 template <int D, int BITS, int MODE, int RT, int NB>
 hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
   const dim3 grid(a.ranges, a.st.n_kv_heads * a.sharers, a.n_seqs), block(ObPlan<D, BITS, MODE, RT>::NW * 64);
@@ -680,9 +686,7 @@ hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((observe_kernel<D, BITS, MODE, RT, NB, true>), grid, block, 0, s, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int64_t keys = (int64_t)a.blocks * kBlockTokens;
-  hipLaunchKernelGGL(observe_sum_kernel, dim3((unsigned)((keys + 255) / 256), a.n_seqs), dim3(256), 0, s, a);
-  return hipGetLastError();
+  return launch_sum(a, s);
 }
 template <int D, int BITS, int MODE>
 hipError_t launch_ob(const ObserveArgs& a, hipStream_t s) {
@@ -720,6 +724,7 @@ size_t observe_plan(ObserveArgs& a, int cus) {
 }
 
 hipError_t launch_observe(const ObserveArgs& a, hipStream_t s) {
+  if (a.n_q == 0) return launch_sum(a, s);  // (of no partials: the weights as they were)
   const BlockLayout& L = a.st.layout;
   if (L.mode == kAffine) {
     switch (L.head_dim * 16 + L.bits) {

@@ -473,7 +473,8 @@ int fmkv_paged_weighing_decode_step(fmkv_pool* pool, const void* k_bf16, const v
  * the positions j <= p), whose keys are in the pool already. V is not read, and no
  * attention is returned (fmkv_paged_prefill_step and the windowed calls give it).
  * q: bf16 [n_seqs][n_new][n_q_heads][head_dim]. max_seq_len bounds start_pos + n_new.
- * Queries at positions below 0 (a padded row's) add nothing. At most 8 query heads per KV
+ * Queries at positions below 0 (a padded row's) add nothing, and n_new 0 stores
+ * `weights` alone, of the positions j < start_pos (q may be NULL then). At most 8 query heads per KV
  * head, every cache mode. Needs the pool's workspace: 4 bytes for each element of q
  * (quantized caches), and up to 2 KiB for each position of max_seq_len (4 bytes per
  * sequence and KV head where those are more than 512). The current GPU has to be the

@@ -96,6 +96,31 @@ def test_hidden_keys(gpu, ora, mode, bits, D, Hkv, Hq):
     assert torch.equal(got, want) and bool(torch.isfinite(got).all())
 
 
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[2], FORMS[8]])
+def test_no_queries(gpu, ora, mode, bits, D, Hkv, Hq):
+    """An empty chunk adds nothing: what was accumulated, or zeros, of the positions
+    before it, in a buffer that holds something else, and in place."""
+    import torch
+
+    lens = [300, 17, 0, 9]
+    b = Paged(gpu, ora, mode, D, bits, Hkv, lens, seed=3)
+    q = torch.empty((4, 0, Hq, D), dtype=torch.bfloat16, device="cuda")
+    start = b.lens_dev([300, 17, 0, -2])
+    seen = [300, 17, 0, 0]
+    old = torch.rand((4, 303), generator=torch.Generator().manual_seed(1)).cuda()
+    sums = torch.full((4, 303), 7.0, device="cuda")
+    assert b.pool.attention_weights(q, b.table(), start, 300, old, weights_out=sums) is sums
+    for s, t in enumerate(seen):
+        assert torch.equal(sums[s, :t], old[s, :t]) and bool((sums[s, t:] == 7.0).all())
+    sums.fill_(7.0)
+    b.pool.attention_weights(q, b.table(), start, 300, weights_out=sums)
+    for s, t in enumerate(seen):
+        assert not sums[s, :t].any() and bool((sums[s, t:] == 7.0).all())
+    same = old.clone()
+    assert b.pool.attention_weights(q, b.table(), start, 300, same) is same
+    assert torch.equal(same, old)
+
+
 def test_graph(gpu, ora):
     import torch
 
