@@ -1908,7 +1908,8 @@ int fmkv_heaviest_tokens(const float* weights, int32_t weights_width, const int3
   if (!weights || !seq_lens || !keep || !n_keep)
     return fail(FMKV_ERR_INVALID_ARG, "weights/seq_lens/keep/n_keep are null");
   if (kept_weights) {
-    if (kept_width < max_keep) return fail(FMKV_ERR_INVALID_ARG, "kept_width must be at least max_keep");
+    if (kept_width < max_keep || kept_width > (1 << 30))
+      return fail(FMKV_ERR_INVALID_ARG, "kept_width must be in [max_keep, 2^30]");
     if (overlaps(weights, (int64_t)n_seqs * weights_width * 4, kept_weights, (int64_t)n_seqs * kept_width * 4))
       return fail(FMKV_ERR_INVALID_ARG, "kept_weights overlaps weights");
   }

@@ -39,6 +39,15 @@ def test_heaviest_tokens_refuses(change):
     assert rc == BAD
 
 
+@pytest.mark.parametrize("width", [(1 << 30) + 1, 2 ** 31 - 1])
+def test_heaviest_tokens_refuses_wide_outputs(width):
+    """Past the documented width (an output that is the weights: refused in any case)."""
+    lib, a = fmkv.load_library(), HEAVIEST
+    args = (a["weights"], a["width"], a["lens"], a["n"], a["most"], a["sinks"], a["recent"], a["keep"], a["n_keep"])
+    assert lib.fmkv_heaviest_tokens(*args, a["weights"], width, None) == BAD
+    assert b"kept_width" in lib.fmkv_last_error()
+
+
 def test_heaviest_tokens_of_nothing():
     lib = fmkv.load_library()
     assert lib.fmkv_heaviest_tokens(None, 64, None, 0, 16, 2, 4, None, None, None, 0, None) == fmkv.FMKV_OK
