@@ -44,10 +44,11 @@ namespace {
 constexpr int kObRows = 64;
 constexpr float kObSlack = 8.0f;  // (base 2) a score may exceed its row's reference by
 
-// A power of 2 of the codes' offset that goes to the scales it is multiplied with,
-// so that neither that nor the sums of q times the rest leave f16.
-template <int BITS>
-constexpr float kScaleUp = BITS == 8 ? 64.0f : 1.0f;
+// Affine caches hold q_rot, its sums over 64 dims and those times the codes' offset as f16
+// operands (q_rot times kCodeScale). A row in which one of them would come near f16's largest
+// value, 65504 (|q_rot| or a sixteenth of a sum's offset part past 4000), is held as so much less by a power of 2,
+// and its scores are multiplied back in f32: a row of any size has finite operands.
+constexpr float kObMost = 4000.0f;
 
 // Blocks of a wave's step in calls of many keys: what the registers hold.
 constexpr int many_blocks(int mode) { return mode == kAffine ? 3 : 4; }
@@ -72,6 +73,8 @@ struct ObPlan {
   static constexpr int kLut = MODE == kCodebook ? CbLut<BITS == 16 ? 2 : BITS>::kBytes : 16;
   // A tile's operands in memory, as a launch of their own leaves them: 1 KiB each, the biases' last.
   static constexpr int kPieces = kOperands + (MODE == kAffine ? RT : 0);
+  // The powers of 2 of the rows behind them.
+  static constexpr int kTile = kPieces * 1024 + (MODE == kAffine ? kObRows * 4 : 0);
 };
 
 // Calls of more than 16 rows rotate them in a launch of their own, which every range
@@ -100,21 +103,42 @@ __device__ inline ObSeq ob_seq(const ObserveArgs& a, int seq) {
 }
 
 // Row r of a tile, rotated but for the signs (x: the lane's D / 64 dims), as its places
-// in the operands: at `ops`, OP bytes apart, and `sums`.
+// in the operands: at `ops`, OP bytes apart, and `sums`. ups: the rows' powers of 2 (affine).
 template <int D, int BITS, int MODE, int RT, int OP>
-__device__ inline void store_row(const float (&x)[D / 64], uint8_t* ops, uint8_t* sums, int r, int lane,
-                                 uint32_t sbits, float cs_lane) {
+__device__ inline void store_row(const float (&x)[D / 64], uint8_t* ops, uint8_t* sums, float* ups, int r,
+                                 int lane, uint32_t sbits, float cs_lane) {
   using P = ObPlan<D, BITS, MODE, RT>;
   constexpr int E = P::E, LPG = 64 / E;  // lanes of a 64-dim group
   const int rt = r >> 4, rc = r & 15, d0 = lane * E, o = d0 & 63;
-  float gs = 0.0f;
+  float gs = 0.0f, v[E];
   _Float16 hv[E], lv[E];
 #pragma unroll
   for (int i = 0; i < E; i++) {
-    const float v = apply_sign(x[i] * cs_lane, sbits, i);
-    gs += v;
-    hv[i] = (_Float16)v;
-    lv[i] = (_Float16)(v - (float)hv[i]);
+    v[i] = apply_sign(x[i] * cs_lane, sbits, i);
+    gs += v[i];
+  }
+  if constexpr (MODE == kAffine) {
+    gs = group_sum<LPG>(gs, lane);
+    float most = fabsf(gs) * (kCodeOffset<BITS> / 16.0f), up = 1.0f;
+#pragma unroll
+    for (int i = 0; i < E; i++) most = fmaxf(most, fabsf(v[i]));
+    if (__any(most > kObMost)) {
+      most = group_max<64>(most, lane);
+      if (most < INFINITY) {  // to [2^10, 2^11)
+        const uint32_t e = (__float_as_uint(most) >> 23) - 127u - 10u;
+        const float down = __uint_as_float((127u - e) << 23);
+        up = __uint_as_float((127u + e) << 23);
+        gs *= down;
+#pragma unroll
+        for (int i = 0; i < E; i++) v[i] *= down;
+      }
+    }
+    if (lane == 0) ups[r] = up;
+  }
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    hv[i] = (_Float16)v[i];
+    lv[i] = (_Float16)(v[i] - (float)hv[i]);
     if constexpr (MODE == kAffine) {  // (exact)
       hv[i] = hv[i] * (_Float16)kCodeScale<BITS>;
       lv[i] = lv[i] * (_Float16)kCodeScale<BITS>;
@@ -128,12 +152,11 @@ __device__ inline void store_row(const float (&x)[D / 64], uint8_t* ops, uint8_t
   store_halves<E>(p + P::index(0, rt, 2 * g + s) * OP, hv);
   store_halves<E>(p + P::index(1, rt, 2 * g + s) * OP, lv);
   if constexpr (MODE == kAffine) {
-    gs = group_sum<LPG>(gs, lane);
     if ((lane & (LPG - 1)) == 0) {
       // sums of 64 dims, high parts and residuals, against the biases; and
       // the sums that the codes' offset adds, against the scales
       _Float16* q = reinterpret_cast<_Float16*>(sums + rt * 1024) + rc * 8 + g;
-      const float off = gs * (-kCodeOffset<BITS> / kScaleUp<BITS>);
+      const float off = gs * -kCodeOffset<BITS>;
       const _Float16 h = (_Float16)gs, ho = (_Float16)off;
       q[0] = h;
       q[16 * 8] = (_Float16)(gs - (float)h);
@@ -155,8 +178,9 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
   const int tile = blockIdx.x / RT, rt = blockIdx.x % RT, kvh = blockIdx.y, seq = blockIdx.z;
   const int G = a.group, QP = kObRows / G, qi0 = tile * QP;
   const int rows = (a.n_q - qi0 < QP ? a.n_q - qi0 : QP) * G;
-  uint8_t* const ops = a.rows + (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * (P::kPieces * 1024);
+  uint8_t* const ops = a.rows + (((int64_t)seq * a.st.n_kv_heads + kvh) * a.tiles + tile) * P::kTile;
   uint8_t* const sums = ops + P::kOperands * 1024;
+  float* const ups = reinterpret_cast<float*>(ops + P::kPieces * 1024);
   const uint32_t sbits = lane_sign_bits<D>(a.sign_bits, lane);
   const float cs_lane = fwht_lane_sign(lane) * a.c;
   const int r0 = rt * 16 + wave * 4;
@@ -177,7 +201,7 @@ __global__ __launch_bounds__(256) void observe_rows_kernel(ObserveArgs a) {
       x[2 * i + 1] = __uint_as_float(w & 0xffff0000u) * a.qscale;
     }
     wave_fwht_signed<E>(x, lane);
-    store_row<D, BITS, MODE, RT, 1024>(x, ops, sums, r0 + k, lane, sbits, cs_lane);
+    store_row<D, BITS, MODE, RT, 1024>(x, ops, sums, ups, r0 + k, lane, sbits, cs_lane);
     if (MODE == kAffine && NG < 8 && lane < 4 * (8 - NG))  // (groups that the dims do not have)
       reinterpret_cast<_Float16*>(sums + rt * 1024)[(lane & 3) * 128 + ((r0 + k) & 15) * 8 + NG + (lane >> 2)] =
           (_Float16)0.0f;
@@ -193,11 +217,11 @@ void observe_kernel(ObserveArgs a) {
   using P = ObPlan<D, BITS, MODE, RT>;
   constexpr BlockLayout L = P::L;
   constexpr int NG = P::NG, NW = P::NW, E = P::E, KW = P::KW;
-  constexpr int LPG = 64 / E;  // lanes of a 64-dim group
   constexpr int CB = MODE == kCodebook ? BITS : 2;
   __shared__ __align__(16) uint8_t rows_s[P::kRows];
   __shared__ __align__(16) uint8_t lut[P::kLut];
   __shared__ int row_pos[RT * 16];
+  __shared__ float row_up[MODE == kAffine ? RT * 16 : 1];
   __shared__ float2 stat[SUMS ? 1 : NW][RT * 16];  // (m, l) of the waves; SUMS: M, 1 / L
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -316,8 +340,11 @@ void observe_kernel(ObserveArgs a) {
     load(bp, 0, cur);
     load_bias(bp, bias);
 
+    float up = 1.0f;
     if constexpr (kObRotated<MODE, RT>) {
-      const u32x4 rs = buffer_rsrc(a.rows + ml_row / kObRows * (P::kPieces * 1024), P::kPieces * 1024);
+      const uint8_t* image = a.rows + ml_row / kObRows * P::kTile;
+      if (MODE == kAffine && tid < RT * 16) up = reinterpret_cast<const float*>(image + P::kPieces * 1024)[tid];
+      const u32x4 rs = buffer_rsrc(image, P::kPieces * 1024);
       const uint32_t to = lds_addr(rows_s);
 #pragma unroll 1
       for (int o = wave; o < P::kPieces; o += NW)
@@ -347,6 +374,7 @@ void observe_kernel(ObserveArgs a) {
       }
     }
     if constexpr (kObRotated<MODE, RT>) {
+      if (MODE == kAffine && tid < RT * 16) row_up[tid] = up;
       wait_vmcnt<0>();
     } else {
       // Four rows of a wave at a time, the next four on their way meanwhile
@@ -390,12 +418,15 @@ void observe_kernel(ObserveArgs a) {
 #pragma unroll
             for (int i = 0; i < E / 2; i++) reinterpret_cast<uint32_t*>(p)[i] = raw[k][i];
           } else {
-            store_row<D, BITS, MODE, RT, P::kStride>(x[k], rows_s, rows_s + P::kSums, r, lane, sbits, cs_lane);
+            store_row<D, BITS, MODE, RT, P::kStride>(x[k], rows_s, rows_s + P::kSums, row_up, r, lane, sbits,
+                                                        cs_lane);
           }
         }
       }
-      }
+    }
     __syncthreads();
+    // (kObMost; any row of the tile)
+    const bool scaled = MODE == kAffine && __any(row_up[lane & (RT * 16 - 1)] != 1.0f);
 
     int p_row[RT];
     float m_run[RT], l_run[RT];  // SUMS: M and 1 / L of the lane's rows
@@ -408,6 +439,7 @@ void observe_kernel(ObserveArgs a) {
         const float2 x = stat[0][rt * 16 + c];
         m_run[rt] = x.x;
         l_run[rt] = x.y;
+        if (scaled) m_run[rt] /= row_up[rt * 16 + c];
       }
     }
 
@@ -450,7 +482,7 @@ void observe_kernel(ObserveArgs a) {
         half8_t kb{};
         if constexpr (MODE == kAffine) {
 #pragma unroll
-          for (int g = 0; g < 8; g++) kb[g] = bias[b][g] * (j < 2 ? (_Float16)1.0f : (_Float16)kScaleUp<BITS>);
+          for (int g = 0; g < 8; g++) kb[g] = bias[b][g];
         }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
@@ -459,7 +491,7 @@ void observe_kernel(ObserveArgs a) {
           if constexpr (MODE == kAffine) {
             const half8_t qb = *reinterpret_cast<const half8_t*>(rows_s + P::kSums + rt * 1024 + lane * 16);
             s[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qb, s[rt][b], 0, 0, 0);
-              __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
@@ -555,6 +587,13 @@ void observe_kernel(ObserveArgs a) {
 #pragma unroll
       for (int b = 0; b < NB; b++) bp[b] = bn[b];
       load_bias(bp, bias);
+
+      if (MODE == kAffine && scaled) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int b = 0; b < NB; b++) s[rt][b] *= row_up[rt * 16 + c];
+      }
 
       // ---- softmax: lane (j, c) has keys 16 b + 4 j + i of rows 16 rt + c ----
       const bool full = key0 + NB * kBlockTokens - 1 <= p_first && rows == RT * 16 && p_first >= 0;
@@ -716,10 +755,10 @@ size_t observe_plan(ObserveArgs& a, int cus) {
   const int ragged = a.n_seqs > 2 ? 3 : 1;
   a.ranges = (int32_t)std::clamp<int64_t>(ragged * places / (per_tile * a.sharers), 1, steps);
   a.part_width = (int64_t)a.blocks * kBlockTokens;
-  // operands of a tile: high parts and residuals of 64 rows, and 4 KiB for the biases
+  // operands of a tile: high parts and residuals of 64 rows, 4 KiB for the biases and the powers of 2
   a.images = a.st.layout.mode == kPlain || a.n_q * a.group <= 16
                  ? 0
-                 : rows * (kObRows * a.st.layout.head_dim + (a.st.layout.mode == kAffine ? 1024 : 0));
+                 : rows * (kObRows * a.st.layout.head_dim + (a.st.layout.mode == kAffine ? 1024 + kObRows : 0));
   return (size_t)(a.images + rows * a.ranges * kObRows * 2 + per_tile * a.sharers * a.part_width);
 }
 

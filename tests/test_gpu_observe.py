@@ -96,6 +96,32 @@ def test_hidden_keys(gpu, ora, mode, bits, D, Hkv, Hq):
     assert torch.equal(got, want) and bool(torch.isfinite(got).all())
 
 
+@pytest.mark.parametrize("lens,n", [([300, 40], 2), ([400, 131], 45)], ids=str)
+@pytest.mark.parametrize("power", [7, 12, 16])
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [f for f in FORMS if f[0] == AFFINE] + [(AFFINE, 8, 512, 1, 7), FORMS[2], FORMS[8]])
+def test_large_queries(gpu, ora, mode, bits, D, Hkv, Hq, power, lens, n):
+    """Queries whose sums over 64 dims and offset parts f16 does not hold, beside ordinary
+    ones, over keys so much smaller: scores as everywhere else."""
+    import torch
+
+    b = Paged(gpu, ora, mode, D, bits, Hkv, lens, seed=2)
+    for s, t in enumerate(lens):  # the same keys, times 2^-power (exact: bits of bf16)
+        k, v = (fast_kv(10 * s + 2 + 5 * i, t, Hkv, D, outliers=False) for i in (0, 1))
+        k = np.where(k & 0x7f80, k - (power << 7), 0).astype(np.uint16)
+        b.oracles[s] = ora.OracleCache(Hkv, D, bits, 0, t + 1, mode=mode)
+        b.oracles[s].append(k, v)
+        b.pool.append(dev_bf16(k[None]), dev_bf16(v[None]), b.table(s),
+                      torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = np.stack([queries(50 + s, n, Hq, Hkv, D) for s in range(len(lens))])
+    large = np.arange(n) % 3 != 1
+    q[:, large] = np.where(q[:, large] & 0x7f80, q[:, large] + (power << 7), 0).astype(np.uint16)
+    want = [reference(ora, oc, q[s], t, D ** -0.5) for s, (oc, t) in enumerate(zip(b.oracles, lens))]
+    got = b.pool.attention_weights(dev_bf16(q), b.table(), b.lens_dev([t - n for t in lens]), max(lens),
+                                   scale=D ** -0.5)
+    for s, t in enumerate(lens):
+        check_weights(got[s, :t].double().cpu().numpy(), np.zeros(t), want[s], f"sequence {s}")
+
+
 @pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[2], FORMS[8]])
 def test_no_queries(gpu, ora, mode, bits, D, Hkv, Hq):
     """An empty chunk adds nothing: what was accumulated, or zeros, of the positions
