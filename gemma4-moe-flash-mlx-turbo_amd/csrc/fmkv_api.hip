@@ -1731,7 +1731,8 @@ int prefix_decode_impl(fmkv_pool* p, bool step, const void* k, const void* v, co
   at.n_seqs = n_seqs;
   // (sequences that mostly read a common prefix are much alike)
   const bool ragged = shared || n_groups >= n_seqs || n_groups == 0 || max_rest_len > max_prefix_len / 2;
-  const int32_t bound = shared ? max_rest_len : (int32_t)std::min<int64_t>((int64_t)max_prefix_len + max_rest_len, width);
+  const int32_t bound = shared ? max_rest_len
+                               : (int32_t)std::min({(int64_t)max_prefix_len + max_rest_len, width, (int64_t)INT32_MAX});
   rc = prepare_paged_attention(p, q, block_tables, max_blocks, seq_lens, n_seqs, bound,
                                n_q_heads, scale, 0.0f, out, out_dtype, step ? 1 : 0, s, &at, kNoWindow, 0, ragged);
   if (rc) return rc;

@@ -68,6 +68,22 @@ def test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch, way):
         check_window(out, want, big, f"{batch} {dtype} {bound}")
 
 
+def test_bounds_of_two_billion(gpu, ora):
+    """A batch that reads its own tables, wide enough for bounds whose sum 32 bits do not hold."""
+    import torch
+
+    b = Shared(gpu, ora, AFFINE, 128, 4, 1, [(40, [50])], seed=25)
+    q = queries(43, 1, 1, 1, 128)
+    tables, lens, prefix, starts, longest, rest = b.args()
+    wide = torch.zeros((1, 1 << 28), dtype=torch.int32, device="cuda")
+    wide[:, :tables.shape[1]] = tables
+    want = reference(ora, b, q, 128 ** -0.5)
+    for bounds in ((longest, rest), (2 ** 31 - 1, rest), (2 ** 31 - 1, 2 ** 31 - 1)):
+        out = b.pool.prefix_attention(dev_bf16(q), wide, lens, prefix, starts, *bounds, scale=128 ** -0.5,
+                                      dtype=torch.float32)
+        check_window(out, want, vmax(b), f"{bounds}")
+
+
 @every_way
 @pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [FORMS[0], FORMS[2], FORMS[7]])
 def test_more_groups_than_lanes(gpu, ora, mode, bits, D, Hkv, Hq, way):
