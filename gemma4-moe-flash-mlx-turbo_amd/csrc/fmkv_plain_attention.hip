@@ -327,8 +327,8 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
         for (int t = 0; t < TW; t++) cur.v[t].x &= seen[0], cur.v[t].y &= seen[1];
       }
       // kTiles: rows differ in what they see. Values that are not finite become 0, and
-      // infinite the accumulators of the rows that do see them: a product of ones
-      // counts how many of them a row sees, per dim.
+      // NaN the accumulators of the rows that do see them (which may be an infinity of
+      // either sign, or none): a product of ones counts how many of them a row sees, per dim.
       if constexpr (TILES) {
         auto bad_of = [](uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u; };
 #pragma unroll
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(kPlThreads) void plain_decode_kernel(AttnArgs a) {
               __builtin_bit_cast(short4_t, make_uint2(seen[0] & 0x3f803f80u, seen[1] & 0x3f803f80u)),
               (float4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; r++) o[t][r] = fmaf(n[r] * 0x1p127f, 0x1p127f, o[t][r]);
+          for (int r = 0; r < 4; r++) o[t][r] = fmaf(n[r] * 0x1p127f * 0x1p127f, 0.0f, o[t][r]);  // inf * 0, or 0
           cur.v[t].x &= ~(b0 * 0xffffu);
           cur.v[t].y &= ~(b1 * 0xffffu);
         }

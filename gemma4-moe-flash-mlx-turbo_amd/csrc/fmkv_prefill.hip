@@ -1024,8 +1024,8 @@ void prefill_attn_kernel(PrefillArgs a) {
 
   // V values (affine: scales and biases) that are not finite, in a step whose
   // keys some rows do not see: a hidden key's weight 0 makes NaN of them. They
-  // become 0, and infinite (or NaN) the accumulators of the rows that do see
-  // them. (In arithmetic without compares: their masks would crowd the scalar
+  // become 0, and NaN the accumulators of the rows that do see
+  // them: what those sum to is an infinity of either sign, or none. (In arithmetic without compares: their masks would crowd the scalar
   // registers of the whole kernel, and the loop ran up to 10% slower.)
   auto hide_not_finite = [&](int step) __attribute__((always_inline)) {
     // 1 in each half of w that is not finite: its exponent is all ones
@@ -1049,7 +1049,7 @@ void prefill_attn_kernel(PrefillArgs a) {
       return ~(uint32_t)((kp - vlo) | (vhi - 1 - kp)) >> 31;
     };
     auto poison = [](float x, float n) __attribute__((always_inline)) -> float {  // n = 0: x
-      return fmaf(n * 0x1p127f, 0x1p127f, x);
+      return fmaf(n * 0x1p127f * 0x1p127f, 0.0f, x);  // inf * 0
     };
     if constexpr (MODE == kPlain) {
 #pragma unroll

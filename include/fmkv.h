@@ -627,7 +627,8 @@ int fmkv_set_sparse_v_gather(int32_t on);
  * step): AUTO (the default) by estimates from a call's sizes; ALONE: every sequence
  * reads its own table's blocks; ROWS: eight rows (sequences times q heads per KV
  * head) at a time read a prefix once; TILES: 64 rows. Each gives the same
- * attention. No reference counterpart (a tuning and test switch). */
+ * attention (a row that sees a value that is not finite is not finite either: NaN, or the
+ * infinity that it makes). No reference counterpart (a tuning and test switch). */
 #define FMKV_PREFIX_AUTO 0
 #define FMKV_PREFIX_ALONE 1
 #define FMKV_PREFIX_ROWS 2

@@ -173,6 +173,68 @@ def test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, way):
     assert not torch.equal(after[0], before[0])  # (which sees them)
 
 
+def not_finite_but_where_the_formula_is(out, kind, what):
+    """out: results that a value of `kind` goes into: that infinity, or NaN."""
+    o = out.cpu().numpy()
+    assert not np.isfinite(o).any(), what
+    assert (np.isnan(o) | (o == kind)).all(), f"{what}: {o[~(np.isnan(o) | (o == kind))]}"
+
+
+@every_way
+@pytest.mark.parametrize("D,Hkv,Hq", [(128, 4, 8), (512, 1, 8), (256, 2, 6)])
+def test_values_that_are_not_finite(gpu, ora, D, Hkv, Hq, way):
+    """bf16 values of either sign that are not finite, in blocks that every row sees and
+    in ones that a member does not see whole: the members that see them have that
+    infinity or NaN in that dim, the others and the other dims what they had."""
+    import torch
+
+    b = Shared(gpu, ora, PLAIN, D, 16, Hkv, [(160, [180, 175, 160])], ((), (20,)), seed=7)
+    q = queries(13, 4, Hq, Hkv, D)
+    tables, lens, prefix, starts, longest, rest = b.args()
+    short = b.ints([180, 37, 160, 20])
+    args = (dev_bf16(q), tables, short, prefix, starts, longest, rest)
+    before = b.pool.prefix_attention(*args, scale=D ** -0.5, dtype=torch.float32)
+    st = b.pool.storage()
+    bad = {5: (-np.inf, 0xff80), 9: (np.nan, 0x7fc0), 11: (np.inf, 0x7f80), 70: (np.nan, 0xffff)}
+    for d, (_, bits) in bad.items():
+        token = 38 + d % 3  # (past the short member's, in the block that it sees in part)
+        o = 32 * D + d * 2 * TOKENS + 2 * (token % TOKENS)
+        block = st[int(b.tables[0, token // TOKENS])]
+        block[:, o], block[:, o + 1] = bits & 255, bits >> 8
+    after = b.pool.prefix_attention(*args, scale=D ** -0.5, dtype=torch.float32)
+    rest_dims = [d for d in range(D) if d not in bad]
+    assert torch.equal(after[3], before[3])
+    check_window(after[1:2], attend_reference(ora, b.oracles[1], q[1], 37, D ** -0.5)[0][None], vmax(b), "the short member")
+    for s in (0, 2):
+        assert torch.equal(after[s][:, rest_dims], before[s][:, rest_dims])
+        for d, (kind, _) in bad.items():
+            not_finite_but_where_the_formula_is(after[s, :, d], kind, f"sequence {s}, {kind}")
+
+
+@pytest.mark.parametrize("window", [0, 100])
+def test_prefill_values_that_are_not_finite(gpu, ora, window):
+    """The same of a chunk's queries."""
+    import torch
+
+    D, Hkv, Hq, prefix, n = 128, 2, 4, 20, 150
+    book = Shared(gpu, ora, PLAIN, D, 16, Hkv, [(0, [prefix + n])], seed=9)
+    q = dev_bf16(np.stack([queries(300 + i, 1, Hq, Hkv, D)[0] for i in range(n)])[None])
+    start = book.ints([prefix])
+    st = book.pool.storage()
+    for kind, bits in ((-np.inf, 0xff80), (np.nan, 0x7fc0), (np.inf, 0x7f80)):
+        token, d = 56, 7
+        o = 32 * D + d * 2 * TOKENS + 2 * (token % TOKENS)
+        block = st[int(book.tables[0, token // TOKENS])]
+        block[:, o], block[:, o + 1] = bits & 255, bits >> 8
+        out = book.pool.window_prefill(q, book.table(), start, window or 2 ** 30, scale=D ** -0.5, dtype=torch.float32)[0]
+        sees = np.arange(prefix, prefix + n)
+        sees = (sees >= token) & (sees < token + (window or 2 ** 30))
+        assert torch.isfinite(out[torch.from_numpy(~sees).cuda()]).all()
+        others = [x for x in range(D) if x != d]
+        assert torch.isfinite(out[:, :, others]).all()
+        not_finite_but_where_the_formula_is(out[torch.from_numpy(sees).cuda()][:, :, d], kind, f"{kind}")
+
+
 @every_way
 def test_graph_and_streams(gpu, ora, way):
     """A captured step replayed with eager calls between, on tensors of another
