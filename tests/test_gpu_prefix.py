@@ -236,6 +236,16 @@ def test_prefill_values_that_are_not_finite(gpu, ora, window):
 
 
 @every_way
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [(CODEBOOK, 4, 128, 2, 6), (CODEBOOK, 2, 256, 1, 3), (CODEBOOK, 2, 512, 1, 2)])
+def test_other_codebooks(gpu, ora, mode, bits, D, Hkv, Hq, way):
+    """The widths that are not among the forms above, over slots full of NaNs."""
+    for batch in BATCHES:
+        test_attention(gpu, ora, mode, bits, D, Hkv, Hq, batch, way)
+    test_step(gpu, ora, mode, bits, D, Hkv, Hq, way)
+    test_hidden_slots(gpu, ora, mode, bits, D, Hkv, Hq, way)
+
+
+@every_way
 def test_graph_and_streams(gpu, ora, way):
     """A captured step replayed with eager calls between, on tensors of another
     stream; the same bits each time."""

@@ -97,6 +97,14 @@ def test_weighing_step(gpu, ora, mode, bits, D, Hkv, Hq):
         check_codes(codes[slots], meta[slots], b.oracles[s], slots=at, what=f"sequence {s}")
 
 
+@pytest.mark.parametrize("mode,bits,D,Hkv,Hq", [(CODEBOOK, 4, 128, 2, 6), (CODEBOOK, 2, 256, 1, 8), (CODEBOOK, 3, 512, 1, 4)])
+def test_weighing_other_codebooks(gpu, ora, mode, bits, D, Hkv, Hq):
+    """The widths that are not among the forms above, over slots full of NaNs."""
+    for lens in LENS:
+        test_weighing_attention(gpu, ora, mode, bits, D, Hkv, Hq, lens)
+    test_weighing_step(gpu, ora, mode, bits, D, Hkv, Hq)
+
+
 def test_weighing_graph(gpu, ora):
     """A captured call replayed with eager ones between: each replay adds the same."""
     import torch
