@@ -862,9 +862,11 @@ int prepare_paged_attention(fmkv_pool* p, const void* q, const int32_t* block_ta
   if (win == kNoWindow) {
     // Lengths that nothing makes alike (`ragged`: not those of sequences that mostly read a
     // common prefix): where splits come out long, sequences count half of the longest, at most
-    // 64 blocks a split, and first splits of four times that as above. (Scores stored, seven of 65 ..
-    // 20011 tokens, 8 bits, 2 heads of 512 dims: 35 blocks 33.5 us, the longest's
-    // plan, 68 and 64 blocks, 42.5 and 40.6, 24: 44.3; 32 of 512 .. 16384, 4 bits, 8
+    // 64 blocks a split, and first splits of four times that as above. (us of calls on the same
+    // inputs again. Scores stored, seven of 65 ..
+    // 20011 tokens, 8 bits, 2 heads of 512 dims: 35 blocks 32.9, the longest's
+    // plan, 68 and 64 blocks, 42.5 and 40.6, 24: 44.3; all of 20011 tokens lose by it: 76.5, where the
+    // longest's plan takes 59 without the scores; 32 of 512 .. 16384, 4 bits, 8
     // heads of 256 dims: 64 blocks, first splits four times that, 106; 171: 163. In groups of
     // one, 32 of up to 16000: 76 so, 145 as of equal ones; 16 of 1000 .. 13000, 8 bits, 2
     // heads of 512 dims: 62 and 53. What 41 sequences have behind

@@ -128,10 +128,7 @@ __device__ inline int64_t tile_part_row(const AttnArgs& a, const TileRows& r, in
 __device__ inline WinGeom tile_window(const AttnArgs& a, const TileRows& r) {
   return r.tile ? win_geometry(r.T, r.T, 0, a.st.table_stride) : attn_window(a, r.seq, r.T);
 }
-// Whether the lane's row sees `slot`, without a branch: where the lanes of a
-// wave differ, `if (!vis) { s[i] = -inf; v[i] = 0; }` after short-circuit tests
-// was compiled to an empty branch (the hidden value lost) in the codebook
-// kernel's 2- and 3-bit forms; selects on this are not.
+// Whether the lane's row sees `slot`, for selects: the rows of a wave differ in it.
 __device__ inline bool tile_sees(const TileRows& r, const WinGeom& g, int64_t sinks, int64_t ex_slot,
                                  int64_t slot) {
   return ((slot >= g.lo) | (slot < sinks)) & (slot < r.row_end) & (slot != ex_slot);

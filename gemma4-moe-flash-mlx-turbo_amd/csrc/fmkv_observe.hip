@@ -12,7 +12,7 @@
 // A work-group holds 64 rows (64 / G consecutive queries of a KV head's G heads) as
 // matrix-core operands in LDS, rotated in a launch of their own where they are many (four
 // prompts of 700 .. 8000 positions, 33 queries, 8 bits, 2 heads of 512 dims: 99.8 us a call with the
-// rotation in each work-group, 77.6 without); its waves take different keys, NB blocks of 16 a step,
+// rotation in each work-group, 78.4 without); its waves take different keys, NB blocks of 16 a step,
 // straight from memory to registers, where a code is turned into an operand once
 // for all rows. Nothing is exchanged between the waves while they run. Over the
 // 64-dim groups of a step the scores of the 64 rows with the step's keys stay in
@@ -23,7 +23,7 @@
 //
 // Bound by the issue of matrix and vector instructions, which hardly overlap in two waves a
 // SIMD (128 queries of 16 heads over 32768 keys, 4 bits, 8 heads of 256 dims: 79.5 us a launch, 0.86
-// PFLOP/s on the matrix cores, busy 48% of the cycles, vector issue about 38%); calls of few steps by their first
+// PFLOP/s on the matrix cores, busy 48% of the cycles, vector issue 39% and 36%); calls of few steps by their first
 // loads and last merges. Priorities of waves, a later start for half of them, and one tile's products
 // under the scales of the one before changed nothing.
 //

@@ -262,7 +262,9 @@ int fmkv_pool_destroy(fmkv_pool* pool);
  * [n_seqs][n_new][n_kv_heads][head_dim]. block_tables: int32 device
  * [n_seqs][max_blocks]; start_pos: int32 device [n_seqs], the position of
  * each sequence's first new token. Positions below 0 (a padded row's), past the
- * table's width or of blocks outside the pool are not written. */
+ * table's width or of blocks outside the pool are not written. A block that this or a
+ * step writes to is its sequence's alone (fmkv_pages_fork names the one to copy): others
+ * would read its slots while their bits change. */
 int fmkv_paged_append(fmkv_pool* pool, const void* k_bf16, const void* v_bf16,
                       const int32_t* block_tables, int32_t max_blocks, const int32_t* start_pos,
                       int32_t n_seqs, int32_t n_new, void* stream);
@@ -474,11 +476,13 @@ int fmkv_paged_weighing_decode_step(fmkv_pool* pool, const void* k_bf16, const v
  * attention is returned (fmkv_paged_prefill_step and the windowed calls give it).
  * q: bf16 [n_seqs][n_new][n_q_heads][head_dim]. max_seq_len bounds start_pos + n_new.
  * Queries at positions below 0 (a padded row's) add nothing, and n_new 0 stores
- * `weights` alone, of the positions j < start_pos (q may be NULL then). At most 8 query heads per KV
- * head, every cache mode. Needs the pool's workspace: 4 bytes for each element of q
- * (quantized caches), and up to 2 KiB for each position of max_seq_len (4 bytes per
- * sequence and KV head where those are more than 512). The current GPU has to be the
- * pool's; for calls on several streams, and graphs, see the windowed calls above. */
+ * `weights` alone, of the positions j < start_pos (q may be NULL then). At most 8 query
+ * heads per KV head, G of them here, every cache mode. Needs the pool's workspace: 2 KiB for
+ * each position of max_seq_len in whole blocks (4 bytes per sequence and KV head where those
+ * are more than 512), 384 KiB, and for each sequence, KV head and tile of 64 / G queries 1 KiB
+ * and, in quantized caches if n_new * G > 16, 256 * head_dim bytes (affine: 4352 more). The
+ * current GPU has to be the pool's; for calls on several streams, and graphs, see the
+ * windowed calls above. */
 int fmkv_paged_attention_weights(fmkv_pool* pool, const void* q_bf16, const int32_t* block_tables,
                                  int32_t max_blocks, const int32_t* start_pos, int32_t n_seqs,
                                  int32_t n_new, int32_t max_seq_len, const float* weights,
@@ -627,7 +631,7 @@ int fmkv_set_sparse_v_gather(int32_t on);
  * step): AUTO (the default) by estimates from a call's sizes; ALONE: every sequence
  * reads its own table's blocks; ROWS: eight rows (sequences times q heads per KV
  * head) at a time read a prefix once; TILES: 64 rows. Each gives the same
- * attention (a row that sees a value that is not finite is not finite either: NaN, or the
+ * attention (a row that sees a V that is not finite is not finite either: NaN, or the
  * infinity that it makes). No reference counterpart (a tuning and test switch). */
 #define FMKV_PREFIX_AUTO 0
 #define FMKV_PREFIX_ALONE 1
