@@ -44,10 +44,10 @@ namespace {
 constexpr int kObRows = 64;
 constexpr float kObSlack = 8.0f;  // (base 2) a score may exceed its row's reference by
 
-// Affine caches hold q_rot, its sums over 64 dims and those times the codes' offset as f16
-// operands (q_rot times kCodeScale). A row in which one of them would come near f16's largest
-// value, 65504 (|q_rot| or a sixteenth of a sum's offset part past 4000), is held as so much less by a power of 2,
-// and its scores are multiplied back in f32: a row of any size has finite operands.
+// Affine caches hold q_rot (times kCodeScale), its sums over 64 dims and those times the codes'
+// offset as f16 operands. A row in which one of them would come near f16's largest value, 65504
+// (|q_rot|, or a sixteenth of a sum's offset part, past 4000), is held as so much less by a power
+// of 2, and its scores are multiplied back in f32: a row of any size has finite operands.
 constexpr float kObMost = 4000.0f;
 
 // Blocks of a wave's step in calls of many keys: what the registers hold.

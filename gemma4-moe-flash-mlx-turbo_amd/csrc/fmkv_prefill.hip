@@ -1024,9 +1024,9 @@ void prefill_attn_kernel(PrefillArgs a) {
 
   // V values (affine: scales and biases) that are not finite, in a step whose
   // keys some rows do not see: a hidden key's weight 0 makes NaN of them. They
-  // become 0, and NaN the accumulators of the rows that do see
-  // them: what those sum to is an infinity of either sign, or none. (In arithmetic without compares: their masks would crowd the scalar
-  // registers of the whole kernel, and the loop ran up to 10% slower.)
+  // become 0, and NaN the accumulators of the rows that do see them, whose sums
+  // are an infinity of either sign, or none. (In arithmetic without compares:
+  // their masks would crowd the scalar registers of the whole kernel, and the loop ran up to 10% slower.)
   auto hide_not_finite = [&](int step) __attribute__((always_inline)) {
     // 1 in each half of w that is not finite: its exponent is all ones
     auto bad_of = [&](uint32_t w) __attribute__((always_inline)) -> uint32_t {
